@@ -97,7 +97,7 @@ def parse_args(argv=None):
     ap.add_argument("--frames", type=int, default=65)
     ap.add_argument("--audio-tokens", type=int, default=None)
     ap.add_argument("--text-tokens", type=int, default=256)
-    ap.add_argument("--weights", choices=["bf16", "int8", "mxfp8"], default="mxfp8")
+    ap.add_argument("--weights", choices=["bf16", "int8", "mxfp8", "mxfp4"], default="mxfp8")
     ap.add_argument("--no-graph", action="store_true", help="time eager launches instead of HIP graph replay")
     ap.add_argument("--kernel-steps", type=int, default=2, help="eager steps for the dominant-kernel timing")
     ap.add_argument("--guided-steps", type=int, default=3,

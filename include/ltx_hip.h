@@ -26,6 +26,7 @@
  *                                  transformer.py:40-50, :387, :484, :598, :625)
  *   ltx_qknorm_rope_bf16        <- model/transformer/attention.py:578-584
  *                                  (RMSNorm :320-329 + rope.py:16-89)
+ *   ltx_rotary                  <- rope.py:16-89 (both layouts, no norm)
  *   ltx_output_norm_modulate_bf16 <- model/transformer/model.py:1312-1342
  *   ltx_euler_x0_step_bf16      <- model.py:1519-1525 (X0Model.denoise) +
  *                                  components/diffusion_steps.py:19-69
@@ -158,6 +159,39 @@ int ltx_qknorm_rope_axes_bf16(void* q, int64_t q_stride, int64_t rows_q, const f
                               const float* sin_k, const int32_t* idx_k, int64_t axes_k,
                               int64_t tab_rows_k, int64_t D, int64_t head_dim, float eps,
                               void* stream);
+
+/*
+ * Rotary positions of queries and, in the same launch, keys (k NULL: none), from
+ * positions and frequencies instead of tables:
+ *   a' = factor * (a cos t - b sin t),  b' = factor * (b cos t + a sin t),
+ *   t = position * inv_freq[i],  i < rotary_dim / 2,
+ * on the first rotary_dim channels of every head, the others copied: pairs
+ * (i, i + rotary_dim / 2), or with LTX_ROTARY_INTERLEAVED (2 i, 2 i + 1) -- the
+ * reference's split and interleaved layouts (rope.py:16-89).  With
+ * LTX_ROTARY_TRANSPOSE the angle is negated: the map from output gradients to
+ * input gradients.  Angles are formed and reduced in fp64, the rotation is
+ * fp32, rounded once.
+ * x / out: element (batch, token, head, channel) at x + batch * x_batch +
+ * token * x_token + head * x_head + channel, of dtype 0 bf16, 1 fp16, 2 fp32;
+ * out may be x with the same strides, otherwise the two must not overlap.  No
+ * alignment beyond an element's is needed; 16-byte aligned rows are fastest.
+ * positions: (batch, tokens) of pos_type 0 int32, 1 int64, 2 fp32, 3 fp64,
+ * batch stride pos_batch (0: one row for all), token stride 1.  inv_freq: fp64
+ * (rotary_dim / 2) device values.  rotary_dim even, at most head_dim; head_dim
+ * at most 512.
+ */
+#define LTX_ROTARY_INTERLEAVED 1
+#define LTX_ROTARY_TRANSPOSE 2
+typedef struct ltx_rotary_rows {
+  const void* x;
+  int64_t x_batch, x_token, x_head;
+  void* out;
+  int64_t out_batch, out_token, out_head;
+  int64_t heads;
+} ltx_rotary_rows;
+int ltx_rotary(const ltx_rotary_rows* q, const ltx_rotary_rows* k, int dtype, int64_t batch, int64_t tokens,
+               int64_t head_dim, int64_t rotary_dim, const void* positions, int pos_type, int64_t pos_batch,
+               const double* inv_freq, double factor, int flags, void* stream);
 
 /*
  * Output head modulation (model.py:1312-1342):
@@ -353,6 +387,41 @@ int ltx_gemm_mx_gelu_mxfp8(const uint8_t* A, int64_t lda, const uint8_t* a_scale
                            const float* bias, uint8_t* Cq, int64_t ldcq, uint8_t* c_scale, int64_t ld_cscale,
                            int64_t M, int64_t N, int64_t K, int flags, void* stream);
 
+/* ---- MXFP4 products ----------------------------------------------------------
+ * MXFP4 (OCP Microscaling v1.0 with E2M1 elements, blocks of 32 along K, E8M0
+ * scales): code bytes (rows, K / 2), the even k in the low nibble, row stride
+ * in bytes; scale words (ceil(K / 128), ld), word [k / 128][row] holding the
+ * E8M0 bytes of the row's four blocks of those 128 k, the first in its low
+ * byte; ld (in words) at least the rows, a multiple of 4.  Bytes of a last
+ * word that lie past K are not used, nor are words past the rows.  No
+ * counterpart in the reference, whose caches hold MXFP8.
+ *
+ * ltx_gemm_mxfp4_bf16: bf16 rows A (M, K) x MXFP4 weights (N, K), decoded to
+ * bf16 exactly.  K % 64 == 0, N % 8 == 0.
+ * ltx_gemm_mx4_bf16: MXFP4 rows x MXFP4 weights on the scaled FP4 MFMA
+ * (v_mfma_scale_f32_16x16x128_f8f6f4).  K % 128 == 0, N % 8 == 0, operands
+ * below 2 GiB each.
+ * fp32 accumulation; epilogues LTX_GEMM_EPI_*, LTX_GEMM_ROUND_THEN_BIAS and
+ * sigmoid_from as above, except that GELU and the head gate act on the fp32
+ * value (no bf16 rounding before them).  Code and row strides 16-byte
+ * multiples, pointers 16-byte aligned (bias and gate 4).
+ * Products of few tiles split K: they need `workspace` (device memory, 16-byte
+ * aligned) of ltx_gemm_*_workspace_bytes(M, N, K) bytes, 0 where none is
+ * needed (workspace may then be NULL); calls that may run at the same time
+ * need their own.  The split sum has a fixed order.
+ */
+int64_t ltx_gemm_mxfp4_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int ltx_gemm_mxfp4_bf16(const void* A, int64_t lda, const uint8_t* Wq, int64_t ldw, const uint32_t* w_scale,
+                        int64_t ld_scale, const float* bias, void* C, int64_t ldc, int64_t M, int64_t N, int64_t K,
+                        int epilogue, const void* residual, int64_t ldr, const float* gate, int64_t sigmoid_from,
+                        float* workspace, int64_t workspace_bytes, void* stream);
+int64_t ltx_gemm_mx4_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int ltx_gemm_mx4_bf16(const uint8_t* A, int64_t lda, const uint32_t* a_scale, int64_t ld_ascale, const uint8_t* Wq,
+                      int64_t ldw, const uint32_t* w_scale, int64_t ld_scale, const float* bias, void* C,
+                      int64_t ldc, int64_t M, int64_t N, int64_t K, int epilogue, const void* residual, int64_t ldr,
+                      const float* gate, int64_t sigmoid_from, float* workspace, int64_t workspace_bytes,
+                      void* stream);
+
 /* Split-K forms of the three GEMMs for products of few output tiles (the
  * 68-token audio stream, short clips): `splits` blocks per output tile each
  * accumulate K / splits of the product into an fp32 partial tile in
@@ -447,6 +516,19 @@ int ltx_quantize_w8_bf16(const void* W, int64_t ldw, int64_t N, int64_t K, int8_
                          int64_t ldq, float* scale, void* stream);
 int ltx_dequantize_w8_bf16(const int8_t* q, int64_t ldq, const float* scale, int64_t N,
                            int64_t K, void* out, int64_t ldo, void* stream);
+
+/* MXFP4 rows (storage: "MXFP4 products" above; weights and activations alike):
+ *   X = floor(log2(max|v|)) - 2 clamped to [-127, 127] (-127 for a zero block),
+ *   scale = X + 127, code = E2M1(v / 2^X), round-to-nearest-even, saturated to
+ *   +-6, the sign kept on zeros.  A block with a NaN or an infinity gets scale
+ *   255 (NaN) and codes 0.
+ * x: (rows, K) of dtype 0 bf16, 1 fp16, 2 fp32, row stride ldx, 16-byte aligned
+ * rows; K % 32 == 0.  The decoder writes bf16 (rows, K), exact; a block of
+ * scale 255 decodes to NaN.  Words past the rows are left as they were. */
+int ltx_quantize_mxfp4(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t K, uint8_t* q, int64_t ldq,
+                       uint32_t* scales, int64_t ld_scale, void* stream);
+int ltx_dequantize_mxfp4_bf16(const uint8_t* q, int64_t ldq, const uint32_t* scales, int64_t ld_scale,
+                              int64_t rows, int64_t K, void* out, int64_t ldo, void* stream);
 
 /* FP8 checkpoint tensor dequantisation -- the numeric step of
  * loader/transformer_cache.py:658-708 (_iter_fp8_checkpoint_weights):

@@ -1,0 +1,127 @@
+// MXFP4 operands of the projection GEMMs (gemm_fp4.hip: bf16 rows x MXFP4
+// weights; gemm_mx4.hip: MXFP4 rows x MXFP4 weights) and their epilogue.
+//
+// Storage: E2M1 codes (rows, K / 2 bytes), the even k in the low nibble, and
+// the E8M0 scales of 32-element blocks as words (ceil(K / 128), ld): word
+// [k / 128][row] holds the four blocks of those 128 k, the first in its low
+// byte.  The words of neighbouring rows are neighbours, so the scales of a
+// tile's rows for 128 k are one contiguous piece (a (rows, K / 32) array gives
+// every row's few bytes a line of its own: beside 4-bit codes those lines
+// would be a third of all requests).  Bytes past K hold no block and are not
+// used.
+#pragma once
+
+#include "gemm_common.h"
+
+namespace ltx {
+
+// eight codes of one word and one block -> bf16, exact (E2M1 has one mantissa
+// bit; 2^X from the scale)
+__device__ __forceinline__ bf16x8 fp4x8_bf16(uint32_t w, float s) {
+  uint32_t o[4];
+  o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
+  o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
+  o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
+  o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
+  return __builtin_bit_cast(bf16x8, u32x4{o[0], o[1], o[2], o[3]});
+}
+
+// Four consecutive columns n .. n + 3 of output row m from their fp32 sums.
+// MXFP4 products reproduce no reference arithmetic, so GELU and the head gate
+// act on the fp32 value, without the other formats' bf16 rounding before them.
+// A residual epilogue keeps that rounding of the branch (its tiles are staged
+// as bf16 rows).
+template <int EPI>
+__device__ __forceinline__ bf16x4 fp4_branch4(const GemmArgs& p, f32x4 a, f32x4 bias, int n) {
+  bf16x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float y = (p.round_then_bias ? round_bf(a[e]) : a[e]) + bias[e];
+    if (EPI == LTX_GEMM_EPI_GELU) y = gelu_tanh(y);
+    if (EPI == LTX_GEMM_EPI_SIGMOID2) y = sigmoid2_bf(y);
+    if (EPI == LTX_GEMM_EPI_BIAS && n + e >= p.sig_from) y = sigmoid2_bf(y);
+    v[e] = (bf16)y;
+  }
+  return v;
+}
+template <int EPI>
+__device__ __forceinline__ bf16 fp4_residual(bf16 y, bf16 r, float g) {
+  return (bf16)(EPI == LTX_GEMM_EPI_RESIDUAL ? fmaf(g, (float)y, (float)r) : round_bf((float)y * g) + (float)r);
+}
+template <int EPI>
+__device__ __forceinline__ void fp4_store4(const GemmArgs& p, f32x4 a, int m, int n) {
+  f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (p.bias)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bias[e] = p.bias[n + e];
+  bf16x4 v = fp4_branch4<EPI>(p, a, bias, n);
+  if constexpr (EPI == LTX_GEMM_EPI_RESIDUAL || EPI == LTX_GEMM_EPI_RESIDUAL_ROUND) {
+    const bf16x4 r = *reinterpret_cast<const bf16x4*>(p.R + (int64_t)m * p.ldr + n);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = fp4_residual<EPI>(v[e], r[e], p.gate[n + e]);
+  }
+  *reinterpret_cast<bf16x4*>(p.C + (int64_t)m * p.ldc + n) = v;
+}
+
+// sum of `splits` partial products (fp32, split order) and the epilogue
+int fp4_combine(const GemmArgs& p, int epi, int splits, hipStream_t s);
+
+// f<EPI>() of an epilogue code; false for an unknown one
+template <class F>
+static bool fp4_epilogue(int epi, F&& f) {
+  switch (epi) {
+    case LTX_GEMM_EPI_BIAS: f(std::integral_constant<int, LTX_GEMM_EPI_BIAS>{}); return true;
+    case LTX_GEMM_EPI_GELU: f(std::integral_constant<int, LTX_GEMM_EPI_GELU>{}); return true;
+    case LTX_GEMM_EPI_RESIDUAL: f(std::integral_constant<int, LTX_GEMM_EPI_RESIDUAL>{}); return true;
+    case LTX_GEMM_EPI_RESIDUAL_ROUND: f(std::integral_constant<int, LTX_GEMM_EPI_RESIDUAL_ROUND>{}); return true;
+    case LTX_GEMM_EPI_SIGMOID2: f(std::integral_constant<int, LTX_GEMM_EPI_SIGMOID2>{}); return true;
+  }
+  return false;
+}
+
+// Checks shared by the two products; `a_bytes` bytes per row of K activations.
+static inline int fp4_check(const void* A, int64_t lda, const void* W, int64_t ldw, const void* w_scale,
+                            int64_t ld_scale, const float* bias, const void* C, int64_t ldc, int64_t M, int64_t N,
+                            int64_t K, int epilogue, const void* R, int64_t ldr, const float* gate, int64_t lda_min,
+                            int64_t lda_unit) {
+  auto al = [](const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; };
+  if (!A || !W || !w_scale || !C || M < 0 || N < 0 || K < 0) return LTX_ERR_INVALID_ARG;
+  if (M > INT32_MAX / 2 || N > INT32_MAX / 2 || K > INT32_MAX / 2) return LTX_ERR_UNSUPPORTED;
+  const int epi = epilogue & 0xff;
+  if (epilogue & ~(0xff | LTX_GEMM_ROUND_THEN_BIAS) || epi > LTX_GEMM_EPI_SIGMOID2) return LTX_ERR_INVALID_ARG;
+  const bool resid = epi == LTX_GEMM_EPI_RESIDUAL || epi == LTX_GEMM_EPI_RESIDUAL_ROUND;
+  if (resid && (!R || !gate || ldr < N)) return LTX_ERR_INVALID_ARG;
+  if (K % 64 != 0 || N % 8 != 0) return LTX_ERR_UNSUPPORTED;
+  if (lda < lda_min || ldw < K / 2 || ldc < N || ld_scale < N) return LTX_ERR_INVALID_ARG;
+  if (!al(A, 16) || !al(W, 16) || !al(C, 16) || !al(w_scale, 16) || !al(bias, 4) || !al(gate, 4) ||
+      lda % lda_unit || ldw % 16 || ldc % 8 || ld_scale % 4 || (resid && (!al(R, 16) || ldr % 8)))
+    return LTX_ERR_ALIGNMENT;
+  return LTX_OK;
+}
+
+static inline GemmArgs fp4_args(const void* A, int64_t lda, const void* W, int64_t ldw, const uint32_t* w_scale,
+                                int64_t ld_scale, const float* bias, void* C, int64_t ldc, int64_t M, int64_t N,
+                                int64_t K, int epilogue, const void* R, int64_t ldr, const float* gate,
+                                int64_t sigmoid_from) {
+  GemmArgs p = {};
+  p.A = (const bf16*)A;
+  p.lda = lda;
+  p.B = W;
+  p.ldb = ldw;
+  p.bscale = w_scale;
+  p.ld_scale = ld_scale;
+  p.bias = bias;
+  p.C = (bf16*)C;
+  p.ldc = ldc;
+  p.R = (const bf16*)R;
+  p.ldr = ldr;
+  p.gate = gate;
+  p.sig_from = (int)(sigmoid_from < N ? (sigmoid_from < 0 ? 0 : sigmoid_from) : N);
+  p.round_then_bias = (epilogue & LTX_GEMM_ROUND_THEN_BIAS) != 0;
+  p.M = (int)M;
+  p.N = (int)N;
+  p.K = (int)K;
+  return p;
+}
+
+}  // namespace ltx

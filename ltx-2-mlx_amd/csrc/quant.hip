@@ -14,9 +14,16 @@
 // int8 W8A16 (per output channel, symmetric):
 //     s[n] = max_k |w[n,k]| / 127 (fp32), q = clamp(rint(w / s), -127, 127);
 //     a zero row has s = 0 and q = 0.  Decode: w' = bf16(fp32(q) * s).
+// MXFP4 (OCP Microscaling v1.0, element E2M1, block 32 along K, scale E8M0):
+//     X = floor(log2(max|v|)) - 2 (2 = E2M1 emax), clamped to [-127, 127],
+//     scale byte = X + 127, code = E2M1(v / 2^X) rounded to nearest-even and
+//     saturated to +-6, the sign kept on zeros.  An all-zero block gets X = -127.
+//     E2M1 has no NaN: a block with a NaN or an infinity gets scale byte 255
+//     (NaN) and codes 0, and decodes to NaN throughout.
+//     Codes two to a byte, the even k low; scale words as gemm_fp4.h lays out.
 #include <type_traits>
 
-#include "ltx_common.h"
+#include "gemm_fp4.h"
 
 namespace ltx {
 
@@ -75,6 +82,99 @@ __global__ void mxfp8_dequantize_kernel(const uint8_t* __restrict__ q, int64_t l
     o[2 * d + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[d], scale, true));
   }
   *reinterpret_cast<u32x4*>(out + n * ldo + c * 8) = u32x4{o[0], o[1], o[2], o[3]};
+}
+
+// ---- MXFP4 -------------------------------------------------------------------
+// Row loads of eight elements as fp32.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  if constexpr (std::is_same_v<T, float>) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = a[e];
+      v[4 + e] = b[e];
+    }
+  } else {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    const t8 x = *reinterpret_cast<const t8*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)x[e];
+  }
+}
+
+// A workgroup encodes 16 rows x 512 k, a wave a row at a time (lane l elements
+// 8 l .. 8 l + 7, lanes 4 b .. 4 b + 3 forming block b).  The scale words of a
+// k range are contiguous over rows, so they meet in LDS and leave as 64-byte
+// pieces.
+constexpr int kQ4Rows = 16;
+template <typename T>
+__global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows,
+                                                             int64_t K, uint8_t* __restrict__ q, int64_t ldq,
+                                                             uint32_t* __restrict__ sc, int64_t lds) {
+  __shared__ uint8_t scale[4][kQ4Rows][4];  // [128 k][row][block]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t chunks = (K + 511) / 512;
+  const int64_t r0 = (int64_t)blockIdx.x / chunks * kQ4Rows, k0 = (int64_t)blockIdx.x % chunks * 512;
+  const int64_t col = k0 + lane * 8;
+  const bool in = col < K;  // K % 32 == 0: a block's four lanes agree
+#pragma unroll
+  for (int i = 0; i < kQ4Rows / 4; ++i) {
+    const int lr = i * 4 + wave;
+    const int64_t r = r0 + lr;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+    if (in && r < rows) load8(x + r * ldx + col, v);
+    // the block's largest magnitude, as bits: those of a NaN or an infinity
+    // are above every finite one's
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t b = __float_as_uint(v[e]) & 0x7fffffffu;
+      top = b > top ? b : top;
+    }
+    const uint32_t t1 = __shfl_xor(top, 1, 64);
+    top = t1 > top ? t1 : top;
+    const uint32_t t2 = __shfl_xor(top, 2, 64);
+    top = t2 > top ? t2 : top;
+    const bool bad = top >= 0x7f800000u;
+    // floor(log2): the exponent field; below 2^-126 (and 0) X is -127 anyway
+    int X = (int)(top >> 23) - 127 - 2;
+    X = X < -127 ? -127 : X;
+    if ((lane & 3) == 0) scale[lane >> 4][lr][(lane >> 2) & 3] = !in ? 0 : (bad ? 255 : (uint8_t)(X + 127));
+    if (!in || r >= rows) continue;
+    const float s = ldexpf(1.0f, X), lim = 6.0f * s;  // lim: X <= 125
+    uint32_t w = 0;
+    auto cl = [lim](float f) { return fabsf(f) >= lim ? __builtin_copysignf(lim, f) : f; };
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, cl(v[0]), cl(v[1]), s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, cl(v[2]), cl(v[3]), s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, cl(v[4]), cl(v[5]), s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, cl(v[6]), cl(v[7]), s, 3);
+    *reinterpret_cast<uint32_t*>(q + r * ldq + col / 2) = bad ? 0u : w;
+  }
+  __syncthreads();
+  const int64_t words = (K + 127) / 128;
+  const int t = threadIdx.x;
+  if (t < 4 * kQ4Rows) {
+    const int64_t w = k0 / 128 + t / kQ4Rows, r = r0 + t % kQ4Rows;
+    if (w < words && r < rows)
+      sc[w * lds + r] = *reinterpret_cast<const uint32_t*>(scale[t / kQ4Rows][t % kQ4Rows]);
+  }
+}
+
+// Eight codes per lane (4 bytes in, 16 out).
+__global__ __launch_bounds__(256) void mxfp4_dequantize_kernel(const uint8_t* __restrict__ q, int64_t ldq,
+                                                               const uint32_t* __restrict__ sc, int64_t lds,
+                                                               int64_t rows, int64_t K, bf16* __restrict__ out,
+                                                               int64_t ldo) {
+  const int64_t per_row = K / 8;
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (idx >= rows * per_row) return;
+  const int64_t r = idx / per_row, c = idx % per_row * 8;
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(q + r * ldq + c / 2);
+  const uint32_t e = (sc[c / 128 * lds + r] >> (c / 32 % 4 * 8)) & 0xffu;
+  *reinterpret_cast<bf16x8*>(out + r * ldo + c) = fp4x8_bf16(w, e8m0_to_f32(e));
 }
 
 // One wave per row.
@@ -233,6 +333,41 @@ extern "C" int ltx_dequantize_w8_bf16(const int8_t* q, int64_t ldq, const float*
   if (total == 0) return LTX_OK;
   w8_dequantize_kernel<<<(int)((total + 255) / 256), 256, 0, (hipStream_t)stream>>>(
       q, ldq, scale, N, K, (bf16*)out, ldo);
+  return ltx_launch_status();
+}
+
+extern "C" int ltx_quantize_mxfp4(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t K, uint8_t* q,
+                                  int64_t ldq, uint32_t* scales, int64_t ld_scale, void* stream) {
+  if (!x || !q || !scales || rows < 0 || K < 0) return LTX_ERR_INVALID_ARG;
+  if (dtype < 0 || dtype > 2 || K % 32) return LTX_ERR_UNSUPPORTED;
+  if (ldx < K || ldq < K / 2 || ld_scale < rows) return LTX_ERR_INVALID_ARG;
+  if (!a16(x) || !a16(q) || !a16(scales) || ldx % (dtype == 2 ? 4 : 8) || ldq % 16 || ld_scale % 4)
+    return LTX_ERR_ALIGNMENT;
+  if (rows == 0 || K == 0) return LTX_OK;
+  const int64_t chunks = (K + 511) / 512, groups = (rows + kQ4Rows - 1) / kQ4Rows;
+  if (chunks > INT32_MAX / groups) return LTX_ERR_UNSUPPORTED;
+  const int blocks = (int)(chunks * groups);
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == 0)
+    mxfp4_quantize_kernel<<<blocks, 256, 0, s>>>((const bf16*)x, ldx, rows, K, q, ldq, scales, ld_scale);
+  else if (dtype == 1)
+    mxfp4_quantize_kernel<<<blocks, 256, 0, s>>>((const _Float16*)x, ldx, rows, K, q, ldq, scales, ld_scale);
+  else
+    mxfp4_quantize_kernel<<<blocks, 256, 0, s>>>((const float*)x, ldx, rows, K, q, ldq, scales, ld_scale);
+  return ltx_launch_status();
+}
+
+extern "C" int ltx_dequantize_mxfp4_bf16(const uint8_t* q, int64_t ldq, const uint32_t* scales, int64_t ld_scale,
+                                         int64_t rows, int64_t K, void* out, int64_t ldo, void* stream) {
+  if (!q || !scales || !out || rows < 0 || K < 0) return LTX_ERR_INVALID_ARG;
+  if (K % 32) return LTX_ERR_UNSUPPORTED;
+  if (ldq < K / 2 || ldo < K || ld_scale < rows) return LTX_ERR_INVALID_ARG;
+  if (!a16(out) || !a16(q) || !a16(scales) || ldq % 16 || ldo % 8 || ld_scale % 4) return LTX_ERR_ALIGNMENT;
+  if (rows == 0 || K == 0) return LTX_OK;
+  if (K / 8 > (int64_t)INT32_MAX * 256 / rows) return LTX_ERR_UNSUPPORTED;
+  const int64_t total = rows * (K / 8);
+  mxfp4_dequantize_kernel<<<(int)((total + 255) / 256), 256, 0, (hipStream_t)stream>>>(
+      q, ldq, scales, ld_scale, rows, K, (bf16*)out, ldo);
   return ltx_launch_status();
 }
 

@@ -19,10 +19,11 @@ LIB_PATH = Path(os.environ.get("LTX_HIP_LIB", Path(__file__).with_name(LIB_NAME)
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _vp = ctypes.c_void_p
 
-# name -> argtypes (every function returns int: a status, or for
-# ltx_gemm_auto_splits / _rows the choice)
+# name -> argtypes (functions return int: a status, or for
+# ltx_gemm_auto_splits / _rows the choice; those of SIZES an int64)
 SIGNATURES: dict[str, list] = {
     "ltx_version": [],
     "ltx_device_clock_stamp": [_vp, _vp],
@@ -67,6 +68,15 @@ SIGNATURES: dict[str, list] = {
     "ltx_dequantize_mxfp8_bf16": [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp],
     "ltx_quantize_w8_bf16": [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp],
     "ltx_dequantize_w8_bf16": [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp],
+    "ltx_gemm_mxfp4_workspace_bytes": [_i64, _i64, _i64],
+    "ltx_gemm_mx4_workspace_bytes": [_i64, _i64, _i64],
+    "ltx_gemm_mxfp4_bf16": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _int, _vp, _i64, _vp,
+                            _i64, _vp, _i64, _vp],
+    "ltx_gemm_mx4_bf16": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _int, _vp,
+                          _i64, _vp, _i64, _vp, _i64, _vp],
+    "ltx_quantize_mxfp4": [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp],
+    "ltx_dequantize_mxfp4_bf16": [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp],
+    "ltx_rotary": [_vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _int, _i64, _vp, _f64, _int, _vp],
     "ltx_dequantize_fp8_e4m3": [_vp, _i64, _vp, _vp, _int, _vp],
     "ltx_attn_transpose_v_bf16": [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp],
     "ltx_flash_attn_bf16": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _vp],
@@ -94,6 +104,17 @@ SIGNATURES: dict[str, list] = {
     "ltx_gemma_features_bf16": [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _f32, _f32, _f32, _vp, _vp, _i64, _vp],
 }
 
+# Functions of SIGNATURES whose result is a size (int64)
+SIZES = ("ltx_gemm_mxfp4_workspace_bytes", "ltx_gemm_mx4_workspace_bytes")
+
+
+class RotaryRows(ctypes.Structure):
+    """``ltx_rotary_rows``: a tensor and where its result goes."""
+
+    _fields_ = [("x", _vp), ("x_batch", _i64), ("x_token", _i64), ("x_head", _i64),
+                ("out", _vp), ("out_batch", _i64), ("out_token", _i64), ("out_head", _i64), ("heads", _i64)]
+
+
 # Flag values (include/ltx_hip.h)
 ADALN_ROUND_NORM = 1
 ADALN_NO_NORM = 2
@@ -112,6 +133,8 @@ GEMM_TILE_256x128 = 4 << 8
 GEMM_TILE_G8 = 5 << 8
 GEMM_TILE_G8_128 = 6 << 8
 GEMM_ROUND_THEN_BIAS = 1 << 12
+ROTARY_INTERLEAVED = 1
+ROTARY_TRANSPOSE = 2
 # Status of a request above the fixed scratch of a no-allocation entry point
 ERR_SCRATCH_LIMIT = -5
 ATTN_NOALLOC_SCRATCH_BYTES = 32 << 20
@@ -133,6 +156,8 @@ def lib() -> ctypes.CDLL:
             fn = getattr(handle, name)
             fn.argtypes = argtypes
             fn.restype = ctypes.c_int
+        for name in SIZES:
+            getattr(handle, name).restype = _i64
         handle.ltx_attn_vt_padded_len.argtypes = [_i64]
         handle.ltx_attn_vt_padded_len.restype = _i64
         handle.ltx_attn_splitkv_workspace_bytes.argtypes = [_i64, _i64, _i64, _i64]
@@ -162,6 +187,23 @@ def call(name: str, *args, detail: str = "") -> None:
     status = getattr(lib(), name)(*args)
     if status != 0:
         raise LtxKernelError(name, status, detail)
+
+
+def call_on(t: torch.Tensor, name: str, *args, detail: str = "") -> None:
+    """:func:`call` with t's device current (a launch goes to the current device)."""
+    if t.get_device() == torch._C._cuda_getDevice():
+        call(name, *args, detail=detail)
+    else:
+        with torch.cuda.device(t.device):
+            call(name, *args, detail=detail)
+
+
+def same_device(*tensors: torch.Tensor | None) -> None:
+    """Raise unless every given tensor is on the first one's GPU."""
+    first = tensors[0]
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device != first.device):
+            raise ValueError(f"expected device tensors on one GPU, got {first.device} and {t.device}")
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

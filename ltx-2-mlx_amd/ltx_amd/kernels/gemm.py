@@ -1,7 +1,7 @@
 """Projection GEMMs: ``y = epilogue(x @ W.T + b)`` on gfx950 matrix cores.
 
-One entry point, :func:`linear`, for the three resident weight formats of
-:class:`LinearWeight` (bf16, int8 W8A16, MXFP8).  It replaces ``nn.Linear`` /
+One entry point, :func:`linear`, for the resident weight formats of
+:class:`LinearWeight` (bf16, int8 W8A16, MXFP8, MXFP4).  It replaces ``nn.Linear`` /
 ``mx.addmm`` (model/transformer/attention.py:425-437,
 feed_forward.py:91-112) and ``mx.quantized_matmul`` for the mxfp8 cache
 (loader/transformer_cache.py:177-193).  The epilogues fuse what the reference
@@ -20,6 +20,12 @@ weights multiply MXFP8-quantised activations on the scaled fp8 MFMA
 (:func:`linear_mx`) instead of bf16 activations.  That is not the reference's
 arithmetic -- its MXFP8 path keeps the activations in bf16 -- and the
 activations' E4M3 rounding moves outputs by a few percent of their range.
+
+MXFP4 (E2M1 codes, an E8M0 scale per 32 along K) has no counterpart in the
+reference: weights at half MXFP8's bytes, times bf16 activations in
+:func:`linear`, or times MXFP4 activations (:class:`Mx4Rows`, from
+:func:`quantize_rows_mxfp4`) on the scaled FP4 MFMA.  Its GELU and head gate
+act on the fp32 value, without the bf16 rounding before them.
 """
 
 from __future__ import annotations
@@ -40,7 +46,7 @@ EPI_SIGMOID2 = _lib.GEMM_EPI_SIGMOID2
 TILE_AUTO, TILE_256, TILE_128, TILE_256_DMA, TILE_256x128, TILE_G8, TILE_G8_128 = 0, 1, 2, 3, 4, 5, 6
 
 
-FORMATS = ("bf16", "int8", "mxfp8")
+FORMATS = ("bf16", "int8", "mxfp8", "mxfp4")
 
 # Opt-in quantised-activation path for MXFP8 weights (see the module text):
 # products with at least this many 256x256 tiles quantise their activations
@@ -60,7 +66,10 @@ class LinearWeight:
 
     ``w`` is (N, K) in nn.Linear layout: bf16, int8 codes, or E4M3 codes
     (uint8).  ``scale`` is fp32 (N) for int8 and E8M0 uint8 (N, K/32) for
-    mxfp8.  ``bias`` is fp32 (N) or None.
+    mxfp8.  ``bias`` is fp32 (N) or None.  mxfp4: ``w`` is (N, K/2) uint8, two
+    E2M1 codes per byte, the even k low, and ``scale`` int32 words
+    (ceil(K/128), N rounded up to 4), word [k/128, n] the E8M0 bytes of row n's
+    four blocks of those 128 k (:func:`mxfp4_scale_words`).
 
     ``qlinear`` selects the reference module whose arithmetic the GEMM
     reproduces: False for ``nn.Linear`` (``mx.addmm``: bias added to the fp32
@@ -84,7 +93,7 @@ class LinearWeight:
 
     @property
     def in_features(self) -> int:
-        return self.w.shape[1]
+        return self.w.shape[1] * (2 if self.kind == "mxfp4" else 1)
 
     def nbytes(self) -> int:
         n = self.w.numel() * self.w.element_size()
@@ -110,13 +119,16 @@ def _quantize(kind: str, w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         _lib.call("ltx_quantize_mxfp8_bf16", w.data_ptr(), k, n, k, q.data_ptr(), k, s.data_ptr(), k // 32,
                   stream, detail=f"N={n} K={k}")
         return q, s
+    if kind == "mxfp4":
+        rows = quantize_rows_mxfp4(w)
+        return rows.codes, rows.scales
     raise ValueError(f"unknown quantised format {kind!r}")
 
 
 def make_weight(w: torch.Tensor, bias: torch.Tensor | None = None, kind: str = "bf16") -> LinearWeight:
     """Build a resident weight from a bf16 (N, K) device tensor.
 
-    ``kind="int8"`` / ``"mxfp8"`` quantise on the device with the library's
+    ``kind="int8"`` / ``"mxfp8"`` / ``"mxfp4"`` quantise on the device with the library's
     encoders (include/ltx_hip.h "weight formats").
     """
     if w.dtype != torch.bfloat16 or w.dim() != 2 or not w.is_cuda:
@@ -130,6 +142,8 @@ def make_weight(w: torch.Tensor, bias: torch.Tensor | None = None, kind: str = "
 
 def dequantize(weight: LinearWeight) -> torch.Tensor:
     """bf16 (N, K) values of a weight, decoded exactly per its format."""
+    if weight.kind == "mxfp4":
+        return dequantize_rows_mxfp4(Mx4Rows(weight.w, weight.scale))
     n, k = weight.w.shape
     if weight.kind == "bf16":
         return weight.w
@@ -389,6 +403,163 @@ def linear_mx_gelu(x: MxRows, weight: LinearWeight) -> MxRows:
     return MxRows(codes, scales)
 
 
+@dataclass
+class Mx4Rows:
+    """Rows in MXFP4: code bytes (M, K/2) uint8 and scale words (ceil(K/128), M
+    rounded up to 4) int32, as :class:`LinearWeight` holds them."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def shape(self):
+        return torch.Size((self.codes.shape[0], self.codes.shape[1] * 2))
+
+
+def _check_mxfp4(what: str, codes: torch.Tensor, scales: torch.Tensor) -> tuple[int, int]:
+    """(rows, K) of MXFP4 codes whose scale words fit them."""
+    if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.stride(1) != 1:
+        raise ValueError(f"{what}: MXFP4 codes are (rows, K/2) uint8 of unit column stride")
+    rows, k = codes.shape[0], codes.shape[1] * 2
+    if (scales is None or scales.dtype != torch.int32 or scales.dim() != 2 or scales.stride(1) != 1
+            or scales.shape[0] < (k + 127) // 128 or scales.shape[1] < rows):
+        raise ValueError(f"{what}: MXFP4 scales of {rows} x {k} values are int32 words ({(k + 127) // 128}, "
+                         f">= {rows}) of unit column stride")
+    return rows, k
+
+
+def mxfp4_scale_words(scales: torch.Tensor) -> torch.Tensor:
+    """E8M0 bytes (rows, K/32) uint8 as the scale words that MXFP4 operands
+    hold: int32 (ceil(K/128), rows rounded up to 4)."""
+    rows, blocks = scales.shape
+    words = (blocks + 3) // 4
+    out = torch.zeros((words, (rows + 3) // 4 * 4, 4), dtype=torch.uint8, device=scales.device)
+    padded = torch.nn.functional.pad(scales, (0, words * 4 - blocks))
+    out[:, :rows] = padded.view(rows, words, 4).transpose(0, 1)
+    return out.view(torch.int32).squeeze(-1)
+
+
+def mxfp4_block_scales(words: torch.Tensor, rows: int, k: int) -> torch.Tensor:
+    """E8M0 bytes (rows, K/32) uint8 of scale words (:func:`mxfp4_scale_words`)."""
+    b = words[:, :rows].contiguous().view(torch.uint8).view(-1, rows, 4)
+    return b.transpose(0, 1).reshape(rows, -1)[:, :k // 32].contiguous()
+
+
+_QUANT_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def quantize_rows_mxfp4(x: torch.Tensor) -> Mx4Rows:
+    """MXFP4 of the rows of x (..., K) bf16, fp16 or fp32 (blocks of 32 along K,
+    the OCP rule: X = floor(log2 max|v|) - 2, E2M1 to nearest even, saturated).
+    A block with a NaN or an infinity decodes to NaN."""
+    k = x.shape[-1]
+    if x.dtype not in _QUANT_DTYPES:
+        raise TypeError(f"quantize_rows_mxfp4 takes bf16, fp16 or fp32 rows, got {x.dtype}")
+    if k % 32:
+        raise ValueError(f"K={k} is not a multiple of 32")
+    xv, ldx = _lib.row_view(x, k)
+    m = x.numel() // k if k else 0
+    ld = (m + 3) // 4 * 4
+    codes = torch.empty((m, k // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(((k + 127) // 128, ld), dtype=torch.int32, device=x.device)
+    if m and k:
+        _lib.call_on(x, "ltx_quantize_mxfp4", _lib.ptr(xv), _QUANT_DTYPES[x.dtype], ldx, m, k, codes.data_ptr(),
+                     k // 2, scales.data_ptr(), ld, _lib.stream_of(x), detail=f"{x.dtype} rows M={m} K={k} ld={ldx}")
+    return Mx4Rows(codes, scales)
+
+
+def dequantize_rows_mxfp4(rows: Mx4Rows) -> torch.Tensor:
+    """bf16 (M, K) values of MXFP4 rows, exact."""
+    m, k = _check_mxfp4("dequantize_rows_mxfp4", rows.codes, rows.scales)
+    _lib.same_device(rows.codes, rows.scales)
+    out = torch.empty((m, k), dtype=torch.bfloat16, device=rows.codes.device)
+    if m and k:
+        _lib.call_on(out, "ltx_dequantize_mxfp4_bf16", rows.codes.data_ptr(), rows.codes.stride(0),
+                     rows.scales.data_ptr(), rows.scales.stride(0), m, k, out.data_ptr(), k, _lib.stream_of(out),
+                     detail=f"M={m} K={k}")
+    return out
+
+
+def _workspace(nbytes: int, like: torch.Tensor) -> torch.Tensor | None:
+    return torch.empty(nbytes // 4, dtype=torch.float32, device=like.device) if nbytes else None
+
+
+@functools.lru_cache(maxsize=4096)
+def _mxfp4_workspace_bytes(name: str, m: int, n: int, k: int) -> int:
+    return getattr(_lib.lib(), name)(m, n, k)
+
+
+def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int, out: torch.Tensor | None,
+                  residual: torch.Tensor | None, gate: torch.Tensor | None,
+                  sigmoid_from: int | None) -> torch.Tensor:
+    """:func:`linear` on MXFP4 weights, for bf16 or MXFP4 rows."""
+    n, k = _check_mxfp4("weight", weight.w, weight.scale)
+    quantised = isinstance(x, Mx4Rows)
+    if quantised:
+        m, kx = _check_mxfp4("activations", x.codes, x.scales)
+        src, lda, lead = x.codes, x.codes.stride(0), (m,)
+    else:
+        if x.dtype != torch.bfloat16:
+            raise TypeError(f"linear expects bf16 or MXFP4 activations, got {x.dtype}")
+        kx = x.shape[-1]
+        src, lda = _lib.row_view(x, kx)
+        m, lead = x.numel() // kx if kx else 0, x.shape[:-1]
+    if kx != k:
+        raise ValueError(f"activations have K={kx}, the weight {k}")
+    if out is None:
+        out = torch.empty((*lead, n), dtype=torch.bfloat16, device=src.device)
+    elif out.dtype != torch.bfloat16 or out.shape != (*lead, n):
+        raise ValueError(f"out must be bf16 {(*lead, n)}, got {out.dtype} {tuple(out.shape)}")
+    ov, ldc = _lib.row_view(out, n)
+    if ov.data_ptr() != out.data_ptr():
+        raise ValueError("out must be a row-strided view")
+    rptr, ldr, gptr = None, 0, None
+    if epilogue in (EPI_RESIDUAL, EPI_RESIDUAL_ROUND):
+        if residual is None or gate is None:
+            raise ValueError("residual epilogues need residual and gate")
+        if residual.dtype != torch.bfloat16 or residual.shape[-1] != n or residual.numel() != m * n:
+            raise ValueError(f"residual must be bf16 ({m}, {n}), got {residual.dtype} {tuple(residual.shape)}")
+        rv, ldr = _lib.row_view(residual, n)
+        if rv.data_ptr() != residual.data_ptr():
+            raise ValueError("residual must be a row-strided view")
+        rptr = rv.data_ptr()
+        if gate.dtype != torch.float32 or gate.numel() != n:
+            raise ValueError("gate must be fp32 with N elements")
+        gate = _lib.flat(gate)
+        gptr = gate.data_ptr()
+    else:
+        residual = gate = None
+    bias = weight.bias
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != n or not bias.is_contiguous()):
+        raise ValueError(f"bias must be {n} contiguous fp32 values")
+    _lib.same_device(src, x.scales if quantised else None, weight.w, weight.scale, bias, out, residual, gate)
+    flags = epilogue
+    if weight.qlinear and bias is not None:
+        flags |= _lib.GEMM_ROUND_THEN_BIAS
+    if m == 0:
+        return out
+    ws_bytes = _mxfp4_workspace_bytes(
+        "ltx_gemm_mx4_workspace_bytes" if quantised else "ltx_gemm_mxfp4_workspace_bytes", m, n, k)
+    ws = _workspace(ws_bytes, src)
+    tail = (weight.w.data_ptr(), weight.w.stride(0), weight.scale.data_ptr(), weight.scale.stride(0),
+            None if bias is None else bias.data_ptr(), ov.data_ptr(), ldc, m, n, k, flags, rptr, ldr, gptr,
+            n if sigmoid_from is None else int(sigmoid_from), None if ws is None else ws.data_ptr(), ws_bytes,
+            _lib.stream_of(src))
+    detail = f"mxfp4 {'x mxfp4' if quantised else 'x bf16'} M={m} N={n} K={k} epi={epilogue}"
+    hook = LAUNCH_HOOK
+    info = (weight.kind, m, n, k, epilogue)
+    if hook is not None:
+        hook("pre", info)
+    if quantised:
+        _lib.call_on(src, "ltx_gemm_mx4_bf16", src.data_ptr(), lda, x.scales.data_ptr(), x.scales.stride(0), *tail,
+                     detail=detail)
+    else:
+        _lib.call_on(src, "ltx_gemm_mxfp4_bf16", src.data_ptr(), lda, *tail, detail=detail)
+    if hook is not None:
+        hook("post", info)
+    return out
+
+
 def _mx_eligible(m: int, n: int, k: int, weight: LinearWeight, tile: int) -> bool:
     return (MX_ACTIVATIONS and weight.kind == "mxfp8" and tile in (TILE_AUTO, TILE_G8) and k % 512 == 0
             and ((m + 255) // 256) * ((n + 255) // 256) >= MX_MIN_TILES)
@@ -462,7 +633,7 @@ def linear_rowss(x: torch.Tensor, weight: LinearWeight, ss_cols: int, *, sigmoid
     return out, ss
 
 
-def linear(x: torch.Tensor, weight: LinearWeight, *, epilogue: int = EPI_BIAS,
+def linear(x: torch.Tensor | MxRows | Mx4Rows, weight: LinearWeight, *, epilogue: int = EPI_BIAS,
            out: torch.Tensor | None = None, residual: torch.Tensor | None = None,
            gate: torch.Tensor | None = None, tile: int = TILE_AUTO,
            sigmoid_from: int | None = None, splits: int | None = None) -> torch.Tensor:
@@ -477,7 +648,15 @@ def linear(x: torch.Tensor, weight: LinearWeight, *, epilogue: int = EPI_BIAS,
     partials from a workspace.
     With ``ROWS_KERNEL`` set, few-row products with ``splits=None`` and the
     automatic tile choice run on :func:`linear_rows`.
+    MXFP4 weights take bf16 rows or :class:`Mx4Rows` and choose tiles and
+    splits themselves (``tile`` and ``splits`` stay at their defaults).
     """
+    if weight.kind == "mxfp4" or isinstance(x, Mx4Rows):
+        if weight.kind != "mxfp4" or isinstance(x, MxRows):
+            raise ValueError(f"{type(x).__name__} activations do not go with {weight.kind} weights")
+        if tile != TILE_AUTO or splits is not None:
+            raise ValueError("MXFP4 products take no explicit tile or split count")
+        return _linear_mxfp4(x, weight, epilogue, out, residual, gate, sigmoid_from)
     k = weight.in_features
     n = weight.out_features
     if (splits is None and tile == TILE_AUTO and not isinstance(x, MxRows)

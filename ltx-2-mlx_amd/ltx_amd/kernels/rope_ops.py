@@ -1,4 +1,5 @@
-"""QK-RMSNorm + split RoPE (in place) and the RoPE table layout.
+"""QK-RMSNorm + split RoPE (in place), the RoPE table layout, and rotary
+positions without a norm (:func:`rotary`).
 
 Replaces the ``q_norm``/``k_norm`` + ``apply_rotary_emb`` sequence of
 ``Attention.__call__`` (model/transformer/attention.py:578-584) with one HIP
@@ -8,6 +9,9 @@ they are built (rope.py:274-283).
 """
 
 from __future__ import annotations
+
+import ctypes
+import math
 
 import torch
 
@@ -78,3 +82,112 @@ def tables_from_reference_layout(cos: torch.Tensor, sin: torch.Tensor) -> tuple[
     def tm(a):
         return a[0].permute(1, 0, 2).reshape(t, h * half).float().contiguous()
     return tm(cos), tm(sin)
+
+
+ROTARY_LAYOUTS = ("half", "interleaved")
+ROTARY_SCALINGS = ("none", "linear", "ntk", "yarn")
+_ROTARY_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_POSITION_DTYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
+
+
+def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, *, scaling: str = "none", stretch: float = 1.0,
+                       original_length: int = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                       device="cuda") -> tuple[torch.Tensor, float]:
+    """What :func:`rotary` takes as ``inv_freq`` and ``factor``: the angle per
+    position of every channel pair, theta^(-2i/rotary_dim), fp64 on ``device``,
+    and the factor on the rotated values.
+
+    ``scaling`` adapts them to sequences ``stretch`` times ``original_length``:
+    "linear" divides every frequency by it; "ntk" raises theta so that the
+    slowest one is; "yarn" divides the pairs with fewer than ``beta_slow``
+    turns over the original length, keeps those with more than ``beta_fast``,
+    blends linearly between, and gives the factor 0.1 ln(stretch) + 1.
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if scaling not in ROTARY_SCALINGS:
+        raise ValueError(f"scaling must be one of {ROTARY_SCALINGS}, got {scaling!r}")
+    if not (theta > 1.0 and stretch >= 1.0 and original_length > 0):
+        raise ValueError(f"theta > 1, stretch >= 1 and original_length > 0 wanted, got {theta}, {stretch}, "
+                         f"{original_length}")
+    d = rotary_dim
+    if scaling == "ntk" and d > 2:
+        theta = theta * stretch ** (d / (d - 2))
+    inv = theta ** (-torch.arange(0, d, 2, dtype=torch.float64) / d)
+    factor = 1.0
+    if scaling == "linear":
+        inv = inv / stretch
+    elif scaling == "yarn" and stretch > 1.0:
+        def pair(turns: float) -> float:  # the (fractional) pair with this many turns over the original length
+            return d * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+        lo, hi = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), d - 1)
+        ramp = ((torch.arange(d // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        inv = inv * (1 - ramp) + inv / stretch * ramp
+        factor = 0.1 * math.log(stretch) + 1.0
+    return inv.to(device), factor
+
+
+def _rotary_side(name: str, x: torch.Tensor, out: torch.Tensor | None) -> tuple[_lib.RotaryRows, torch.Tensor]:
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        raise ValueError(f"{name} must have unit channel stride")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or (out.stride(-1) != 1 and x.shape[-1] > 1):
+        raise ValueError(f"{name}'s out must be {x.dtype} {tuple(x.shape)} of unit channel stride")
+    def strides(t):
+        st = t.stride()
+        return (st[0] if t.dim() == 4 else 0, st[-3], st[-2])
+    return _lib.RotaryRows(x.data_ptr(), *strides(x), out.data_ptr(), *strides(out), x.shape[-2]), out
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *,
+           layout: str = "half", factor: float = 1.0, transpose: bool = False,
+           out: tuple[torch.Tensor, torch.Tensor | None] | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotary positions of queries and keys, one launch: returns (q', k').
+
+    q: (T, H, dh) or (B, T, H, dh) bf16, fp16 or fp32, any strides but the
+    channels'; k likewise with its own number of heads, or None.  The first
+    2 * len(inv_freq) channels of a head rotate, the others are copied:
+    channels (i, i + d/2) in the "half" layout, (2i, 2i+1) "interleaved" -- the
+    reference's split and interleaved forms (model/transformer/rope.py:16-89)
+    -- by the angle positions * inv_freq[i], scaled by ``factor``
+    (:func:`rotary_frequencies`).  positions: (T) for every sequence of the
+    batch, or (B, T); int32, int64, fp32 or fp64.  ``transpose`` rotates back
+    (times ``factor`` again): with the outputs' gradients for q and k it gives
+    the inputs' gradients.  ``out`` may be (q, k) itself (in place).
+    """
+    if layout not in ROTARY_LAYOUTS:
+        raise ValueError(f"layout must be one of {ROTARY_LAYOUTS}, got {layout!r}")
+    if q.dim() not in (3, 4) or q.dtype not in _ROTARY_DTYPES:
+        raise ValueError(f"q must be (T, H, dh) or (B, T, H, dh) in bf16, fp16 or fp32, got {q.dtype} "
+                         f"{tuple(q.shape)}")
+    if k is not None and (k.dim() != q.dim() or k.dtype != q.dtype or k.shape[:-2] != q.shape[:-2]
+                          or k.shape[-1] != q.shape[-1]):
+        raise ValueError(f"k {k.dtype} {tuple(k.shape)} does not go with q {q.dtype} {tuple(q.shape)}")
+    batch, tokens = (q.shape[0], q.shape[1]) if q.dim() == 4 else (1, q.shape[0])
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous fp64 vector (rotary_frequencies)")
+    d = 2 * inv_freq.numel()
+    if not 2 <= d <= q.shape[-1]:
+        raise ValueError(f"{d} rotary channels do not fit heads of {q.shape[-1]}")
+    if positions.dtype not in _POSITION_DTYPES or positions.shape not in ((tokens,), (batch, tokens)):
+        raise ValueError(f"positions must be int32, int64, fp32 or fp64 ({tokens},) or ({batch}, {tokens}), got "
+                         f"{positions.dtype} {tuple(positions.shape)}")
+    if positions.stride(-1) != 1 and tokens > 1:
+        positions = positions.contiguous()
+    oq, ok = out if out is not None else (None, None)
+    if k is None and ok is not None:
+        raise ValueError("out has a tensor for k, but there is no k")
+    sq, oq = _rotary_side("q", q, oq)
+    sk, ok = _rotary_side("k", k, ok) if k is not None else (None, None)
+    _lib.same_device(q, k, positions, inv_freq, oq, ok)
+    if batch * tokens == 0:
+        return oq, ok
+    flags = (_lib.ROTARY_INTERLEAVED if layout == "interleaved" else 0) | (_lib.ROTARY_TRANSPOSE if transpose else 0)
+    _lib.call_on(q, "ltx_rotary", ctypes.addressof(sq), None if sk is None else ctypes.addressof(sk),
+                 _ROTARY_DTYPES[q.dtype], batch, tokens, q.shape[-1], d, positions.data_ptr(),
+                 _POSITION_DTYPES[positions.dtype], positions.stride(0) if positions.dim() == 2 else 0,
+                 inv_freq.data_ptr(), float(factor), flags, _lib.stream_of(q),
+                 detail=f"{q.dtype} B={batch} T={tokens} dh={q.shape[-1]} rotary={d}")
+    return oq, ok

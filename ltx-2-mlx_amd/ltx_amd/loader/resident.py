@@ -33,7 +33,7 @@ Resident formats: MXFP8 cache weights stay MXFP8 (bytes copied); plain and
 pretransposed weights load as bf16; MXFP8 caches quantised along N
 (``mxfp8-blocks-pretranspose``) are decoded exactly to bf16, because the
 GEMMs read scales blocked along K.  ``weight_format`` forces a resident
-format ("bf16", "int8" or "mxfp8", quantised on the device).  A projection
+format ("bf16", "int8", "mxfp8" or "mxfp4", quantised on the device).  A projection
 that the reference runs as a quantised linear keeps that arithmetic
 (``LinearWeight.qlinear``: bias added after the bf16 product), also when
 decoded to bf16.
@@ -561,7 +561,7 @@ def _run_linear(job: _LinearJob, src: WeightSource, weight_format: str | None, d
         target = "mxfp8" if all(r.fmt == "mxfp8" for r in parts) else "bf16"
     qlinear = target == "mxfp8" or (target == "bf16" and quantized)
     cur = getattr(job.owner, job.attr)
-    reuse = cur is not None and cur.kind == target and tuple(cur.w.shape) == (n_total, k)
+    reuse = cur is not None and cur.kind == target and (cur.out_features, cur.in_features) == (n_total, k)
     if target == "bf16":
         w = cur.w if reuse else torch.empty((n_total, k), dtype=torch.bfloat16, device=device)
         scale = None
@@ -571,6 +571,10 @@ def _run_linear(job: _LinearJob, src: WeightSource, weight_format: str | None, d
     elif target == "int8":
         w = cur.w if reuse else torch.empty((n_total, k), dtype=torch.int8, device=device)
         scale = cur.scale if reuse else torch.empty((n_total,), dtype=torch.float32, device=device)
+    elif target == "mxfp4":
+        w = cur.w if reuse else torch.empty((n_total, k // 2), dtype=torch.uint8, device=device)
+        scale = cur.scale if reuse else torch.empty(((k + 127) // 128, (n_total + 3) // 4 * 4), dtype=torch.int32,
+                                                    device=device)
     else:
         raise ValueError(f"unknown resident weight format {target!r}")
     bias = cur.bias if reuse and cur.bias is not None else torch.empty((n_total,), dtype=torch.float32,
@@ -590,6 +594,10 @@ def _run_linear(job: _LinearJob, src: WeightSource, weight_format: str | None, d
             elif target == "mxfp8":
                 _lib.call("ltx_quantize_mxfp8_bf16", _lib.ptr(vals), k, n, k, _lib.ptr(w[rows]), k,
                           _lib.ptr(scale[rows]), k // 32, _lib.stream_of(vals), detail=rec.base)
+            elif target == "mxfp4":
+                part = gemm.quantize_rows_mxfp4(vals)
+                w[rows].copy_(part.codes)
+                scale[:, rows].copy_(part.scales[:, :n])
             else:
                 _lib.call("ltx_quantize_w8_bf16", _lib.ptr(vals), k, n, k, _lib.ptr(w[rows]), k,
                           _lib.ptr(scale[rows]), _lib.stream_of(vals), detail=rec.base)

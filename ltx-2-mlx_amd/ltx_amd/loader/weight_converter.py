@@ -55,7 +55,7 @@ def load_transformer_weights(model, weights_path: str | Path, include_audio: boo
 
     ``include_audio`` defaults to whether the model has the audio stream.
     ``weight_format`` picks the resident format of the block projections
-    (``None``/"bf16" as stored, "mxfp8" or "int8" quantised on the device).
+    (``None``/"bf16" as stored, "mxfp8", "mxfp4" or "int8" quantised on the device).
     """
     from .resident import CheckpointSource, install_weights
 

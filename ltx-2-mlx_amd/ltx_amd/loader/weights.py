@@ -45,6 +45,10 @@ def linear_weight(n: int, k: int, *, gen, device, weight_format: str, bias: bool
         if weight_format == "mxfp8":
             return gemm.LinearWeight("mxfp8", torch.empty((n, k), dtype=torch.uint8, device=device),
                                      torch.empty((n, k // 32), dtype=torch.uint8, device=device), b, qlinear=True)
+        if weight_format == "mxfp4":
+            return gemm.LinearWeight("mxfp4", torch.empty((n, k // 2), dtype=torch.uint8, device=device),
+                                     torch.empty(((k + 127) // 128, (n + 3) // 4 * 4), dtype=torch.int32,
+                                                 device=device), b)
         raise ValueError(f"unknown weight format {weight_format!r}")
     if init != "random":
         raise ValueError(f"init must be 'random' or 'empty', got {init!r}")

@@ -149,3 +149,56 @@ def linear(x, W, b=None, *, epilogue: str = "bias", residual=None, gate=None, ex
     if epilogue == "residual_round":
         return bf16r(r + bf16r(g * y).astype(np.float64))
     raise ValueError(epilogue)
+
+
+# ---- MXFP4 (OCP MX v1.0, E2M1 elements, blocks of 32, E8M0 scales) ---------------
+# No counterpart in the reference; the OCP rule restated, in float64.
+
+E2M1_VALUES = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+
+
+def e2m1_encode(v) -> np.ndarray:
+    """Nearest E2M1 code (ties to the even code), saturating at +-6, the sign
+    kept on zeros: nearest by distance over the eight magnitudes."""
+    v = np.asarray(v, np.float64)
+    a = np.minimum(np.abs(v), 6.0)
+    d = np.abs(a[..., None] - E2M1_VALUES)
+    code = d.argmin(-1)
+    up = np.minimum(code + 1, 7)
+    tie = np.take_along_axis(d, up[..., None], -1)[..., 0] == d.min(-1)
+    code = np.where(tie & (up > code) & (code % 2 == 1), up, code)
+    return (code | np.where(np.signbit(v), 8, 0)).astype(np.uint8)
+
+
+def mxfp4_quantize(x) -> tuple[np.ndarray, np.ndarray]:
+    """(N, K) -> E2M1 codes (N, K), one per byte, and E8M0 scales (N, K/32)."""
+    x = np.asarray(x, np.float64)
+    n, k = x.shape
+    blocks = x.reshape(n, k // 32, 32)
+    bad = ~np.isfinite(blocks).all(-1)
+    blocks = np.where(bad[..., None], 0.0, blocks)
+    amax = np.abs(blocks).max(-1)
+    _, e = np.frexp(amax)
+    X = np.clip(np.where(amax > 0, e - 1 - 2, -127), -127, 127)
+    codes = e2m1_encode(np.ldexp(blocks, -X[..., None]))
+    codes = np.where(bad[..., None], 0, codes).astype(np.uint8)
+    return codes.reshape(n, k), np.where(bad, 255, X + 127).astype(np.uint8)
+
+
+def mxfp4_dequantize(codes, scales) -> np.ndarray:
+    """float64 values of codes (N, K) with E8M0 scales (N, K/32); 255 is NaN."""
+    codes, scales = np.asarray(codes), np.asarray(scales)
+    v = E2M1_VALUES[codes & 7] * np.where(codes & 8, -1.0, 1.0)
+    s = np.where(scales == 255, np.nan, np.ldexp(1.0, scales.astype(np.int64) - 127))
+    return (v.reshape(*scales.shape, 32) * s[..., None]).reshape(codes.shape)
+
+
+def mxfp4_pack(codes, scales) -> tuple[np.ndarray, np.ndarray]:
+    """Stored form: code bytes (N, K/2), the even k low, and scale words
+    (ceil(K/128), N rounded up to 4) int32, the first block in the low byte."""
+    codes, scales = np.asarray(codes), np.asarray(scales)
+    n, b = scales.shape
+    words = np.zeros(((b + 3) // 4, (n + 3) // 4 * 4), np.uint32)
+    for i in range(b):
+        words[i // 4, :n] |= scales[:, i].astype(np.uint32) << (8 * (i % 4))
+    return (codes[:, ::2] | codes[:, 1::2] << 4).astype(np.uint8), words.view(np.int32)
