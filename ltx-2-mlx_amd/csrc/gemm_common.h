@@ -13,7 +13,8 @@ namespace ltx {
 // B_MX: MXFP8 weights and MXFP8 activations (E4M3 codes + E8M0 scale per 32
 // along K on both operands), multiplied by the scaled fp8 MFMA -- an opt-in
 // path with quantised activations, only on the 8-wave kernel.
-enum BKind { B_BF16 = 0, B_INT8 = 1, B_MXFP8 = 2, B_MX = 3 };
+// B_MXFP4: MXFP4 weights (two E2M1 codes per byte, scale words: gemm_fp4.h).
+enum BKind { B_BF16 = 0, B_INT8 = 1, B_MXFP8 = 2, B_MX = 3, B_MXFP4 = 4 };
 
 // workgroups are dealt to the 8 XCDs round-robin (block b runs on XCD b % 8)
 constexpr int kNumXcd = 8;
@@ -65,6 +66,17 @@ __device__ __forceinline__ float e8m0_to_f32_valu(uint32_t s) {
   return x + (x - x);
 }
 
+
+// eight E2M1 codes of one word and one block -> bf16, exact (E2M1 has one
+// mantissa bit; 2^X from the scale)
+__device__ __forceinline__ bf16x8 fp4x8_bf16(uint32_t w, float s) {
+  uint32_t o[4];
+  o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
+  o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
+  o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
+  o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
+  return __builtin_bit_cast(bf16x8, u32x4{o[0], o[1], o[2], o[3]});
+}
 
 // LDS-DMA helpers: each lane of a wave writes the 16 bytes it loads to
 // `lds_wave_base + 16 * lane`; the per-lane source address implements the
@@ -119,7 +131,7 @@ struct GemmArgs {
   const void* B;
   int64_t ldb;
   const void* bscale;  // int8: fp32 (N); mxfp8: uint8 (N, K/32)
-  int64_t ld_scale;    // mxfp8 scale row stride (bytes)
+  int64_t ld_scale;    // mxfp8 scale row stride (bytes); mxfp4: word row stride (words)
   const float* bias;   // fp32 (N) or null
   bf16* C;
   int64_t ldc;

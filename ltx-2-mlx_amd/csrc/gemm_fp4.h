@@ -15,17 +15,6 @@
 
 namespace ltx {
 
-// eight codes of one word and one block -> bf16, exact (E2M1 has one mantissa
-// bit; 2^X from the scale)
-__device__ __forceinline__ bf16x8 fp4x8_bf16(uint32_t w, float s) {
-  uint32_t o[4];
-  o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
-  o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
-  o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
-  o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
-  return __builtin_bit_cast(bf16x8, u32x4{o[0], o[1], o[2], o[3]});
-}
-
 // Four consecutive columns n .. n + 3 of output row m from their fp32 sums.
 // MXFP4 products reproduce no reference arithmetic, so GELU and the head gate
 // act on the fp32 value, without the other formats' bf16 rounding before them.

@@ -4,6 +4,7 @@
 //
 // Operand storage: gemm_fp4.h.  The weights are decoded to bf16 (exact) in
 // registers and multiplied on v_mfma_f32_16x16x32_bf16, fp32 accumulation.
+#include "gemm8.h"
 #include "gemm_fp4.h"
 
 namespace ltx {
@@ -103,6 +104,91 @@ __global__ __launch_bounds__(kFrThreads) void fp4_rows_kernel(GemmArgs p, int k_
   }
 }
 
+// ---- one to 16 rows ----------------------------------------------------------
+// Bound by latency and the weight bytes: one launch, no workspace, a wave's
+// loads of up to 512 k issued before their first use.  A workgroup computes 16
+// columns; its waves split K, each streaming its range of the codes (and the
+// activations, which the L2 holds) straight to registers, and meet once
+// through LDS, in wave order.  Weights from HBM: 1 x 4096 -> 4096 6.0 us (10.8 in 8
+// K ranges and a combining launch of the few-row tiles, 11.2 in 4 of the
+// mid-size kernel; a launch that does next to nothing takes 4.0), 1 x 4096 ->
+// 16384 13.8, 16 x 4096 -> 4096 8.2.  Holding the next 512 k in flight as well cost
+// more in occupancy than it gave (1 x 4096 -> 16384 16.9); 16 waves are no faster.
+constexpr int kSkWaves = 8;
+
+template <int EPI>
+__global__ __launch_bounds__(kSkWaves * 64) void fp4_skinny_kernel(GemmArgs p) {
+  __shared__ __attribute__((aligned(16))) f32x4 part[kSkWaves][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, q = lane >> 4;
+  const int n0 = (int)blockIdx.x * 16;
+  int gn = n0 + r16;  // columns past N re-read the last one, rows past M the last row
+  gn = gn < p.N ? gn : p.N - 1;
+  const uint8_t* wrow = (const uint8_t*)p.B + (int64_t)gn * p.ldb + q * 16;
+  const uint32_t* srow = (const uint32_t*)p.bscale + gn;
+  const bf16* xrow = p.A + (int64_t)(r16 < p.M ? r16 : p.M - 1) * p.lda + q * 32;
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+
+  // U units of 128 k from unit u on.  HALF: only the first 64 k of one exist; the
+  // upper quarters take the lower ones' codes, with scale 1, and zeros for x
+  auto run = [&](int u, auto uc, auto hc) __attribute__((always_inline)) {
+    constexpr int U = decltype(uc)::value;
+    constexpr bool HALF = decltype(hc)::value;
+    const bool out = HALF && q >= 2;
+    const int back = out ? 64 : 0;  // in k
+    u32x4 w[U];
+    uint32_t sc[U];
+#pragma unroll
+    for (int b = 0; b < U; ++b) {
+      w[b] = *reinterpret_cast<const u32x4*>(wrow + (u + b) * 64 - back / 2);
+      sc[b] = srow[(int64_t)(u + b) * p.ld_scale];
+    }
+    bf16x8 x[U][4];
+#pragma unroll
+    for (int b = 0; b < U; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[b][j] = *reinterpret_cast<const bf16x8*>(xrow + (u + b) * 128 - back + j * 8);
+        if (out) x[b][j] = bf16x8{};
+      }
+#pragma unroll
+    for (int b = 0; b < U; ++b) {
+      const float s = out ? 1.0f : e8m0_to_f32_valu((sc[b] >> (8 * q)) & 0xffu);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4x8_bf16(w[b][j], s), x[b][j], acc, 0, 0, 0);
+    }
+  };
+  const int units = p.K >> 7;
+  int u = units * wave / kSkWaves;
+  const int end = units * (wave + 1) / kSkWaves;
+  constexpr std::integral_constant<int, 4> c4;
+  constexpr std::integral_constant<int, 2> c2;
+  constexpr std::integral_constant<int, 1> c1;
+  constexpr std::false_type whole;
+  for (; u + 4 <= end; u += 4) run(u, c4, whole);
+  if (u + 2 <= end) {
+    run(u, c2, whole);
+    u += 2;
+  }
+  if (u < end) run(u, c1, whole);
+  if ((p.K & 64) && wave == kSkWaves - 1) run(units, c1, std::true_type{});
+
+  part[wave][lane] = acc;
+  __syncthreads();
+  if (tid >= 64) return;
+  const int n = n0 + 4 * q;  // N % 8 == 0: four columns inside or outside
+  f32x4 a = part[0][lane];
+#pragma unroll
+  for (int z = 1; z < kSkWaves; ++z) {
+    const f32x4 b = part[z][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] += b[e];
+  }
+  if (r16 < p.M && n < p.N) fp4_store4<EPI>(p, a, r16, n);
+}
+
 // sum of the partial products in split order, then the epilogue
 template <int EPI>
 __global__ __launch_bounds__(256) void fp4_combine_kernel(GemmArgs p, int splits) {
@@ -129,37 +215,126 @@ int fp4_combine(const GemmArgs& p, int epi, int splits, hipStream_t s) {
   return ltx_launch_status();
 }
 
-// How a product runs: rows per tile and K ranges.
+// ---- which kernel ------------------------------------------------------------
+// kFp4Skinny, kFp4Rows: above.  kFp4Mid: the mid-size kernel (gemm_kg.hip), tiles
+// of 64, 128 or 192 x 128, whole units of 128 k.  kFp4Large: the 8-wave kernel
+// (gemm8.h), 256 or 128 x 256.
+enum Fp4Kernel { kFp4Skinny, kFp4Rows, kFp4Mid, kFp4Large };
 struct Fp4Plan {
-  int mb;       // 16-row blocks of a tile
+  int kernel;
+  int bm;       // rows of a tile
   int splits;   // K ranges
   int k_split;  // k of one (a multiple of 128)
 };
 
+// Modelled times (us).  Mid-size: a round of one workgroup per CU costs `unit` us
+// per 128 k, the L2s deliver 13 TB/s of tile operands at most, 4 us of launch,
+// first loads and epilogue, a split's second launch and its partials.  Against
+// measured: 1296 x 4096 -> 4096 tiles of 192 / 128 / 64 rows 39 / 53 / 57 against
+// 40 / 56 / 56, 68 x 2048 -> 8192 64 rows 13 / 12, 68 x 8192 -> 2048 in 8 splits 64
+// rows 14 / 16, 256 x 4096 -> 8192 22 / 21, 1296 x 4096 -> 12320 192 rows 108 / 112.
+static double fp4_mid_time(double M, double N, double K, int bm, int splits) {
+  const double unit = bm == 64 ? 0.55 : (bm == 128 ? 0.77 : 1.08);
+  const double wgs = ceil(M / bm) * ceil(N / 128) * splits, units = K / 128 / splits;
+  double t = ceil(wgs / 256) * units * unit;
+  const double bytes = wgs * units * 128 * (2.0 * bm + 64);
+  if (bytes / 13e6 > t) t = bytes / 13e6;
+  t += 4.0;
+  if (splits > 1) t += 3.5 + M * N * splits * 8 / 3.5e6;
+  return t;
+}
+// 8-wave: a round of 256-row tiles 2.3 us per 128 k, of 128-row tiles 1.5 (3456 x
+// 4096 -> 4096 in one round 79; 3456 x 16384 -> 4096 287; 1296 x 4096 -> 4096 in
+// 128-row tiles 50).
+static double fp4_large_time(double M, double N, double K, int bm) {
+  const double units = ceil(K / 128);
+  if (bm == 128) return 4.0 + ceil(ceil(M / 128) * ceil(N / 256) / 256) * units * 1.5;
+  const int r0 = g8_split_rows((int)M, (int)N);
+  double t = ceil(ceil(r0 / 256.0) * ceil(N / 256) / 256) * 2.3;
+  if (r0 < M) t += ceil(ceil((M - r0) / 128) * ceil(N / 256) / 256) * 1.5;
+  return 4.0 + t * units;
+}
+
 static Fp4Plan fp4_plan(int64_t M, int64_t N, int64_t K) {
-  Fp4Plan pl;
-  pl.mb = M <= 16 ? 1 : (M <= 32 ? 2 : 4);
-  const int64_t tiles = ((M + pl.mb * 16 - 1) / (pl.mb * 16)) * ((N + kFrBN - 1) / kFrBN);
-  const int64_t units = (K + 127) / 128;
-  int64_t s = 512 / tiles;
-  if (s > units / 4) s = units / 4;
-  if (s > 32) s = 32;
-  if (s < 1) s = 1;
-  const int64_t per = (units + s - 1) / s;
-  pl.k_split = (int)(per * 128);
-  pl.splits = (int)((units + per - 1) / per);
+  Fp4Plan pl = {kFp4Skinny, 16, 1, (int)((K + 127) / 128 * 128)};
+  // beyond that many activations (each workgroup reads all of them) splitting
+  // K over workgroups is faster: 16 x 16384 -> 4096 25 us, 18 on the mid-size
+  // kernel; 1 x 16384 -> 4096 13.7 against 16.6
+  if (M <= 16 && (M * K <= 131072 || K % 128 != 0)) return pl;
+  if (K % 128 != 0 && M <= 64) {
+    pl.kernel = kFp4Rows;
+    pl.bm = M <= 32 ? 32 : 64;
+    const int64_t tiles = (N + kFrBN - 1) / kFrBN, units = (K + 127) / 128;
+    int64_t s = 512 / tiles;  // two workgroups per CU, ranges of at least 512 k
+    s = s > units / 4 ? units / 4 : s;
+    s = s > 32 ? 32 : (s < 1 ? 1 : s);
+    const int64_t per = (units + s - 1) / s;
+    pl.k_split = (int)(per * 128);
+    pl.splits = (int)((units + per - 1) / per);
+    return pl;
+  }
+  pl.kernel = kFp4Large;
+  pl.bm = 128;
+  double best = fp4_large_time(M, N, K, 128);
+  const double t256 = fp4_large_time(M, N, K, 256);
+  if (t256 < best) {
+    best = t256;
+    pl.bm = 256;
+  }
+  if (K % 128 == 0) {
+    const int64_t units = K / 128;
+    for (int bm = 64; bm <= 192; bm += 64) {
+      const int64_t tiles = ((M + bm - 1) / bm) * ((N + 127) / 128);
+      for (int s = 1; s <= 16; ++s) {
+        // splits: whole units, at least 256 k each, within one round of the CUs,
+        // and 10 % faster (a launch and a workspace more)
+        if (s > 1 && (units % s || units / s < 2 || tiles * s > 256)) continue;
+        const double t = fp4_mid_time(M, N, K, bm, s);
+        if (t < best * (s > 1 ? 0.9 : 1.0)) {
+          best = t;
+          pl = {kFp4Mid, bm, s, (int)(K / s)};
+        }
+      }
+    }
+  }
   return pl;
 }
 
 template <int EPI>
-static void fp4_launch_rows(const GemmArgs& p, const Fp4Plan& pl, hipStream_t s) {
+static void fp4_launch_rows(const GemmArgs& p, int bm, int splits, int k_split, hipStream_t s) {
   GemmArgs a = p;
-  a.tiles_m = (p.M + pl.mb * 16 - 1) / (pl.mb * 16);
+  a.tiles_m = (p.M + bm - 1) / bm;
   a.tiles_n = (p.N + kFrBN - 1) / kFrBN;
-  const int blocks = a.tiles_m * a.tiles_n * pl.splits;
-  if (pl.mb == 1) fp4_rows_kernel<1, EPI><<<blocks, kFrThreads, 0, s>>>(a, pl.k_split);
-  else if (pl.mb == 2) fp4_rows_kernel<2, EPI><<<blocks, kFrThreads, 0, s>>>(a, pl.k_split);
-  else fp4_rows_kernel<4, EPI><<<blocks, kFrThreads, 0, s>>>(a, pl.k_split);
+  const int blocks = a.tiles_m * a.tiles_n * splits;
+  if (bm == 32) fp4_rows_kernel<2, EPI><<<blocks, kFrThreads, 0, s>>>(a, k_split);
+  else fp4_rows_kernel<4, EPI><<<blocks, kFrThreads, 0, s>>>(a, k_split);
+}
+
+// one launch of the plan's kernel (EPI kEpiPartial: its K ranges)
+template <int EPI>
+static void fp4_launch(const GemmArgs& p, const Fp4Plan& pl, hipStream_t s) {
+  if (pl.kernel == kFp4Rows) {
+    fp4_launch_rows<EPI>(p, pl.bm, pl.splits, pl.k_split, s);
+  } else if (pl.kernel == kFp4Mid) {
+    GemmArgs a = p;
+    if (EPI == kEpiPartial) {
+      a.K = pl.k_split;
+      a.ldc = p.N;
+    }
+    kg_launch(B_MXFP4, a, EPI, pl.bm, pl.splits, s);
+  } else if constexpr (EPI != kEpiPartial) {
+    if (pl.kernel == kFp4Skinny) {
+      fp4_skinny_kernel<EPI><<<(p.N + 15) / 16, kSkWaves * 64, 0, s>>>(p);
+      return;
+    }
+    const int r0 = pl.bm == 256 ? g8_split_rows(p.M, p.N) : 0;
+    if (r0 > 0) {
+      GemmArgs top = p;
+      top.M = r0;
+      launch_g8<B_MXFP4, EPI>(top, s);
+    }
+    if (r0 < p.M) launch_g8<B_MXFP4, EPI, 128>(rows_from(p, r0), s);
+  }
 }
 
 }  // namespace ltx
@@ -183,7 +358,7 @@ extern "C" int ltx_gemm_mxfp4_bf16(const void* A, int64_t lda, const uint8_t* Wq
   if (st != LTX_OK) return st;
   if (M == 0 || N == 0) return LTX_OK;
   if (K == 0) return LTX_ERR_UNSUPPORTED;
-  const Fp4Plan pl = fp4_plan(M, N, K);
+  Fp4Plan pl = fp4_plan(M, N, K);
   const int64_t need = pl.splits > 1 ? (int64_t)pl.splits * M * N * 4 : 0;
   if (need > 0 && (!workspace || workspace_bytes < need)) return LTX_ERR_INVALID_ARG;
   if (need > 0 && ((uintptr_t)workspace & 15u)) return LTX_ERR_ALIGNMENT;
@@ -191,12 +366,33 @@ extern "C" int ltx_gemm_mxfp4_bf16(const void* A, int64_t lda, const uint8_t* Wq
                         sigmoid_from);
   hipStream_t s = (hipStream_t)stream;
   const int epi = epilogue & 0xff;
+  // The mid-size and 8-wave kernels address their operands by 31-bit byte
+  // offsets: longer activations go in pieces of whole tiles, and what does not
+  // fit them otherwise (a weight of 2 GiB) to the few-row tiles.
+  int64_t piece = M;
+  if (pl.kernel == kFp4Mid || pl.kernel == kFp4Large) {
+    const int64_t lim = (int64_t)1 << 31;
+    const bool w_fits = N <= (lim - 1) / ldw && ld_scale <= (lim - 1) / 4 / ((K + 127) / 128);
+    const int64_t rows = (lim - 1) / (lda * 2) / 768 * 768;  // tiles of 64, 128, 192, 256 rows
+    if (w_fits && (M <= (lim - 1) / (lda * 2) || (rows > 0 && pl.splits == 1))) {
+      if (M > (lim - 1) / (lda * 2)) piece = rows;
+    } else {
+      pl.kernel = kFp4Rows;
+      pl.bm = 64;
+    }
+  }
   if (pl.splits > 1) {
     p.partial = workspace;
-    fp4_launch_rows<kEpiPartial>(p, pl, s);
+    fp4_launch<kEpiPartial>(p, pl, s);
     const int e = ltx_launch_status();
     return e != LTX_OK ? e : fp4_combine(p, epi, pl.splits, s);
   }
-  fp4_epilogue(epi, [&](auto e) { fp4_launch_rows<decltype(e)::value>(p, pl, s); });
-  return ltx_launch_status();
+  for (int64_t r0 = 0; r0 < M; r0 += piece) {
+    GemmArgs part = rows_from(p, r0);
+    part.M = (int)(M - r0 < piece ? M - r0 : piece);
+    fp4_epilogue(epi, [&](auto e) { fp4_launch<decltype(e)::value>(part, pl, s); });
+    const int e = ltx_launch_status();
+    if (e != LTX_OK) return e;
+  }
+  return LTX_OK;
 }

@@ -40,16 +40,19 @@ constexpr int kKgThreads = 512;
 
 template <int BKIND, int BM_>
 struct KgCfg {
-  static constexpr bool BF = BKIND == B_BF16, MXS = BKIND == B_MXFP8;
+  static constexpr bool BF = BKIND == B_BF16, MXS = BKIND == B_MXFP8, FP4 = BKIND == B_MXFP4;
+  static constexpr bool SCALED = MXS || FP4;  // E8M0 scales, loaded for four units at a time
   static constexpr int BM = BM_, BN = 128;
   static constexpr int KU = BF ? 32 : 64;            // k per group and unit
-  static constexpr int ES = BF ? 2 : 1;              // weight bytes per element
+  static constexpr int EH = BF ? 4 : (FP4 ? 1 : 2);  // weight half-bytes per element
   static constexpr int KS = KU / 32;                 // MFMA k-steps per group and unit
   static constexpr int WM = BM / 2, WN = 64;         // wave tile
   static constexpr int AM = WM / 16, AN = WN / 16;   // its 16x16 accumulator blocks
   static constexpr int HM = AM / 2;                  // row blocks kept per group after the exchange
-  static constexpr int A_ROWB = 128, B_ROWB = 128;   // LDS row bytes
-  static constexpr int A_BYTES = BM * 2 * KU, B_BYTES = BN * KU * ES;  // one group's stage
+  // LDS row bytes.  MXFP4: both groups' halves of a unit are 64 bytes (half the
+  // bytes in as many requests as the 8-bit codes)
+  static constexpr int A_ROWB = 128, B_ROWB = FP4 ? 64 : 128;
+  static constexpr int A_BYTES = BM * 2 * KU, B_BYTES = BN * KU * EH / 2;  // one group's stage
   // ring depths in units.  192-row tiles of 8-bit weights: three whole units
   // exceed the LDS, so the activations (mostly L2 hits) run one unit ahead
   // and the weights (HBM) two.
@@ -61,14 +64,14 @@ struct KgCfg {
   // unit u + 1, the scale load of a unit with h == 0 among them
   static constexpr int in_flight(int h) {
     int n = (RA - 2) * (A_DMA + B_DMA) + (RB > RA ? B_DMA : 0);
-    if (MXS)
+    if (SCALED)
       for (int t = 1; t <= RA - 2; ++t) n += (h - t + 8) % 4 == 0 ? 1 : 0;
     return n;
   }
   static constexpr int B_OFF = RA * 2 * A_BYTES;
   // E8M0 bytes of four units, [row][16], double buffered
   static constexpr int SC_OFF = B_OFF + RB * 2 * B_BYTES;
-  static constexpr int RING = SC_OFF + (MXS ? 2 * BN * 16 : 0);
+  static constexpr int RING = SC_OFF + (SCALED ? 2 * BN * 16 : 0);
   // after the loop: the exchanged accumulator halves, the bf16 output tile,
   // the column values
   static constexpr int X_WAVE = HM * AN * 64 * 16, X_BYTES = 8 * X_WAVE;
@@ -77,10 +80,10 @@ struct KgCfg {
   static constexpr int EPI = COL_OFF + 2 * BN * 4;
   static constexpr int LDS_BYTES = RING > EPI ? RING : EPI;
   static_assert(AM % 2 == 0 && AN == 4, "accumulator row blocks split between the groups");
-  static_assert((2 * A_BYTES) % 8192 == 0 && B_BYTES == 8192, "whole direct-load instructions per wave");
+  static_assert((2 * A_BYTES) % 8192 == 0 && (2 * B_BYTES) % 8192 == 0, "whole direct-load instructions per wave");
   static_assert(RB == RA || RB == RA + 1, "ring depths");
   static_assert(in_flight(0) < 60, "vmcnt range");
-  static_assert(!MXS || RA <= 4, "a scale load lands within the four units before its use");
+  static_assert(!SCALED || RA <= 4, "a scale load lands within the four units before its use");
   static_assert(LDS_BYTES <= 160 * 1024, "LDS");
 };
 
@@ -94,10 +97,10 @@ __device__ __forceinline__ void kg_dma4(const void* base, int num_records, uint3
 template <int BKIND, int EPI, int BM_>
 __global__ __launch_bounds__(kKgThreads, 1) void gemm_kg_kernel(GemmArgs p) {
   using Cfg = KgCfg<BKIND, BM_>;
-  constexpr bool BF = Cfg::BF, MXS = Cfg::MXS;
+  constexpr bool BF = Cfg::BF, MXS = Cfg::MXS, FP4 = Cfg::FP4, SCALED = Cfg::SCALED;
   constexpr int BM = Cfg::BM, BN = Cfg::BN, WM = Cfg::WM, WN = Cfg::WN, AM = Cfg::AM, AN = Cfg::AN, HM = Cfg::HM;
   constexpr int A_ROWB = Cfg::A_ROWB, B_ROWB = Cfg::B_ROWB, A_BYTES = Cfg::A_BYTES, B_BYTES = Cfg::B_BYTES;
-  constexpr int A_DMA = Cfg::A_DMA, B_DMA = Cfg::B_DMA, RA = Cfg::RA, RB = Cfg::RB, ES = Cfg::ES;
+  constexpr int A_DMA = Cfg::A_DMA, B_DMA = Cfg::B_DMA, RA = Cfg::RA, RB = Cfg::RB, EH = Cfg::EH;
   constexpr bool RESID = EPI == LTX_GEMM_EPI_RESIDUAL || EPI == LTX_GEMM_EPI_RESIDUAL_ROUND;
   constexpr bool PARTIAL = EPI == kEpiPartial;
   __shared__ __attribute__((aligned(1024))) char lds[Cfg::LDS_BYTES];
@@ -130,7 +133,7 @@ __global__ __launch_bounds__(kKgThreads, 1) void gemm_kg_kernel(GemmArgs p) {
   // re-read the last row.  The record counts bound the lane offsets to their
   // operand; the scalar offset, which they do not cover, stays inside the row
   // because past the last unit that one is loaded again.
-  const int a_records = (int)((int64_t)p.M * p.lda * 2), b_records = (int)((int64_t)p.N * p.ldb * ES);
+  const int a_records = (int)((int64_t)p.M * p.lda * 2), b_records = (int)((int64_t)p.N * p.ldb * (BF ? 2 : 1));
   uint32_t a_src[A_DMA];
 #pragma unroll
   for (int d = 0; d < A_DMA; ++d) {
@@ -144,23 +147,37 @@ __global__ __launch_bounds__(kKgThreads, 1) void gemm_kg_kernel(GemmArgs p) {
   uint32_t b_src[B_DMA];
 #pragma unroll
   for (int d = 0; d < B_DMA; ++d) {
-    const int r = 8 * (8 * d + wave) + (lane >> 3);
+    // MXFP4: rows of 64 bytes, 16 per instruction, chunks XORed by (row / 4) % 4:
+    // a fragment read's 16 rows x 8 bytes lie in 16 different pieces of 256 bytes
+    const int r = FP4 ? 16 * (8 * d + wave) + (lane >> 2) : 8 * (8 * d + wave) + (lane >> 3);
     int gn = n0 + r;
     gn = gn < p.N ? gn : p.N - 1;
-    b_src[d] = (uint32_t)(((int64_t)gn * p.ldb + k0) * ES) + pair_chunk(lane) * 16;
+    if constexpr (FP4) b_src[d] = (uint32_t)((int64_t)gn * p.ldb + k0 / 2) + ((lane & 3) ^ ((r >> 2) & 3)) * 16;
+    else b_src[d] = (uint32_t)(((int64_t)gn * p.ldb + k0) * (EH / 2)) + pair_chunk(lane) * 16;
   }
   // MXFP8 scales, four units at a time: 16 bytes per weight row, a dword per
   // lane of 16 rows per wave (a dword per unit of 64 rows per wave would
   // touch 64 cache lines per instruction, as much address work as the whole
   // unit's data: 28.5 against ~20 us on 256 x 4096 -> 8192)
   uint32_t sc_src = 0;
-  const int sc_records = MXS ? (int)((int64_t)p.N * p.ld_scale) : 0;
+  const int sc_records = MXS ? (int)((int64_t)p.N * p.ld_scale)
+                             : (FP4 ? (int)((k0 + p.K) / 128 * p.ld_scale * 4) : 0);
+  if constexpr (FP4) {  // wave w: the words of unit 4 o + w / 2, rows 64 (w % 2) on
+    int gn = n0 + 64 * (wave & 1) + lane;
+    gn = gn < p.N ? gn : p.N - 1;
+    sc_src = (uint32_t)((k0 / 128 * p.ld_scale + gn) * 4);
+  }
   if constexpr (MXS) {
     int gn = n0 + 16 * wave + (lane >> 2);
     gn = gn < p.N ? gn : p.N - 1;
     sc_src = (uint32_t)((int64_t)gn * p.ld_scale + k0 / 32) + (lane & 3) * 4;
   }
   auto load_scales = [&](int o) __attribute__((always_inline)) {  // of units 4 o .. 4 o + 3
+    if constexpr (FP4) {
+      const int u = clamp_unit(4 * o + (wave >> 1), KT);
+      kg_dma4(p.bscale, sc_records, sc_src + (uint32_t)((int64_t)u * p.ld_scale * 4), 0,
+              lds + Cfg::SC_OFF + (o & 1) * BN * 16 + wave * 256);
+    }
     if constexpr (MXS)
       kg_dma4(p.bscale, sc_records, sc_src, (4 * o < KT ? o : KT / 4 - 1) * 16,
               lds + Cfg::SC_OFF + (o & 1) * BN * 16 + wave * 256);
@@ -174,7 +191,7 @@ __global__ __launch_bounds__(kKgThreads, 1) void gemm_kg_kernel(GemmArgs p) {
       buffer_dma16(p.A, a_records, a_src[l < A_DMA ? l : 0], ua * 4 * Cfg::KU,
                    lds + sa * 2 * A_BYTES + (8 * l + wave) * 1024);
     else
-      buffer_dma16(p.B, b_records, b_src[l >= A_DMA ? l - A_DMA : 0], ub * 2 * Cfg::KU * ES,
+      buffer_dma16(p.B, b_records, b_src[l >= A_DMA ? l - A_DMA : 0], ub * Cfg::KU * EH,
                    lds + Cfg::B_OFF + sb * 2 * B_BYTES + (8 * (l - A_DMA) + wave) * 1024);
   };
 
@@ -188,8 +205,9 @@ __global__ __launch_bounds__(kKgThreads, 1) void gemm_kg_kernel(GemmArgs p) {
   for (int s = 0; s < Cfg::KS; ++s)
     a_rd[s] = (wm * WM + r16) * A_ROWB + (BF ? ((4 * grp + q) ^ swz_pair(r16)) * 16
                                              : grp * A_BYTES + ((2 * q + s) ^ g8_swz128(r16, true)) * 16);
-  const int w_rd = Cfg::B_OFF + (wn * WN + r16) * B_ROWB + ((4 * grp + q) ^ swz_pair(r16)) * 16;
-  const int s_rd = Cfg::SC_OFF + (wn * WN + r16) * 16 + 2 * grp + (q >> 1);  // the lane's k-block of 32
+  const int w_rd = Cfg::B_OFF + (wn * WN + r16) * B_ROWB +
+                   (FP4 ? ((2 * grp + (q >> 1)) ^ (r16 >> 2)) * 16 + (q & 1) * 8 : ((4 * grp + q) ^ swz_pair(r16)) * 16);
+  const int s_rd = Cfg::SC_OFF + (wn * WN + r16) * (FP4 ? 4 : 16) + 2 * grp + (q >> 1);  // the lane's k-block of 32
 
   float s_i8[AN];
 #pragma unroll
@@ -217,12 +235,22 @@ __global__ __launch_bounds__(kKgThreads, 1) void gemm_kg_kernel(GemmArgs p) {
   auto read_w = [&](u32x4 (&w)[AN], uint32_t (&sc)[AN], int u, int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < AN; ++j) {
+      if constexpr (FP4) {  // 16 codes: words 0 and 1
+        const u32x2 c = *reinterpret_cast<const u32x2*>(lds + w_rd + slot * 2 * B_BYTES + j * 16 * B_ROWB);
+        w[j][0] = c[0];
+        w[j][1] = c[1];
+        sc[j] = *reinterpret_cast<const uint8_t*>(lds + s_rd + ((u >> 2) & 1) * BN * 16 + (u & 3) * BN * 4 + j * 64);
+        continue;
+      }
       w[j] = *reinterpret_cast<const u32x4*>(lds + w_rd + slot * 2 * B_BYTES + j * 16 * B_ROWB);
       if constexpr (MXS)
         sc[j] = *reinterpret_cast<const uint8_t*>(lds + s_rd + ((u >> 2) & 1) * BN * 16 + (u & 3) * 4 + j * 256);
     }
   };
-  auto dequant = [&](uint32_t w0, uint32_t w1, float sc) __attribute__((always_inline)) -> bf16x8 {
+  // k-step s of a weight fragment's codes
+  auto dequant = [&](u32x4 w, int s, float sc) __attribute__((always_inline)) -> bf16x8 {
+    if constexpr (FP4) return fp4x8_bf16(w[s], sc);
+    const uint32_t w0 = w[2 * s], w1 = w[2 * s + 1];
     uint32_t o[4];
     if constexpr (MXS) {
       o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, sc, false));
@@ -282,7 +310,7 @@ __global__ __launch_bounds__(kKgThreads, 1) void gemm_kg_kernel(GemmArgs p) {
     wait_lgkmcnt0();
     wait_vmcnt<Cfg::in_flight(h)>();
     barrier_nofence();
-    if (MXS && h == 0) load_scales((u >> 2) + 1);
+    if (SCALED && h == 0) load_scales((u >> 2) + 1);
   };
   auto next_slots = [&]() __attribute__((always_inline)) {
     sa = sa + 1 < RA ? sa + 1 : 0;
@@ -339,12 +367,12 @@ __global__ __launch_bounds__(kKgThreads, 1) void gemm_kg_kernel(GemmArgs p) {
     float sf[AN];
     auto scales = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < AN; ++j) sf[j] = MXS ? e8m0_to_f32_valu(sc[j]) : s_i8[j];
+      for (int j = 0; j < AN; ++j) sf[j] = SCALED ? e8m0_to_f32_valu(sc[j]) : s_i8[j];
     };
     read_a(x[0], 0, 0, I0{}, IA{});
     read_w(w[0], sc, 0, 0);
     scales();
-    wf[0] = dequant(w[0][0][0], w[0][0][1], sf[0]);
+    wf[0] = dequant(w[0][0], 0, sf[0]);
     auto unit = [&](int u, auto hc) __attribute__((always_inline)) {
       constexpr int h = decltype(hc)::value & 1;
       int fa = 0, fb = 0;
@@ -367,10 +395,10 @@ __global__ __launch_bounds__(kKgThreads, 1) void gemm_kg_kernel(GemmArgs p) {
         }
         if (f + 1 < 2 * AN) {
           const int s = (f + 1) / AN, j = (f + 1) % AN;
-          wf[(f + 1) & 1] = dequant(w[h][j][2 * s], w[h][j][2 * s + 1], sf[j]);
+          wf[(f + 1) & 1] = dequant(w[h][j], s, sf[j]);
         } else {
           scales();
-          wf[0] = dequant(w[1 - h][0][0], w[1 - h][0][1], sf[0]);
+          wf[0] = dequant(w[1 - h][0], 0, sf[0]);
         }
         multiply(x[f / AN], wf[f & 1], f % AN);
         __builtin_amdgcn_sched_barrier(0);
@@ -465,8 +493,10 @@ __global__ __launch_bounds__(kKgThreads, 1) void gemm_kg_kernel(GemmArgs p) {
           for (int e = 0; e < 4; ++e) y[e] += bias4[e];
           if (EPI == LTX_GEMM_EPI_GELU || EPI == LTX_GEMM_EPI_SIGMOID2 || SIG) {
             float r[4] = {y[0], y[1], y[2], y[3]};
-            round_bf2(r[0], r[1]);
-            round_bf2(r[2], r[3]);
+            if constexpr (!FP4) {  // MXFP4 reproduces no reference rounding here
+              round_bf2(r[0], r[1]);
+              round_bf2(r[2], r[3]);
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               if (EPI == LTX_GEMM_EPI_GELU) y[e] = gelu_tanh(r[e]);
@@ -564,6 +594,7 @@ bool kg_launch(int bkind, const GemmArgs& p, int epi, int bm, int splits, hipStr
   if (bkind == B_BF16) return kg_launch_kind<B_BF16>(p, epi, bm, splits, s);
   if (bkind == B_INT8) return kg_launch_kind<B_INT8>(p, epi, bm, splits, s);
   if (bkind == B_MXFP8) return kg_launch_kind<B_MXFP8>(p, epi, bm, splits, s);
+  if (bkind == B_MXFP4) return kg_launch_kind<B_MXFP4>(p, epi, bm, splits, s);
   return false;
 }
 

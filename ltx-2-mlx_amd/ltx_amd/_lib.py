@@ -189,21 +189,23 @@ def call(name: str, *args, detail: str = "") -> None:
         raise LtxKernelError(name, status, detail)
 
 
-def call_on(t: torch.Tensor, name: str, *args, detail: str = "") -> None:
-    """:func:`call` with t's device current (a launch goes to the current device)."""
-    if t.get_device() == torch._C._cuda_getDevice():
-        call(name, *args, detail=detail)
-    else:
-        with torch.cuda.device(t.device):
-            call(name, *args, detail=detail)
+def launch(device: int, name: str, *args) -> int:
+    """Status of an entry point, called with ``device`` current (a launch goes
+    to the current device) and that device's current stream as last argument."""
+    fn = getattr(_LIB or lib(), name)
+    if device == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    with torch.cuda.device(device):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(device))
 
 
-def same_device(*tensors: torch.Tensor | None) -> None:
-    """Raise unless every given tensor is on the first one's GPU."""
-    first = tensors[0]
+def same_device(*tensors: torch.Tensor | None) -> int:
+    """The GPU index of the given tensors; raises unless all are on one GPU."""
+    device = tensors[0].get_device()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device != first.device):
-            raise ValueError(f"expected device tensors on one GPU, got {first.device} and {t.device}")
+        if t is not None and (t.get_device() != device or device < 0):
+            raise ValueError(f"expected device tensors on one GPU, got {tensors[0].device} and {t.device}")
+    return device
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

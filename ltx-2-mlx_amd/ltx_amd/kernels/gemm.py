@@ -416,16 +416,20 @@ class Mx4Rows:
         return torch.Size((self.codes.shape[0], self.codes.shape[1] * 2))
 
 
-def _check_mxfp4(what: str, codes: torch.Tensor, scales: torch.Tensor) -> tuple[int, int]:
-    """(rows, K) of MXFP4 codes whose scale words fit them."""
-    if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.stride(1) != 1:
-        raise ValueError(f"{what}: MXFP4 codes are (rows, K/2) uint8 of unit column stride")
-    rows, k = codes.shape[0], codes.shape[1] * 2
-    if (scales is None or scales.dtype != torch.int32 or scales.dim() != 2 or scales.stride(1) != 1
-            or scales.shape[0] < (k + 127) // 128 or scales.shape[1] < rows):
-        raise ValueError(f"{what}: MXFP4 scales of {rows} x {k} values are int32 words ({(k + 127) // 128}, "
-                         f">= {rows}) of unit column stride")
-    return rows, k
+def _check_mxfp4(what: str, codes: torch.Tensor, scales: torch.Tensor) -> tuple[int, int, int, int]:
+    """(rows, K, code row stride, word row stride) of MXFP4 codes whose scale
+    words fit them."""
+    if codes.dtype is torch.uint8 and codes.dim() == 2 and scales is not None and scales.dtype is torch.int32 \
+            and scales.dim() == 2:
+        rows, half = codes.shape
+        words, ld = scales.shape
+        ldc, unit = codes.stride()
+        lds, sunit = scales.stride()
+        if words * 64 >= half and ld >= rows and unit == sunit == 1:
+            return rows, half * 2, ldc, lds
+    raise ValueError(f"{what}: MXFP4 operands are code bytes (rows, K/2) uint8 and scale words (ceil(K/128), >= rows) "
+                     f"int32 of unit column stride, got {codes.dtype} {tuple(codes.shape)} and "
+                     f"{None if scales is None else (scales.dtype, tuple(scales.shape))}")
 
 
 def mxfp4_scale_words(scales: torch.Tensor) -> torch.Tensor:
@@ -453,7 +457,8 @@ def quantize_rows_mxfp4(x: torch.Tensor) -> Mx4Rows:
     the OCP rule: X = floor(log2 max|v|) - 2, E2M1 to nearest even, saturated).
     A block with a NaN or an infinity decodes to NaN."""
     k = x.shape[-1]
-    if x.dtype not in _QUANT_DTYPES:
+    dtype = _QUANT_DTYPES.get(x.dtype)
+    if dtype is None:
         raise TypeError(f"quantize_rows_mxfp4 takes bf16, fp16 or fp32 rows, got {x.dtype}")
     if k % 32:
         raise ValueError(f"K={k} is not a multiple of 32")
@@ -463,25 +468,24 @@ def quantize_rows_mxfp4(x: torch.Tensor) -> Mx4Rows:
     codes = torch.empty((m, k // 2), dtype=torch.uint8, device=x.device)
     scales = torch.empty(((k + 127) // 128, ld), dtype=torch.int32, device=x.device)
     if m and k:
-        _lib.call_on(x, "ltx_quantize_mxfp4", _lib.ptr(xv), _QUANT_DTYPES[x.dtype], ldx, m, k, codes.data_ptr(),
-                     k // 2, scales.data_ptr(), ld, _lib.stream_of(x), detail=f"{x.dtype} rows M={m} K={k} ld={ldx}")
+        st = _lib.launch(_lib.same_device(xv), "ltx_quantize_mxfp4", xv.data_ptr(), dtype, ldx, m, k,
+                         codes.data_ptr(), k // 2, scales.data_ptr(), ld)
+        if st:
+            raise _lib.LtxKernelError("ltx_quantize_mxfp4", st, f"{x.dtype} rows M={m} K={k} ld={ldx}")
     return Mx4Rows(codes, scales)
 
 
 def dequantize_rows_mxfp4(rows: Mx4Rows) -> torch.Tensor:
     """bf16 (M, K) values of MXFP4 rows, exact."""
-    m, k = _check_mxfp4("dequantize_rows_mxfp4", rows.codes, rows.scales)
-    _lib.same_device(rows.codes, rows.scales)
-    out = torch.empty((m, k), dtype=torch.bfloat16, device=rows.codes.device)
+    codes, scales = rows.codes, rows.scales
+    m, k, ldq, lds = _check_mxfp4("dequantize_rows_mxfp4", codes, scales)
+    out = torch.empty((m, k), dtype=torch.bfloat16, device=codes.device)
     if m and k:
-        _lib.call_on(out, "ltx_dequantize_mxfp4_bf16", rows.codes.data_ptr(), rows.codes.stride(0),
-                     rows.scales.data_ptr(), rows.scales.stride(0), m, k, out.data_ptr(), k, _lib.stream_of(out),
-                     detail=f"M={m} K={k}")
+        st = _lib.launch(_lib.same_device(codes, scales), "ltx_dequantize_mxfp4_bf16", codes.data_ptr(), ldq,
+                         scales.data_ptr(), lds, m, k, out.data_ptr(), k)
+        if st:
+            raise _lib.LtxKernelError("ltx_dequantize_mxfp4_bf16", st, f"M={m} K={k}")
     return out
-
-
-def _workspace(nbytes: int, like: torch.Tensor) -> torch.Tensor | None:
-    return torch.empty(nbytes // 4, dtype=torch.float32, device=like.device) if nbytes else None
 
 
 @functools.lru_cache(maxsize=4096)
@@ -492,69 +496,74 @@ def _mxfp4_workspace_bytes(name: str, m: int, n: int, k: int) -> int:
 def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int, out: torch.Tensor | None,
                   residual: torch.Tensor | None, gate: torch.Tensor | None,
                   sigmoid_from: int | None) -> torch.Tensor:
-    """:func:`linear` on MXFP4 weights, for bf16 or MXFP4 rows."""
-    n, k = _check_mxfp4("weight", weight.w, weight.scale)
+    """:func:`linear` on MXFP4 weights, for bf16 or MXFP4 rows.  (Small products
+    are bound by the host: this path reads each tensor's properties once.)"""
+    w, scale, bias = weight.w, weight.scale, weight.bias
+    n, k, ldw, ldws = _check_mxfp4("weight", w, scale)
     quantised = isinstance(x, Mx4Rows)
     if quantised:
-        m, kx = _check_mxfp4("activations", x.codes, x.scales)
-        src, lda, lead = x.codes, x.codes.stride(0), (m,)
+        src, xs = x.codes, x.scales
+        m, kx, lda, ldas = _check_mxfp4("activations", src, xs)
+        shape = (m, n)
     else:
-        if x.dtype != torch.bfloat16:
+        if x.dtype is not torch.bfloat16:
             raise TypeError(f"linear expects bf16 or MXFP4 activations, got {x.dtype}")
-        kx = x.shape[-1]
+        *lead, kx = x.shape
         src, lda = _lib.row_view(x, kx)
-        m, lead = x.numel() // kx if kx else 0, x.shape[:-1]
+        xs, shape = None, (*lead, n)
+        m = x.numel() // kx if kx else 0
     if kx != k:
         raise ValueError(f"activations have K={kx}, the weight {k}")
     if out is None:
-        out = torch.empty((*lead, n), dtype=torch.bfloat16, device=src.device)
-    elif out.dtype != torch.bfloat16 or out.shape != (*lead, n):
-        raise ValueError(f"out must be bf16 {(*lead, n)}, got {out.dtype} {tuple(out.shape)}")
-    ov, ldc = _lib.row_view(out, n)
-    if ov.data_ptr() != out.data_ptr():
-        raise ValueError("out must be a row-strided view")
+        out = src.new_empty(shape) if not quantised else torch.empty(shape, dtype=torch.bfloat16, device=src.device)
+        ldc = n
+    else:
+        if out.dtype is not torch.bfloat16 or out.shape != shape:
+            raise ValueError(f"out must be bf16 {shape}, got {out.dtype} {tuple(out.shape)}")
+        ov, ldc = _lib.row_view(out, n)
+        if ov.data_ptr() != out.data_ptr():
+            raise ValueError("out must be a row-strided view")
     rptr, ldr, gptr = None, 0, None
-    if epilogue in (EPI_RESIDUAL, EPI_RESIDUAL_ROUND):
+    if epilogue == EPI_RESIDUAL or epilogue == EPI_RESIDUAL_ROUND:
         if residual is None or gate is None:
             raise ValueError("residual epilogues need residual and gate")
-        if residual.dtype != torch.bfloat16 or residual.shape[-1] != n or residual.numel() != m * n:
+        if residual.dtype is not torch.bfloat16 or residual.shape[-1] != n or residual.numel() != m * n:
             raise ValueError(f"residual must be bf16 ({m}, {n}), got {residual.dtype} {tuple(residual.shape)}")
         rv, ldr = _lib.row_view(residual, n)
-        if rv.data_ptr() != residual.data_ptr():
-            raise ValueError("residual must be a row-strided view")
         rptr = rv.data_ptr()
-        if gate.dtype != torch.float32 or gate.numel() != n:
+        if rptr != residual.data_ptr():
+            raise ValueError("residual must be a row-strided view")
+        if gate.dtype is not torch.float32 or gate.numel() != n:
             raise ValueError("gate must be fp32 with N elements")
         gate = _lib.flat(gate)
         gptr = gate.data_ptr()
     else:
         residual = gate = None
-    bias = weight.bias
-    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != n or not bias.is_contiguous()):
-        raise ValueError(f"bias must be {n} contiguous fp32 values")
-    _lib.same_device(src, x.scales if quantised else None, weight.w, weight.scale, bias, out, residual, gate)
-    flags = epilogue
-    if weight.qlinear and bias is not None:
-        flags |= _lib.GEMM_ROUND_THEN_BIAS
+    flags, bptr = epilogue, None
+    if bias is not None:
+        if bias.dtype is not torch.float32 or bias.numel() != n or not bias.is_contiguous():
+            raise ValueError(f"bias must be {n} contiguous fp32 values")
+        bptr = bias.data_ptr()
+        if weight.qlinear:
+            flags |= _lib.GEMM_ROUND_THEN_BIAS
+    device = _lib.same_device(src, xs, w, scale, bias, out, residual, gate)
     if m == 0:
         return out
-    ws_bytes = _mxfp4_workspace_bytes(
-        "ltx_gemm_mx4_workspace_bytes" if quantised else "ltx_gemm_mxfp4_workspace_bytes", m, n, k)
-    ws = _workspace(ws_bytes, src)
-    tail = (weight.w.data_ptr(), weight.w.stride(0), weight.scale.data_ptr(), weight.scale.stride(0),
-            None if bias is None else bias.data_ptr(), ov.data_ptr(), ldc, m, n, k, flags, rptr, ldr, gptr,
-            n if sigmoid_from is None else int(sigmoid_from), None if ws is None else ws.data_ptr(), ws_bytes,
-            _lib.stream_of(src))
-    detail = f"mxfp4 {'x mxfp4' if quantised else 'x bf16'} M={m} N={n} K={k} epi={epilogue}"
+    name = "ltx_gemm_mx4_bf16" if quantised else "ltx_gemm_mxfp4_bf16"
+    ws_bytes = _mxfp4_workspace_bytes("ltx_gemm_mx4_workspace_bytes" if quantised
+                                      else "ltx_gemm_mxfp4_workspace_bytes", m, n, k)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=src.device) if ws_bytes else None
     hook = LAUNCH_HOOK
     info = (weight.kind, m, n, k, epilogue)
     if hook is not None:
         hook("pre", info)
-    if quantised:
-        _lib.call_on(src, "ltx_gemm_mx4_bf16", src.data_ptr(), lda, x.scales.data_ptr(), x.scales.stride(0), *tail,
-                     detail=detail)
-    else:
-        _lib.call_on(src, "ltx_gemm_mxfp4_bf16", src.data_ptr(), lda, *tail, detail=detail)
+    a_scale = (xs.data_ptr(), ldas) if quantised else ()
+    st = _lib.launch(device, name, src.data_ptr(), lda, *a_scale, w.data_ptr(), ldw, scale.data_ptr(), ldws, bptr,
+                     out.data_ptr(), ldc, m, n, k, flags, rptr, ldr, gptr,
+                     n if sigmoid_from is None else int(sigmoid_from), None if ws is None else ws.data_ptr(),
+                     ws_bytes)
+    if st:
+        raise _lib.LtxKernelError(name, st, f"M={m} N={n} K={k} epi={epilogue} lda={lda} ldw={ldw} ldc={ldc}")
     if hook is not None:
         hook("post", info)
     return out

@@ -10,8 +10,8 @@ they are built (rope.py:274-283).
 
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 
 import torch
 
@@ -128,17 +128,23 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, *, scaling: str 
     return inv.to(device), factor
 
 
-def _rotary_side(name: str, x: torch.Tensor, out: torch.Tensor | None) -> tuple[_lib.RotaryRows, torch.Tensor]:
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
-        raise ValueError(f"{name} must have unit channel stride")
+_ROTARY_ROWS = struct.Struct("9q").pack  # ltx_rotary_rows: x, its strides, out, its strides, heads
+
+
+def _rotary_side(name: str, x: torch.Tensor, out: torch.Tensor | None) -> tuple[bytes, torch.Tensor]:
+    shape, st = x.shape, x.stride()
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or (out.stride(-1) != 1 and x.shape[-1] > 1):
-        raise ValueError(f"{name}'s out must be {x.dtype} {tuple(x.shape)} of unit channel stride")
-    def strides(t):
-        st = t.stride()
-        return (st[0] if t.dim() == 4 else 0, st[-3], st[-2])
-    return _lib.RotaryRows(x.data_ptr(), *strides(x), out.data_ptr(), *strides(out), x.shape[-2]), out
+        out = x.new_empty(shape)
+    elif out.shape != shape or out.dtype is not x.dtype:
+        raise ValueError(f"{name}'s out must be {x.dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
+    so = out.stride()
+    if (st[-1] != 1 or so[-1] != 1) and shape[-1] > 1:
+        raise ValueError(f"{name} and its out must have unit channel stride")
+    if len(st) == 3:
+        rows = _ROTARY_ROWS(x.data_ptr(), 0, st[0], st[1], out.data_ptr(), 0, so[0], so[1], shape[1])
+    else:
+        rows = _ROTARY_ROWS(x.data_ptr(), st[0], st[1], st[2], out.data_ptr(), so[0], so[1], so[2], shape[2])
+    return rows, out
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *,
@@ -159,35 +165,39 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     """
     if layout not in ROTARY_LAYOUTS:
         raise ValueError(f"layout must be one of {ROTARY_LAYOUTS}, got {layout!r}")
-    if q.dim() not in (3, 4) or q.dtype not in _ROTARY_DTYPES:
+    shape = q.shape
+    dtype = _ROTARY_DTYPES.get(q.dtype)
+    if dtype is None or not 3 <= len(shape) <= 4:
         raise ValueError(f"q must be (T, H, dh) or (B, T, H, dh) in bf16, fp16 or fp32, got {q.dtype} "
-                         f"{tuple(q.shape)}")
-    if k is not None and (k.dim() != q.dim() or k.dtype != q.dtype or k.shape[:-2] != q.shape[:-2]
-                          or k.shape[-1] != q.shape[-1]):
-        raise ValueError(f"k {k.dtype} {tuple(k.shape)} does not go with q {q.dtype} {tuple(q.shape)}")
-    batch, tokens = (q.shape[0], q.shape[1]) if q.dim() == 4 else (1, q.shape[0])
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+                         f"{tuple(shape)}")
+    *lead, _, dh = shape
+    if k is not None:
+        *lead_k, _, dk = k.shape
+        if k.dtype is not q.dtype or lead_k != lead or dk != dh:
+            raise ValueError(f"k {k.dtype} {tuple(k.shape)} does not go with q {q.dtype} {tuple(shape)}")
+    batch, tokens = lead if len(lead) == 2 else (1, lead[0])
+    if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous fp64 vector (rotary_frequencies)")
     d = 2 * inv_freq.numel()
-    if not 2 <= d <= q.shape[-1]:
-        raise ValueError(f"{d} rotary channels do not fit heads of {q.shape[-1]}")
-    if positions.dtype not in _POSITION_DTYPES or positions.shape not in ((tokens,), (batch, tokens)):
+    if not 2 <= d <= dh:
+        raise ValueError(f"{d} rotary channels do not fit heads of {dh}")
+    pos_type, pos_shape = _POSITION_DTYPES.get(positions.dtype), positions.shape
+    if pos_type is None or (pos_shape != (tokens,) and pos_shape != (batch, tokens)):
         raise ValueError(f"positions must be int32, int64, fp32 or fp64 ({tokens},) or ({batch}, {tokens}), got "
-                         f"{positions.dtype} {tuple(positions.shape)}")
-    if positions.stride(-1) != 1 and tokens > 1:
+                         f"{positions.dtype} {tuple(pos_shape)}")
+    if not positions.is_contiguous():
         positions = positions.contiguous()
     oq, ok = out if out is not None else (None, None)
     if k is None and ok is not None:
         raise ValueError("out has a tensor for k, but there is no k")
     sq, oq = _rotary_side("q", q, oq)
     sk, ok = _rotary_side("k", k, ok) if k is not None else (None, None)
-    _lib.same_device(q, k, positions, inv_freq, oq, ok)
+    device = _lib.same_device(q, k, positions, inv_freq, oq, ok)
     if batch * tokens == 0:
         return oq, ok
     flags = (_lib.ROTARY_INTERLEAVED if layout == "interleaved" else 0) | (_lib.ROTARY_TRANSPOSE if transpose else 0)
-    _lib.call_on(q, "ltx_rotary", ctypes.addressof(sq), None if sk is None else ctypes.addressof(sk),
-                 _ROTARY_DTYPES[q.dtype], batch, tokens, q.shape[-1], d, positions.data_ptr(),
-                 _POSITION_DTYPES[positions.dtype], positions.stride(0) if positions.dim() == 2 else 0,
-                 inv_freq.data_ptr(), float(factor), flags, _lib.stream_of(q),
-                 detail=f"{q.dtype} B={batch} T={tokens} dh={q.shape[-1]} rotary={d}")
+    st = _lib.launch(device, "ltx_rotary", sq, sk, dtype, batch, tokens, dh, d, positions.data_ptr(), pos_type,
+                     tokens if len(pos_shape) == 2 else 0, inv_freq.data_ptr(), factor, flags)
+    if st:
+        raise _lib.LtxKernelError("ltx_rotary", st, f"{q.dtype} B={batch} T={tokens} dh={dh} rotary={d}")
     return oq, ok

@@ -160,6 +160,21 @@ def test_strided_operands_and_what_lies_beside_them(m, k, n, quantised):
     assert torch.equal(inplace, got)
 
 
+@pytest.mark.parametrize("rows,stride,k,n", [(2100, 1 << 19, 256, 264), (150, 1 << 23, 512, 136), (40, 1 << 25, 320, 72)])
+def test_activations_past_two_gib(rows, stride, k, n):
+    """Rows so far apart that byte offsets pass 31 and 32 bits: the product goes
+    in pieces of rows, or to the kernel with 64-bit addresses."""
+    from ltx_amd.kernels import gemm
+
+    buf = torch.empty(rows, stride, dtype=torch.bfloat16, device=DEV)
+    x = buf[:, :k]
+    g = torch.Generator(device=DEV).manual_seed(8)
+    x.copy_(torch.randn(rows, k, generator=g, device=DEV))
+    wc, ws, w = _codes_words(n, k, seed=2)
+    got = gemm.linear(x, gemm.LinearWeight("mxfp4", wc, ws))
+    _check(got, *_reference(x.double(), w, None, "bias", None, None, None, False))
+
+
 @pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "mx"])
 @pytest.mark.parametrize("m,n", [(1, 64), (90, 200), (2000, 4096)])
 def test_non_finite_rows_and_columns_stay_theirs(m, n, quantised):
