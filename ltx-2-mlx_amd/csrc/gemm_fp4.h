@@ -20,16 +20,22 @@ namespace ltx {
 // act on the fp32 value, without the other formats' bf16 rounding before them.
 // A residual epilogue keeps that rounding of the branch (its tiles are staged
 // as bf16 rows).
-template <int EPI>
+// SIG: columns from sig_from on may be among these; RTB: round_then_bias.
+template <int EPI, bool SIG, bool RTB>
 __device__ __forceinline__ bf16x4 fp4_branch4(const GemmArgs& p, f32x4 a, f32x4 bias, int n) {
   bf16x4 v;
+  float y[4] = {a[0], a[1], a[2], a[3]};
+  if (RTB) {
+    round_bf2(y[0], y[1]);
+    round_bf2(y[2], y[3]);
+  }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    float y = (p.round_then_bias ? round_bf(a[e]) : a[e]) + bias[e];
-    if (EPI == LTX_GEMM_EPI_GELU) y = gelu_tanh(y);
-    if (EPI == LTX_GEMM_EPI_SIGMOID2) y = sigmoid2_bf(y);
-    if (EPI == LTX_GEMM_EPI_BIAS && n + e >= p.sig_from) y = sigmoid2_bf(y);
-    v[e] = (bf16)y;
+    y[e] += bias[e];
+    if (EPI == LTX_GEMM_EPI_GELU) y[e] = gelu_tanh(y[e]);
+    if (EPI == LTX_GEMM_EPI_SIGMOID2) y[e] = sigmoid2_bf(y[e]);
+    if (SIG) y[e] = n + e >= p.sig_from ? sigmoid2_bf(y[e]) : y[e];
+    v[e] = (bf16)y[e];
   }
   return v;
 }
@@ -43,7 +49,8 @@ __device__ __forceinline__ void fp4_store4(const GemmArgs& p, f32x4 a, int m, in
   if (p.bias)
 #pragma unroll
     for (int e = 0; e < 4; ++e) bias[e] = p.bias[n + e];
-  bf16x4 v = fp4_branch4<EPI>(p, a, bias, n);
+  constexpr bool SIG = EPI == LTX_GEMM_EPI_BIAS;
+  bf16x4 v = p.round_then_bias ? fp4_branch4<EPI, SIG, true>(p, a, bias, n) : fp4_branch4<EPI, SIG, false>(p, a, bias, n);
   if constexpr (EPI == LTX_GEMM_EPI_RESIDUAL || EPI == LTX_GEMM_EPI_RESIDUAL_ROUND) {
     const bf16x4 r = *reinterpret_cast<const bf16x4*>(p.R + (int64_t)m * p.ldr + n);
 #pragma unroll

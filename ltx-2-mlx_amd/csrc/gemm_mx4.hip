@@ -17,41 +17,40 @@
 
 namespace ltx {
 
-constexpr int kM4Threads = 256;
-
-template <int BM_, int BN_>
-struct M4Cfg {
-  static constexpr int BM = BM_, BN = BN_, WM = BM / 2, WN = BN / 2, AM = WM / 16, AN = WN / 16;
+template <int BM_, int BN_, int WAVES_M_, int WAVES_N_, int NST_>
+struct M4Tile {
+  static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, NST = NST_;
+  static constexpr int WAVES = WAVES_M * WAVES_N, THREADS = WAVES * 64;
+  static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, AM = WM / 16, AN = WN / 16;
   static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128;
   // two scale words per row; at least one direct-load instruction (1 KiB)
   static constexpr int SA_BYTES = BM * 8 < 1024 ? 1024 : BM * 8, SB_BYTES = BN * 8 < 1024 ? 1024 : BN * 8;
   static constexpr int B_OFF = A_BYTES, SA_OFF = B_OFF + B_BYTES, SB_OFF = SA_OFF + SA_BYTES;
   static constexpr int STAGE = SB_OFF + SB_BYTES;
-  static constexpr int NST = BM * BN >= 256 * 256 ? 2 : 3;
   // direct loads of a wave per stage: code rows, and a share of the scales'
-  static constexpr int A_DMA = BM / 32, B_DMA = BN / 32;
+  static constexpr int A_DMA = BM / 8 / WAVES, B_DMA = BN / 8 / WAVES;
   static constexpr int SA_DMA = SA_BYTES / 1024, SB_DMA = SB_BYTES / 1024;
-  // scale instructions go to the waves in turn: S_DMA per wave, the same count
-  // for each (a wave without one of its own repeats one)
-  static constexpr int S_DMA = (SA_DMA + SB_DMA + 3) / 4;
+  // scale instructions go to the waves in turn, the same count for each (a
+  // wave without one of its own repeats one)
+  static constexpr int S_DMA = (SA_DMA + SB_DMA + WAVES - 1) / WAVES;
   static constexpr int DMA = A_DMA + B_DMA + S_DMA;
   static constexpr int EPI_ROWB = WN * 2, EPI_WAVE = WM * EPI_ROWB;
-  static constexpr int RING = NST * STAGE, EPI = 4 * EPI_WAVE;
+  static constexpr int RING = NST * STAGE, EPI = WAVES * EPI_WAVE;
   static constexpr int LDS_BYTES = RING > EPI ? RING : EPI;
+  static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole direct-load instructions per wave");
   static_assert(LDS_BYTES <= 160 * 1024 && (NST - 1) * DMA < 60, "LDS, vmcnt range");
 };
 
-template <int BM_, int BN_, int EPI>
-__global__ __launch_bounds__(kM4Threads, 1) void gemm_mx4_kernel(GemmArgs p, int k_split) {
-  using Cfg = M4Cfg<BM_, BN_>;
+template <class Cfg, int EPI>
+__global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, int k_split) {
   constexpr int BM = Cfg::BM, BN = Cfg::BN, WM = Cfg::WM, WN = Cfg::WN, AM = Cfg::AM, AN = Cfg::AN;
-  constexpr int NST = Cfg::NST, A_DMA = Cfg::A_DMA, B_DMA = Cfg::B_DMA;
+  constexpr int NST = Cfg::NST, A_DMA = Cfg::A_DMA, B_DMA = Cfg::B_DMA, WAVES = Cfg::WAVES;
   constexpr bool RESID = EPI == LTX_GEMM_EPI_RESIDUAL || EPI == LTX_GEMM_EPI_RESIDUAL_ROUND;
   __shared__ __attribute__((aligned(1024))) char lds[Cfg::LDS_BYTES];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave & 1, wn = wave >> 1;
+  const int wm = wave % Cfg::WAVES_M, wn = wave / Cfg::WAVES_M;
   const int r16 = lane & 15, q = lane >> 4;
   const int tiles = p.tiles_m * p.tiles_n;
   const int kz = EPI == kEpiPartial ? (int)blockIdx.x / tiles : 0;
@@ -75,70 +74,84 @@ __global__ __launch_bounds__(kM4Threads, 1) void gemm_mx4_kernel(GemmArgs p, int
   uint32_t a_src[A_DMA], b_src[B_DMA];
 #pragma unroll
   for (int d = 0; d < A_DMA; ++d) {
-    int gm = m0 + 8 * (4 * d + wave) + (lane >> 3);
+    int gm = m0 + 8 * (WAVES * d + wave) + (lane >> 3);
     gm = gm < p.M ? gm : p.M - 1;
     a_src[d] = (uint32_t)((int64_t)gm * p.lda + k0 / 2) + chunk * 16;
   }
 #pragma unroll
   for (int d = 0; d < B_DMA; ++d) {
-    int gn = n0 + 8 * (4 * d + wave) + (lane >> 3);
+    int gn = n0 + 8 * (WAVES * d + wave) + (lane >> 3);
     gn = gn < p.N ? gn : p.N - 1;
     b_src[d] = (uint32_t)((int64_t)gn * p.ldb + k0 / 2) + chunk * 16;
   }
   // Scales: 16 bytes (4 rows' words) per lane.  Piece i of an operand's stage
   // (BM or BN words for each of the two k-steps) is words 4 i .. 4 i + 3.  Rows
   // past the padded count and k-steps past the last re-read the last.
+  constexpr int S_DMA = Cfg::S_DMA, SA_DMA = Cfg::SA_DMA, SB_DMA = Cfg::SB_DMA;
   const int words = p.K / 128;
-  auto scale_src = [&](int piece, int rows, int row0, int64_t ld, int t) __attribute__((always_inline)) {
-    int kw = k0 / 128 + 2 * t + (piece * 4) / rows;
-    int row = row0 + (piece * 4) % rows;
-    kw = kw < words ? kw : words - 1;
-    row = row + 4 <= (int)ld ? row : (int)ld - 4;
-    return (uint32_t)(((int64_t)kw * ld + row) * 4);
-  };
-  const int sa_records = (int)((int64_t)words * p.ld_ascale * 4), sb_records = (int)((int64_t)words * p.ld_scale * 4);
+  const void* s_base[S_DMA];
+  int s_ld[S_DMA], s_dst[S_DMA];
+  int s_row[S_DMA], s_ks[S_DMA];
+#pragma unroll
+  for (int d = 0; d < S_DMA; ++d) {
+    int i = (WAVES * d + wave) % (SA_DMA + SB_DMA);  // the activations' instructions, then the weights'
+    const bool of_a = i < SA_DMA;
+    i = of_a ? i : i - SA_DMA;
+    const int rows = of_a ? BM : BN, piece = i * 64 + lane;
+    s_base[d] = of_a ? (const void*)p.ascale : p.bscale;
+    s_ld[d] = (int)(of_a ? p.ld_ascale : p.ld_scale);
+    s_dst[d] = (of_a ? Cfg::SA_OFF : Cfg::SB_OFF) + i * 1024;
+    s_ks[d] = k0 / 128 + piece * 4 / rows;
+    const int row = (of_a ? m0 : n0) + piece * 4 % rows;
+    s_row[d] = row + 4 <= s_ld[d] ? row : s_ld[d] - 4;
+  }
   auto load_stage = [&](int t, int slot) __attribute__((always_inline)) {
     t = t < T ? t : T - 1;
     char* S = lds + slot * Cfg::STAGE;
     const uint32_t bk = half && t == T - 1 ? back : 0;
 #pragma unroll
     for (int d = 0; d < A_DMA; ++d)
-      buffer_dma16(p.A, a_records, a_src[d] - bk, t * 128, S + (4 * d + wave) * 1024);
+      buffer_dma16(p.A, a_records, a_src[d] - bk, t * 128, S + (WAVES * d + wave) * 1024);
 #pragma unroll
     for (int d = 0; d < B_DMA; ++d)
-      buffer_dma16(p.B, b_records, b_src[d] - bk, t * 128, S + Cfg::B_OFF + (4 * d + wave) * 1024);
+      buffer_dma16(p.B, b_records, b_src[d] - bk, t * 128, S + Cfg::B_OFF + (WAVES * d + wave) * 1024);
 #pragma unroll
-    for (int d = 0; d < Cfg::S_DMA; ++d) {
-      int i = 4 * d + wave;  // scale instruction: the activations', then the weights'
-      i = i < Cfg::SA_DMA + Cfg::SB_DMA ? i : i % (Cfg::SA_DMA + Cfg::SB_DMA);
-      if (i < Cfg::SA_DMA)
-        buffer_dma16(p.ascale, sa_records, scale_src(i * 64 + lane, BM, m0, p.ld_ascale, t), 0,
-                     S + Cfg::SA_OFF + i * 1024);
-      else
-        buffer_dma16(p.bscale, sb_records, scale_src((i - Cfg::SA_DMA) * 64 + lane, BN, n0, p.ld_scale, t), 0,
-                     S + Cfg::SB_OFF + (i - Cfg::SA_DMA) * 1024);
+    for (int d = 0; d < S_DMA; ++d) {
+      int kw = s_ks[d] + 2 * t;
+      kw = kw < words ? kw : words - 1;
+      buffer_dma16(s_base[d], words * s_ld[d] * 4, (uint32_t)(kw * s_ld[d] + s_row[d]) * 4, 0, S + s_dst[d]);
     }
   };
 
-  // ---- fragments
-  struct Frag {
-    u32x4 a[AM], b[AN];
-    uint32_t sa[AM], sb[AN];
+  // ---- fragments.  A k-step runs in two phases of half the weight fragments
+  // each: in the first the second half arrives, in the second the next k-step's
+  // first half, and over both the next k-step's activation fragments, which all
+  // MFMAs of a k-step use.
+  constexpr int AH = AN / 2;
+  struct Rows {
+    u32x4 a[AM];
+    uint32_t s[AM];
   };
+  struct Half {
+    u32x4 w[AH];
+    uint32_t s[AH];
+  };
+  Rows x0, x1;
+  Half w0, w1;
   int c_off[2];
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) c_off[ks] = ((4 * ks + q) ^ swz_pair(r16)) * 16;
   const int a_rd = (wm * WM + r16) * 128, b_rd = Cfg::B_OFF + (wn * WN + r16) * 128;
   const int sa_rd = Cfg::SA_OFF + (wm * WM + r16) * 4 + q, sb_rd = Cfg::SB_OFF + (wn * WN + r16) * 4 + q;
-  auto read_a = [&](Frag& f, int slot, int ks, int i) __attribute__((always_inline)) {
+  auto read_a = [&](Rows& x, int slot, int ks, int i) __attribute__((always_inline)) {
     const char* S = lds + slot * Cfg::STAGE;
-    f.a[i] = *reinterpret_cast<const u32x4*>(S + a_rd + c_off[ks] + i * 2048);
-    f.sa[i] = *reinterpret_cast<const uint8_t*>(S + sa_rd + ks * BM * 4 + i * 64);
+    x.a[i] = *reinterpret_cast<const u32x4*>(S + a_rd + c_off[ks] + i * 2048);
+    x.s[i] = *reinterpret_cast<const uint8_t*>(S + sa_rd + ks * BM * 4 + i * 64);
   };
-  auto read_b = [&](Frag& f, int slot, int ks, int j) __attribute__((always_inline)) {
+  auto read_w = [&](Half& h, int slot, int ks, int part, int j) __attribute__((always_inline)) {
     const char* S = lds + slot * Cfg::STAGE;
-    f.b[j] = *reinterpret_cast<const u32x4*>(S + b_rd + c_off[ks] + j * 2048);
-    f.sb[j] = *reinterpret_cast<const uint8_t*>(S + sb_rd + ks * BN * 4 + j * 64);
+    h.w[j] = *reinterpret_cast<const u32x4*>(S + b_rd + c_off[ks] + (part * AH + j) * 2048);
+    h.s[j] = *reinterpret_cast<const uint8_t*>(S + sb_rd + ks * BN * 4 + (part * AH + j) * 64);
   };
 
   f32x4 acc[AM][AN];
@@ -150,25 +163,26 @@ __global__ __launch_bounds__(kM4Threads, 1) void gemm_mx4_kernel(GemmArgs p, int
     const i32x4 x = __builtin_bit_cast(i32x4, v);
     return __builtin_shufflevector(x, x, 0, 1, 2, 3, -1, -1, -1, -1);
   };
-  // the MFMAs of weight fragment j (weights as the MFMA's first operand: a
-  // lane then holds four consecutive output columns)
-  auto multiply = [&](const Frag& f, int j) __attribute__((always_inline)) {
+  // the MFMAs of weight fragment j of a half (weights as the MFMA's first
+  // operand: a lane then holds four consecutive output columns)
+  auto multiply = [&](const Rows& x, const Half& h, int part, int j) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < AM; ++i)
-      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(f.b[j]), wide(f.a[i]), acc[i][j], 4, 4, 0,
-                                                                   (int)f.sb[j], 0, (int)f.sa[i]);
+      acc[i][part * AH + j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+          wide(h.w[j]), wide(x.a[i]), acc[i][part * AH + j], 4, 4, 0, (int)h.s[j], 0, (int)x.s[i]);
   };
-  // a k-step's MFMAs, the reads of the next one spread over them
-  constexpr int RPJ = (AM + AN + AN - 1) / AN;  // reads per group
-  auto step = [&](const Frag& f, Frag& nx, int slot, int ks) __attribute__((always_inline)) {
+  // k-step (x, first half in w0); the next is `ks` of `slot`, and `cks` / `cslot`
+  // is this one
+  constexpr int HA = (AM + 1) / 2, RPJ = (HA + AH - 1) / AH;  // activation reads per phase and per group
+  auto phase = [&](const Rows& x, const Half& h, int part, Half& nh, int hslot, int hks, Rows& nx, int slot,
+                   int ks) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < AN; ++j) {
+    for (int j = 0; j < AH; ++j) {
+      read_w(nh, hslot, hks, 1 - part, j);
 #pragma unroll
-      for (int r = j * RPJ; r < (j + 1) * RPJ && r < AM + AN; ++r) {
-        if (r < AN) read_b(nx, slot, ks, r < AN ? r : 0);
-        else read_a(nx, slot, ks, r >= AN ? r - AN : 0);
-      }
-      multiply(f, j);
+      for (int r = j * RPJ; r < (j + 1) * RPJ && r < HA; ++r)
+        if (part * HA + r < AM) read_a(nx, slot, ks, part * HA + r);
+      multiply(x, h, part, j);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -177,29 +191,52 @@ __global__ __launch_bounds__(kM4Threads, 1) void gemm_mx4_kernel(GemmArgs p, int
   static_for<0, NST>([&](auto ic) { load_stage(decltype(ic)::value, decltype(ic)::value); });
   wait_vmcnt<(NST - 1) * Cfg::DMA>();
   barrier_nofence();
-  Frag f0, f1;
 #pragma unroll
-  for (int j = 0; j < AN; ++j) read_b(f0, 0, 0, j);
+  for (int j = 0; j < AH; ++j) read_w(w0, 0, 0, 0, j);
 #pragma unroll
-  for (int i = 0; i < AM; ++i) read_a(f0, 0, 0, i);
+  for (int i = 0; i < AM; ++i) read_a(x0, 0, 0, i);
 
-  // Stage t: k-step 0 while k-step 1's fragments arrive; then, with every read
-  // of the stage done and stage t + 1 landed, the barrier, the loads of stage
-  // t + NST into this slot, and k-step 1 while the next stage's first
-  // fragments arrive.  Past the last stage the loads repeat it.
+  // Stage t: k-step 0 while k-step 1's fragments arrive, and the second half
+  // of k-step 1's weights in its first phase; then, with every read of the stage
+  // done and stage t + 1 landed, the barrier, and the loads of stage t + NST into
+  // this slot.  Past the last stage the loads repeat it.
   int slot = 0;
   for (int t = 0; t < depth / 256; ++t) {
-    step(f0, f1, slot, 1);
+    phase(x0, w0, 0, w1, slot, 0, x1, slot, 1);
+    phase(x0, w1, 1, w0, slot, 1, x1, slot, 1);
+    const int next = slot + 1 < NST ? slot + 1 : 0;
+#pragma unroll
+    for (int j = 0; j < AH; ++j) read_w(w1, slot, 1, 1, j);
     wait_lgkmcnt0();
     wait_vmcnt<(NST - 2) * Cfg::DMA>();
     barrier_nofence();
     load_stage(t + NST, slot);
-    slot = slot + 1 < NST ? slot + 1 : 0;
-    step(f1, f0, slot, 0);
-  }
-  if (half)
+    slot = next;
 #pragma unroll
-    for (int j = 0; j < AN; ++j) multiply(f0, j);
+    for (int j = 0; j < AH; ++j) {
+#pragma unroll
+      for (int r = j * RPJ; r < (j + 1) * RPJ && r < HA; ++r) read_a(x0, slot, 0, r);
+      multiply(x1, w0, 0, j);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int j = 0; j < AH; ++j) {
+      read_w(w0, slot, 0, 0, j);
+#pragma unroll
+      for (int r = j * RPJ; r < (j + 1) * RPJ && r < HA; ++r)
+        if (HA + r < AM) read_a(x0, slot, 0, HA + r);
+      multiply(x1, w1, 1, j);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  if (half) {
+#pragma unroll
+    for (int j = 0; j < AH; ++j) read_w(w1, slot, 0, 1, j);
+#pragma unroll
+    for (int j = 0; j < AH; ++j) multiply(x0, w0, 0, j);
+#pragma unroll
+    for (int j = 0; j < AH; ++j) multiply(x0, w1, 1, j);
+  }
   wait_vmcnt<0>();
   if constexpr (EPI == kEpiPartial) {
     float* P = p.partial + (int64_t)kz * p.M * p.N;
@@ -218,21 +255,31 @@ __global__ __launch_bounds__(kM4Threads, 1) void gemm_mx4_kernel(GemmArgs p, int
     // that both the 8-byte writes and the 16-byte reads spread over the banks
     __syncthreads();
     constexpr int CH = WN / 8, RPI = 64 / CH, ITS = WM / RPI;
-    auto swz = [](int row) { return CH == 16 ? row & 15 : (row >> 1) & 7; };
+    auto swz = [](int row) { return CH == 16 ? row & 15 : (CH == 8 ? (row >> 1) & 7 : (row >> 2) & 3); };
     char* E = lds + wave * Cfg::EPI_WAVE;
+    auto phase1 = [&](auto sig_tag, auto rtb_tag) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < AN; ++j) {
-      const int gn = n0 + wn * WN + j * 16 + 4 * q;
-      f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (p.bias && gn < p.N)
+      for (int j = 0; j < AN; ++j) {
+        const int gn = n0 + wn * WN + j * 16 + 4 * q;
+        f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (p.bias && gn < p.N)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bias[e] = p.bias[gn + e];
+          for (int e = 0; e < 4; ++e) bias[e] = p.bias[gn + e];
 #pragma unroll
-      for (int i = 0; i < AM; ++i) {
-        const int row = i * 16 + r16;
-        *reinterpret_cast<bf16x4*>(E + row * Cfg::EPI_ROWB + ((2 * j + (q >> 1)) ^ swz(row)) * 16 + (q & 1) * 8) =
-            fp4_branch4<EPI>(p, acc[i][j], bias, gn);
+        for (int i = 0; i < AM; ++i) {
+          const int row = i * 16 + r16;
+          *reinterpret_cast<bf16x4*>(E + row * Cfg::EPI_ROWB + ((2 * j + (q >> 1)) ^ swz(row)) * 16 + (q & 1) * 8) =
+              fp4_branch4<EPI, decltype(sig_tag)::value, decltype(rtb_tag)::value>(p, acc[i][j], bias, gn);
+        }
       }
+    };
+    const bool sig = EPI == LTX_GEMM_EPI_BIAS && n0 + wn * WN + WN > p.sig_from;
+    if (p.round_then_bias) {
+      if (sig) phase1(std::true_type{}, std::true_type{});
+      else phase1(std::false_type{}, std::true_type{});
+    } else {
+      if (sig) phase1(std::true_type{}, std::false_type{});
+      else phase1(std::false_type{}, std::false_type{});
     }
     // a wave reads back only what it wrote itself
     wait_lgkmcnt0();
@@ -258,6 +305,10 @@ __global__ __launch_bounds__(kM4Threads, 1) void gemm_mx4_kernel(GemmArgs p, int
     }
   }
 }
+
+using M4Large = M4Tile<256, 256, 4, 2, 2>;
+using M4Mid = M4Tile<128, 128, 2, 4, 4>;
+using M4Small = M4Tile<64, 128, 2, 4, 4>;
 
 struct Mx4Plan {
   int bm, bn, splits, k_split;
@@ -285,9 +336,13 @@ static void mx4_launch(const GemmArgs& p, const Mx4Plan& pl, hipStream_t s) {
   a.tiles_m = (p.M + pl.bm - 1) / pl.bm;
   a.tiles_n = (p.N + pl.bn - 1) / pl.bn;
   const int blocks = a.tiles_m * a.tiles_n * pl.splits;
-  if (pl.bm == 256) gemm_mx4_kernel<256, 256, EPI><<<blocks, kM4Threads, 0, s>>>(a, pl.k_split);
-  else if (pl.bm == 128) gemm_mx4_kernel<128, 128, EPI><<<blocks, kM4Threads, 0, s>>>(a, pl.k_split);
-  else gemm_mx4_kernel<64, 128, EPI><<<blocks, kM4Threads, 0, s>>>(a, pl.k_split);
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    gemm_mx4_kernel<T, EPI><<<blocks, T::THREADS, 0, s>>>(a, pl.k_split);
+  };
+  if (pl.bm == 256) go(M4Large{});
+  else if (pl.bm == 128) go(M4Mid{});
+  else go(M4Small{});
 }
 
 }  // namespace ltx
