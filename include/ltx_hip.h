@@ -399,7 +399,7 @@ int ltx_gemm_mx_gelu_mxfp8(const uint8_t* A, int64_t lda, const uint8_t* a_scale
  * ltx_gemm_mxfp4_bf16: bf16 rows A (M, K) x MXFP4 weights (N, K), decoded to
  * bf16 exactly.  K % 64 == 0, N % 8 == 0.
  * ltx_gemm_mx4_bf16: MXFP4 rows x MXFP4 weights on the scaled FP4 MFMA
- * (v_mfma_scale_f32_16x16x128_f8f6f4).  K % 128 == 0, N % 8 == 0, operands
+ * (v_mfma_scale_f32_32x32x64_f8f6f4).  K % 128 == 0, N % 8 == 0, operands
  * below 2 GiB each.
  * fp32 accumulation; epilogues LTX_GEMM_EPI_*, LTX_GEMM_ROUND_THEN_BIAS and
  * sigmoid_from as above, except that GELU and the head gate act on the fp32

@@ -1,18 +1,26 @@
 // Projection GEMMs of MXFP4 rows and MXFP4 weights on the scaled FP4 MFMA
-// (v_mfma_scale_f32_16x16x128_f8f6f4):
+// (v_mfma_scale_f32_32x32x64_f8f6f4):
 //
 //   C[m, n] = epilogue( sum_k a[m, k] w[n, k] + bias[n] ),
 //   a = e2m1(A) 2^(XA), w = e2m1(W) 2^(XW), a scale per 32 k on both sides.
 //
 // Operand storage: gemm_fp4.h.
 //
-// A workgroup of 4 waves (2 x 2) computes a BM x BN tile.  A stage is 256 k:
-// rows of 128 code bytes, one line each, and two scale words per row; stages
-// reach LDS by direct loads into a ring of NST.  A stage has two k-steps of 128;
-// lane (row r16, quarter q) of a fragment holds the 16 bytes of its row's block
-// q, and its scale operand that block's byte.  The fragments of the next
-// k-step are read while the MFMAs of the current one run, also across the
-// one barrier per stage.
+// A workgroup computes a BM x BN tile.  A stage is 256 k: rows of 128 code bytes,
+// one line each, and two scale words per row; stages reach LDS by direct loads
+// into a ring of NST.  A stage has four k-steps of 64; lane (row r32, half h) of a
+// fragment holds the 16 bytes of its row's block h, and its scale operand that
+// block's byte.  The fragments of the next k-step are read while the MFMAs of the
+// current one run, also across the one barrier per stage.
+//
+// What bounds it: 256 x 256 tiles with all CUs busy run at 3.9-4.1 PFLOP/s (3456 x
+// 16384 -> 4096 115 us, 1.75 us per stage).  A loop of nothing but these MFMAs on
+// random codes reaches 5.9-6.4 at the chip's power limit (9.8 on zeros, and this
+// kernel 4.9); its loads and fragment reads alone take 1.15 us per stage, the
+// MFMAs without loads 1.65.  Measured beside it: the 16 x 16 x 128 form 117 us; four
+// waves of 128 x 128 117 (a third less LDS traffic); all loads in one k-step 117
+// against 113 for two; touching the lines two stages ahead, to take the L2
+// misses off the loads, 116: no change.
 #include "gemm_fp4.h"
 
 namespace ltx {
@@ -21,7 +29,7 @@ template <int BM_, int BN_, int WAVES_M_, int WAVES_N_, int NST_>
 struct M4Tile {
   static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, NST = NST_;
   static constexpr int WAVES = WAVES_M * WAVES_N, THREADS = WAVES * 64;
-  static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, AM = WM / 16, AN = WN / 16;
+  static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, AM = WM / 32, AN = WN / 32;
   static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128;
   // two scale words per row; at least one direct-load instruction (1 KiB)
   static constexpr int SA_BYTES = BM * 8 < 1024 ? 1024 : BM * 8, SB_BYTES = BN * 8 < 1024 ? 1024 : BN * 8;
@@ -51,7 +59,7 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % Cfg::WAVES_M, wn = wave / Cfg::WAVES_M;
-  const int r16 = lane & 15, q = lane >> 4;
+  const int r32 = lane & 31, h = lane >> 5;
   const int tiles = p.tiles_m * p.tiles_n;
   const int kz = EPI == kEpiPartial ? (int)blockIdx.x / tiles : 0;
   int tmi, tni;
@@ -69,7 +77,7 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
   // missing k-step load the other's bytes.
   const int a_records = (int)((int64_t)(p.M - 1) * p.lda + p.K / 2);
   const int b_records = (int)((int64_t)(p.N - 1) * p.ldb + p.K / 2);
-  const int chunk = pair_chunk(lane);
+  const int chunk = (lane & 7) ^ g8_swz128(8 * wave + (lane >> 3), false);  // (8 waves a multiple of 16 rows)
   const int back = (chunk & 4) * 16;
   uint32_t a_src[A_DMA], b_src[B_DMA];
 #pragma unroll
@@ -105,149 +113,143 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
     const int row = (of_a ? m0 : n0) + piece * 4 % rows;
     s_row[d] = row + 4 <= s_ld[d] ? row : s_ld[d] - 4;
   }
-  auto load_stage = [&](int t, int slot) __attribute__((always_inline)) {
+  // load instruction l of stage t: code rows, then scales
+  auto load = [&](int t, int slot, int l) __attribute__((always_inline)) {
     t = t < T ? t : T - 1;
     char* S = lds + slot * Cfg::STAGE;
     const uint32_t bk = half && t == T - 1 ? back : 0;
-#pragma unroll
-    for (int d = 0; d < A_DMA; ++d)
-      buffer_dma16(p.A, a_records, a_src[d] - bk, t * 128, S + (WAVES * d + wave) * 1024);
-#pragma unroll
-    for (int d = 0; d < B_DMA; ++d)
+    if (l < A_DMA) {
+      buffer_dma16(p.A, a_records, a_src[l < A_DMA ? l : 0] - bk, t * 128, S + (WAVES * l + wave) * 1024);
+    } else if (l < A_DMA + B_DMA) {
+      const int d = l >= A_DMA && l < A_DMA + B_DMA ? l - A_DMA : 0;
       buffer_dma16(p.B, b_records, b_src[d] - bk, t * 128, S + Cfg::B_OFF + (WAVES * d + wave) * 1024);
-#pragma unroll
-    for (int d = 0; d < S_DMA; ++d) {
+    } else {
+      const int d = l >= A_DMA + B_DMA ? l - A_DMA - B_DMA : 0;
       int kw = s_ks[d] + 2 * t;
       kw = kw < words ? kw : words - 1;
       buffer_dma16(s_base[d], words * s_ld[d] * 4, (uint32_t)(kw * s_ld[d] + s_row[d]) * 4, 0, S + s_dst[d]);
     }
   };
 
-  // ---- fragments.  A k-step runs in two phases of half the weight fragments
-  // each: in the first the second half arrives, in the second the next k-step's
-  // first half, and over both the next k-step's activation fragments, which all
-  // MFMAs of a k-step use.
-  constexpr int AH = AN / 2;
-  struct Rows {
-    u32x4 a[AM];
-    uint32_t s[AM];
+  // ---- fragments of a k-step of 64: lane (row r32, half h) holds the 16 bytes of
+  // block h, chunk 2 ks + h of its row, and that block's scale byte
+  struct Frags {
+    u32x4 a[AM], w[AN];
+    uint32_t sa[AM], sw[AN];
   };
-  struct Half {
-    u32x4 w[AH];
-    uint32_t s[AH];
-  };
-  Rows x0, x1;
-  Half w0, w1;
-  int c_off[2];
+  Frags f0, f1;
+  int c_off[4];
 #pragma unroll
-  for (int ks = 0; ks < 2; ++ks) c_off[ks] = ((4 * ks + q) ^ swz_pair(r16)) * 16;
-  const int a_rd = (wm * WM + r16) * 128, b_rd = Cfg::B_OFF + (wn * WN + r16) * 128;
-  const int sa_rd = Cfg::SA_OFF + (wm * WM + r16) * 4 + q, sb_rd = Cfg::SB_OFF + (wn * WN + r16) * 4 + q;
-  auto read_a = [&](Rows& x, int slot, int ks, int i) __attribute__((always_inline)) {
+  for (int ks = 0; ks < 4; ++ks) c_off[ks] = ((2 * ks + h) ^ g8_swz128(r32, false)) * 16;
+  const int a_rd = (wm * WM + r32) * 128, w_rd = Cfg::B_OFF + (wn * WN + r32) * 128;
+  const int sa_rd = Cfg::SA_OFF + (wm * WM + r32) * 4 + h, sw_rd = Cfg::SB_OFF + (wn * WN + r32) * 4 + h;
+  auto read_a = [&](Frags& f, int slot, int ks, int i) __attribute__((always_inline)) {
     const char* S = lds + slot * Cfg::STAGE;
-    x.a[i] = *reinterpret_cast<const u32x4*>(S + a_rd + c_off[ks] + i * 2048);
-    x.s[i] = *reinterpret_cast<const uint8_t*>(S + sa_rd + ks * BM * 4 + i * 64);
+    f.a[i] = *reinterpret_cast<const u32x4*>(S + a_rd + c_off[ks] + i * 4096);
+    f.sa[i] = *reinterpret_cast<const uint8_t*>(S + sa_rd + (ks >> 1) * BM * 4 + (ks & 1) * 2 + i * 128);
   };
-  auto read_w = [&](Half& h, int slot, int ks, int part, int j) __attribute__((always_inline)) {
+  auto read_w = [&](Frags& f, int slot, int ks, int j) __attribute__((always_inline)) {
     const char* S = lds + slot * Cfg::STAGE;
-    h.w[j] = *reinterpret_cast<const u32x4*>(S + b_rd + c_off[ks] + (part * AH + j) * 2048);
-    h.s[j] = *reinterpret_cast<const uint8_t*>(S + sb_rd + ks * BN * 4 + (part * AH + j) * 64);
+    f.w[j] = *reinterpret_cast<const u32x4*>(S + w_rd + c_off[ks] + j * 4096);
+    f.sw[j] = *reinterpret_cast<const uint8_t*>(S + sw_rd + (ks >> 1) * BN * 4 + (ks & 1) * 2 + j * 128);
   };
 
-  f32x4 acc[AM][AN];
+  f32x16 acc[AM][AN];
 #pragma unroll
   for (int i = 0; i < AM; ++i)
 #pragma unroll
-    for (int j = 0; j < AN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < AN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
   auto wide = [](u32x4 v) __attribute__((always_inline)) {
     const i32x4 x = __builtin_bit_cast(i32x4, v);
     return __builtin_shufflevector(x, x, 0, 1, 2, 3, -1, -1, -1, -1);
   };
-  // the MFMAs of weight fragment j of a half (weights as the MFMA's first
-  // operand: a lane then holds four consecutive output columns)
-  auto multiply = [&](const Rows& x, const Half& h, int part, int j) __attribute__((always_inline)) {
+  // a k-step's MFMAs in groups of one weight fragment (weights as the MFMA's first
+  // operand: a lane then holds runs of four consecutive output columns); f(j)
+  // issues what goes beside group j
+  auto step = [&](const Frags& x, auto f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < AM; ++i)
-      acc[i][part * AH + j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-          wide(h.w[j]), wide(x.a[i]), acc[i][part * AH + j], 4, 4, 0, (int)h.s[j], 0, (int)x.s[i]);
-  };
-  // k-step (x, first half in w0); the next is `ks` of `slot`, and `cks` / `cslot`
-  // is this one
-  constexpr int HA = (AM + 1) / 2, RPJ = (HA + AH - 1) / AH;  // activation reads per phase and per group
-  auto phase = [&](const Rows& x, const Half& h, int part, Half& nh, int hslot, int hks, Rows& nx, int slot,
-                   int ks) __attribute__((always_inline)) {
+    for (int j = 0; j < AN; ++j) {
+      f(j);
 #pragma unroll
-    for (int j = 0; j < AH; ++j) {
-      read_w(nh, hslot, hks, 1 - part, j);
-#pragma unroll
-      for (int r = j * RPJ; r < (j + 1) * RPJ && r < HA; ++r)
-        if (part * HA + r < AM) read_a(nx, slot, ks, part * HA + r);
-      multiply(x, h, part, j);
+      for (int i = 0; i < AM; ++i)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(x.w[j]), wide(x.a[i]), acc[i][j], 4, 4, 0,
+                                                                    (int)x.sw[j], 0, (int)x.sa[i]);
       __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  // the reads of k-step ks, share j of AN
+  auto read_share = [&](Frags& f, int slot, int ks, int j) __attribute__((always_inline)) {
+    if (j < AN) read_w(f, slot, ks, j);
+#pragma unroll
+    for (int i = 0; i < AM; ++i)
+      if (i * AN / AM == j) read_a(f, slot, ks, i);
   };
 
   // ---- prologue: the ring filled, stage 0 landed
-  static_for<0, NST>([&](auto ic) { load_stage(decltype(ic)::value, decltype(ic)::value); });
-  wait_vmcnt<(NST - 1) * Cfg::DMA>();
+  // (of the last slot's stage the first HL loads)
+  constexpr int HL = (Cfg::DMA + 1) / 2;
+#pragma unroll
+  for (int t = 0; t < NST; ++t)
+#pragma unroll
+    for (int l = 0; l < (t < NST - 1 ? Cfg::DMA : HL); ++l) load(t, t, l);
+  wait_vmcnt<(NST - 2) * Cfg::DMA + HL>();
   barrier_nofence();
 #pragma unroll
-  for (int j = 0; j < AH; ++j) read_w(w0, 0, 0, 0, j);
-#pragma unroll
-  for (int i = 0; i < AM; ++i) read_a(x0, 0, 0, i);
+  for (int j = 0; j < AN; ++j) read_share(f0, 0, 0, j);
 
-  // Stage t: k-step 0 while k-step 1's fragments arrive, and the second half
-  // of k-step 1's weights in its first phase; then, with every read of the stage
-  // done and stage t + 1 landed, the barrier, and the loads of stage t + NST into
-  // this slot.  Past the last stage the loads repeat it.
+  // Stage t: each k-step's MFMAs while the next one's fragments arrive; before the
+  // last, with every read of the stage done and stage t + 1 landed, the barrier,
+  // after which the loads of stage t + NST go into this slot.  Past the last
+  // stage the loads repeat it.
   int slot = 0;
+  constexpr int LPJ = (HL + AN - 1) / AN;  // load instructions per group
+  int prev = NST - 1;                      // the slot of stage t - 1
   for (int t = 0; t < depth / 256; ++t) {
-    phase(x0, w0, 0, w1, slot, 0, x1, slot, 1);
-    phase(x0, w1, 1, w0, slot, 1, x1, slot, 1);
-    const int next = slot + 1 < NST ? slot + 1 : 0;
+    step(f0, [&](int j) __attribute__((always_inline)) {
+      read_share(f1, slot, 1, j);
 #pragma unroll
-    for (int j = 0; j < AH; ++j) read_w(w1, slot, 1, 1, j);
+      for (int l = HL; l < Cfg::DMA; ++l)
+        if ((l - HL) / LPJ == j) load(t + NST - 1, prev, l);
+    });
+    step(f1, [&](int j) __attribute__((always_inline)) { read_share(f0, slot, 2, j); });
+    step(f0, [&](int j) __attribute__((always_inline)) {
+      if (j == 0)
+#pragma unroll
+        for (int i = 0; i < AN; ++i) read_share(f1, slot, 3, i);
+    });
     wait_lgkmcnt0();
     wait_vmcnt<(NST - 2) * Cfg::DMA>();
     barrier_nofence();
-    load_stage(t + NST, slot);
-    slot = next;
+    prev = slot;
+    slot = slot + 1 < NST ? slot + 1 : 0;
+    step(f1, [&](int j) __attribute__((always_inline)) {
+      read_share(f0, slot, 0, j);
 #pragma unroll
-    for (int j = 0; j < AH; ++j) {
-#pragma unroll
-      for (int r = j * RPJ; r < (j + 1) * RPJ && r < HA; ++r) read_a(x0, slot, 0, r);
-      multiply(x1, w0, 0, j);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#pragma unroll
-    for (int j = 0; j < AH; ++j) {
-      read_w(w0, slot, 0, 0, j);
-#pragma unroll
-      for (int r = j * RPJ; r < (j + 1) * RPJ && r < HA; ++r)
-        if (HA + r < AM) read_a(x0, slot, 0, HA + r);
-      multiply(x1, w1, 1, j);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+      for (int l = 0; l < HL; ++l)
+        if (l / LPJ == j) load(t + NST, prev, l);
+    });
   }
   if (half) {
-#pragma unroll
-    for (int j = 0; j < AH; ++j) read_w(w1, slot, 0, 1, j);
-#pragma unroll
-    for (int j = 0; j < AH; ++j) multiply(x0, w0, 0, j);
-#pragma unroll
-    for (int j = 0; j < AH; ++j) multiply(x0, w1, 1, j);
+    step(f0, [&](int j) __attribute__((always_inline)) { read_share(f1, slot, 1, j); });
+    step(f1, [](int) {});
   }
   wait_vmcnt<0>();
   if constexpr (EPI == kEpiPartial) {
     float* P = p.partial + (int64_t)kz * p.M * p.N;
 #pragma unroll
     for (int i = 0; i < AM; ++i) {
-      const int gm = m0 + wm * WM + i * 16 + r16;
+      const int gm = m0 + wm * WM + i * 32 + r32;
 #pragma unroll
-      for (int j = 0; j < AN; ++j) {
-        const int gn = n0 + wn * WN + j * 16 + 4 * q;  // N % 8 == 0: four columns inside or outside
-        if (gm < p.M && gn < p.N) *reinterpret_cast<f32x4*>(P + (int64_t)gm * p.N + gn) = acc[i][j];
-      }
+      for (int j = 0; j < AN; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int gn = n0 + wn * WN + j * 32 + 8 * g + 4 * h;  // N % 8 == 0: four columns inside or outside
+          if (gm < p.M && gn < p.N)
+            *reinterpret_cast<f32x4*>(P + (int64_t)gm * p.N + gn) =
+                f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        }
     }
     return;
   } else {
@@ -260,16 +262,20 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
     auto phase1 = [&](auto sig_tag, auto rtb_tag) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < AN; ++j) {
-        const int gn = n0 + wn * WN + j * 16 + 4 * q;
-        f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (p.bias && gn < p.N)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) bias[e] = p.bias[gn + e];
+        for (int g = 0; g < 4; ++g) {
+          const int gn = n0 + wn * WN + j * 32 + 8 * g + 4 * h;
+          f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
+          if (p.bias && gn < p.N)
 #pragma unroll
-        for (int i = 0; i < AM; ++i) {
-          const int row = i * 16 + r16;
-          *reinterpret_cast<bf16x4*>(E + row * Cfg::EPI_ROWB + ((2 * j + (q >> 1)) ^ swz(row)) * 16 + (q & 1) * 8) =
-              fp4_branch4<EPI, decltype(sig_tag)::value, decltype(rtb_tag)::value>(p, acc[i][j], bias, gn);
+            for (int e = 0; e < 4; ++e) bias[e] = p.bias[gn + e];
+#pragma unroll
+          for (int i = 0; i < AM; ++i) {
+            const int row = i * 32 + r32;
+            const f32x4 y = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+            *reinterpret_cast<bf16x4*>(E + row * Cfg::EPI_ROWB + ((4 * j + g) ^ swz(row)) * 16 + h * 8) =
+                fp4_branch4<EPI, decltype(sig_tag)::value, decltype(rtb_tag)::value>(p, y, bias, gn);
+          }
         }
       }
     };
@@ -306,27 +312,57 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
   }
 }
 
-using M4Large = M4Tile<256, 256, 4, 2, 2>;
+using M4Large = M4Tile<256, 256, 2, 4, 2>;
+using M4Tall = M4Tile<256, 128, 4, 2, 3>;
 using M4Mid = M4Tile<128, 128, 2, 4, 4>;
 using M4Small = M4Tile<64, 128, 2, 4, 4>;
 
+
 struct Mx4Plan {
-  int bm, bn, splits, k_split;
+  int bm, bn, splits;
+  int k_split;  // k of one range, a multiple of 256
 };
+
+// Modelled time (us): a round of one workgroup per CU costs `fixed` (first loads
+// and epilogue) and per 256 k `idle` to `full`, as it fills the CUs (they share the
+// L2s and the chip's power); a split's second launch and its partials.  Model
+// against measured: 1296 x 4096 -> 4096 in tiles of 256 x 256, 256 x 128, 128 x 128,
+// 64 x 128 29 / 21 / 24 / 28 against 26 / 20 / 25 / 28, 3456 x 4096 -> 4096 34 / 41 /
+// 48 / 66 against 35 / 43 / 55 / 70, 1296 x 4096 -> 12320 60 / 58 / 59 / 71 against 58 /
+// 55 / 60 / 72, 68 x 8192 -> 2048 64 x 128 in 4 splits 11 / 11, 256 x 4096 -> 8192 64 x
+// 128 11 / 11, 6144 x 1024 -> 16384 256 x 256 77 / 79.
+static double mx4_time(double M, double N, int bm, int bn, int splits, double per) {
+  const double wgs = ceil(M / bm) * ceil(N / bn) * splits;
+  double fixed = 2.2, idle = 0.37, full = 0.40;
+  if (bm == 256 && bn == 256) fixed = 5.5, idle = 1.15, full = 1.75;
+  else if (bm == 256) fixed = 4.3, idle = 0.80, full = 0.94;
+  else if (bm == 128) fixed = 2.6, idle = 0.49, full = 0.57;
+  const double rounds = floor(wgs / 256), rest = wgs / 256 - rounds;
+  double t = 2.2 + rounds * (fixed + per * full);
+  if (rest > 0) t += fixed + per * (idle + (full - idle) * rest);
+  if (splits > 1) t += 2.5 + M * N * splits * 8 / 4e6;
+  return t;
+}
+
 static Mx4Plan mx4_plan(int64_t M, int64_t N, int64_t K) {
-  Mx4Plan pl;
-  const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
-  pl.bm = big >= 160 ? 256 : (M <= 64 ? 64 : 128);
-  pl.bn = big >= 160 ? 256 : 128;
-  const int64_t tiles = ((M + pl.bm - 1) / pl.bm) * ((N + pl.bn - 1) / pl.bn);
+  static const int tile[4][2] = {{256, 256}, {256, 128}, {128, 128}, {64, 128}};
   const int64_t units = (K + 255) / 256;
-  int64_t s = 256 / tiles;
-  if (s > units / 2) s = units / 2;
-  if (s > 32) s = 32;
-  if (s < 1) s = 1;
-  const int64_t per = (units + s - 1) / s;
-  pl.k_split = (int)(per * 256);
-  pl.splits = (int)((units + per - 1) / per);
+  Mx4Plan pl = {64, 128, 1, (int)(units * 256)};
+  double best = 1e30;
+  for (const auto& t : tile) {
+    const int64_t tiles = ((M + t[0] - 1) / t[0]) * ((N + t[1] - 1) / t[1]);
+    for (int want = 1; want <= 16; ++want) {
+      // splits: at least two stages each, within one round of the CUs, 10 % faster
+      if (want > 1 && (units / want < 2 || tiles * want > 256)) break;
+      const int64_t per = (units + want - 1) / want;
+      const int s = (int)((units + per - 1) / per);
+      const double us = mx4_time((double)M, (double)N, t[0], t[1], s, (double)per);
+      if (us < best * (s > 1 ? 0.9 : 1.0)) {
+        best = us;
+        pl = {t[0], t[1], s, (int)(per * 256)};
+      }
+    }
+  }
   return pl;
 }
 
@@ -340,7 +376,8 @@ static void mx4_launch(const GemmArgs& p, const Mx4Plan& pl, hipStream_t s) {
     using T = decltype(t);
     gemm_mx4_kernel<T, EPI><<<blocks, T::THREADS, 0, s>>>(a, pl.k_split);
   };
-  if (pl.bm == 256) go(M4Large{});
+  if (pl.bm == 256 && pl.bn == 256) go(M4Large{});
+  else if (pl.bm == 256) go(M4Tall{});
   else if (pl.bm == 128) go(M4Mid{});
   else go(M4Small{});
 }
