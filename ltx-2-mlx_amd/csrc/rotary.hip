@@ -49,11 +49,22 @@ struct alignas(sizeof(T) * VEC) RotVec {
 
 // VEC elements per load and store: the largest power of two up to 16 bytes
 // that divides the extents, strides and addresses.
+//
+// An item is two vectors of a head: the two halves of VEC pairs, or two vectors
+// of neighbouring pairs, or two that are only copied (the second may repeat the
+// first at an odd end).  The items of the workgroup's tokens and heads form
+// one list that the threads go through, kBatch items each at a time: as many
+// loads in flight whatever the head layout (a loop over heads with a fixed item
+// per thread left them idle where tokens have few heads: 14639 tokens x 40 heads
+// of 64 fp32 99 us).
+constexpr int kRotBatch = 4;
 template <typename T, int VEC, bool INTERLEAVED>
 __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs p) {
   using V = RotVec<T, VEC>;
+  constexpr bool NEIGHBOURS = INTERLEAVED && VEC > 1;  // a vector holds whole pairs
   __shared__ __attribute__((aligned(16))) float cs[kRotTokens][kRotMaxDim / 2];
   __shared__ __attribute__((aligned(16))) float sn[kRotTokens][kRotMaxDim / 2];
+  __shared__ int64_t row_x[2][kRotTokens], row_out[2][kRotTokens];
   const int pairs = p.rotary / 2;
   const int64_t all = p.batch * p.tokens;
   const int64_t first = (int64_t)blockIdx.x * p.per_block;
@@ -69,77 +80,93 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs p) {
     cs[t][j] = c * p.factor;
     sn[t][j] = (p.transpose ? -s : s) * p.factor;
   }
+  if (threadIdx.x < 2 * kRotTokens) {
+    const int side = threadIdx.x / kRotTokens, t = threadIdx.x % kRotTokens;
+    const ltx_rotary_rows& r = p.side[side];
+    const int64_t row = first + t, b = row / p.tokens, tok = row % p.tokens;
+    row_x[side][t] = b * r.x_batch + tok * r.x_token;
+    row_out[side][t] = b * r.out_batch + tok * r.out_token;
+  }
   __syncthreads();
 
-  // items of a head: vectors of pairs (half layout: two loads), then vectors of
-  // the channels that are only copied.  A thread keeps its item over the heads.
-  constexpr bool NEIGHBOURS = INTERLEAVED && VEC > 1;  // a vector holds whole pairs
-  const int rot_items = NEIGHBOURS ? p.rotary / VEC : pairs / VEC;
-  const int all_items = rot_items + (p.head_dim - p.rotary) / VEC;
-  const int lanes = all_items < kRotThreads ? all_items : kRotThreads;
-  const int step = kRotThreads / lanes;
-  const int i0 = threadIdx.x % lanes, h0 = threadIdx.x / lanes;
-  if (h0 >= step) return;
+  const int rot_vecs = NEIGHBOURS ? p.rotary / VEC : 2 * (pairs / VEC), copy_vecs = (p.head_dim - p.rotary) / VEC;
+  const int rot_items = (rot_vecs + 1) / 2, all_items = rot_items + (copy_vecs + 1) / 2;
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     const ltx_rotary_rows& r = p.side[side];
-    if (r.heads == 0) continue;
+    const int heads = (int)r.heads;
+    if (heads == 0) continue;
     const bool in_place = r.x == r.out && r.x_batch == r.out_batch && r.x_token == r.out_token && r.x_head == r.out_head;
     const int items = in_place ? rot_items : all_items;
-    for (int t = 0; t < count; ++t) {
-      const int64_t row = first + t, b = row / p.tokens, tok = row % p.tokens;
-      const T* x = (const T*)r.x + b * r.x_batch + tok * r.x_token;
-      T* out = (T*)r.out + b * r.out_batch + tok * r.out_token;
-      for (int i = i0; i < items; i += lanes) {
-        if (i >= rot_items) {
-          const int c = p.rotary + (i - rot_items) * VEC;
-#pragma unroll 2
-          for (int64_t h = h0; h < r.heads; h += step)
-            *reinterpret_cast<V*>(out + h * r.out_head + c) = *reinterpret_cast<const V*>(x + h * r.x_head + c);
-          continue;
+    const T* x = (const T*)r.x;
+    T* out = (T*)r.out;
+    // (token, head, item) of this thread, and what kRotThreads items add to it
+    int i = threadIdx.x % items, h = threadIdx.x / items % heads, t = threadIdx.x / items / heads;
+    const int di = kRotThreads % items, dh = kRotThreads / items % heads, dt = kRotThreads / items / heads;
+    while (t < count) {
+      V a[kRotBatch], b[kRotBatch];
+      T* dst[kRotBatch];
+      int c0[kRotBatch], c1[kRotBatch], at[kRotBatch];
+#pragma unroll
+      for (int e = 0; e < kRotBatch; ++e) {
+        at[e] = t;
+        if (t < count) {
+          const int j = i - rot_items;
+          if (j >= 0) {
+            c0[e] = p.rotary + 2 * j * VEC;
+            c1[e] = p.rotary + (2 * j + 1 < copy_vecs ? 2 * j + 1 : 2 * j) * VEC;
+          } else if (NEIGHBOURS) {
+            c0[e] = 2 * i * VEC;
+            c1[e] = (2 * i + 1 < rot_vecs ? 2 * i + 1 : 2 * i) * VEC;
+          } else {
+            c0[e] = INTERLEAVED ? 2 * i : i * VEC;
+            c1[e] = INTERLEAVED ? 2 * i + 1 : i * VEC + pairs;
+          }
+          const T* src = x + row_x[side][t] + h * r.x_head;
+          dst[e] = out + row_out[side][t] + h * r.out_head;
+          a[e] = *reinterpret_cast<const V*>(src + c0[e]);
+          b[e] = *reinterpret_cast<const V*>(src + c1[e]);
         }
-        if constexpr (NEIGHBOURS) {
-          const int c = i * VEC;
-          float ca[VEC / 2], sa[VEC / 2];
+        i += di;
+        h += dh;
+        t += dt;
+        if (i >= items) {
+          i -= items;
+          ++h;
+        }
+        if (h >= heads) {
+          h -= heads;
+          ++t;
+        }
+      }
 #pragma unroll
-          for (int e = 0; e < VEC / 2; ++e) {
-            ca[e] = cs[t][c / 2 + e];
-            sa[e] = sn[t][c / 2 + e];
-          }
-#pragma unroll 2
-          for (int64_t h = h0; h < r.heads; h += step) {
-            V v = *reinterpret_cast<const V*>(x + h * r.x_head + c);
+      for (int e = 0; e < kRotBatch; ++e) {
+        if (at[e] >= count) break;
+        if (c0[e] < p.rotary) {
+          const float* cv = cs[at[e]];
+          const float* sv = sn[at[e]];
+          if constexpr (NEIGHBOURS) {
 #pragma unroll
-            for (int e = 0; e < VEC / 2; ++e) {
-              const float u = (float)v.v[2 * e], w = (float)v.v[2 * e + 1];
-              v.v[2 * e] = (T)(u * ca[e] - w * sa[e]);
-              v.v[2 * e + 1] = (T)(w * ca[e] + u * sa[e]);
+            for (int k = 0; k < VEC / 2; ++k) {
+              const float ca = cv[c0[e] / 2 + k], sa = sv[c0[e] / 2 + k], u = (float)a[e].v[2 * k], w = (float)a[e].v[2 * k + 1];
+              a[e].v[2 * k] = (T)(u * ca - w * sa);
+              a[e].v[2 * k + 1] = (T)(w * ca + u * sa);
+              const float cb = cv[c1[e] / 2 + k], sb = sv[c1[e] / 2 + k], y = (float)b[e].v[2 * k], z = (float)b[e].v[2 * k + 1];
+              b[e].v[2 * k] = (T)(y * cb - z * sb);
+              b[e].v[2 * k + 1] = (T)(z * cb + y * sb);
             }
-            *reinterpret_cast<V*>(out + h * r.out_head + c) = v;
-          }
-        } else {
-          const int c = i * VEC, c0 = INTERLEAVED ? 2 * c : c, c1 = INTERLEAVED ? 2 * c + 1 : c + pairs;
-          float ca[VEC], sa[VEC];
+          } else {
+            const int j = INTERLEAVED ? c0[e] / 2 : c0[e];
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            ca[e] = cs[t][c + e];
-            sa[e] = sn[t][c + e];
-          }
-#pragma unroll 2
-          for (int64_t h = h0; h < r.heads; h += step) {
-            const V u = *reinterpret_cast<const V*>(x + h * r.x_head + c0);
-            const V w = *reinterpret_cast<const V*>(x + h * r.x_head + c1);
-            V o, n;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              const float a = (float)u.v[e], d = (float)w.v[e];
-              o.v[e] = (T)(a * ca[e] - d * sa[e]);
-              n.v[e] = (T)(d * ca[e] + a * sa[e]);
+            for (int k = 0; k < VEC; ++k) {
+              const float ca = cv[j + k], sa = sv[j + k], u = (float)a[e].v[k], w = (float)b[e].v[k];
+              a[e].v[k] = (T)(u * ca - w * sa);
+              b[e].v[k] = (T)(w * ca + u * sa);
             }
-            *reinterpret_cast<V*>(out + h * r.out_head + c0) = o;
-            *reinterpret_cast<V*>(out + h * r.out_head + c1) = n;
           }
         }
+        *reinterpret_cast<V*>(dst[e] + c0[e]) = a[e];
+        *reinterpret_cast<V*>(dst[e] + c1[e]) = b[e];
       }
     }
   }
