@@ -218,21 +218,24 @@ int fp4_combine(const GemmArgs& p, int epi, int splits, hipStream_t s) {
 // ---- which kernel ------------------------------------------------------------
 // kFp4Skinny, kFp4Rows: above.  kFp4Mid: the mid-size kernel (gemm_kg.hip), tiles
 // of 64, 128 or 192 x 128, whole units of 128 k.  kFp4Large: the 8-wave kernel
-// (gemm8.h), 256 or 128 x 256.
+// (gemm8.h), 128 x 256.  Before it, rows [0, head) on the 8-wave kernel's 256 x 256
+// tiles: where those make whole rounds of the CUs and another kernel takes the
+// rows left over for less than one more round.
 enum Fp4Kernel { kFp4Skinny, kFp4Rows, kFp4Mid, kFp4Large };
 struct Fp4Plan {
-  int kernel;
-  int bm;       // rows of a tile
-  int splits;   // K ranges
-  int k_split;  // k of one (a multiple of 128)
+  int64_t head;  // a multiple of 256, or M: all rows
+  int kernel;    // of the rows from head on
+  int bm;        // rows of its tiles
+  int splits;    // its K ranges (1 with a head)
+  int k_split;   // k of one (a multiple of 128)
 };
 
-// Modelled times (us).  Mid-size: a round of one workgroup per CU costs `unit` us
-// per 128 k, the L2s deliver 13 TB/s of tile operands at most, 4 us of launch,
-// first loads and epilogue, a split's second launch and its partials.  Against
-// measured: 1296 x 4096 -> 4096 tiles of 192 / 128 / 64 rows 39 / 53 / 57 against
-// 40 / 56 / 56, 68 x 2048 -> 8192 64 rows 13 / 12, 68 x 8192 -> 2048 in 8 splits 64
-// rows 14 / 16, 256 x 4096 -> 8192 22 / 21, 1296 x 4096 -> 12320 192 rows 108 / 112.
+// Modelled times (us) of one launch.  Mid-size: a round of one workgroup per CU
+// costs `unit` us per 128 k, the L2s deliver 13 TB/s of tile operands at most, 4 us
+// of launch, first loads and epilogue, a split's second launch and its partials.
+// Against measured: 1296 x 4096 -> 4096 tiles of 192 / 128 / 64 rows 39 / 53 / 57
+// against 40 / 56 / 56, 68 x 2048 -> 8192 64 rows 13 / 12, 68 x 8192 -> 2048 in 8
+// splits 64 rows 14 / 16, 256 x 4096 -> 8192 22 / 21.
 static double fp4_mid_time(double M, double N, double K, int bm, int splits) {
   const double unit = bm == 64 ? 0.55 : (bm == 128 ? 0.77 : 1.08);
   const double wgs = ceil(M / bm) * ceil(N / 128) * splits, units = K / 128 / splits;
@@ -247,21 +250,52 @@ static double fp4_mid_time(double M, double N, double K, int bm, int splits) {
 // 4096 -> 4096 in one round 79; 3456 x 16384 -> 4096 287; 1296 x 4096 -> 4096 in
 // 128-row tiles 50).
 static double fp4_large_time(double M, double N, double K, int bm) {
-  const double units = ceil(K / 128);
-  if (bm == 128) return 4.0 + ceil(ceil(M / 128) * ceil(N / 256) / 256) * units * 1.5;
-  const int r0 = g8_split_rows((int)M, (int)N);
-  double t = ceil(ceil(r0 / 256.0) * ceil(N / 256) / 256) * 2.3;
-  if (r0 < M) t += ceil(ceil((M - r0) / 128) * ceil(N / 256) / 256) * 1.5;
-  return 4.0 + t * units;
+  return 4.0 + ceil(ceil(M / bm) * ceil(N / 256) / 256) * ceil(K / 128) * (bm == 256 ? 2.3 : 1.5);
+}
+// Up to 16 rows: every workgroup reads all activations (16 x 4096 -> 4096 8.2 us,
+// 8 x 2048 -> 8192 7.3, 1 x 4096 -> 16384 13.8).
+static double fp4_skinny_time(double M, double N, double K) {
+  const double weights = N * K * 0.53 / 3.6e6, rows = N / 4096 * M * K * 2 / 47e3;
+  return 4.0 + (weights > rows ? weights + 0.5 * rows : rows + 0.5 * weights);
+}
+
+// The fastest single launch (or, where `split`, K ranges and a combining one)
+static double fp4_one(int64_t M, int64_t N, int64_t K, bool split, Fp4Plan* pl) {
+  const int whole = (int)((K + 127) / 128 * 128);
+  double best = fp4_large_time(M, N, K, 128);
+  *pl = {0, kFp4Large, 128, 1, whole};
+  if (M <= 16) {
+    const double t = fp4_skinny_time(M, N, K);
+    if (t < best) {
+      best = t;
+      *pl = {0, kFp4Skinny, 16, 1, whole};
+    }
+  }
+  if (K % 128 != 0) return best;
+  const int64_t units = K / 128;
+  for (int bm = 64; bm <= 192; bm += 64) {
+    const int64_t tiles = ((M + bm - 1) / bm) * ((N + 127) / 128);
+    for (int s = 1; s <= (split ? 16 : 1); ++s) {
+      // splits: whole units, at least 256 k each, within one round of the CUs,
+      // and 10 % faster (a launch and a workspace more)
+      if (s > 1 && (units % s || units / s < 2 || tiles * s > 256)) continue;
+      const double t = fp4_mid_time(M, N, K, bm, s);
+      if (t < best * (s > 1 ? 0.9 : 1.0)) {
+        best = t;
+        *pl = {0, kFp4Mid, bm, s, (int)(K / s)};
+      }
+    }
+  }
+  return best;
 }
 
 static Fp4Plan fp4_plan(int64_t M, int64_t N, int64_t K) {
-  Fp4Plan pl = {kFp4Skinny, 16, 1, (int)((K + 127) / 128 * 128)};
-  // beyond that many activations (each workgroup reads all of them) splitting
-  // K over workgroups is faster: 16 x 16384 -> 4096 25 us, 18 on the mid-size
-  // kernel; 1 x 16384 -> 4096 13.7 against 16.6
-  if (M <= 16 && (M * K <= 131072 || K % 128 != 0)) return pl;
+  Fp4Plan pl;
   if (K % 128 != 0 && M <= 64) {
+    // half a scale word past the last unit: neither the mid-size kernel nor,
+    // for so few rows, the 8-wave kernel
+    pl = {0, kFp4Skinny, 16, 1, (int)((K + 127) / 128 * 128)};
+    if (M <= 16) return pl;
     pl.kernel = kFp4Rows;
     pl.bm = M <= 32 ? 32 : 64;
     const int64_t tiles = (N + kFrBN - 1) / kFrBN, units = (K + 127) / 128;
@@ -273,28 +307,20 @@ static Fp4Plan fp4_plan(int64_t M, int64_t N, int64_t K) {
     pl.splits = (int)((units + per - 1) / per);
     return pl;
   }
-  pl.kernel = kFp4Large;
-  pl.bm = 128;
-  double best = fp4_large_time(M, N, K, 128);
-  const double t256 = fp4_large_time(M, N, K, 256);
-  if (t256 < best) {
-    best = t256;
-    pl.bm = 256;
+  double best = fp4_one(M, N, K, true, &pl);
+  if (M <= 128) return pl;
+  const double all = fp4_large_time(M, N, K, 256);
+  if (all < best) {
+    best = all;
+    pl = {M, kFp4Large, 128, 1, (int)((K + 127) / 128 * 128)};
   }
-  if (K % 128 == 0) {
-    const int64_t units = K / 128;
-    for (int bm = 64; bm <= 192; bm += 64) {
-      const int64_t tiles = ((M + bm - 1) / bm) * ((N + 127) / 128);
-      for (int s = 1; s <= 16; ++s) {
-        // splits: whole units, at least 256 k each, within one round of the CUs,
-        // and 10 % faster (a launch and a workspace more)
-        if (s > 1 && (units % s || units / s < 2 || tiles * s > 256)) continue;
-        const double t = fp4_mid_time(M, N, K, bm, s);
-        if (t < best * (s > 1 ? 0.9 : 1.0)) {
-          best = t;
-          pl = {kFp4Mid, bm, s, (int)(K / s)};
-        }
-      }
+  for (int64_t b = (M - 1) / 256, tries = 0; b >= 1 && tries < 16; --b, ++tries) {
+    Fp4Plan rest;
+    const double t = fp4_large_time(256 * b, N, K, 256) + fp4_one(M - 256 * b, N, K, false, &rest);
+    if (t < 0.97 * best) {
+      best = t;
+      pl = rest;
+      pl.head = 256 * b;
     }
   }
   return pl;
@@ -323,17 +349,8 @@ static void fp4_launch(const GemmArgs& p, const Fp4Plan& pl, hipStream_t s) {
     }
     kg_launch(B_MXFP4, a, EPI, pl.bm, pl.splits, s);
   } else if constexpr (EPI != kEpiPartial) {
-    if (pl.kernel == kFp4Skinny) {
-      fp4_skinny_kernel<EPI><<<(p.N + 15) / 16, kSkWaves * 64, 0, s>>>(p);
-      return;
-    }
-    const int r0 = pl.bm == 256 ? g8_split_rows(p.M, p.N) : 0;
-    if (r0 > 0) {
-      GemmArgs top = p;
-      top.M = r0;
-      launch_g8<B_MXFP4, EPI>(top, s);
-    }
-    if (r0 < p.M) launch_g8<B_MXFP4, EPI, 128>(rows_from(p, r0), s);
+    if (pl.kernel == kFp4Skinny) fp4_skinny_kernel<EPI><<<(p.N + 15) / 16, kSkWaves * 64, 0, s>>>(p);
+    else launch_g8<B_MXFP4, EPI, 128>(p, s);
   }
 }
 
@@ -366,33 +383,53 @@ extern "C" int ltx_gemm_mxfp4_bf16(const void* A, int64_t lda, const uint8_t* Wq
                         sigmoid_from);
   hipStream_t s = (hipStream_t)stream;
   const int epi = epilogue & 0xff;
-  // The mid-size and 8-wave kernels address their operands by 31-bit byte
-  // offsets: longer activations go in pieces of whole tiles, and what does not
-  // fit them otherwise (a weight of 2 GiB) to the few-row tiles.
-  int64_t piece = M;
-  if (pl.kernel == kFp4Mid || pl.kernel == kFp4Large) {
-    const int64_t lim = (int64_t)1 << 31;
-    const bool w_fits = N <= (lim - 1) / ldw && ld_scale <= (lim - 1) / 4 / ((K + 127) / 128);
-    const int64_t rows = (lim - 1) / (lda * 2) / 768 * 768;  // tiles of 64, 128, 192, 256 rows
-    if (w_fits && (M <= (lim - 1) / (lda * 2) || (rows > 0 && pl.splits == 1))) {
-      if (M > (lim - 1) / (lda * 2)) piece = rows;
-    } else {
+  if (pl.splits > 1) {
+    // (the mid-size kernel addresses its operands by 31-bit byte offsets)
+    const int64_t lim = ((int64_t)1 << 31) - 1;
+    if (pl.kernel == kFp4Mid && (M > lim / (lda * 2) || N > lim / ldw || ld_scale > lim / 4 / ((K + 127) / 128))) {
       pl.kernel = kFp4Rows;
       pl.bm = 64;
     }
-  }
-  if (pl.splits > 1) {
     p.partial = workspace;
     fp4_launch<kEpiPartial>(p, pl, s);
     const int e = ltx_launch_status();
     return e != LTX_OK ? e : fp4_combine(p, epi, pl.splits, s);
   }
-  for (int64_t r0 = 0; r0 < M; r0 += piece) {
-    GemmArgs part = rows_from(p, r0);
-    part.M = (int)(M - r0 < piece ? M - r0 : piece);
-    fp4_epilogue(epi, [&](auto e) { fp4_launch<decltype(e)::value>(part, pl, s); });
-    const int e = ltx_launch_status();
-    if (e != LTX_OK) return e;
+  // rows [r0, r1) on a kernel: the mid-size and 8-wave kernels in pieces of whole
+  // tiles below 2 GiB of activations; what does not fit them otherwise (a weight
+  // of 2 GiB) on the few-row tiles
+  auto run = [&](int64_t r0, int64_t r1, bool head) {
+    int64_t piece = r1 - r0;
+    Fp4Plan q = pl;
+    bool large = head;
+    if (head || q.kernel == kFp4Mid || q.kernel == kFp4Large) {
+      const int64_t lim = ((int64_t)1 << 31) - 1, rows = lim / (lda * 2);
+      const bool w_fits = N <= lim / ldw && ld_scale <= lim / 4 / ((K + 127) / 128);
+      if (!w_fits || (piece > rows && rows < 768)) {
+        q.kernel = kFp4Rows;
+        q.bm = 64;
+        q.splits = 1;
+        q.k_split = (int)((K + 127) / 128 * 128);
+        large = false;
+      } else if (piece > rows) {
+        piece = rows / 768 * 768;  // tiles of 64, 128, 192, 256 rows
+      }
+    }
+    for (; r0 < r1; r0 += piece) {
+      GemmArgs part = rows_from(p, r0);
+      part.M = (int)(r1 - r0 < piece ? r1 - r0 : piece);
+      fp4_epilogue(epi, [&](auto e) {
+        if (large) launch_g8<B_MXFP4, decltype(e)::value>(part, s);
+        else fp4_launch<decltype(e)::value>(part, q, s);
+      });
+      const int e = ltx_launch_status();
+      if (e != LTX_OK) return e;
+    }
+    return LTX_OK;
+  };
+  if (pl.head > 0) {
+    const int e = run(0, pl.head, true);
+    if (e != LTX_OK || pl.head >= M) return e;
   }
-  return LTX_OK;
+  return run(pl.head, M, false);
 }

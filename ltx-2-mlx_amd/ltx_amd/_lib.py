@@ -140,6 +140,8 @@ ERR_SCRATCH_LIMIT = -5
 ATTN_NOALLOC_SCRATCH_BYTES = 32 << 20
 
 _LIB: ctypes.CDLL | None = None
+_current_device = getattr(torch._C, "_cuda_getDevice", None)  # (None: a torch without a GPU backend)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def lib() -> ctypes.CDLL:
@@ -193,10 +195,10 @@ def launch(device: int, name: str, *args) -> int:
     """Status of an entry point, called with ``device`` current (a launch goes
     to the current device) and that device's current stream as last argument."""
     fn = getattr(_LIB or lib(), name)
-    if device == torch._C._cuda_getDevice():
-        return fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if device == _current_device():
+        return fn(*args, _raw_stream(device))
     with torch.cuda.device(device):
-        return fn(*args, torch._C._cuda_getCurrentRawStream(device))
+        return fn(*args, _raw_stream(device))
 
 
 def same_device(*tensors: torch.Tensor | None) -> int:

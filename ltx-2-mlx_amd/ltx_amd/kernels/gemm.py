@@ -465,8 +465,8 @@ def quantize_rows_mxfp4(x: torch.Tensor) -> Mx4Rows:
     xv, ldx = _lib.row_view(x, k)
     m = x.numel() // k if k else 0
     ld = (m + 3) // 4 * 4
-    codes = torch.empty((m, k // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(((k + 127) // 128, ld), dtype=torch.int32, device=x.device)
+    codes = x.new_empty((m, k // 2), dtype=torch.uint8)
+    scales = x.new_empty(((k + 127) // 128, ld), dtype=torch.int32)
     if m and k:
         st = _lib.launch(_lib.same_device(xv), "ltx_quantize_mxfp4", xv.data_ptr(), dtype, ldx, m, k,
                          codes.data_ptr(), k // 2, scales.data_ptr(), ld)
@@ -479,7 +479,7 @@ def dequantize_rows_mxfp4(rows: Mx4Rows) -> torch.Tensor:
     """bf16 (M, K) values of MXFP4 rows, exact."""
     codes, scales = rows.codes, rows.scales
     m, k, ldq, lds = _check_mxfp4("dequantize_rows_mxfp4", codes, scales)
-    out = torch.empty((m, k), dtype=torch.bfloat16, device=codes.device)
+    out = codes.new_empty((m, k), dtype=torch.bfloat16)
     if m and k:
         st = _lib.launch(_lib.same_device(codes, scales), "ltx_dequantize_mxfp4_bf16", codes.data_ptr(), ldq,
                          scales.data_ptr(), lds, m, k, out.data_ptr(), k)
@@ -515,7 +515,7 @@ def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int
     if kx != k:
         raise ValueError(f"activations have K={kx}, the weight {k}")
     if out is None:
-        out = src.new_empty(shape) if not quantised else torch.empty(shape, dtype=torch.bfloat16, device=src.device)
+        out = src.new_empty(shape, dtype=torch.bfloat16)
         ldc = n
     else:
         if out.dtype is not torch.bfloat16 or out.shape != shape:
@@ -552,7 +552,7 @@ def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int
     name = "ltx_gemm_mx4_bf16" if quantised else "ltx_gemm_mxfp4_bf16"
     ws_bytes = _mxfp4_workspace_bytes("ltx_gemm_mx4_workspace_bytes" if quantised
                                       else "ltx_gemm_mxfp4_workspace_bytes", m, n, k)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=src.device) if ws_bytes else None
+    ws = src.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     hook = LAUNCH_HOOK
     info = (weight.kind, m, n, k, epilogue)
     if hook is not None:

@@ -134,7 +134,7 @@ _ROTARY_ROWS = struct.Struct("9q").pack  # ltx_rotary_rows: x, its strides, out,
 def _rotary_side(name: str, x: torch.Tensor, out: torch.Tensor | None) -> tuple[bytes, torch.Tensor]:
     shape, st = x.shape, x.stride()
     if out is None:
-        out = x.new_empty(shape)
+        out = torch.empty_like(x)
     elif out.shape != shape or out.dtype is not x.dtype:
         raise ValueError(f"{name}'s out must be {x.dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
     so = out.stride()
