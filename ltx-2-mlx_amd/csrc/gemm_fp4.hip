@@ -236,26 +236,28 @@ struct Fp4Plan {
 // Against measured: 1296 x 4096 -> 4096 tiles of 192 / 128 / 64 rows 39 / 53 / 57
 // against 40 / 56 / 56, 68 x 2048 -> 8192 64 rows 13 / 12, 68 x 8192 -> 2048 in 8
 // splits 64 rows 14 / 16, 256 x 4096 -> 8192 22 / 21.
-static double fp4_mid_time(double M, double N, double K, int bm, int splits) {
+static inline int64_t fp4_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+static double fp4_mid_time(int64_t M, int64_t N, int64_t K, int bm, int splits) {
   const double unit = bm == 64 ? 0.55 : (bm == 128 ? 0.77 : 1.08);
-  const double wgs = ceil(M / bm) * ceil(N / 128) * splits, units = K / 128 / splits;
-  double t = ceil(wgs / 256) * units * unit;
-  const double bytes = wgs * units * 128 * (2.0 * bm + 64);
+  const int64_t wgs = fp4_up(M, bm) * fp4_up(N, 128) * splits;
+  const double units = (double)(K / 128) / splits;
+  double t = (double)fp4_up(wgs, 256) * units * unit;
+  const double bytes = (double)wgs * units * 128 * (2.0 * bm + 64);
   if (bytes / 13e6 > t) t = bytes / 13e6;
   t += 4.0;
-  if (splits > 1) t += 3.5 + M * N * splits * 8 / 3.5e6;
+  if (splits > 1) t += 3.5 + (double)(M * N) * splits * 8 / 3.5e6;
   return t;
 }
 // 8-wave: a round of 256-row tiles 2.3 us per 128 k, of 128-row tiles 1.5 (3456 x
 // 4096 -> 4096 in one round 79; 3456 x 16384 -> 4096 287; 1296 x 4096 -> 4096 in
 // 128-row tiles 50).
-static double fp4_large_time(double M, double N, double K, int bm) {
-  return 4.0 + ceil(ceil(M / bm) * ceil(N / 256) / 256) * ceil(K / 128) * (bm == 256 ? 2.3 : 1.5);
+static double fp4_large_time(int64_t M, int64_t N, int64_t K, int bm) {
+  return 4.0 + (double)(fp4_up(fp4_up(M, bm) * fp4_up(N, 256), 256) * fp4_up(K, 128)) * (bm == 256 ? 2.3 : 1.5);
 }
 // Up to 16 rows: every workgroup reads all activations (16 x 4096 -> 4096 8.2 us,
 // 8 x 2048 -> 8192 7.3, 1 x 4096 -> 16384 13.8).
-static double fp4_skinny_time(double M, double N, double K) {
-  const double weights = N * K * 0.53 / 3.6e6, rows = N / 4096 * M * K * 2 / 47e3;
+static double fp4_skinny_time(int64_t M, int64_t N, int64_t K) {
+  const double weights = (double)(N * K) * 0.53 / 3.6e6, rows = (double)N / 4096 * (double)(M * K) * 2 / 47e3;
   return 4.0 + (weights > rows ? weights + 0.5 * rows : rows + 0.5 * weights);
 }
 
@@ -278,7 +280,8 @@ static double fp4_one(int64_t M, int64_t N, int64_t K, bool split, Fp4Plan* pl) 
     for (int s = 1; s <= (split ? 16 : 1); ++s) {
       // splits: whole units, at least 256 k each, within one round of the CUs,
       // and 10 % faster (a launch and a workspace more)
-      if (s > 1 && (units % s || units / s < 2 || tiles * s > 256)) continue;
+      if (s > 1 && (tiles * s > 256 || units / s < 2)) break;
+      if (units % s) continue;
       const double t = fp4_mid_time(M, N, K, bm, s);
       if (t < best * (s > 1 ? 0.9 : 1.0)) {
         best = t;
@@ -307,6 +310,7 @@ static Fp4Plan fp4_plan(int64_t M, int64_t N, int64_t K) {
     pl.splits = (int)((units + per - 1) / per);
     return pl;
   }
+  if (M <= 16 && M * K <= 16384) return {0, kFp4Skinny, 16, 1, (int)K};  // a few rows: the launch, not the choice, counts
   double best = fp4_one(M, N, K, true, &pl);
   if (M <= 128) return pl;
   const double all = fp4_large_time(M, N, K, 256);

@@ -331,16 +331,16 @@ struct Mx4Plan {
 // 48 / 66 against 35 / 43 / 55 / 70, 1296 x 4096 -> 12320 60 / 58 / 59 / 71 against 58 /
 // 55 / 60 / 72, 68 x 8192 -> 2048 64 x 128 in 4 splits 11 / 11, 256 x 4096 -> 8192 64 x
 // 128 11 / 11, 6144 x 1024 -> 16384 256 x 256 77 / 79.
-static double mx4_time(double M, double N, int bm, int bn, int splits, double per) {
-  const double wgs = ceil(M / bm) * ceil(N / bn) * splits;
+static double mx4_time(int64_t M, int64_t N, int bm, int bn, int splits, double per) {
+  const double wgs = (double)(((M + bm - 1) / bm) * ((N + bn - 1) / bn) * splits);
   double fixed = 2.2, idle = 0.37, full = 0.40;
   if (bm == 256 && bn == 256) fixed = 5.5, idle = 1.15, full = 1.75;
   else if (bm == 256) fixed = 4.3, idle = 0.80, full = 0.94;
   else if (bm == 128) fixed = 2.6, idle = 0.49, full = 0.57;
-  const double rounds = floor(wgs / 256), rest = wgs / 256 - rounds;
+  const double rounds = (double)(int64_t)(wgs / 256), rest = wgs / 256 - rounds;
   double t = 2.2 + rounds * (fixed + per * full);
   if (rest > 0) t += fixed + per * (idle + (full - idle) * rest);
-  if (splits > 1) t += 2.5 + M * N * splits * 8 / 4e6;
+  if (splits > 1) t += 2.5 + (double)(M * N) * splits * 8 / 4e6;
   return t;
 }
 
@@ -356,7 +356,7 @@ static Mx4Plan mx4_plan(int64_t M, int64_t N, int64_t K) {
       if (want > 1 && (units / want < 2 || tiles * want > 256)) break;
       const int64_t per = (units + want - 1) / want;
       const int s = (int)((units + per - 1) / per);
-      const double us = mx4_time((double)M, (double)N, t[0], t[1], s, (double)per);
+      const double us = mx4_time(M, N, t[0], t[1], s, (double)per);
       if (us < best * (s > 1 ? 0.9 : 1.0)) {
         best = us;
         pl = {t[0], t[1], s, (int)(per * 256)};

@@ -426,7 +426,8 @@ def _check_mxfp4(what: str, codes: torch.Tensor, scales: torch.Tensor) -> tuple[
         ldc, unit = codes.stride()
         lds, sunit = scales.stride()
         if words * 64 >= half and ld >= rows and unit == sunit == 1:
-            return rows, half * 2, ldc, lds
+            # (the stride of an axis of one entry says nothing)
+            return rows, half * 2, ldc if rows > 1 else half, lds if words > 1 else (ld + 3) // 4 * 4
     raise ValueError(f"{what}: MXFP4 operands are code bytes (rows, K/2) uint8 and scale words (ceil(K/128), >= rows) "
                      f"int32 of unit column stride, got {codes.dtype} {tuple(codes.shape)} and "
                      f"{None if scales is None else (scales.dtype, tuple(scales.shape))}")
@@ -464,6 +465,10 @@ def quantize_rows_mxfp4(x: torch.Tensor) -> Mx4Rows:
         raise ValueError(f"K={k} is not a multiple of 32")
     xv, ldx = _lib.row_view(x, k)
     m = x.numel() // k if k else 0
+    if m == 1:
+        ldx = k  # (the stride of an axis of one entry says nothing)
+    elif ldx < k:  # one row for all
+        xv, ldx = xv.contiguous(), k
     ld = (m + 3) // 4 * 4
     codes = x.new_empty((m, k // 2), dtype=torch.uint8)
     scales = x.new_empty(((k + 127) // 128, ld), dtype=torch.int32)
@@ -508,10 +513,19 @@ def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int
     else:
         if x.dtype is not torch.bfloat16:
             raise TypeError(f"linear expects bf16 or MXFP4 activations, got {x.dtype}")
-        *lead, kx = x.shape
-        src, lda = _lib.row_view(x, kx)
-        xs, shape = None, (*lead, n)
-        m = x.numel() // kx if kx else 0
+        shape, st = x.shape, x.stride()
+        if len(shape) == 2 and st[1] == 1:  # rows of a matrix
+            m, kx = shape
+            src, lda, shape = x, st[0], (m, n)
+        else:
+            *lead, kx = shape
+            src, lda = _lib.row_view(x, kx)
+            m, shape = x.numel() // kx if kx else 0, (*lead, n)
+        if m == 1:
+            lda = kx  # (the stride of an axis of one entry says nothing)
+        elif lda < kx:  # one row for all
+            src, lda = src.contiguous(), kx
+        xs = None
     if kx != k:
         raise ValueError(f"activations have K={kx}, the weight {k}")
     if out is None:
@@ -521,8 +535,9 @@ def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int
         if out.dtype is not torch.bfloat16 or out.shape != shape:
             raise ValueError(f"out must be bf16 {shape}, got {out.dtype} {tuple(out.shape)}")
         ov, ldc = _lib.row_view(out, n)
-        if ov.data_ptr() != out.data_ptr():
+        if ov.data_ptr() != out.data_ptr() or (ldc < n and m > 1):
             raise ValueError("out must be a row-strided view")
+        ldc = ldc if m > 1 else n
     rptr, ldr, gptr = None, 0, None
     if epilogue == EPI_RESIDUAL or epilogue == EPI_RESIDUAL_ROUND:
         if residual is None or gate is None:
@@ -531,8 +546,9 @@ def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int
             raise ValueError(f"residual must be bf16 ({m}, {n}), got {residual.dtype} {tuple(residual.shape)}")
         rv, ldr = _lib.row_view(residual, n)
         rptr = rv.data_ptr()
-        if rptr != residual.data_ptr():
+        if rptr != residual.data_ptr() or (ldr < n and m > 1):
             raise ValueError("residual must be a row-strided view")
+        ldr = ldr if m > 1 else n
         if gate.dtype is not torch.float32 or gate.numel() != n:
             raise ValueError("gate must be fp32 with N elements")
         gate = _lib.flat(gate)

@@ -346,3 +346,57 @@ def test_streams_and_graphs():
         torch.cuda.synchronize()
         for a, b in zip(outs, want):
             assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_rows_whose_strides_say_nothing():
+    """One row under any stride, one row broadcast over many, a vector, one scale
+    word row, a batch of rows."""
+    from ltx_amd.kernels import gemm
+
+    g = torch.Generator(device=DEV).manual_seed(4)
+    col = torch.randn(128, 1, generator=g, device=DEV).bfloat16()
+    w = gemm.make_weight(torch.randn(64, 128, generator=g, device=DEV).bfloat16(), kind="mxfp4")
+    row = col.t()  # (1, 128), strides (1, 1)
+    want = gemm.linear(row.contiguous(), w)
+    assert torch.equal(gemm.linear(row, w), want)
+    assert torch.equal(gemm.linear(row.expand(5, 128), w), want.expand(5, 64))
+    assert torch.equal(gemm.linear(col[:, 0], w), want[0])
+    a, b = gemm.quantize_rows_mxfp4(row), gemm.quantize_rows_mxfp4(row.contiguous())
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales[:, :1], b.scales[:, :1])
+    e = gemm.quantize_rows_mxfp4(row.expand(5, 128))
+    assert torch.equal(e.codes, b.codes.expand(5, 64)) and torch.equal(e.scales[:, :5], b.scales[:, :1].expand(1, 5))
+    many = gemm.linear(e, w)
+    assert torch.equal(many, gemm.linear(b, w).expand(5, 64))
+    out = torch.empty(64, 1, dtype=torch.bfloat16, device=DEV).t()
+    assert torch.equal(gemm.linear(row, w, out=out), want)
+    with pytest.raises(ValueError):
+        gemm.linear(row.expand(5, 128), w, out=out.expand(5, 64))
+    res = torch.randn(64, 1, generator=g, device=DEV).bfloat16().t()
+    gate = torch.randn(64, generator=g, device=DEV)
+    kw = dict(epilogue=gemm.EPI_RESIDUAL, gate=gate)
+    assert torch.equal(gemm.linear(row, w, residual=res, **kw), gemm.linear(row.contiguous(), w,
+                                                                             residual=res.contiguous(), **kw))
+    with pytest.raises(ValueError):
+        gemm.linear(row.expand(5, 128), w, residual=res.expand(5, 64), **kw)
+
+
+@pytest.mark.parametrize("m", [5, 200, 2200])
+def test_misaligned_operands_are_refused(m):
+    from ltx_amd import _lib
+    from ltx_amd.kernels import gemm
+
+    w = gemm.make_weight(torch.randn(64, 128, device=DEV).bfloat16(), kind="mxfp4")
+    buf = torch.zeros(m, 160, dtype=torch.bfloat16, device=DEV)
+    for x in (buf[:, 4:132], torch.zeros(m, 130, dtype=torch.bfloat16, device=DEV)[:, :128]):
+        with pytest.raises(_lib.LtxKernelError):
+            gemm.linear(x, w)
+        with pytest.raises(_lib.LtxKernelError):
+            gemm.quantize_rows_mxfp4(x)
+    with pytest.raises(_lib.LtxKernelError):
+        gemm.linear(buf[:, :128], w, out=torch.empty(m, 68, dtype=torch.bfloat16, device=DEV)[:, 4:])
+    with pytest.raises(_lib.LtxKernelError):  # K of no 128: bf16 rows only
+        v = gemm.make_weight(torch.randn(64, 192, device=DEV).bfloat16(), kind="mxfp4")
+        gemm.linear(gemm.quantize_rows_mxfp4(torch.zeros(m, 192, device=DEV)), v)
+    with pytest.raises(_lib.LtxKernelError):  # N of no 8
+        v = gemm.make_weight(torch.randn(60, 128, device=DEV).bfloat16(), kind="mxfp4")
+        gemm.linear(buf[:, :128], v)
