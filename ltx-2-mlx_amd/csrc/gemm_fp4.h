@@ -34,7 +34,11 @@ __device__ __forceinline__ bf16x4 fp4_branch4(const GemmArgs& p, f32x4 a, f32x4 
     y[e] += bias[e];
     if (EPI == LTX_GEMM_EPI_GELU) y[e] = gelu_tanh(y[e]);
     if (EPI == LTX_GEMM_EPI_SIGMOID2) y[e] = sigmoid2_bf(y[e]);
-    if (SIG) y[e] = n + e >= p.sig_from ? sigmoid2_bf(y[e]) : y[e];
+    if (SIG) {  // both, then a choice: not a branch per value
+      float g = sigmoid2_bf(y[e]);
+      asm("" : "+v"(g));
+      y[e] = n + e >= p.sig_from ? g : y[e];
+    }
     v[e] = (bf16)y[e];
   }
   return v;

@@ -140,6 +140,8 @@ def _rotary_side(name: str, x: torch.Tensor, out: torch.Tensor | None) -> tuple[
     so = out.stride()
     if (st[-1] != 1 or so[-1] != 1) and shape[-1] > 1:
         raise ValueError(f"{name} and its out must have unit channel stride")
+    if 0 in so and any(st == 0 and size > 1 for st, size in zip(so, shape)):
+        raise ValueError(f"{name}'s out has one element in several places")
     if len(st) == 3:
         rows = _ROTARY_ROWS(x.data_ptr(), 0, st[0], st[1], out.data_ptr(), 0, so[0], so[1], shape[1])
     else:

@@ -400,3 +400,19 @@ def test_misaligned_operands_are_refused(m):
     with pytest.raises(_lib.LtxKernelError):  # N of no 8
         v = gemm.make_weight(torch.randn(60, 128, device=DEV).bfloat16(), kind="mxfp4")
         gemm.linear(buf[:, :128], v)
+
+
+@pytest.mark.parametrize("m", [1, 30, 50, 150, 900])
+@pytest.mark.parametrize("k", [64, 192, 320, 1088])
+def test_bytes_past_the_last_block_are_not_used(m, k):
+    """Depths that end inside a scale word: its unused bytes may hold anything."""
+    from ltx_amd.kernels import gemm
+
+    n = 136
+    wc, ws, w = _codes_words(n, k, seed=k)
+    x = torch.randn(m, k, generator=torch.Generator(device=DEV).manual_seed(m), device=DEV).bfloat16()
+    ws[-1] |= -65536  # blocks 2 and 3: NaN scales
+    got = gemm.linear(x, gemm.LinearWeight("mxfp4", wc, ws))
+    _check(got, *_reference(x.double(), w, None, "bias", None, None, None, False))
+    val = gemm.dequantize(gemm.LinearWeight("mxfp4", wc, ws))
+    assert torch.equal(val.double(), w)

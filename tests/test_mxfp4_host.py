@@ -159,7 +159,8 @@ def test_python_refusals_without_a_gpu():
 
     q, pos = torch.zeros(5, 4, 64, dtype=torch.bfloat16), torch.arange(5)
     inv, _ = rope_ops.rotary_frequencies(64, device="cpu")
-    for kw in (dict(layout="quarter"), dict(out=(q.float(), None)), dict(out=(q, q))):
+    for kw in (dict(layout="quarter"), dict(out=(q.float(), None)), dict(out=(q, q)),
+               dict(out=(q[:, :1].expand(5, 4, 64), None))):
         with pytest.raises(ValueError):
             rope_ops.rotary(q, None, pos, inv, **kw)
     for a in ((q[0], None, pos, inv), (q, q[:4], pos, inv), (q, q[..., :32], pos, inv), (q, None, pos[:4], inv),
