@@ -4,7 +4,8 @@ Usage: python ltx-2-mlx_amd/build_lib.py [--jobs N]
 
 Each translation unit is compiled to an object with hipcc, then linked into
 ltx-2-mlx_amd/ltx_amd/libltx_hip.so, which the ctypes loader in
-ltx_amd/_lib.py opens.  The build always recompiles (it is the "does it
+ltx_amd/_lib.py opens; csrc/calls.cpp, the native host side of small calls,
+becomes ltx_amd/_calls.so.  The build always recompiles (it is the "does it
 build" check) and writes to a temporary name first, so a failed build never
 leaves a half-written library behind.
 """
@@ -17,6 +18,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_ROOT = Path(__file__).resolve().parent
@@ -56,14 +58,37 @@ def _compile(src: Path) -> Path:
     return obj
 
 
+def build_calls() -> Path:
+    """ltx_amd/_calls.so: the native host calls (a CPython module on torch's
+    headers; the kernels stay behind the C ABI)."""
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    lib_dir = Path(torch.__file__).parent / "lib"
+    out = LIB_PATH.with_name("_calls.so")
+    tmp = out.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f for p in include_paths() for f in ("-isystem", p)), f"-I{sysconfig.get_paths()['include']}",
+           str(CSRC / "calls.cpp"), "-o", str(tmp), f"-L{lib_dir}", "-ltorch_python", "-ltorch_cpu", "-lc10",
+           f"-Wl,-rpath,{lib_dir}"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed for calls.cpp:\n{proc.stderr}")
+    os.replace(tmp, out)
+    return out
+
+
 def build(jobs: int | None = None, verbose: bool = True) -> Path:
     OBJ_DIR.mkdir(exist_ok=True)
     srcs = sources()
     if not srcs:
         raise RuntimeError(f"no HIP sources under {CSRC}")
-    jobs = jobs or min(len(srcs), os.cpu_count() or 4, 8)
+    jobs = jobs or min(len(srcs) + 1, os.cpu_count() or 4, 8)
     with cf.ThreadPoolExecutor(max_workers=jobs) as pool:
+        calls = pool.submit(build_calls)
         objs = list(pool.map(_compile, srcs))
+        calls.result()
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
     proc = subprocess.run(cmd, capture_output=True, text=True)

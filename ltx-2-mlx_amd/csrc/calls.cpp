@@ -1,0 +1,228 @@
+// Host side of the small MXFP4 and rotary calls: argument checks, output
+// allocation and the launch in one native call.  A product of one row or the
+// rotation of one token takes the GPU 3-6 us; checking the tensors and making
+// the call from Python takes 7-10, from here 4-6.
+//
+// Every function does the usual case only and returns None for anything else
+// (an unusual stride, a type or size that does not fit, a failed launch); the
+// caller's Python path then does the work or raises.  No state is kept.
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <ATen/ATen.h>
+#include <Python.h>
+
+#include "../../include/ltx_hip.h"
+
+namespace {
+
+struct Entry {
+  decltype(&ltx_gemm_mxfp4_bf16) gemm;
+  decltype(&ltx_gemm_mxfp4_workspace_bytes) gemm_ws;
+  decltype(&ltx_gemm_mx4_bf16) mx4;
+  decltype(&ltx_gemm_mx4_workspace_bytes) mx4_ws;
+  decltype(&ltx_quantize_mxfp4) quantize;
+  decltype(&ltx_dequantize_mxfp4_bf16) dequantize;
+  decltype(&ltx_rotary) rotary;
+} entry = {};
+
+PyObject* general() { Py_RETURN_NONE; }
+
+// the tensor of an argument that is exactly one; null otherwise
+const at::Tensor* tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
+bool on(const at::Tensor& t, int64_t device) { return t.is_cuda() && t.get_device() == device; }
+
+at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const at::Tensor& like) {
+  return at::empty(size, like.options().dtype(type));
+}
+
+// dense-column (rows, K / 2) codes with scale words that cover them
+bool mxfp4(const at::Tensor* codes, const at::Tensor* words, int64_t device, int64_t* rows, int64_t* k) {
+  if (!codes || !words || codes->scalar_type() != at::kByte || words->scalar_type() != at::kInt || codes->dim() != 2 ||
+      words->dim() != 2 || !on(*codes, device) || !on(*words, device))
+    return false;
+  *rows = codes->size(0);
+  *k = codes->size(1) * 2;
+  return codes->stride(1) == 1 && words->stride(1) == 1 && codes->stride(0) >= codes->size(1) &&
+         words->stride(0) >= words->size(1) && words->size(0) * 128 >= *k && words->size(1) >= *rows;
+}
+
+// linear(x, x_words or None, codes, words, bias or None, flags, epilogue, residual or None, gate or None,
+//        sigmoid_from or -1, device, stream)
+PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 12 || !entry.gemm) return general();
+  const at::Tensor *x = tensor(a[0]), *xs = tensor(a[1]), *w = tensor(a[2]), *ws = tensor(a[3]), *bias = tensor(a[4]),
+                   *res = tensor(a[7]), *gate = tensor(a[8]);
+  const int64_t flags = PyLong_AsLongLong(a[5]), epi = PyLong_AsLongLong(a[6]), sig = PyLong_AsLongLong(a[9]),
+                device = PyLong_AsLongLong(a[10]);
+  void* stream = PyLong_AsVoidPtr(a[11]);
+  if (PyErr_Occurred()) return nullptr;
+  int64_t N, K, M, kx;
+  if (!x || (!xs && a[1] != Py_None) || (!bias && a[4] != Py_None) || !mxfp4(w, ws, device, &N, &K)) return general();
+  if (xs) {
+    if (!mxfp4(x, xs, device, &M, &kx)) return general();
+  } else {
+    if (x->dim() != 2 || x->scalar_type() != at::kBFloat16 || !on(*x, device) || x->stride(1) != 1) return general();
+    M = x->size(0);
+    kx = x->size(1);
+  }
+  if (kx != K || M < 1 || K < 1 || N < 1) return general();
+  const int64_t width = x->size(1), lda = M > 1 ? x->stride(0) : width;
+  if (lda < width) return general();
+  if (bias && (bias->scalar_type() != at::kFloat || bias->numel() != N || !bias->is_contiguous() || !on(*bias, device)))
+    return general();
+  const bool resid = epi == LTX_GEMM_EPI_RESIDUAL || epi == LTX_GEMM_EPI_RESIDUAL_ROUND;
+  int64_t ldr = 0;
+  if (resid) {
+    if (!res || !gate || res->dim() != 2 || res->scalar_type() != at::kBFloat16 || res->size(0) != M ||
+        res->size(1) != N || res->stride(1) != 1 || !on(*res, device) || gate->scalar_type() != at::kFloat ||
+        gate->numel() != N || !gate->is_contiguous() || !on(*gate, device))
+      return general();
+    ldr = M > 1 ? res->stride(0) : N;
+    if (ldr < N) return general();
+  }
+  at::Tensor out = empty({M, N}, at::kBFloat16, *x);
+  const int64_t bytes = xs ? entry.mx4_ws(M, N, K) : entry.gemm_ws(M, N, K);
+  at::Tensor work;
+  if (bytes > 0) work = empty({bytes}, at::kByte, *x);
+  float* wp = bytes > 0 ? static_cast<float*>(work.data_ptr()) : nullptr;
+  const float* bp = bias ? bias->const_data_ptr<float>() : nullptr;
+  const int64_t ldw = N > 1 ? w->stride(0) : K / 2;
+  const void* rp = resid ? res->const_data_ptr() : nullptr;
+  const float* gp = resid ? gate->const_data_ptr<float>() : nullptr;
+  const int64_t from = sig < 0 ? N : sig;
+  const auto* wc = static_cast<const uint8_t*>(w->const_data_ptr());
+  const auto* wsp = static_cast<const uint32_t*>(ws->const_data_ptr());
+  const int st = xs ? entry.mx4(static_cast<const uint8_t*>(x->const_data_ptr()), lda,
+                                static_cast<const uint32_t*>(xs->const_data_ptr()), xs->stride(0), wc, ldw, wsp,
+                                ws->stride(0), bp, out.data_ptr(), N, M, N, K, (int)(epi | flags), rp, ldr, gp, from, wp,
+                                bytes, stream)
+                    : entry.gemm(x->const_data_ptr(), lda, wc, ldw, wsp, ws->stride(0), bp, out.data_ptr(), N, M, N, K,
+                                 (int)(epi | flags), rp, ldr, gp, from, wp, bytes, stream);
+  return st == LTX_OK ? THPVariable_Wrap(std::move(out)) : general();
+}
+
+// quantize(x, device, stream) -> (codes, words)
+PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 3 || !entry.quantize) return general();
+  const at::Tensor* x = tensor(a[0]);
+  const int64_t device = PyLong_AsLongLong(a[1]);
+  void* stream = PyLong_AsVoidPtr(a[2]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!x || x->dim() != 2 || !on(*x, device) || x->stride(1) != 1) return general();
+  const auto type = x->scalar_type();
+  const int dtype = type == at::kBFloat16 ? 0 : (type == at::kHalf ? 1 : (type == at::kFloat ? 2 : -1));
+  const int64_t rows = x->size(0), k = x->size(1), ldx = rows > 1 ? x->stride(0) : k;
+  if (dtype < 0 || rows < 1 || k < 32 || k % 32 || ldx < k) return general();
+  const int64_t ld = (rows + 3) / 4 * 4;
+  at::Tensor codes = empty({rows, k / 2}, at::kByte, *x), words = empty({(k + 127) / 128, ld}, at::kInt, *x);
+  if (entry.quantize(x->const_data_ptr(), dtype, ldx, rows, k, static_cast<uint8_t*>(codes.data_ptr()), k / 2,
+                     static_cast<uint32_t*>(words.data_ptr()), ld, stream) != LTX_OK)
+    return general();
+  PyObject *c = THPVariable_Wrap(std::move(codes)), *s = THPVariable_Wrap(std::move(words));
+  PyObject* r = c && s ? PyTuple_Pack(2, c, s) : nullptr;
+  Py_XDECREF(c);
+  Py_XDECREF(s);
+  return r;
+}
+
+// dequantize(codes, words, device, stream)
+PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 4 || !entry.dequantize) return general();
+  const at::Tensor *codes = tensor(a[0]), *words = tensor(a[1]);
+  const int64_t device = PyLong_AsLongLong(a[2]);
+  void* stream = PyLong_AsVoidPtr(a[3]);
+  if (PyErr_Occurred()) return nullptr;
+  int64_t rows, k;
+  if (!mxfp4(codes, words, device, &rows, &k) || rows < 1 || k < 1) return general();
+  at::Tensor out = empty({rows, k}, at::kBFloat16, *codes);
+  if (entry.dequantize(static_cast<const uint8_t*>(codes->const_data_ptr()), rows > 1 ? codes->stride(0) : k / 2,
+                       static_cast<const uint32_t*>(words->const_data_ptr()), words->stride(0), rows, k, out.data_ptr(),
+                       k, stream) != LTX_OK)
+    return general();
+  return THPVariable_Wrap(std::move(out));
+}
+
+// one side of a rotation into a new tensor
+bool side(const at::Tensor& x, const at::Tensor& out, ltx_rotary_rows* r) {
+  const int b = x.dim() == 4 ? 1 : 0;
+  if (x.stride(b + 2) != 1) return false;
+  *r = {x.const_data_ptr(), b ? x.stride(0) : 0, x.stride(b), x.stride(b + 1),
+        out.data_ptr(),     b ? out.stride(0) : 0, out.stride(b), out.stride(b + 1), x.size(b + 1)};
+  return true;
+}
+
+// rotary(q, k or None, positions, inv_freq, flags, factor, device, stream) -> (q', k' or None)
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 8 || !entry.rotary) return general();
+  const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *pos = tensor(a[2]), *inv = tensor(a[3]);
+  const int64_t flags = PyLong_AsLongLong(a[4]), device = PyLong_AsLongLong(a[6]);
+  const double factor = PyFloat_AsDouble(a[5]);
+  void* stream = PyLong_AsVoidPtr(a[7]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!q || (!k && a[1] != Py_None) || !pos || !inv || (q->dim() != 3 && q->dim() != 4)) return general();
+  const int64_t dims = q->dim(), batch = dims == 4 ? q->size(0) : 1, tokens = q->size(dims - 3), dh = q->size(dims - 1);
+  const auto type = q->scalar_type(), ptype = pos->scalar_type();
+  const int dtype = type == at::kBFloat16 ? 0 : (type == at::kHalf ? 1 : (type == at::kFloat ? 2 : -1));
+  const int pos_type = ptype == at::kInt ? 0 : (ptype == at::kLong ? 1 : (ptype == at::kFloat ? 2 : (ptype == at::kDouble ? 3 : -1)));
+  if (dtype < 0 || pos_type < 0 || batch < 1 || tokens < 1 || q->size(dims - 2) < 1 || !on(*q, device) ||
+      !on(*pos, device) || !on(*inv, device) || inv->scalar_type() != at::kDouble || inv->dim() != 1 ||
+      !inv->is_contiguous() || !pos->is_contiguous())
+    return general();
+  const bool own = pos->dim() == 2;
+  if ((own && (pos->size(0) != batch || pos->size(1) != tokens)) || (!own && (pos->dim() != 1 || pos->size(0) != tokens)))
+    return general();
+  const int64_t d = 2 * inv->numel();
+  if (d < 2 || d > dh) return general();
+  if (k && (k->dim() != dims || k->scalar_type() != type || !on(*k, device) || k->size(dims - 1) != dh ||
+            k->size(dims - 3) != tokens || (dims == 4 && k->size(0) != batch) || k->size(dims - 2) < 1))
+    return general();
+  at::Tensor oq = empty(q->sizes(), type, *q), ok;
+  if (k) ok = empty(k->sizes(), type, *k);
+  ltx_rotary_rows rq, rk;
+  if (!side(*q, oq, &rq) || (k && !side(*k, ok, &rk))) return general();
+  if (entry.rotary(&rq, k ? &rk : nullptr, dtype, batch, tokens, dh, d, pos->const_data_ptr(), pos_type, own ? tokens : 0,
+                   inv->const_data_ptr<double>(), factor, (int)flags, stream) != LTX_OK)
+    return general();
+  PyObject* po = THPVariable_Wrap(std::move(oq));
+  PyObject* pk = k ? THPVariable_Wrap(std::move(ok)) : (Py_INCREF(Py_None), Py_None);
+  PyObject* r = po && pk ? PyTuple_Pack(2, po, pk) : nullptr;
+  Py_XDECREF(po);
+  Py_XDECREF(pk);
+  return r;
+}
+
+// a C++ exception (no memory for an output) becomes a Python one
+template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
+PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  try {
+    return F(self, a, n);
+  } catch (...) {
+    return general();  // the Python path meets the same condition and raises torch's error for it
+  }
+}
+
+// bind(addresses of the entry points, in the order of Entry)
+PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  void** slots[] = {(void**)&entry.gemm,     (void**)&entry.gemm_ws,    (void**)&entry.mx4,   (void**)&entry.mx4_ws,
+                    (void**)&entry.quantize, (void**)&entry.dequantize, (void**)&entry.rotary};
+  if (n != 7) {
+    PyErr_SetString(PyExc_TypeError, "bind takes seven addresses");
+    return nullptr;
+  }
+  for (int i = 0; i < 7; ++i) *slots[i] = PyLong_AsVoidPtr(a[i]);
+  if (PyErr_Occurred()) return nullptr;
+  Py_RETURN_NONE;
+}
+
+PyMethodDef methods[] = {
+    {"bind", (PyCFunction)(void (*)())bind, METH_FASTCALL, "entry point addresses"},
+    {"linear", (PyCFunction)(void (*)())guarded<linear>, METH_FASTCALL, "an MXFP4 product, or None"},
+    {"quantize", (PyCFunction)(void (*)())guarded<quantize>, METH_FASTCALL, "rows to MXFP4, or None"},
+    {"dequantize", (PyCFunction)(void (*)())guarded<dequantize>, METH_FASTCALL, "MXFP4 rows to bf16, or None"},
+    {"rotary", (PyCFunction)(void (*)())guarded<rotary>, METH_FASTCALL, "rotary positions, or None"},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__calls() { return PyModule_Create(&module); }

@@ -140,13 +140,18 @@ ERR_SCRATCH_LIMIT = -5
 ATTN_NOALLOC_SCRATCH_BYTES = 32 << 20
 
 _LIB: ctypes.CDLL | None = None
+# Native host side of the small MXFP4 and rotary calls (csrc/calls.cpp), once the
+# library is loaded; None where it was not built: their Python path does the same
+CALLS = None
+_CALLS_ENTRIES = ("ltx_gemm_mxfp4_bf16", "ltx_gemm_mxfp4_workspace_bytes", "ltx_gemm_mx4_bf16",
+                  "ltx_gemm_mx4_workspace_bytes", "ltx_quantize_mxfp4", "ltx_dequantize_mxfp4_bf16", "ltx_rotary")
 _current_device = getattr(torch._C, "_cuda_getDevice", None)  # (None: a torch without a GPU backend)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def lib() -> ctypes.CDLL:
     """Return the loaded library, loading it on first call."""
-    global _LIB
+    global _LIB, CALLS
     if _LIB is None:
         if not LIB_PATH.exists():
             raise RuntimeError(
@@ -172,6 +177,11 @@ def lib() -> ctypes.CDLL:
         handle.ltx_gemm_rows_counter_words.restype = _i64
         handle.ltx_status_string.argtypes = [ctypes.c_int]
         handle.ltx_status_string.restype = ctypes.c_char_p
+        if LIB_PATH.with_name("_calls.so").exists():
+            from . import _calls
+
+            _calls.bind(*(ctypes.cast(getattr(handle, name), _vp).value for name in _CALLS_ENTRIES))
+            CALLS = _calls
         _LIB = handle
     return _LIB
 
@@ -199,6 +209,15 @@ def launch(device: int, name: str, *args) -> int:
         return fn(*args, _raw_stream(device))
     with torch.cuda.device(device):
         return fn(*args, _raw_stream(device))
+
+
+def fast_stream(t: torch.Tensor) -> tuple[int, int] | None:
+    """(device, its current stream) for a native host call on t's GPU; None
+    where t is not on the current GPU."""
+    device = t.get_device()
+    if device < 0 or device != _current_device():
+        return None
+    return device, _raw_stream(device)
 
 
 def same_device(*tensors: torch.Tensor | None) -> int:

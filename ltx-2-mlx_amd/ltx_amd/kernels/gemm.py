@@ -457,6 +457,11 @@ def quantize_rows_mxfp4(x: torch.Tensor) -> Mx4Rows:
     """MXFP4 of the rows of x (..., K) bf16, fp16 or fp32 (blocks of 32 along K,
     the OCP rule: X = floor(log2 max|v|) - 2, E2M1 to nearest even, saturated).
     A block with a NaN or an infinity decodes to NaN."""
+    if _lib.CALLS is not None:
+        where = _lib.fast_stream(x)
+        rows = None if where is None else _lib.CALLS.quantize(x, *where)
+        if rows is not None:
+            return Mx4Rows(*rows)
     k = x.shape[-1]
     dtype = _QUANT_DTYPES.get(x.dtype)
     if dtype is None:
@@ -483,6 +488,11 @@ def quantize_rows_mxfp4(x: torch.Tensor) -> Mx4Rows:
 def dequantize_rows_mxfp4(rows: Mx4Rows) -> torch.Tensor:
     """bf16 (M, K) values of MXFP4 rows, exact."""
     codes, scales = rows.codes, rows.scales
+    if _lib.CALLS is not None:
+        where = _lib.fast_stream(codes)
+        out = None if where is None else _lib.CALLS.dequantize(codes, scales, *where)
+        if out is not None:
+            return out
     m, k, ldq, lds = _check_mxfp4("dequantize_rows_mxfp4", codes, scales)
     out = codes.new_empty((m, k), dtype=torch.bfloat16)
     if m and k:
@@ -502,8 +512,18 @@ def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int
                   residual: torch.Tensor | None, gate: torch.Tensor | None,
                   sigmoid_from: int | None) -> torch.Tensor:
     """:func:`linear` on MXFP4 weights, for bf16 or MXFP4 rows.  (Small products
-    are bound by the host: this path reads each tensor's properties once.)"""
+    are bound by the host: the usual call is one native call, csrc/calls.cpp;
+    this path, for all others, reads each tensor's properties once.)"""
     w, scale, bias = weight.w, weight.scale, weight.bias
+    if _lib.CALLS is not None and out is None and LAUNCH_HOOK is None:
+        where = _lib.fast_stream(w)
+        if where is not None:
+            src, xs = (x.codes, x.scales) if isinstance(x, Mx4Rows) else (x, None)
+            y = _lib.CALLS.linear(src, xs, w, scale, bias,
+                                  _lib.GEMM_ROUND_THEN_BIAS if weight.qlinear and bias is not None else 0, epilogue,
+                                  residual, gate, -1 if sigmoid_from is None else max(int(sigmoid_from), 0), *where)
+            if y is not None:
+                return y
     n, k, ldw, ldws = _check_mxfp4("weight", w, scale)
     quantised = isinstance(x, Mx4Rows)
     if quantised:

@@ -167,6 +167,12 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     """
     if layout not in ROTARY_LAYOUTS:
         raise ValueError(f"layout must be one of {ROTARY_LAYOUTS}, got {layout!r}")
+    flags = (_lib.ROTARY_INTERLEAVED if layout == "interleaved" else 0) | (_lib.ROTARY_TRANSPOSE if transpose else 0)
+    if _lib.CALLS is not None and out is None:
+        where = _lib.fast_stream(q)
+        rotated = None if where is None else _lib.CALLS.rotary(q, k, positions, inv_freq, flags, factor, *where)
+        if rotated is not None:
+            return rotated
     shape = q.shape
     dtype = _ROTARY_DTYPES.get(q.dtype)
     if dtype is None or not 3 <= len(shape) <= 4:
@@ -197,7 +203,6 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     device = _lib.same_device(q, k, positions, inv_freq, oq, ok)
     if batch * tokens == 0:
         return oq, ok
-    flags = (_lib.ROTARY_INTERLEAVED if layout == "interleaved" else 0) | (_lib.ROTARY_TRANSPOSE if transpose else 0)
     st = _lib.launch(device, "ltx_rotary", sq, sk, dtype, batch, tokens, dh, d, positions.data_ptr(), pos_type,
                      tokens if len(pos_shape) == 2 else 0, inv_freq.data_ptr(), factor, flags)
     if st:
