@@ -273,8 +273,25 @@ static double fp4_one(int64_t M, int64_t N, int64_t K, bool split, Fp4Plan* pl) 
       *pl = {0, kFp4Skinny, 16, 1, whole};
     }
   }
-  if (K % 128 != 0) return best;
-  const int64_t units = K / 128;
+  const int64_t units = fp4_up(K, 128);
+  if (K % 128 != 0) {
+    // half a scale word past the last unit: not the mid-size kernel's.  Few-row
+    // tiles in any K ranges of at least 512 k (a round of 256 workgroups 1.6 us
+    // per 128 k: 256 x 4096 -> 8192 55, 68 x 8192 -> 2048 in 8 ranges 21)
+    const int bm = M <= 32 ? 32 : 64;
+    const int64_t tiles = fp4_up(M, bm) * fp4_up(N, kFrBN);
+    for (int s = 1; s <= (split ? 32 : 1); ++s) {
+      if (s > 1 && (tiles * s > 512 || units / s < 4)) break;
+      const int64_t per = fp4_up(units, s), n = fp4_up(units, per);
+      double t = 4.0 + (double)(fp4_up(tiles * n, 256) * per) * 1.6;
+      if (n > 1) t += 3.5 + (double)(M * N * n) * 8 / 3.5e6;
+      if (t < best * (n > 1 ? 0.9 : 1.0)) {
+        best = t;
+        *pl = {0, kFp4Rows, bm, (int)n, (int)(per * 128)};
+      }
+    }
+    return best;
+  }
   for (int bm = 64; bm <= 192; bm += 64) {
     const int64_t tiles = ((M + bm - 1) / bm) * ((N + 127) / 128);
     for (int s = 1; s <= (split ? 16 : 1); ++s) {
@@ -294,22 +311,6 @@ static double fp4_one(int64_t M, int64_t N, int64_t K, bool split, Fp4Plan* pl) 
 
 static Fp4Plan fp4_plan(int64_t M, int64_t N, int64_t K) {
   Fp4Plan pl;
-  if (K % 128 != 0 && M <= 64) {
-    // half a scale word past the last unit: neither the mid-size kernel nor,
-    // for so few rows, the 8-wave kernel
-    pl = {0, kFp4Skinny, 16, 1, (int)((K + 127) / 128 * 128)};
-    if (M <= 16) return pl;
-    pl.kernel = kFp4Rows;
-    pl.bm = M <= 32 ? 32 : 64;
-    const int64_t tiles = (N + kFrBN - 1) / kFrBN, units = (K + 127) / 128;
-    int64_t s = 512 / tiles;  // two workgroups per CU, ranges of at least 512 k
-    s = s > units / 4 ? units / 4 : s;
-    s = s > 32 ? 32 : (s < 1 ? 1 : s);
-    const int64_t per = (units + s - 1) / s;
-    pl.k_split = (int)(per * 128);
-    pl.splits = (int)((units + per - 1) / per);
-    return pl;
-  }
   if (M <= 16 && M * K <= 16384) return {0, kFp4Skinny, 16, 1, (int)K};  // a few rows: the launch, not the choice, counts
   double best = fp4_one(M, N, K, true, &pl);
   if (M <= 128) return pl;
