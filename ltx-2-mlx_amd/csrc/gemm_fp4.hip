@@ -107,28 +107,36 @@ __global__ __launch_bounds__(kFrThreads) void fp4_rows_kernel(GemmArgs p, int k_
 // ---- one to 16 rows ----------------------------------------------------------
 // Bound by latency and the weight bytes: one launch, no workspace, a wave's
 // loads of up to 512 k issued before their first use.  A workgroup computes 16
-// columns; its waves split K, each streaming its range of the codes (and the
+// columns (NB times 16); its waves split K, each streaming its range of the codes (and the
 // activations, which the L2 holds) straight to registers, and meet once
-// through LDS, in wave order.  Weights from HBM: 1 x 4096 -> 4096 6.0 us (10.8 in 8
+// through LDS, in wave order.  NB = 2: 32 columns, half the reads of the
+// activations, where that leaves workgroups for every CU.  Weights from HBM: 1 x 4096 -> 4096 6.0 us (10.8 in 8
 // K ranges and a combining launch of the few-row tiles, 11.2 in 4 of the
 // mid-size kernel; a launch that does next to nothing takes 4.0), 1 x 4096 ->
-// 16384 13.8, 16 x 4096 -> 4096 8.2.  Holding the next 512 k in flight as well cost
+// 16384 12.5, 16 x 4096 -> 4096 8.7.  Holding the next 512 k in flight as well cost
 // more in occupancy than it gave (1 x 4096 -> 16384 16.9); 16 waves are no faster.
 constexpr int kSkWaves = 8;
 
-template <int EPI>
+template <int NB, int EPI>
 __global__ __launch_bounds__(kSkWaves * 64) void fp4_skinny_kernel(GemmArgs p) {
-  __shared__ __attribute__((aligned(16))) f32x4 part[kSkWaves][64];
+  __shared__ __attribute__((aligned(16))) f32x4 part[kSkWaves][NB][64];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, q = lane >> 4;
-  const int n0 = (int)blockIdx.x * 16;
-  int gn = n0 + r16;  // columns past N re-read the last one, rows past M the last row
-  gn = gn < p.N ? gn : p.N - 1;
-  const uint8_t* wrow = (const uint8_t*)p.B + (int64_t)gn * p.ldb + q * 16;
-  const uint32_t* srow = (const uint32_t*)p.bscale + gn;
+  const int n0 = (int)blockIdx.x * (16 * NB);
+  const uint8_t* wrow[NB];
+  const uint32_t* srow[NB];
+#pragma unroll
+  for (int c = 0; c < NB; ++c) {
+    int gn = n0 + c * 16 + r16;  // columns past N re-read the last one, rows past M the last row
+    gn = gn < p.N ? gn : p.N - 1;
+    wrow[c] = (const uint8_t*)p.B + (int64_t)gn * p.ldb + q * 16;
+    srow[c] = (const uint32_t*)p.bscale + gn;
+  }
   const bf16* xrow = p.A + (int64_t)(r16 < p.M ? r16 : p.M - 1) * p.lda + q * 32;
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 acc[NB];
+#pragma unroll
+  for (int c = 0; c < NB; ++c) acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   // U units of 128 k from unit u on.  HALF: only the first 64 k of one exist; the
   // upper quarters take the lower ones' codes, with scale 1, and zeros for x
@@ -137,13 +145,15 @@ __global__ __launch_bounds__(kSkWaves * 64) void fp4_skinny_kernel(GemmArgs p) {
     constexpr bool HALF = decltype(hc)::value;
     const bool out = HALF && q >= 2;
     const int back = out ? 64 : 0;  // in k
-    u32x4 w[U];
-    uint32_t sc[U];
+    u32x4 w[U][NB];
+    uint32_t sc[U][NB];
 #pragma unroll
-    for (int b = 0; b < U; ++b) {
-      w[b] = *reinterpret_cast<const u32x4*>(wrow + (u + b) * 64 - back / 2);
-      sc[b] = srow[(int64_t)(u + b) * p.ld_scale];
-    }
+    for (int b = 0; b < U; ++b)
+#pragma unroll
+      for (int c = 0; c < NB; ++c) {
+        w[b][c] = *reinterpret_cast<const u32x4*>(wrow[c] + (u + b) * 64 - back / 2);
+        sc[b][c] = srow[c][(int64_t)(u + b) * p.ld_scale];
+      }
     bf16x8 x[U][4];
 #pragma unroll
     for (int b = 0; b < U; ++b)
@@ -153,12 +163,14 @@ __global__ __launch_bounds__(kSkWaves * 64) void fp4_skinny_kernel(GemmArgs p) {
         if (out) x[b][j] = bf16x8{};
       }
 #pragma unroll
-    for (int b = 0; b < U; ++b) {
-      const float s = out ? 1.0f : e8m0_to_f32_valu((sc[b] >> (8 * q)) & 0xffu);
+    for (int b = 0; b < U; ++b)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4x8_bf16(w[b][j], s), x[b][j], acc, 0, 0, 0);
-    }
+      for (int c = 0; c < NB; ++c) {
+        const float s = out ? 1.0f : e8m0_to_f32_valu((sc[b][c] >> (8 * q)) & 0xffu);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4x8_bf16(w[b][c][j], s), x[b][j], acc[c], 0, 0, 0);
+      }
   };
   const int units = p.K >> 7;
   int u = units * wave / kSkWaves;
@@ -175,14 +187,15 @@ __global__ __launch_bounds__(kSkWaves * 64) void fp4_skinny_kernel(GemmArgs p) {
   if (u < end) run(u, c1, whole);
   if ((p.K & 64) && wave == kSkWaves - 1) run(units, c1, std::true_type{});
 
-  part[wave][lane] = acc;
+#pragma unroll
+  for (int c = 0; c < NB; ++c) part[wave][c][lane] = acc[c];
   __syncthreads();
-  if (tid >= 64) return;
-  const int n = n0 + 4 * q;  // N % 8 == 0: four columns inside or outside
-  f32x4 a = part[0][lane];
+  if (wave >= NB) return;
+  const int n = n0 + wave * 16 + 4 * q;  // N % 8 == 0: four columns inside or outside
+  f32x4 a = part[0][wave][lane];
 #pragma unroll
   for (int z = 1; z < kSkWaves; ++z) {
-    const f32x4 b = part[z][lane];
+    const f32x4 b = part[z][wave][lane];
 #pragma unroll
     for (int e = 0; e < 4; ++e) a[e] += b[e];
   }
@@ -225,7 +238,7 @@ enum Fp4Kernel { kFp4Skinny, kFp4Rows, kFp4Mid, kFp4Large };
 struct Fp4Plan {
   int64_t head;  // a multiple of 256, or M: all rows
   int kernel;    // of the rows from head on
-  int bm;        // rows of its tiles
+  int bm;        // rows of its tiles (kFp4Skinny: columns of a workgroup)
   int splits;    // its K ranges (1 with a head)
   int k_split;   // k of one (a multiple of 128)
 };
@@ -254,10 +267,13 @@ static double fp4_mid_time(int64_t M, int64_t N, int64_t K, int bm, int splits) 
 static double fp4_large_time(int64_t M, int64_t N, int64_t K, int bm) {
   return 4.0 + (double)(fp4_up(fp4_up(M, bm) * fp4_up(N, 256), 256) * fp4_up(K, 128)) * (bm == 256 ? 2.3 : 1.5);
 }
-// Up to 16 rows: every workgroup reads all activations (16 x 4096 -> 4096 8.2 us,
-// 8 x 2048 -> 8192 7.3, 1 x 4096 -> 16384 13.8).
+// Up to 16 rows: every workgroup reads all activations; 32 columns each where
+// that leaves one for every CU (16 / 32 columns: 16 x 4096 -> 12320 22.5 / 15.3 us,
+// 4 x 4096 -> 16384 15.9 / 13.4, 1 x 2048 -> 8192 5.9 / 5.9, 16 x 4096 -> 4096 8.7 / 9.4,
+// 1 x 16384 -> 4096 14.8 / 19.9).
+static int fp4_skinny_cols(int64_t N) { return N >= 32 * 256 ? 32 : 16; }
 static double fp4_skinny_time(int64_t M, int64_t N, int64_t K) {
-  const double weights = (double)(N * K) * 0.53 / 3.6e6, rows = (double)N / 4096 * (double)(M * K) * 2 / 47e3;
+  const double weights = (double)(N * K) * 0.53 / 3.6e6, rows = (double)N / 256 / fp4_skinny_cols(N) * (double)(M * K) * 2 / 47e3;
   return 4.0 + (weights > rows ? weights + 0.5 * rows : rows + 0.5 * weights);
 }
 
@@ -270,7 +286,7 @@ static double fp4_one(int64_t M, int64_t N, int64_t K, bool split, Fp4Plan* pl) 
     const double t = fp4_skinny_time(M, N, K);
     if (t < best) {
       best = t;
-      *pl = {0, kFp4Skinny, 16, 1, whole};
+      *pl = {0, kFp4Skinny, fp4_skinny_cols(N), 1, whole};
     }
   }
   const int64_t units = fp4_up(K, 128);
@@ -311,7 +327,7 @@ static double fp4_one(int64_t M, int64_t N, int64_t K, bool split, Fp4Plan* pl) 
 
 static Fp4Plan fp4_plan(int64_t M, int64_t N, int64_t K) {
   Fp4Plan pl;
-  if (M <= 16 && M * K <= 16384) return {0, kFp4Skinny, 16, 1, (int)K};  // a few rows: the launch, not the choice, counts
+  if (M <= 16 && M * K <= 16384) return {0, kFp4Skinny, fp4_skinny_cols(N), 1, (int)K};  // a few rows: the launch, not the choice, counts
   double best = fp4_one(M, N, K, true, &pl);
   if (M <= 128) return pl;
   const double all = fp4_large_time(M, N, K, 256);
@@ -354,7 +370,8 @@ static void fp4_launch(const GemmArgs& p, const Fp4Plan& pl, hipStream_t s) {
     }
     kg_launch(B_MXFP4, a, EPI, pl.bm, pl.splits, s);
   } else if constexpr (EPI != kEpiPartial) {
-    if (pl.kernel == kFp4Skinny) fp4_skinny_kernel<EPI><<<(p.N + 15) / 16, kSkWaves * 64, 0, s>>>(p);
+    if (pl.kernel == kFp4Skinny && pl.bm == 32) fp4_skinny_kernel<2, EPI><<<(p.N + 31) / 32, kSkWaves * 64, 0, s>>>(p);
+    else if (pl.kernel == kFp4Skinny) fp4_skinny_kernel<1, EPI><<<(p.N + 15) / 16, kSkWaves * 64, 0, s>>>(p);
     else launch_g8<B_MXFP4, EPI, 128>(p, s);
   }
 }

@@ -133,25 +133,42 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
 
   // ---- fragments of a k-step of 64: lane (row r32, half h) holds the 16 bytes of
   // block h, chunk 2 ks + h of its row, and that block's scale byte
+  // (scales: a word per row holds the blocks of two k-steps; shifted by the
+  // lane's half, byte 0 is the first's and byte 2 the second's)
   struct Frags {
     u32x4 a[AM], w[AN];
-    uint32_t sa[AM], sw[AN];
+  };
+  struct Scales {
+    uint32_t a[AM], w[AN];
   };
   Frags f0, f1;
+  Scales s0, s1;
   int c_off[4];
 #pragma unroll
   for (int ks = 0; ks < 4; ++ks) c_off[ks] = ((2 * ks + h) ^ g8_swz128(r32, false)) * 16;
   const int a_rd = (wm * WM + r32) * 128, w_rd = Cfg::B_OFF + (wn * WN + r32) * 128;
-  const int sa_rd = Cfg::SA_OFF + (wm * WM + r32) * 4 + h, sw_rd = Cfg::SB_OFF + (wn * WN + r32) * 4 + h;
+  const int sa_rd = Cfg::SA_OFF + (wm * WM + r32) * 4, sw_rd = Cfg::SB_OFF + (wn * WN + r32) * 4;
   auto read_a = [&](Frags& f, int slot, int ks, int i) __attribute__((always_inline)) {
     const char* S = lds + slot * Cfg::STAGE;
     f.a[i] = *reinterpret_cast<const u32x4*>(S + a_rd + c_off[ks] + i * 4096);
-    f.sa[i] = *reinterpret_cast<const uint8_t*>(S + sa_rd + (ks >> 1) * BM * 4 + (ks & 1) * 2 + i * 128);
   };
   auto read_w = [&](Frags& f, int slot, int ks, int j) __attribute__((always_inline)) {
     const char* S = lds + slot * Cfg::STAGE;
     f.w[j] = *reinterpret_cast<const u32x4*>(S + w_rd + c_off[ks] + j * 4096);
-    f.sw[j] = *reinterpret_cast<const uint8_t*>(S + sw_rd + (ks >> 1) * BN * 4 + (ks & 1) * 2 + j * 128);
+  };
+
+  auto read_scales = [&](Scales& s, int slot, int pair) __attribute__((always_inline)) {
+    const char* S = lds + slot * Cfg::STAGE;
+#pragma unroll
+    for (int i = 0; i < AM; ++i) s.a[i] = *reinterpret_cast<const uint32_t*>(S + sa_rd + pair * BM * 4 + i * 128);
+#pragma unroll
+    for (int j = 0; j < AN; ++j) s.w[j] = *reinterpret_cast<const uint32_t*>(S + sw_rd + pair * BN * 4 + j * 128);
+  };
+  auto shift = [&](Scales& s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < AM; ++i) s.a[i] >>= 8 * h;
+#pragma unroll
+    for (int j = 0; j < AN; ++j) s.w[j] >>= 8 * h;
   };
 
   f32x16 acc[AM][AN];
@@ -168,14 +185,16 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
   // a k-step's MFMAs in groups of one weight fragment (weights as the MFMA's first
   // operand: a lane then holds runs of four consecutive output columns); f(j)
   // issues what goes beside group j
-  auto step = [&](const Frags& x, auto f) __attribute__((always_inline)) {
+  // (BYTE: of the scale words)
+  auto step = [&](const Frags& x, const Scales& s, auto byte, auto f) __attribute__((always_inline)) {
+    constexpr int BYTE = decltype(byte)::value;
 #pragma unroll
     for (int j = 0; j < AN; ++j) {
       f(j);
 #pragma unroll
       for (int i = 0; i < AM; ++i)
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(x.w[j]), wide(x.a[i]), acc[i][j], 4, 4, 0,
-                                                                    (int)x.sw[j], 0, (int)x.sa[i]);
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(x.w[j]), wide(x.a[i]), acc[i][j], 4, 4,
+                                                                    BYTE, (int)s.w[j], BYTE, (int)s.a[i]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -196,6 +215,9 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
     for (int l = 0; l < (t < NST - 1 ? Cfg::DMA : HL); ++l) load(t, t, l);
   wait_vmcnt<(NST - 2) * Cfg::DMA + HL>();
   barrier_nofence();
+  using Even = std::integral_constant<int, 0>;
+  using Odd = std::integral_constant<int, 2>;
+  read_scales(s0, 0, 0);
 #pragma unroll
   for (int j = 0; j < AN; ++j) read_share(f0, 0, 0, j);
 
@@ -207,14 +229,19 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
   constexpr int LPJ = (HL + AN - 1) / AN;  // load instructions per group
   int prev = NST - 1;                      // the slot of stage t - 1
   for (int t = 0; t < depth / 256; ++t) {
-    step(f0, [&](int j) __attribute__((always_inline)) {
+    shift(s0);
+    step(f0, s0, Even{}, [&](int j) __attribute__((always_inline)) {
       read_share(f1, slot, 1, j);
 #pragma unroll
       for (int l = HL; l < Cfg::DMA; ++l)
         if ((l - HL) / LPJ == j) load(t + NST - 1, prev, l);
     });
-    step(f1, [&](int j) __attribute__((always_inline)) { read_share(f0, slot, 2, j); });
-    step(f0, [&](int j) __attribute__((always_inline)) {
+    step(f1, s0, Odd{}, [&](int j) __attribute__((always_inline)) {
+      if (j == 0) read_scales(s1, slot, 1);
+      read_share(f0, slot, 2, j);
+    });
+    shift(s1);
+    step(f0, s1, Even{}, [&](int j) __attribute__((always_inline)) {
       if (j == 0)
 #pragma unroll
         for (int i = 0; i < AN; ++i) read_share(f1, slot, 3, i);
@@ -224,7 +251,8 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
     barrier_nofence();
     prev = slot;
     slot = slot + 1 < NST ? slot + 1 : 0;
-    step(f1, [&](int j) __attribute__((always_inline)) {
+    step(f1, s1, Odd{}, [&](int j) __attribute__((always_inline)) {
+      if (j == 0) read_scales(s0, slot, 0);
       read_share(f0, slot, 0, j);
 #pragma unroll
       for (int l = 0; l < HL; ++l)
@@ -232,8 +260,9 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
     });
   }
   if (half) {
-    step(f0, [&](int j) __attribute__((always_inline)) { read_share(f1, slot, 1, j); });
-    step(f1, [](int) {});
+    shift(s0);
+    step(f0, s0, Even{}, [&](int j) __attribute__((always_inline)) { read_share(f1, slot, 1, j); });
+    step(f1, s0, Odd{}, [](int) {});
   }
   wait_vmcnt<0>();
   if constexpr (EPI == kEpiPartial) {
