@@ -423,6 +423,27 @@ int main(int argc, char** argv) {
     EXPECT(ltx_ge_correct_f32(fd, fo, fo, 0, 0.5f, 0.5f, 3456 * 128, nullptr), LTX_ERR_HIP);
     EXPECT(ltx_euler_step_bf16(d, fd, 0.5f, d, 3456 * 128, nullptr), LTX_ERR_HIP);
     EXPECT(ltx_swap_axes(d, 9, 128, 384, 2, static_cast<char*>(d) + (1 << 24), nullptr), LTX_ERR_HIP);
+    // MXFP4 rows, weights and products (every kernel of the choice), rotary positions
+    uint32_t* ud = static_cast<uint32_t*>(d);
+    uint8_t* bd = static_cast<uint8_t*>(d);
+    EXPECT(ltx_quantize_mxfp4(d, 0, 4096, 3456, 4096, bd, 2048, ud, 3456, nullptr), LTX_ERR_HIP);
+    EXPECT(ltx_dequantize_mxfp4_bf16(bd, 2048, ud, 3456, 3456, 4096, d, 4096, nullptr), LTX_ERR_HIP);
+    for (int64_t m : {int64_t(1), int64_t(16), int64_t(33), int64_t(68), int64_t(300), int64_t(1296), int64_t(3456)})
+      for (int64_t k : {int64_t(64), int64_t(1088), int64_t(4096)})
+        for (int64_t n : {int64_t(8), int64_t(2048), int64_t(12320)}) {
+          const int64_t ld = (n + 3) / 4 * 4, need = ltx_gemm_mxfp4_workspace_bytes(m, n, k);
+          EXPECT(need >= 0, 1);
+          EXPECT(ltx_gemm_mxfp4_bf16(d, k, bd, k / 2, ud, ld, fd, d, n, m, n, k, 0, nullptr, 0, nullptr, n, fo, need,
+                                     nullptr), LTX_ERR_HIP);
+          const int64_t need4 = ltx_gemm_mx4_workspace_bytes(m, n, k);
+          EXPECT(ltx_gemm_mx4_bf16(bd, k / 2, ud, (m + 3) / 4 * 4, bd, k / 2, ud, ld, fd, d, n, m, n, k, 1, nullptr, 0,
+                                   nullptr, n, fo, need4, nullptr), k % 128 ? LTX_ERR_UNSUPPORTED : LTX_ERR_HIP);
+        }
+    const ltx_rotary_rows rows = {d, 0, 4096, 128, d, 0, 4096, 128, 32};
+    for (int type : {0, 1, 2})
+      for (int flags : {0, LTX_ROTARY_INTERLEAVED | LTX_ROTARY_TRANSPOSE})
+        EXPECT(ltx_rotary(&rows, &rows, type, 1, 3456, 128, 64, id, 0, 0, static_cast<const double*>(d), 1.0, flags,
+                          nullptr), LTX_ERR_HIP);
     EXPECT(ltx_gemma_features_bf16(d, 49, 1024, 3840, 1024 * 3840, 3840, id, 1e-6f, 1.0f, 1.0f, d, d, 49 * 3840,
                                    nullptr), LTX_ERR_HIP);
   }

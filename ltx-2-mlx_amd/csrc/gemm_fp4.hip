@@ -15,13 +15,16 @@ namespace ltx {
 // code bytes of its k block of 32 straight from memory: one block, one scale,
 // four MFMA k-steps; the quarter's k run 32 q + 8 j in k-step j, for both
 // operands.  The activation rows go through LDS, KC of k at a time, where all
-// waves read them.  Takes every size that the products allow.
+// waves read them.  Takes every size that the products allow: what the other
+// kernels do not (few rows of a depth that ends inside a scale word, operands of
+// 2 GiB).  Bound by its own serial phases (256 x 4096 -> 8192 55 us, the mid-size
+// kernel 21).
 constexpr int kFrThreads = 512, kFrBN = 128;
 
 template <int MB>
 struct FrCfg {
   static constexpr int BM = MB * 16;
-  static constexpr int KC = MB <= 4 ? 512 : 256;
+  static constexpr int KC = 512;
   // LDS row: KC bf16 and 32 bytes, so that the 16 rows x 16 bytes that a
   // fragment read's lane octets fetch together start in 16-byte pieces two
   // apart; rows 8-15 use the pieces between (their chunks XOR 1)
@@ -106,15 +109,16 @@ __global__ __launch_bounds__(kFrThreads) void fp4_rows_kernel(GemmArgs p, int k_
 
 // ---- one to 16 rows ----------------------------------------------------------
 // Bound by latency and the weight bytes: one launch, no workspace, a wave's
-// loads of up to 512 k issued before their first use.  A workgroup computes 16
-// columns (NB times 16); its waves split K, each streaming its range of the codes (and the
-// activations, which the L2 holds) straight to registers, and meet once
-// through LDS, in wave order.  NB = 2: 32 columns, half the reads of the
-// activations, where that leaves workgroups for every CU.  Weights from HBM: 1 x 4096 -> 4096 6.0 us (10.8 in 8
-// K ranges and a combining launch of the few-row tiles, 11.2 in 4 of the
+// loads of up to 512 k issued before their first use.  A workgroup computes NB *
+// 16 columns; its waves split K, each streaming its range of the codes (and the
+// activations, which the L2 holds) straight to registers, and meet once through
+// LDS, in wave order.  NB = 2 halves the reads of the activations, where that
+// leaves workgroups for every CU.  Weights from HBM: 1 x 4096 -> 4096 6.0 us (10.8
+// in 8 K ranges and a combining launch of the few-row tiles, 11.2 in 4 of the
 // mid-size kernel; a launch that does next to nothing takes 4.0), 1 x 4096 ->
-// 16384 12.5, 16 x 4096 -> 4096 8.7.  Holding the next 512 k in flight as well cost
-// more in occupancy than it gave (1 x 4096 -> 16384 16.9); 16 waves are no faster.
+// 16384 12.5, 16 x 4096 -> 4096 8.7.  Holding the next 512 k in flight as well
+// cost more in occupancy than it gave (1 x 4096 -> 16384, one fragment of columns:
+// 16.9 against 13.8); 16 waves are no faster.
 constexpr int kSkWaves = 8;
 
 template <int NB, int EPI>
