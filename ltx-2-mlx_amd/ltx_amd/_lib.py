@@ -229,6 +229,50 @@ def same_device(*tensors: torch.Tensor | None) -> int:
     return device
 
 
+def _axes(t: torch.Tensor) -> list[tuple[int, int]]:
+    """(stride in bytes, size) of the axes of more than one entry, outermost last."""
+    size = t.element_size()
+    return sorted((st * size, n) for st, n in zip(t.stride(), t.shape) if n != 1)
+
+
+def same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether index for index the two are the same memory."""
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and all(
+        n == 1 or sa == sb for sa, sb, n in zip(a.stride(), b.stride(), a.shape))
+
+
+def overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the two may share memory.  Column ranges of one buffer's rows do
+    not: with a stride in common, what lies inside it is compared."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    xa, xb = _axes(a), _axes(b)
+
+    def extent(axes, size, below=None):  # bytes from the first element to the end of the last
+        return size + sum(st * (n - 1) for st, n in axes if below is None or st < below)
+
+    gap = b.data_ptr() - a.data_ptr()
+    if gap >= extent(xa, a.element_size()) or -gap >= extent(xb, b.element_size()):
+        return False
+    for period in {st for st, _ in xa} & {st for st, _ in xb}:
+        if period == 0 or any(st > period and st % period for st, _ in xa + xb):
+            continue
+        d = gap % period
+        if extent(xa, a.element_size(), period) <= d and d + extent(xb, b.element_size(), period) <= period:
+            return False
+    return True
+
+
+def self_overlaps(t: torch.Tensor) -> bool:
+    """Whether two indices may name the same element."""
+    end = t.element_size()
+    for st, n in _axes(t) if t.numel() else ():
+        if st < end:
+            return True
+        end += st * (n - 1)
+    return False
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     if t is None:
         return None

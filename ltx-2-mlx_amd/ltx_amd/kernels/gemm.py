@@ -548,7 +548,8 @@ def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int
         xs = None
     if kx != k:
         raise ValueError(f"activations have K={kx}, the weight {k}")
-    if out is None:
+    given = out is not None
+    if not given:
         out = src.new_empty(shape, dtype=torch.bfloat16)
         ldc = n
     else:
@@ -582,6 +583,9 @@ def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int
         bptr = bias.data_ptr()
         if weight.qlinear:
             flags |= _lib.GEMM_ROUND_THEN_BIAS
+    if given and (_lib.overlaps(out, src) or (
+            residual is not None and (out.data_ptr() != rptr or ldc != ldr) and _lib.overlaps(out, residual))):
+        raise ValueError("out overlaps the activations, or the residual without being it")
     device = _lib.same_device(src, xs, w, scale, bias, out, residual, gate)
     if m == 0:
         return out

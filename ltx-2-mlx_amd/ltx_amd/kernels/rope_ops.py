@@ -137,11 +137,11 @@ def _rotary_side(name: str, x: torch.Tensor, out: torch.Tensor | None) -> tuple[
         out = torch.empty_like(x)
     elif out.shape != shape or out.dtype is not x.dtype:
         raise ValueError(f"{name}'s out must be {x.dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
+    elif _lib.self_overlaps(out):
+        raise ValueError(f"{name}'s out has one element in several places")
     so = out.stride()
     if (st[-1] != 1 or so[-1] != 1) and shape[-1] > 1:
         raise ValueError(f"{name} and its out must have unit channel stride")
-    if 0 in so and any(st == 0 and size > 1 for st, size in zip(so, shape)):
-        raise ValueError(f"{name}'s out has one element in several places")
     if len(st) == 3:
         rows = _ROTARY_ROWS(x.data_ptr(), 0, st[0], st[1], out.data_ptr(), 0, so[0], so[1], shape[1])
     else:
@@ -163,7 +163,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     (:func:`rotary_frequencies`).  positions: (T) for every sequence of the
     batch, or (B, T); int32, int64, fp32 or fp64.  ``transpose`` rotates back
     (times ``factor`` again): with the outputs' gradients for q and k it gives
-    the inputs' gradients.  ``out`` may be (q, k) itself (in place).
+    the inputs' gradients.  ``out`` may be (q, k) itself (in place);
+    its tensors must not overlap the others in any other way.
     """
     if layout not in ROTARY_LAYOUTS:
         raise ValueError(f"layout must be one of {ROTARY_LAYOUTS}, got {layout!r}")
@@ -200,6 +201,14 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
         raise ValueError("out has a tensor for k, but there is no k")
     sq, oq = _rotary_side("q", q, oq)
     sk, ok = _rotary_side("k", k, ok) if k is not None else (None, None)
+    if out is not None:
+        # workgroups read and write in any order: an output may be its own input, and
+        # must keep off everything else that is read or written
+        for mine, x, other, y in ((oq, q, ok, k), (ok, k, oq, q)):
+            if mine is not None and (
+                    (not _lib.same_view(mine, x) and _lib.overlaps(mine, x)) or
+                    any(t is not None and _lib.overlaps(mine, t) for t in (other, y, positions, inv_freq))):
+                raise ValueError("an output of rotary overlaps another tensor of the call")
     device = _lib.same_device(q, k, positions, inv_freq, oq, ok)
     if batch * tokens == 0:
         return oq, ok

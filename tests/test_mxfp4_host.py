@@ -194,3 +194,51 @@ def test_frequency_stretches():
                 dict(rotary_dim=8, theta=1.0), dict(rotary_dim=8, stretch=0.5)):
         with pytest.raises(ValueError):
             rotary_frequencies(device="cpu", **bad)
+
+
+def test_overlapping_outputs_are_refused():
+    from ltx_amd import _lib
+    from ltx_amd.kernels import gemm, rope_ops
+
+    rng = np.random.default_rng(3)
+    for _ in range(300):  # the rule against the sets of addresses
+        base = torch.zeros(400, dtype=torch.bfloat16)
+        views = []
+        for _ in range(2):
+            sizes = [int(v) for v in rng.integers(1, 5, 3)]
+            strides = [int(v) for v in rng.choice([0, 1, 2, 3, 8, 16, 32, 33], 3)]
+            views.append(base.as_strided(sizes, strides, int(rng.integers(0, 60))))
+        a, b = views
+        at = [torch.arange(400).as_strided(v.shape, v.stride(), v.storage_offset()).flatten().tolist() for v in views]
+        if set(at[0]) & set(at[1]):
+            assert _lib.overlaps(a, b) and _lib.overlaps(b, a)
+        if len(set(at[0])) < len(at[0]):
+            assert _lib.self_overlaps(a)
+    buf = torch.zeros(2, 5, 12, 64, dtype=torch.bfloat16)
+    q, k, rest = buf[:, :, :4], buf[:, :, 4:6], buf[:, :, 6:]
+    assert not _lib.overlaps(q, k) and not _lib.overlaps(rest, q) and not _lib.overlaps(buf[0], buf[1])
+    assert not _lib.overlaps(buf[..., :32], buf[..., 32:]) and _lib.overlaps(buf[..., :33], buf[..., 32:])
+    assert not _lib.self_overlaps(q) and not _lib.self_overlaps(buf.transpose(1, 2)) and _lib.self_overlaps(q[:, :1].expand_as(q))
+
+    pos = torch.arange(5)
+    inv, _ = rope_ops.rotary_frequencies(64, device="cpu")
+    for out in ((k.clone(), q.clone()), (buf[:, :, 1:5], k), (q, buf[:, :, 3:5]), (buf[:, :, 6:10], buf[:, :, 9:11]),
+                (q.transpose(1, 2).reshape(-1).as_strided(q.shape, (0, 256, 64, 1)), None)):
+        with pytest.raises(ValueError):
+            rope_ops.rotary(q, k, pos, inv, out=out)
+    for out in ((q, k), (rest[:, :, :4], rest[:, :, 4:]), (torch.empty_like(q), None)):
+        with pytest.raises(ValueError, match="on one GPU"):  # nothing to object to but the host's memory
+            rope_ops.rotary(q, k, pos, inv, out=out)
+
+    w = gemm.LinearWeight("mxfp4", torch.zeros(128, 64, dtype=torch.uint8), torch.zeros(1, 128, dtype=torch.int32))
+    rows = torch.zeros(6, 256, dtype=torch.bfloat16)
+    gate = torch.zeros(128)
+    x = rows[:4, :128]
+    res = dict(epilogue=gemm.EPI_RESIDUAL, gate=gate)
+    for kw in (dict(out=x), dict(out=rows[1:5, :128]), dict(out=rows[:4, 64:192]),
+               dict(out=rows[:4, 128:], residual=rows[1:5, 128:], **res)):
+        with pytest.raises(ValueError, match="overlaps"):
+            gemm.linear(x, w, **kw)
+    for kw in (dict(out=rows[:4, 128:]), dict(out=rows[:4, 128:], residual=rows[:4, 128:], **res)):
+        with pytest.raises(ValueError, match="on one GPU"):
+            gemm.linear(x, w, **kw)
