@@ -425,7 +425,7 @@ def _check_mxfp4(what: str, codes: torch.Tensor, scales: torch.Tensor) -> tuple[
         words, ld = scales.shape
         ldc, unit = codes.stride()
         lds, sunit = scales.stride()
-        if words * 64 >= half and ld >= rows and unit == sunit == 1:
+        if words * 64 >= half > 0 and ld >= rows and unit == sunit == 1:
             # (the stride of an axis of one entry says nothing)
             return rows, half * 2, ldc if rows > 1 else half, lds if words > 1 else (ld + 3) // 4 * 4
     raise ValueError(f"{what}: MXFP4 operands are code bytes (rows, K/2) uint8 and scale words (ceil(K/128), >= rows) "
@@ -466,10 +466,10 @@ def quantize_rows_mxfp4(x: torch.Tensor) -> Mx4Rows:
     dtype = _QUANT_DTYPES.get(x.dtype)
     if dtype is None:
         raise TypeError(f"quantize_rows_mxfp4 takes bf16, fp16 or fp32 rows, got {x.dtype}")
-    if k % 32:
-        raise ValueError(f"K={k} is not a multiple of 32")
+    if k % 32 or k == 0:
+        raise ValueError(f"K={k} is not a positive multiple of 32")
     xv, ldx = _lib.row_view(x, k)
-    m = x.numel() // k if k else 0
+    m = x.numel() // k
     if m == 1:
         ldx = k  # (the stride of an axis of one entry says nothing)
     elif ldx < k:  # one row for all
@@ -477,7 +477,7 @@ def quantize_rows_mxfp4(x: torch.Tensor) -> Mx4Rows:
     ld = (m + 3) // 4 * 4
     codes = x.new_empty((m, k // 2), dtype=torch.uint8)
     scales = x.new_empty(((k + 127) // 128, ld), dtype=torch.int32)
-    if m and k:
+    if m:
         st = _lib.launch(_lib.same_device(xv), "ltx_quantize_mxfp4", xv.data_ptr(), dtype, ldx, m, k,
                          codes.data_ptr(), k // 2, scales.data_ptr(), ld)
         if st:
@@ -495,7 +495,7 @@ def dequantize_rows_mxfp4(rows: Mx4Rows) -> torch.Tensor:
             return out
     m, k, ldq, lds = _check_mxfp4("dequantize_rows_mxfp4", codes, scales)
     out = codes.new_empty((m, k), dtype=torch.bfloat16)
-    if m and k:
+    if m:
         st = _lib.launch(_lib.same_device(codes, scales), "ltx_dequantize_mxfp4_bf16", codes.data_ptr(), ldq,
                          scales.data_ptr(), lds, m, k, out.data_ptr(), k)
         if st:
@@ -540,7 +540,7 @@ def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int
         else:
             *lead, kx = shape
             src, lda = _lib.row_view(x, kx)
-            m, shape = x.numel() // kx if kx else 0, (*lead, n)
+            m, shape = x.numel() // kx if kx else 0, (*lead, n)  # (K = 0 is refused below)
         if m == 1:
             lda = kx  # (the stride of an axis of one entry says nothing)
         elif lda < kx:  # one row for all

@@ -242,3 +242,16 @@ def test_overlapping_outputs_are_refused():
     for kw in (dict(out=rows[:4, 128:]), dict(out=rows[:4, 128:], residual=rows[:4, 128:], **res)):
         with pytest.raises(ValueError, match="on one GPU"):
             gemm.linear(x, w, **kw)
+
+
+def test_rows_of_no_elements_are_refused():
+    from ltx_amd.kernels import gemm
+
+    codes, words = torch.zeros(8, 0, dtype=torch.uint8), torch.zeros(0, 8, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        gemm.quantize_rows_mxfp4(torch.zeros(5, 0))
+    with pytest.raises(ValueError):
+        gemm.dequantize_rows_mxfp4(gemm.Mx4Rows(codes, words))
+    for x in (torch.zeros(2, 5, 0, dtype=torch.bfloat16), gemm.Mx4Rows(codes, words)):
+        with pytest.raises(ValueError):
+            gemm.linear(x, gemm.LinearWeight("mxfp4", codes, words))
