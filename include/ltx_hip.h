@@ -178,7 +178,7 @@ int ltx_qknorm_rope_axes_bf16(void* q, int64_t q_stride, int64_t rows_q, const f
  * positions: (batch, tokens) of pos_type 0 int32, 1 int64, 2 fp32, 3 fp64,
  * batch stride pos_batch (0: one row for all), token stride 1.  inv_freq: fp64
  * (rotary_dim / 2) device values.  rotary_dim even, at most head_dim; head_dim
- * at most 512.
+ * at most 512; at most 2^26 - 4 tokens over the batch.
  */
 #define LTX_ROTARY_INTERLEAVED 1
 #define LTX_ROTARY_TRANSPOSE 2
@@ -405,6 +405,7 @@ int ltx_gemm_mx_gelu_mxfp8(const uint8_t* A, int64_t lda, const uint8_t* a_scale
  * sigmoid_from as above, except that GELU and the head gate act on the fp32
  * value (no bf16 rounding before them).  Code and row strides 16-byte
  * multiples, pointers 16-byte aligned (bias and gate 4).
+ * At most 2^27 rows or columns and 2^34 outputs.
  * Products of few tiles split K: they need `workspace` (device memory, 16-byte
  * aligned) of ltx_gemm_*_workspace_bytes(M, N, K) bytes, 0 where none is
  * needed (workspace may then be NULL); calls that may run at the same time
@@ -524,7 +525,8 @@ int ltx_dequantize_w8_bf16(const int8_t* q, int64_t ldq, const float* scale, int
  *   255 (NaN) and codes 0.
  * x: (rows, K) of dtype 0 bf16, 1 fp16, 2 fp32, row stride ldx, 16-byte aligned
  * rows; K % 32 == 0.  The decoder writes bf16 (rows, K), exact; a block of
- * scale 255 decodes to NaN.  Words past the rows are left as they were. */
+ * scale 255 decodes to NaN.  Words past the rows are left as they were.  At
+ * most about 2^37 (encoder) and 2^35 (decoder) elements in a call. */
 int ltx_quantize_mxfp4(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t K, uint8_t* q, int64_t ldq,
                        uint32_t* scales, int64_t ld_scale, void* stream);
 int ltx_dequantize_mxfp4_bf16(const uint8_t* q, int64_t ldq, const uint32_t* scales, int64_t ld_scale,

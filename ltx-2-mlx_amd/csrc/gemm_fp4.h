@@ -86,7 +86,11 @@ static inline int fp4_check(const void* A, int64_t lda, const void* W, int64_t l
                             int64_t lda_unit) {
   auto al = [](const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; };
   if (!A || !W || !w_scale || !C || M < 0 || N < 0 || K < 0) return LTX_ERR_INVALID_ARG;
-  if (M > INT32_MAX / 2 || N > INT32_MAX / 2 || K > INT32_MAX / 2) return LTX_ERR_UNSUPPORTED;
+  // a launch has fewer than 2^32 threads: 512 for a tile of at least 32 x 128
+  // outputs, or for 32 columns of a few rows
+  const int64_t size = 1 << 27, stride = (int64_t)1 << 40;
+  if (M > size || N > size || K > INT32_MAX / 2 || M * N > (int64_t)1 << 34) return LTX_ERR_UNSUPPORTED;
+  if (lda > stride || ldw > stride || ldc > stride || ldr > stride || ld_scale > stride) return LTX_ERR_UNSUPPORTED;
   const int epi = epilogue & 0xff;
   if (epilogue & ~(0xff | LTX_GEMM_ROUND_THEN_BIAS) || epi > LTX_GEMM_EPI_SIGMOID2) return LTX_ERR_INVALID_ARG;
   const bool resid = epi == LTX_GEMM_EPI_RESIDUAL || epi == LTX_GEMM_EPI_RESIDUAL_ROUND;

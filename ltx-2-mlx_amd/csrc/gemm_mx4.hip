@@ -346,7 +346,6 @@ using M4Tall = M4Tile<256, 128, 4, 2, 3>;
 using M4Mid = M4Tile<128, 128, 2, 4, 4>;
 using M4Small = M4Tile<64, 128, 2, 4, 4>;
 
-
 struct Mx4Plan {
   int bm, bn, splits;
   int k_split;  // k of one range, a multiple of 256

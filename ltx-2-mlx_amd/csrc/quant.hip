@@ -108,6 +108,7 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
 // k range are contiguous over rows, so they meet in LDS and leave as 64-byte
 // pieces.
 constexpr int kQ4Rows = 16;
+constexpr int64_t kQ4Blocks = (1 << 24) - 1;  // of 256 threads: a launch has fewer than 2^32
 template <typename T>
 __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows,
                                                              int64_t K, uint8_t* __restrict__ q, int64_t ldq,
@@ -345,7 +346,7 @@ extern "C" int ltx_quantize_mxfp4(const void* x, int dtype, int64_t ldx, int64_t
     return LTX_ERR_ALIGNMENT;
   if (rows == 0 || K == 0) return LTX_OK;
   const int64_t chunks = (K + 511) / 512, groups = (rows + kQ4Rows - 1) / kQ4Rows;
-  if (chunks > INT32_MAX / groups) return LTX_ERR_UNSUPPORTED;
+  if (chunks > kQ4Blocks / groups) return LTX_ERR_UNSUPPORTED;
   const int blocks = (int)(chunks * groups);
   hipStream_t s = (hipStream_t)stream;
   if (dtype == 0)
@@ -364,7 +365,7 @@ extern "C" int ltx_dequantize_mxfp4_bf16(const uint8_t* q, int64_t ldq, const ui
   if (ldq < K / 2 || ldo < K || ld_scale < rows) return LTX_ERR_INVALID_ARG;
   if (!a16(out) || !a16(q) || !a16(scales) || ldq % 16 || ldo % 8 || ld_scale % 4) return LTX_ERR_ALIGNMENT;
   if (rows == 0 || K == 0) return LTX_OK;
-  if (K / 8 > (int64_t)INT32_MAX * 256 / rows) return LTX_ERR_UNSUPPORTED;
+  if (K / 8 > kQ4Blocks * 256 / rows) return LTX_ERR_UNSUPPORTED;
   const int64_t total = rows * (K / 8);
   mxfp4_dequantize_kernel<<<(int)((total + 255) / 256), 256, 0, (hipStream_t)stream>>>(
       q, ldq, scales, ld_scale, rows, K, (bf16*)out, ldo);

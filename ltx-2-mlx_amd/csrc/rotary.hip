@@ -241,7 +241,7 @@ extern "C" int ltx_rotary(const ltx_rotary_rows* q, const ltx_rotary_rows* k, in
   const int64_t all = batch * tokens;
   p.per_block = all >= 4096 ? kRotTokens : (all >= 2048 ? 2 : 1);
   const int64_t blocks = (all + p.per_block - 1) / p.per_block;
-  if (blocks > INT32_MAX) return LTX_ERR_UNSUPPORTED;
+  if (blocks > (1 << 24) - 1) return LTX_ERR_UNSUPPORTED;  // a launch has fewer than 2^32 threads
   hipStream_t s = (hipStream_t)stream;
   if (dtype == 0) rotary_launch_vec<bf16>(p, vec, interleaved, (int)blocks, s);
   else if (dtype == 1) rotary_launch_vec<_Float16>(p, vec, interleaved, (int)blocks, s);

@@ -255,3 +255,25 @@ def test_rows_of_no_elements_are_refused():
     for x in (torch.zeros(2, 5, 0, dtype=torch.bfloat16), gemm.Mx4Rows(codes, words)):
         with pytest.raises(ValueError):
             gemm.linear(x, gemm.LinearWeight("mxfp4", codes, words))
+
+
+@pytest.mark.parametrize("name", ["ltx_gemm_mxfp4_bf16", "ltx_gemm_mx4_bf16"])
+def test_products_past_one_launch_are_refused(lib, name):
+    """More threads than one launch has, or strides that overflow a byte offset."""
+    m, n = 1 << 28, 1 << 28
+    assert _gemm(lib, name, M=m, ldas=m) == UNSUPPORTED
+    assert _gemm(lib, name, N=n, ldc=n, ldws=n, sig=n) == UNSUPPORTED
+    m, n = 1 << 18, 1 << 17
+    assert _gemm(lib, name, M=m, ldas=m, N=n, ldc=n, ldws=n, sig=n) == UNSUPPORTED
+    for stride in ("lda", "ldw", "ldc", "ldws"):
+        assert _gemm(lib, name, M=1, **{stride: 1 << 62}) == UNSUPPORTED
+
+
+def test_rows_past_one_launch_are_refused(lib):
+    from ltx_amd import _lib
+
+    k, rows = 512, 1 << 28
+    assert lib.ltx_quantize_mxfp4(16, 0, k, rows, k, 16, k // 2, 16, rows, None) == UNSUPPORTED
+    assert lib.ltx_dequantize_mxfp4_bf16(16, k // 2, 16, rows, rows, k, 16, k, None) == UNSUPPORTED
+    q = _lib.RotaryRows(16, 0, 64, 64, 16, 0, 64, 64, 1)
+    assert lib.ltx_rotary(ctypes.addressof(q), None, 0, 1, 1 << 27, 64, 64, 16, 0, 0, 16, 1.0, 0, None) == UNSUPPORTED
