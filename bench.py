@@ -2,7 +2,7 @@
 
 Workload (default): the LTX-2.3 22B-shape transformer, 48 blocks resident in
 HBM with random-init weights ~N(0, 0.02) stored as MXFP8 (E4M3 codes + E8M0
-scale per 32 along K; --weights bf16|int8 for the other formats), one
+scale per 32 along K; --weights bf16|int8|mxfp4 for the other formats), one
 denoise step at
 768x512x65 -> 3456 video tokens (latent 9x16x24), 68 audio tokens and 256
 text tokens per modality, eight distilled sigmas cycled.  A "step" is one
