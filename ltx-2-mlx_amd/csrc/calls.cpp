@@ -35,6 +35,67 @@ at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const at::Tensor& li
   return at::empty(size, like.options().dtype(type));
 }
 
+// The axes of more than one entry, by ascending stride (in bytes; up to 4)
+struct Axes {
+  int n = 0;
+  int64_t stride[4], size[4], unit;
+  explicit Axes(const at::Tensor& t) : unit(t.element_size()) {
+    for (int64_t d = 0; d < t.dim(); ++d) {
+      if (t.size(d) == 1) continue;
+      int i = n++;
+      for (; i > 0 && stride[i - 1] > t.stride(d) * unit; --i) stride[i] = stride[i - 1], size[i] = size[i - 1];
+      stride[i] = t.stride(d) * unit;
+      size[i] = t.size(d);
+    }
+  }
+  // bytes from the first element to the end of the last, along strides below `period`
+  int64_t extent(int64_t period = INT64_MAX) const {
+    int64_t e = unit;
+    for (int i = 0; i < n && stride[i] < period; ++i) e += stride[i] * (size[i] - 1);
+    return e;
+  }
+  bool whole_periods(int64_t period) const {
+    for (int i = 0; i < n; ++i)
+      if (stride[i] > period && stride[i] % period) return false;
+    return true;
+  }
+};
+
+// whether no two indices name the same element
+bool distinct(const at::Tensor& t) {
+  const Axes x(t);
+  int64_t end = x.unit;
+  for (int i = 0; i < x.n; ++i) {
+    if (x.stride[i] < end) return false;
+    end += x.stride[i] * (x.size[i] - 1);
+  }
+  return true;
+}
+
+// whether the two (not empty) share no memory: apart, or with a stride in common
+// within which they are apart (column ranges of one buffer's rows)
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  const Axes xa(a), xb(b);
+  const int64_t gap = static_cast<const char*>(b.const_data_ptr()) - static_cast<const char*>(a.const_data_ptr());
+  if (gap >= xa.extent() || -gap >= xb.extent()) return true;
+  for (int i = 0; i < xa.n; ++i)
+    for (int j = 0; j < xb.n; ++j) {
+      const int64_t period = xa.stride[i];
+      if (period == 0 || xb.stride[j] != period || !xa.whole_periods(period) || !xb.whole_periods(period)) continue;
+      const int64_t d = (gap % period + period) % period;
+      if (xa.extent(period) <= d && d + xb.extent(period) <= period) return true;
+    }
+  return false;
+}
+
+// whether index for index the two (of one shape) are the same memory
+bool same_view(const at::Tensor& a, const at::Tensor& b) {
+  if (a.const_data_ptr() != b.const_data_ptr()) return false;
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) != 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+
 // dense-column (rows, K / 2) codes with scale words that cover them
 bool mxfp4(const at::Tensor* codes, const at::Tensor* words, int64_t device, int64_t* rows, int64_t* k) {
   if (!codes || !words || codes->scalar_type() != at::kByte || words->scalar_type() != at::kInt || codes->dim() != 2 ||
@@ -47,17 +108,17 @@ bool mxfp4(const at::Tensor* codes, const at::Tensor* words, int64_t device, int
 }
 
 // linear(x, x_words or None, codes, words, bias or None, flags, epilogue, residual or None, gate or None,
-//        sigmoid_from or -1, device, stream)
+//        sigmoid_from or -1, out or None, device, stream)
 PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 12 || !entry.gemm) return general();
+  if (n != 13 || !entry.gemm) return general();
   const at::Tensor *x = tensor(a[0]), *xs = tensor(a[1]), *w = tensor(a[2]), *ws = tensor(a[3]), *bias = tensor(a[4]),
-                   *res = tensor(a[7]), *gate = tensor(a[8]);
+                   *res = tensor(a[7]), *gate = tensor(a[8]), *given = tensor(a[10]);
   const int64_t flags = PyLong_AsLongLong(a[5]), epi = PyLong_AsLongLong(a[6]), sig = PyLong_AsLongLong(a[9]),
-                device = PyLong_AsLongLong(a[10]);
-  void* stream = PyLong_AsVoidPtr(a[11]);
+                device = PyLong_AsLongLong(a[11]);
+  void* stream = PyLong_AsVoidPtr(a[12]);
   if (PyErr_Occurred()) return nullptr;
   int64_t N, K, M, kx;
-  if (!x || (!xs && a[1] != Py_None) || (!bias && a[4] != Py_None) || !mxfp4(w, ws, device, &N, &K)) return general();
+  if (!x || (!xs && a[1] != Py_None) || (!bias && a[4] != Py_None) || (!given && a[10] != Py_None) || !mxfp4(w, ws, device, &N, &K)) return general();
   if (xs) {
     if (!mxfp4(x, xs, device, &M, &kx)) return general();
   } else {
@@ -80,7 +141,16 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     ldr = M > 1 ? res->stride(0) : N;
     if (ldr < N) return general();
   }
-  at::Tensor out = empty({M, N}, at::kBFloat16, *x);
+  int64_t ldc = N;
+  if (given) {
+    if (given->dim() != 2 || given->scalar_type() != at::kBFloat16 || given->size(0) != M || given->size(1) != N ||
+        given->stride(1) != 1 || !on(*given, device) || !apart(*given, *x) ||
+        (resid && !same_view(*given, *res) && !apart(*given, *res)))
+      return general();
+    if (M > 1) ldc = given->stride(0);
+    if (ldc < N) return general();
+  }
+  at::Tensor out = given ? *given : empty({M, N}, at::kBFloat16, *x);
   const int64_t bytes = xs ? entry.mx4_ws(M, N, K) : entry.gemm_ws(M, N, K);
   at::Tensor work;
   if (bytes > 0) work = empty({bytes}, at::kByte, *x);
@@ -94,9 +164,9 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const auto* wsp = static_cast<const uint32_t*>(ws->const_data_ptr());
   const int st = xs ? entry.mx4(static_cast<const uint8_t*>(x->const_data_ptr()), lda,
                                 static_cast<const uint32_t*>(xs->const_data_ptr()), xs->stride(0), wc, ldw, wsp,
-                                ws->stride(0), bp, out.data_ptr(), N, M, N, K, (int)(epi | flags), rp, ldr, gp, from, wp,
+                                ws->stride(0), bp, out.data_ptr(), ldc, M, N, K, (int)(epi | flags), rp, ldr, gp, from, wp,
                                 bytes, stream)
-                    : entry.gemm(x->const_data_ptr(), lda, wc, ldw, wsp, ws->stride(0), bp, out.data_ptr(), N, M, N, K,
+                    : entry.gemm(x->const_data_ptr(), lda, wc, ldw, wsp, ws->stride(0), bp, out.data_ptr(), ldc, M, N, K,
                                  (int)(epi | flags), rp, ldr, gp, from, wp, bytes, stream);
   return st == LTX_OK ? THPVariable_Wrap(std::move(out)) : general();
 }
@@ -142,24 +212,35 @@ PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(out));
 }
 
-// one side of a rotation into a new tensor
+// one side of a rotation
 bool side(const at::Tensor& x, const at::Tensor& out, ltx_rotary_rows* r) {
   const int b = x.dim() == 4 ? 1 : 0;
-  if (x.stride(b + 2) != 1) return false;
+  if (x.stride(b + 2) != 1 || out.stride(b + 2) != 1) return false;
   *r = {x.const_data_ptr(), b ? x.stride(0) : 0, x.stride(b), x.stride(b + 1),
         out.data_ptr(),     b ? out.stride(0) : 0, out.stride(b), out.stride(b + 1), x.size(b + 1)};
   return true;
 }
 
-// rotary(q, k or None, positions, inv_freq, flags, factor, device, stream) -> (q', k' or None)
+// an output that the caller gave for x
+bool fits(const at::Tensor& out, const at::Tensor& x, const at::Tensor* other, const at::Tensor& pos,
+          const at::Tensor& inv) {
+  return out.scalar_type() == x.scalar_type() && out.sizes() == x.sizes() && out.get_device() == x.get_device() &&
+         out.is_cuda() && distinct(out) && (same_view(out, x) || apart(out, x)) && (!other || apart(out, *other)) &&
+         apart(out, pos) && apart(out, inv);
+}
+
+// rotary(q, k or None, positions, inv_freq, flags, factor, q' or None, k' or None, device, stream) -> (q', k' or None)
 PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 8 || !entry.rotary) return general();
-  const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *pos = tensor(a[2]), *inv = tensor(a[3]);
-  const int64_t flags = PyLong_AsLongLong(a[4]), device = PyLong_AsLongLong(a[6]);
+  if (n != 10 || !entry.rotary) return general();
+  const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *pos = tensor(a[2]), *inv = tensor(a[3]), *gq = tensor(a[6]),
+                   *gk = tensor(a[7]);
+  const int64_t flags = PyLong_AsLongLong(a[4]), device = PyLong_AsLongLong(a[8]);
   const double factor = PyFloat_AsDouble(a[5]);
-  void* stream = PyLong_AsVoidPtr(a[7]);
+  void* stream = PyLong_AsVoidPtr(a[9]);
   if (PyErr_Occurred()) return nullptr;
-  if (!q || (!k && a[1] != Py_None) || !pos || !inv || (q->dim() != 3 && q->dim() != 4)) return general();
+  if (!q || (!k && a[1] != Py_None) || !pos || !inv || (q->dim() != 3 && q->dim() != 4) ||
+      (!gq && a[6] != Py_None) || (!gk && a[7] != Py_None) || (gk && !k))
+    return general();
   const int64_t dims = q->dim(), batch = dims == 4 ? q->size(0) : 1, tokens = q->size(dims - 3), dh = q->size(dims - 1);
   const auto type = q->scalar_type(), ptype = pos->scalar_type();
   const int dtype = type == at::kBFloat16 ? 0 : (type == at::kHalf ? 1 : (type == at::kFloat ? 2 : -1));
@@ -176,8 +257,10 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (k && (k->dim() != dims || k->scalar_type() != type || !on(*k, device) || k->size(dims - 1) != dh ||
             k->size(dims - 3) != tokens || (dims == 4 && k->size(0) != batch) || k->size(dims - 2) < 1))
     return general();
-  at::Tensor oq = empty(q->sizes(), type, *q), ok;
-  if (k) ok = empty(k->sizes(), type, *k);
+  if ((gq && !fits(*gq, *q, k, *pos, *inv)) || (gk && !fits(*gk, *k, q, *pos, *inv)) || (gq && gk && !apart(*gq, *gk)))
+    return general();
+  at::Tensor oq = gq ? *gq : empty(q->sizes(), type, *q), ok;
+  if (k) ok = gk ? *gk : empty(k->sizes(), type, *k);
   ltx_rotary_rows rq, rk;
   if (!side(*q, oq, &rq) || (k && !side(*k, ok, &rk))) return general();
   if (entry.rotary(&rq, k ? &rk : nullptr, dtype, batch, tokens, dh, d, pos->const_data_ptr(), pos_type, own ? tokens : 0,

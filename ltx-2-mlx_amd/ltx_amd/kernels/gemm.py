@@ -515,13 +515,14 @@ def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int
     are bound by the host: the usual call is one native call, csrc/calls.cpp;
     this path, for all others, reads each tensor's properties once.)"""
     w, scale, bias = weight.w, weight.scale, weight.bias
-    if _lib.CALLS is not None and out is None and LAUNCH_HOOK is None:
+    if _lib.CALLS is not None and LAUNCH_HOOK is None:
         where = _lib.fast_stream(w)
         if where is not None:
             src, xs = (x.codes, x.scales) if isinstance(x, Mx4Rows) else (x, None)
             y = _lib.CALLS.linear(src, xs, w, scale, bias,
                                   _lib.GEMM_ROUND_THEN_BIAS if weight.qlinear and bias is not None else 0, epilogue,
-                                  residual, gate, -1 if sigmoid_from is None else max(int(sigmoid_from), 0), *where)
+                                  residual, gate, -1 if sigmoid_from is None else max(int(sigmoid_from), 0), out,
+                                  *where)
             if y is not None:
                 return y
     n, k, ldw, ldws = _check_mxfp4("weight", w, scale)

@@ -134,7 +134,7 @@ _ROTARY_ROWS = struct.Struct("9q").pack  # ltx_rotary_rows: x, its strides, out,
 def _rotary_side(name: str, x: torch.Tensor, out: torch.Tensor | None) -> tuple[bytes, torch.Tensor]:
     shape, st = x.shape, x.stride()
     if out is None:
-        out = torch.empty_like(x)
+        out = x.new_empty(shape)  # dense, whatever the strides of x
     elif out.shape != shape or out.dtype is not x.dtype:
         raise ValueError(f"{name}'s out must be {x.dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
     elif _lib.self_overlaps(out):
@@ -169,9 +169,10 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     if layout not in ROTARY_LAYOUTS:
         raise ValueError(f"layout must be one of {ROTARY_LAYOUTS}, got {layout!r}")
     flags = (_lib.ROTARY_INTERLEAVED if layout == "interleaved" else 0) | (_lib.ROTARY_TRANSPOSE if transpose else 0)
-    if _lib.CALLS is not None and out is None:
+    oq, ok = out if out is not None else (None, None)
+    if _lib.CALLS is not None:
         where = _lib.fast_stream(q)
-        rotated = None if where is None else _lib.CALLS.rotary(q, k, positions, inv_freq, flags, factor, *where)
+        rotated = None if where is None else _lib.CALLS.rotary(q, k, positions, inv_freq, flags, factor, oq, ok, *where)
         if rotated is not None:
             return rotated
     shape = q.shape
@@ -196,7 +197,6 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
                          f"{positions.dtype} {tuple(pos_shape)}")
     if not positions.is_contiguous():
         positions = positions.contiguous()
-    oq, ok = out if out is not None else (None, None)
     if k is None and ok is not None:
         raise ValueError("out has a tensor for k, but there is no k")
     sq, oq = _rotary_side("q", q, oq)

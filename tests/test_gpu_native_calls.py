@@ -123,3 +123,42 @@ def test_what_the_native_calls_refuse_raises():
               (q, q.half(), pos, inv), (q[..., :32], None, pos, inv), (q.double(), None, pos, inv)):
         with pytest.raises(ValueError):
             rope_ops.rotary(*a)
+
+
+def test_given_outputs(both):
+    from ltx_amd.kernels import gemm, rope_ops
+
+    g = torch.Generator(device=DEV).manual_seed(1)
+    w = gemm.make_weight(torch.randn(72, 256, generator=g, device=DEV).bfloat16(), torch.zeros(72, device=DEV), kind="mxfp4")
+    gate = torch.randn(72, generator=g, device=DEV)
+    for m in (1, 5, 40):
+        rows = torch.randn(m, 512, generator=g, device=DEV).bfloat16()
+        x, out, res = rows[:, :256], rows[:, 256:328], rows[:, 336:408]
+        want = gemm.linear(x, w, epilogue=gemm.EPI_RESIDUAL, residual=res, gate=gate)
+        got = both(lambda: gemm.linear(x, w, epilogue=gemm.EPI_RESIDUAL, residual=res, gate=gate, out=out))
+        assert got is out and torch.equal(out, want)
+        keep = rows.clone()
+        assert gemm.linear(x, w, epilogue=gemm.EPI_RESIDUAL, residual=res, gate=gate, out=res) is res  # in place
+        assert torch.equal(res, want)
+        keep[:, 336:408] = want
+        assert torch.equal(rows, keep)  # and nothing beside it
+        for bad in (rows[:, 192:264], rows[:, 328:400], out.float(), out[:, :64]):
+            with pytest.raises(ValueError):
+                gemm.linear(x, w, epilogue=gemm.EPI_RESIDUAL, residual=res, gate=gate, out=bad)
+
+    inv, f = rope_ops.rotary_frequencies(64)
+    for lead in ((1,), (9,), (2, 5)):
+        buf = torch.randn(*lead, 10, 64, generator=g, device=DEV).bfloat16()
+        q, k, rest = buf[..., :4, :], buf[..., 4:6, :], buf[..., 6:, :]
+        pos = torch.arange(lead[-1], device=DEV)
+        want = rope_ops.rotary(q, k, pos, inv)
+        keep = buf.clone()
+        got = both(lambda: rope_ops.rotary(q, k, pos, inv, out=(rest, None)))
+        assert got[0] is rest and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        keep[..., 6:, :] = want[0]
+        got = rope_ops.rotary(q, k, pos, inv, out=(q, k))
+        keep[..., :4, :], keep[..., 4:6, :] = want
+        assert got[0] is q and got[1] is k and torch.equal(buf, keep)
+        for bad in ((buf[..., 1:5, :], k), (k, q), (q, buf[..., 3:5, :]), (q[..., :1, :].expand(q.shape), k)):
+            with pytest.raises(ValueError):
+                rope_ops.rotary(q, k, pos, inv, out=bad)
