@@ -12,13 +12,18 @@
 // cosines and sines once into LDS (one pair per thread) and then streams the
 // heads.  The angle is formed and reduced to a fraction of a turn in fp64: at
 // position 10^6 an fp32 angle has lost 0.06 of a radian.
+// Measured: 3456 tokens x 64 heads of 128 bf16 21.5 us (5.3 TB/s), 14640 x 40 heads
+// of 128 bf16 56-59 (5.1-5.3 TB/s), 14639 x 40 heads of 64 fp32 56 (5.3 TB/s), 14639 x
+// 9 heads of 64 bf16 11 (3.1 TB/s), one token 4.
 #include <type_traits>
 
 #include "ltx_common.h"
 
 namespace ltx {
 
-constexpr int kRotThreads = 256, kRotTokens = 4, kRotMaxDim = 512;
+constexpr int kRotThreads = 256, kRotTokens = 16, kRotMaxDim = 512;
+constexpr int kRotTable = 2048;  // cosines (and sines) of a workgroup
+constexpr int64_t kRotBlocks = (1 << 24) - 1;  // a launch has fewer than 2^32 threads
 
 struct RotArgs {
   ltx_rotary_rows side[2];
@@ -31,6 +36,7 @@ struct RotArgs {
   float factor;
   int transpose;
   int per_block;  // tokens of a workgroup
+  int table;      // table entries of a token: its pairs, up to a multiple of 4
 };
 
 __device__ __forceinline__ double rot_position(const RotArgs& p, int64_t i) {
@@ -62,8 +68,7 @@ template <typename T, int VEC, bool INTERLEAVED>
 __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs p) {
   using V = RotVec<T, VEC>;
   constexpr bool NEIGHBOURS = INTERLEAVED && VEC > 1;  // a vector holds whole pairs
-  __shared__ __attribute__((aligned(16))) float cs[kRotTokens][kRotMaxDim / 2];
-  __shared__ __attribute__((aligned(16))) float sn[kRotTokens][kRotMaxDim / 2];
+  __shared__ __attribute__((aligned(16))) float cs[kRotTable], sn[kRotTable];
   __shared__ int64_t row_x[2][kRotTokens], row_out[2][kRotTokens];
   const int pairs = p.rotary / 2;
   const int64_t all = p.batch * p.tokens;
@@ -77,8 +82,8 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs p) {
     turns -= rint(turns);
     float s, c;
     sincospif((float)(2.0 * turns), &s, &c);
-    cs[t][j] = c * p.factor;
-    sn[t][j] = (p.transpose ? -s : s) * p.factor;
+    cs[t * p.table + j] = c * p.factor;
+    sn[t * p.table + j] = (p.transpose ? -s : s) * p.factor;
   }
   if (threadIdx.x < 2 * kRotTokens) {
     const int side = threadIdx.x / kRotTokens, t = threadIdx.x % kRotTokens;
@@ -143,8 +148,8 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs p) {
       for (int e = 0; e < kRotBatch; ++e) {
         if (at[e] >= count) break;
         if (c0[e] < p.rotary) {
-          const float* cv = cs[at[e]];
-          const float* sv = sn[at[e]];
+          const float* cv = (const float*)__builtin_assume_aligned(cs + at[e] * p.table, 16);
+          const float* sv = (const float*)__builtin_assume_aligned(sn + at[e] * p.table, 16);
           if constexpr (NEIGHBOURS) {
 #pragma unroll
             for (int k = 0; k < VEC / 2; ++k) {
@@ -170,6 +175,22 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs p) {
       }
     }
   }
+}
+
+// Tokens of a workgroup: a power of two, of up to 48 KiB of heads (fp32, with half
+// the arithmetic per byte: 32), where 448 workgroups remain, 640 of more than 4 tokens.
+// Fewer tokens wait for a table too often, more leave the CUs uneven.  1 / 2 / 4 / 16 tokens: 14639 x 64 heads
+// of 128 bf16 100 / 90 / 91 us, x 9 heads of 64 bf16 45 / 26 / 17 / 11; 2 / 4 tokens: 14640 x
+// 40 heads of 128 bf16 62 / 56, x 40 heads of 64 fp32 52 / 56, 4096 x 40 heads of 128
+// bf16 18 / 16; 1 / 2: 256 x 64 heads of 128 bf16 5.6 / 6.5, 1000 x 64 heads 8.6 / 8.4;
+// 8 / 16: 9000 x 16 heads of 80 fp16 12.4 / 14.0.
+static int rot_tokens(int64_t all, int64_t token_bytes, int size, int table) {
+  const int64_t most = size == 2 ? 49152 : 32768;
+  int n = 1;
+  while (2 * n <= kRotTokens && 2 * n * table <= kRotTable &&
+         ((2 * n * token_bytes <= most && 2 * n <= all / (n < 4 ? 448 : 640)) || all / n > kRotBlocks))
+    n *= 2;
+  return n;
 }
 
 template <typename T, int VEC>
@@ -225,7 +246,7 @@ extern "C" int ltx_rotary(const ltx_rotary_rows* q, const ltx_rotary_rows* k, in
   }
   if (p.side[0].heads == 0 && p.side[1].heads == 0) return LTX_OK;
   if (batch == 0 || tokens == 0) return LTX_OK;
-  if (tokens > INT64_MAX / 2 / batch) return LTX_ERR_UNSUPPORTED;
+  if (tokens > 4 * kRotBlocks / batch) return LTX_ERR_UNSUPPORTED;  // (4 tokens of any width fit a workgroup)
   int vec = (int)(16 / size);
   while (vec > 1 && (bits & (vec - 1))) vec >>= 1;
   p.batch = batch;
@@ -239,9 +260,9 @@ extern "C" int ltx_rotary(const ltx_rotary_rows* q, const ltx_rotary_rows* k, in
   p.factor = (float)factor;
   p.transpose = (flags & LTX_ROTARY_TRANSPOSE) != 0;
   const int64_t all = batch * tokens;
-  p.per_block = all >= 4096 ? kRotTokens : (all >= 2048 ? 2 : 1);
+  p.table = (int)(rotary_dim / 2 + 3) / 4 * 4;
+  p.per_block = rot_tokens(all, (p.side[0].heads + p.side[1].heads) * head_dim * (int64_t)size, (int)size, p.table);
   const int64_t blocks = (all + p.per_block - 1) / p.per_block;
-  if (blocks > (1 << 24) - 1) return LTX_ERR_UNSUPPORTED;  // a launch has fewer than 2^32 threads
   hipStream_t s = (hipStream_t)stream;
   if (dtype == 0) rotary_launch_vec<bf16>(p, vec, interleaved, (int)blocks, s);
   else if (dtype == 1) rotary_launch_vec<_Float16>(p, vec, interleaved, (int)blocks, s);
