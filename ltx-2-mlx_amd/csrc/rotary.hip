@@ -58,7 +58,8 @@ struct alignas(sizeof(T) * VEC) RotVec {
 //
 // An item is two vectors of a head: the two halves of VEC pairs, or two vectors
 // of neighbouring pairs, or two that are only copied (the second may repeat the
-// first at an odd end).  The items of the workgroup's tokens and heads form
+// first at an odd end), the second half a range after the first, so that the
+// lanes of a load lie side by side.  The items of the workgroup's tokens and heads form
 // one list that the threads go through, kBatch items each at a time: as many
 // loads in flight whatever the head layout (a loop over heads with a fixed item
 // per thread left them idle where tokens have few heads: 14639 tokens x 40 heads
@@ -95,7 +96,7 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs p) {
   __syncthreads();
 
   const int rot_vecs = NEIGHBOURS ? p.rotary / VEC : 2 * (pairs / VEC), copy_vecs = (p.head_dim - p.rotary) / VEC;
-  const int rot_items = (rot_vecs + 1) / 2, all_items = rot_items + (copy_vecs + 1) / 2;
+  const int rot_items = (rot_vecs + 1) / 2, copy_items = (copy_vecs + 1) / 2, all_items = rot_items + copy_items;
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     const ltx_rotary_rows& r = p.side[side];
@@ -118,11 +119,11 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs p) {
         if (t < count) {
           const int j = i - rot_items;
           if (j >= 0) {
-            c0[e] = p.rotary + 2 * j * VEC;
-            c1[e] = p.rotary + (2 * j + 1 < copy_vecs ? 2 * j + 1 : 2 * j) * VEC;
+            c0[e] = p.rotary + j * VEC;
+            c1[e] = p.rotary + (j + copy_items < copy_vecs ? j + copy_items : j) * VEC;
           } else if (NEIGHBOURS) {
-            c0[e] = 2 * i * VEC;
-            c1[e] = (2 * i + 1 < rot_vecs ? 2 * i + 1 : 2 * i) * VEC;
+            c0[e] = i * VEC;
+            c1[e] = (i + rot_items < rot_vecs ? i + rot_items : i) * VEC;
           } else {
             c0[e] = INTERLEAVED ? 2 * i : i * VEC;
             c1[e] = INTERLEAVED ? 2 * i + 1 : i * VEC + pairs;
