@@ -106,7 +106,8 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
 // A workgroup encodes 16 rows x 512 k, a wave a row at a time (lane l elements
 // 8 l .. 8 l + 7, lanes 4 b .. 4 b + 3 forming block b).  The scale words of a
 // k range are contiguous over rows, so they meet in LDS and leave as 64-byte
-// pieces.
+// pieces.  Bound by HBM: 14640 x 4096 bf16 25 us (6.0 TB/s), the decoder 24 (6.6);
+// 68 x 2048 4.1 and 2.6, a launch.
 constexpr int kQ4Rows = 16;
 constexpr int64_t kQ4Blocks = (1 << 24) - 1;  // of 256 threads: a launch has fewer than 2^32
 template <typename T>
