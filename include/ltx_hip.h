@@ -402,8 +402,8 @@ int ltx_gemm_mx_gelu_mxfp8(const uint8_t* A, int64_t lda, const uint8_t* a_scale
  * (v_mfma_scale_f32_32x32x64_f8f6f4).  K % 128 == 0, N % 8 == 0, operands
  * below 2 GiB each.
  * fp32 accumulation; epilogues LTX_GEMM_EPI_*, LTX_GEMM_ROUND_THEN_BIAS and
- * sigmoid_from as above, except that GELU and the head gate act on the fp32
- * value (no bf16 rounding before them).  Code and row strides 16-byte
+ * sigmoid_from as above, except that GELU, the head gate and EPI_RESIDUAL act
+ * on the fp32 value (no bf16 rounding before them).  Code and row strides 16-byte
  * multiples, pointers 16-byte aligned (bias and gate 4).
  * At most 2^27 rows or columns and 2^34 outputs.
  * Products of few tiles split K: they need `workspace` (device memory, 16-byte

@@ -2,7 +2,7 @@
 // weights, MXFP8 x MXFP8; gemm_fp4.hip: MXFP4 weights) and its launches.
 #pragma once
 
-#include "gemm_common.h"
+#include "gemm_fp4.h"
 
 namespace ltx {
 
@@ -670,6 +670,13 @@ __global__ __launch_bounds__(kG8Threads, 1) void gemm8_kernel(GemmArgs p) {
   const int gn2 = n0 + wn * WN + ch * 8;
   const bool col_ok = gn2 < p.N;
   char* E = lds + wave * EPI_WAVE;
+  if constexpr (FP4 && RESID) {
+    static_assert(EPI_WAVE == TM16 / 2 * 4096 && WN == 64, "half the row blocks per pass");
+    fp4_residual_rows<EPI, TM16, TM16 / 2>(
+        p, E, col_lds + wn * WN, col_lds + BN + wn * WN, m0 + wm * WM, n0 + wn * WN, lane,
+        [&](int i, int j) __attribute__((always_inline)) { return acc[i][j]; });
+    return;
+  }
   auto phase1 = [&](auto sig_tag, auto rtb_tag) {
     constexpr bool SIG = decltype(sig_tag)::value;
     constexpr bool RTB = decltype(rtb_tag)::value;

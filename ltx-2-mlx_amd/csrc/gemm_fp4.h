@@ -15,15 +15,13 @@
 
 namespace ltx {
 
-// Four consecutive columns n .. n + 3 of output row m from their fp32 sums.
-// MXFP4 products reproduce no reference arithmetic, so GELU and the head gate
-// act on the fp32 value, without the other formats' bf16 rounding before them.
-// A residual epilogue keeps that rounding of the branch (its tiles are staged
-// as bf16 rows).
+// Four consecutive columns n .. n + 3 of an output row from their fp32 sums, up
+// to the residual.  MXFP4 products reproduce no reference arithmetic, so GELU, the
+// head gate and the gated residual act on the fp32 value, without the other
+// formats' bf16 rounding before them (EPI_RESIDUAL_ROUND is the form that rounds).
 // SIG: columns from sig_from on may be among these; RTB: round_then_bias.
 template <int EPI, bool SIG, bool RTB>
-__device__ __forceinline__ bf16x4 fp4_branch4(const GemmArgs& p, f32x4 a, f32x4 bias, int n) {
-  bf16x4 v;
+__device__ __forceinline__ f32x4 fp4_branch4(const GemmArgs& p, f32x4 a, f32x4 bias, int n) {
   float y[4] = {a[0], a[1], a[2], a[3]};
   if (RTB) {
     round_bf2(y[0], y[1]);
@@ -39,13 +37,13 @@ __device__ __forceinline__ bf16x4 fp4_branch4(const GemmArgs& p, f32x4 a, f32x4 
       asm("" : "+v"(g));
       y[e] = n + e >= p.sig_from ? g : y[e];
     }
-    v[e] = (bf16)y[e];
   }
-  return v;
+  return f32x4{y[0], y[1], y[2], y[3]};
 }
+__device__ __forceinline__ bf16x4 fp4_bf16(f32x4 y) { return bf16x4{(bf16)y[0], (bf16)y[1], (bf16)y[2], (bf16)y[3]}; }
 template <int EPI>
-__device__ __forceinline__ bf16 fp4_residual(bf16 y, bf16 r, float g) {
-  return (bf16)(EPI == LTX_GEMM_EPI_RESIDUAL ? fmaf(g, (float)y, (float)r) : round_bf((float)y * g) + (float)r);
+__device__ __forceinline__ bf16 fp4_residual(float y, bf16 r, float g) {
+  return (bf16)(EPI == LTX_GEMM_EPI_RESIDUAL ? fmaf(g, y, (float)r) : round_bf(round_bf(y) * g) + (float)r);
 }
 template <int EPI>
 __device__ __forceinline__ void fp4_store4(const GemmArgs& p, f32x4 a, int m, int n) {
@@ -54,13 +52,72 @@ __device__ __forceinline__ void fp4_store4(const GemmArgs& p, f32x4 a, int m, in
 #pragma unroll
     for (int e = 0; e < 4; ++e) bias[e] = p.bias[n + e];
   constexpr bool SIG = EPI == LTX_GEMM_EPI_BIAS;
-  bf16x4 v = p.round_then_bias ? fp4_branch4<EPI, SIG, true>(p, a, bias, n) : fp4_branch4<EPI, SIG, false>(p, a, bias, n);
+  const f32x4 y = p.round_then_bias ? fp4_branch4<EPI, SIG, true>(p, a, bias, n) : fp4_branch4<EPI, SIG, false>(p, a, bias, n);
+  bf16x4 v = fp4_bf16(y);
   if constexpr (EPI == LTX_GEMM_EPI_RESIDUAL || EPI == LTX_GEMM_EPI_RESIDUAL_ROUND) {
     const bf16x4 r = *reinterpret_cast<const bf16x4*>(p.R + (int64_t)m * p.ldr + n);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = fp4_residual<EPI>(v[e], r[e], p.gate[n + e]);
+    for (int e = 0; e < 4; ++e) v[e] = fp4_residual<EPI>(y[e], r[e], p.gate[n + e]);
   }
   *reinterpret_cast<bf16x4*>(p.C + (int64_t)m * p.ldc + n) = v;
+}
+
+// Residual epilogue of a wave that holds NB x 4 accumulator blocks of 16 x 16 (lane
+// (r16, q): row r16, columns 4 q .. 4 q + 3), rows row0 on and columns col0 on; acc(i,
+// j) is block (i, j), bias and gate the wave's 64 columns.  The branch stays fp32: PASS
+// row blocks at a time go through PASS * 4 KiB of LDS, which only this wave uses, in
+// rows of 256 bytes with their 16-byte chunks XORed by the row, and come back as rows of
+// eight columns per lane.  All residual rows are read before the first is written.
+template <int EPI, int NB, int PASS, class Acc>
+__device__ __forceinline__ void fp4_residual_rows(const GemmArgs& p, char* E, const float* bias, const float* gate,
+                                                  int row0, int col0, int lane, Acc acc) {
+  static_assert(NB % PASS == 0, "whole passes");
+  const int r16 = lane & 15, q = lane >> 4, ch = lane & 7, rsub = lane >> 3;
+  const int gn = col0 + ch * 8;
+  const bool ok = gn < p.N;  // N % 8 == 0
+  bf16x8 res[NB * 2];
+  float g8[8];
+  auto stage = [&](int i0, auto rtb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4 b = *reinterpret_cast<const f32x4*>(bias + j * 16 + 4 * q);
+#pragma unroll
+      for (int i = 0; i < PASS; ++i) {
+        const int row = i * 16 + r16;
+        *reinterpret_cast<f32x4*>(E + row * 256 + (((4 * j + q) ^ row) & 15) * 16) =
+            fp4_branch4<EPI, false, decltype(rtb)::value>(p, acc(i0 + i, j), b, 0);
+      }
+    }
+  };
+#pragma unroll
+  for (int i0 = 0; i0 < NB; i0 += PASS) {
+    if (p.round_then_bias) stage(i0, std::true_type{});
+    else stage(i0, std::false_type{});
+    if (i0 == 0) {  // (after the first accumulators are in LDS: fewer live registers)
+#pragma unroll
+      for (int it = 0; it < NB * 2; ++it) {
+        int gm = row0 + it * 8 + rsub;
+        gm = gm < p.M ? gm : p.M - 1;
+        res[it] = *reinterpret_cast<const bf16x8*>(p.R + (int64_t)gm * p.ldr + (ok ? gn : 0));
+      }
+      const f32x4 ga = *reinterpret_cast<const f32x4*>(gate + ch * 8), gb = *reinterpret_cast<const f32x4*>(gate + ch * 8 + 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g8[e] = e < 4 ? ga[e & 3] : gb[e & 3];
+    }
+    wait_lgkmcnt0();
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int it = 0; it < PASS * 2; ++it) {
+      const int ml = it * 8 + rsub, gm = row0 + i0 * 16 + ml;
+      const f32x4 a = *reinterpret_cast<const f32x4*>(E + ml * 256 + (((2 * ch) ^ ml) & 15) * 16);
+      const f32x4 b = *reinterpret_cast<const f32x4*>(E + ml * 256 + (((2 * ch + 1) ^ ml) & 15) * 16);
+      bf16x8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = fp4_residual<EPI>(e < 4 ? a[e & 3] : b[e & 3], res[2 * i0 + it][e], g8[e]);
+      if (gm < p.M && ok) *reinterpret_cast<bf16x8*>(p.C + (int64_t)gm * p.ldc + gn) = v;
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
 }
 
 // sum of `splits` partial products (fp32, split order) and the epilogue

@@ -33,7 +33,7 @@
 // -> 2048, 16 workgroups: 43 bytes of weights per ns).  A deeper ring changed
 // nothing.  MXFP4 weights (half the weight bytes, in as many requests) run at the
 // 8-bit codes' rate: 68 x 2048 -> 8192 12 us, 1296 x 4096 -> 4096 40 in 192-row tiles.
-#include "gemm_common.h"
+#include "gemm_fp4.h"
 
 namespace ltx {
 
@@ -76,7 +76,8 @@ struct KgCfg {
   // after the loop: the exchanged accumulator halves, the bf16 output tile,
   // the column values
   static constexpr int X_WAVE = HM * AN * 64 * 16, X_BYTES = 8 * X_WAVE;
-  static constexpr int E_WAVE = HM * 16 * WN * 2;
+  // (MXFP4 residuals: one row block of fp32 at a time)
+  static constexpr int E_WAVE = FP4 && HM == 1 ? 16 * WN * 4 : HM * 16 * WN * 2;
   static constexpr int COL_OFF = X_BYTES + 8 * E_WAVE;
   static constexpr int EPI = COL_OFF + 2 * BN * 4;
   static constexpr int LDS_BYTES = RING > EPI ? RING : EPI;
@@ -459,6 +460,12 @@ __global__ __launch_bounds__(kKgThreads, 1) void gemm_kg_kernel(GemmArgs p) {
     }
     return;
   } else {
+    if constexpr (FP4 && RESID) {
+      fp4_residual_rows<EPI, HM, 1>(p, lds + Cfg::X_BYTES + wave * Cfg::E_WAVE, col_lds + wn * WN,
+                                    col_lds + BN + wn * WN, row0, col0, lane,
+                                    [&](int i, int j) __attribute__((always_inline)) { return sum[i][j]; });
+      return;
+    }
     // ---- epilogue: bf16 tile through LDS (128-byte rows, 16-byte chunks
     // XORed by (row / 2) % 8), then whole 16-byte chunks of rows
     constexpr int ITS = HM * 2;  // 8 rows of 8 chunks per pass

@@ -42,7 +42,10 @@ struct M4Tile {
   // wave without one of its own repeats one)
   static constexpr int S_DMA = (SA_DMA + SB_DMA + WAVES - 1) / WAVES;
   static constexpr int DMA = A_DMA + B_DMA + S_DMA;
-  static constexpr int EPI_ROWB = WN * 2, EPI_WAVE = WM * EPI_ROWB;
+  // staged output rows of a wave: its tile as bf16; a residual's branch as fp32,
+  // R_PASS 32-row blocks at a time
+  static constexpr int EPI_ROWB = WN * 2, R_PASS = AM > 1 ? AM / 2 : 1, R_ROWB = WN * 4;
+  static constexpr int EPI_WAVE = WM * EPI_ROWB > R_PASS * 32 * R_ROWB ? WM * EPI_ROWB : R_PASS * 32 * R_ROWB;
   static constexpr int RING = NST * STAGE, EPI = WAVES * EPI_WAVE;
   static constexpr int LDS_BYTES = RING > EPI ? RING : EPI;
   static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole direct-load instructions per wave");
@@ -282,61 +285,92 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
     }
     return;
   } else {
-    // ---- epilogue: bf16 tile through LDS, 16-byte chunks XORed by the row so
-    // that both the 8-byte writes and the 16-byte reads spread over the banks
+    // ---- epilogue: the tile through LDS, 16-byte chunks XORed by the row so that
+    // both the writes and the 16-byte reads spread over the banks
     __syncthreads();
-    constexpr int CH = WN / 8, RPI = 64 / CH, ITS = WM / RPI;
-    auto swz = [](int row) { return CH == 16 ? row & 15 : (CH == 8 ? (row >> 1) & 7 : (row >> 2) & 3); };
-    char* E = lds + wave * Cfg::EPI_WAVE;
-    auto phase1 = [&](auto sig_tag, auto rtb_tag) __attribute__((always_inline)) {
+    constexpr int CH = WN / 8, RPI = 64 / CH;
+    char* E = lds + wave * Cfg::EPI_WAVE;  // a wave reads back only what it wrote itself
+    const int ch = lane % CH, rsub = lane / CH;
+    const int gn = n0 + wn * WN + ch * 8;
+    // the values of columns 8 g + 4 h on of fragment column j, rows of block i, to put(i, j, g, value)
+    auto branch = [&](int i0, int i1, auto sig_tag, auto rtb_tag, auto put) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < AN; ++j) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const int gn = n0 + wn * WN + j * 32 + 8 * g + 4 * h;
+          const int c = n0 + wn * WN + j * 32 + 8 * g + 4 * h;
           f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
-          if (p.bias && gn < p.N)
+          if (p.bias && c < p.N)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) bias[e] = p.bias[gn + e];
+            for (int e = 0; e < 4; ++e) bias[e] = p.bias[c + e];
 #pragma unroll
           for (int i = 0; i < AM; ++i) {
-            const int row = i * 32 + r32;
+            if (i < i0 || i >= i1) continue;
             const f32x4 y = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-            *reinterpret_cast<bf16x4*>(E + row * Cfg::EPI_ROWB + ((4 * j + g) ^ swz(row)) * 16 + h * 8) =
-                fp4_branch4<EPI, decltype(sig_tag)::value, decltype(rtb_tag)::value>(p, y, bias, gn);
+            put(i, j, g, fp4_branch4<EPI, decltype(sig_tag)::value, decltype(rtb_tag)::value>(p, y, bias, c));
           }
         }
       }
     };
-    const bool sig = EPI == LTX_GEMM_EPI_BIAS && n0 + wn * WN + WN > p.sig_from;
-    if (p.round_then_bias) {
-      if (sig) phase1(std::true_type{}, std::true_type{});
-      else phase1(std::false_type{}, std::true_type{});
-    } else {
-      if (sig) phase1(std::true_type{}, std::false_type{});
-      else phase1(std::false_type{}, std::false_type{});
-    }
-    // a wave reads back only what it wrote itself
-    wait_lgkmcnt0();
-    __builtin_amdgcn_wave_barrier();
-    const int ch = lane % CH, rsub = lane / CH;
-    const int gn = n0 + wn * WN + ch * 8;
-    if (gn >= p.N) return;
-    float g8[8];
-    if constexpr (RESID)
+    if constexpr (RESID) {
+      constexpr int PASS = Cfg::R_PASS, ROWB = Cfg::R_ROWB, C4 = WN / 4, ITS = PASS * 32 / RPI;
+      float g8[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) g8[e] = p.gate[gn + e];
+      for (int e = 0; e < 8; ++e) g8[e] = gn < p.N ? p.gate[gn + e] : 0.0f;
 #pragma unroll
-    for (int it = 0; it < ITS; ++it) {
-      const int row = it * RPI + rsub, gm = m0 + wm * WM + row;
-      if (gm >= p.M) break;
-      bf16x8 v = *reinterpret_cast<const bf16x8*>(E + row * Cfg::EPI_ROWB + (ch ^ swz(row)) * 16);
-      if constexpr (RESID) {
-        const bf16x8 r = *reinterpret_cast<const bf16x8*>(p.R + (int64_t)gm * p.ldr + gn);
+      for (int i0 = 0; i0 < AM; i0 += PASS) {
+        auto put = [&](int i, int j, int g, f32x4 y) __attribute__((always_inline)) {
+          const int row = (i - i0) * 32 + r32;
+          *reinterpret_cast<f32x4*>(E + row * ROWB + (((8 * j + 2 * g + h) ^ row) & (C4 - 1)) * 16) = y;
+        };
+        if (p.round_then_bias) branch(i0, i0 + PASS, std::false_type{}, std::true_type{}, put);
+        else branch(i0, i0 + PASS, std::false_type{}, std::false_type{}, put);
+        bf16x8 res[ITS];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fp4_residual<EPI>(v[e], r[e], g8[e]);
+        for (int it = 0; it < ITS; ++it) {
+          int gm = m0 + wm * WM + i0 * 32 + it * RPI + rsub;
+          gm = gm < p.M ? gm : p.M - 1;
+          res[it] = *reinterpret_cast<const bf16x8*>(p.R + (int64_t)gm * p.ldr + (gn < p.N ? gn : 0));
+        }
+        wait_lgkmcnt0();
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) {
+          const int row = it * RPI + rsub, gm = m0 + wm * WM + i0 * 32 + row;
+          const f32x4 a = *reinterpret_cast<const f32x4*>(E + row * ROWB + (((2 * ch) ^ row) & (C4 - 1)) * 16);
+          const f32x4 b = *reinterpret_cast<const f32x4*>(E + row * ROWB + (((2 * ch + 1) ^ row) & (C4 - 1)) * 16);
+          bf16x8 v;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = fp4_residual<EPI>(e < 4 ? a[e & 3] : b[e & 3], res[it][e], g8[e]);
+          if (gm < p.M && gn < p.N) *reinterpret_cast<bf16x8*>(p.C + (int64_t)gm * p.ldc + gn) = v;
+        }
+        __builtin_amdgcn_wave_barrier();
       }
-      *reinterpret_cast<bf16x8*>(p.C + (int64_t)gm * p.ldc + gn) = v;
+    } else {
+      constexpr int ITS = WM / RPI;
+      auto swz = [](int row) { return CH == 16 ? row & 15 : (CH == 8 ? (row >> 1) & 7 : (row >> 2) & 3); };
+      auto put = [&](int i, int j, int g, f32x4 y) __attribute__((always_inline)) {
+        const int row = i * 32 + r32;
+        *reinterpret_cast<bf16x4*>(E + row * Cfg::EPI_ROWB + ((4 * j + g) ^ swz(row)) * 16 + h * 8) = fp4_bf16(y);
+      };
+      const bool sig = EPI == LTX_GEMM_EPI_BIAS && n0 + wn * WN + WN > p.sig_from;
+      if (p.round_then_bias) {
+        if (sig) branch(0, AM, std::true_type{}, std::true_type{}, put);
+        else branch(0, AM, std::false_type{}, std::true_type{}, put);
+      } else {
+        if (sig) branch(0, AM, std::true_type{}, std::false_type{}, put);
+        else branch(0, AM, std::false_type{}, std::false_type{}, put);
+      }
+      wait_lgkmcnt0();
+      __builtin_amdgcn_wave_barrier();
+      if (gn >= p.N) return;
+#pragma unroll
+      for (int it = 0; it < ITS; ++it) {
+        const int row = it * RPI + rsub, gm = m0 + wm * WM + row;
+        if (gm >= p.M) break;
+        *reinterpret_cast<bf16x8*>(p.C + (int64_t)gm * p.ldc + gn) =
+            *reinterpret_cast<const bf16x8*>(E + row * Cfg::EPI_ROWB + (ch ^ swz(row)) * 16);
+      }
     }
   }
 }

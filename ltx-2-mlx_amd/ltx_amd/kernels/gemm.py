@@ -24,8 +24,9 @@ activations' E4M3 rounding moves outputs by a few percent of their range.
 MXFP4 (E2M1 codes, an E8M0 scale per 32 along K) has no counterpart in the
 reference: weights at half MXFP8's bytes, times bf16 activations in
 :func:`linear`, or times MXFP4 activations (:class:`Mx4Rows`, from
-:func:`quantize_rows_mxfp4`) on the scaled FP4 MFMA.  Its GELU and head gate
-act on the fp32 value, without the bf16 rounding before them.
+:func:`quantize_rows_mxfp4`) on the scaled FP4 MFMA.  Its GELU, head gate
+and ``EPI_RESIDUAL`` act on the fp32 value, without the bf16 rounding before
+them.
 """
 
 from __future__ import annotations
