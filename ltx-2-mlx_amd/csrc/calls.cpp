@@ -4,8 +4,11 @@
 // the call from Python takes 7-10, from here 4-6.
 //
 // Every function does the usual case only and returns None for anything else
-// (an unusual stride, a type or size that does not fit, a failed launch); the
-// caller's Python path then does the work or raises.  No state is kept.
+// (an unusual stride, a type or size that does not fit, a refusal of the entry
+// point), all of it before any launch; the caller's Python path then does the
+// work or raises.  Once something may have been launched, a status other than OK
+// comes back as an int, which the caller raises: the call is never made twice (in
+// place it would be applied twice).  No state is kept.
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
@@ -29,7 +32,25 @@ PyObject* general() { Py_RETURN_NONE; }
 
 // the tensor of an argument that is exactly one; null otherwise
 const at::Tensor* tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
-bool on(const at::Tensor& t, int64_t device) { return t.is_cuda() && t.get_device() == device; }
+// (device -1: host tensors, for entry points that are no GPU's)
+bool on(const at::Tensor& t, int64_t device) { return t.get_device() == device && (t.is_cuda() || device < 0); }
+
+// what a function returns for the entry point's status: `result` (a new
+// reference, null with an error set) if OK, None after a refusal, else the status
+PyObject* outcome(int status, PyObject* result) {
+  if (status == LTX_OK || !result) return result;
+  Py_DECREF(result);
+  if (status == LTX_ERR_INVALID_ARG || status == LTX_ERR_UNSUPPORTED || status == LTX_ERR_ALIGNMENT) return general();
+  return PyLong_FromLong(status);
+}
+PyObject* pair(at::Tensor a, at::Tensor b) {
+  PyObject* pa = THPVariable_Wrap(std::move(a));
+  PyObject* pb = b.defined() ? THPVariable_Wrap(std::move(b)) : (Py_INCREF(Py_None), Py_None);
+  PyObject* r = pa && pb ? PyTuple_Pack(2, pa, pb) : nullptr;
+  Py_XDECREF(pa);
+  Py_XDECREF(pb);
+  return r;
+}
 
 at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const at::Tensor& like) {
   return at::empty(size, like.options().dtype(type));
@@ -162,13 +183,15 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t from = sig < 0 ? N : sig;
   const auto* wc = static_cast<const uint8_t*>(w->const_data_ptr());
   const auto* wsp = static_cast<const uint32_t*>(ws->const_data_ptr());
+  PyObject* result = THPVariable_Wrap(out);  // (before the launch: it may fail)
+  if (!result) return nullptr;
   const int st = xs ? entry.mx4(static_cast<const uint8_t*>(x->const_data_ptr()), lda,
                                 static_cast<const uint32_t*>(xs->const_data_ptr()), xs->stride(0), wc, ldw, wsp,
                                 ws->stride(0), bp, out.data_ptr(), ldc, M, N, K, (int)(epi | flags), rp, ldr, gp, from, wp,
                                 bytes, stream)
                     : entry.gemm(x->const_data_ptr(), lda, wc, ldw, wsp, ws->stride(0), bp, out.data_ptr(), ldc, M, N, K,
                                  (int)(epi | flags), rp, ldr, gp, from, wp, bytes, stream);
-  return st == LTX_OK ? THPVariable_Wrap(std::move(out)) : general();
+  return outcome(st, result);
 }
 
 // quantize(x, device, stream) -> (codes, words)
@@ -185,14 +208,11 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (dtype < 0 || rows < 1 || k < 32 || k % 32 || ldx < k) return general();
   const int64_t ld = (rows + 3) / 4 * 4;
   at::Tensor codes = empty({rows, k / 2}, at::kByte, *x), words = empty({(k + 127) / 128, ld}, at::kInt, *x);
-  if (entry.quantize(x->const_data_ptr(), dtype, ldx, rows, k, static_cast<uint8_t*>(codes.data_ptr()), k / 2,
-                     static_cast<uint32_t*>(words.data_ptr()), ld, stream) != LTX_OK)
-    return general();
-  PyObject *c = THPVariable_Wrap(std::move(codes)), *s = THPVariable_Wrap(std::move(words));
-  PyObject* r = c && s ? PyTuple_Pack(2, c, s) : nullptr;
-  Py_XDECREF(c);
-  Py_XDECREF(s);
-  return r;
+  PyObject* result = pair(codes, words);
+  if (!result) return nullptr;
+  return outcome(entry.quantize(x->const_data_ptr(), dtype, ldx, rows, k, static_cast<uint8_t*>(codes.data_ptr()), k / 2,
+                                static_cast<uint32_t*>(words.data_ptr()), ld, stream),
+                 result);
 }
 
 // dequantize(codes, words, device, stream)
@@ -205,11 +225,13 @@ PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int64_t rows, k;
   if (!mxfp4(codes, words, device, &rows, &k) || rows < 1 || k < 1) return general();
   at::Tensor out = empty({rows, k}, at::kBFloat16, *codes);
-  if (entry.dequantize(static_cast<const uint8_t*>(codes->const_data_ptr()), rows > 1 ? codes->stride(0) : k / 2,
-                       static_cast<const uint32_t*>(words->const_data_ptr()), words->stride(0), rows, k, out.data_ptr(),
-                       k, stream) != LTX_OK)
-    return general();
-  return THPVariable_Wrap(std::move(out));
+  PyObject* result = THPVariable_Wrap(out);
+  if (!result) return nullptr;
+  return outcome(entry.dequantize(static_cast<const uint8_t*>(codes->const_data_ptr()),
+                                  rows > 1 ? codes->stride(0) : k / 2,
+                                  static_cast<const uint32_t*>(words->const_data_ptr()), words->stride(0), rows, k,
+                                  out.data_ptr(), k, stream),
+                 result);
 }
 
 // one side of a rotation
@@ -224,8 +246,8 @@ bool side(const at::Tensor& x, const at::Tensor& out, ltx_rotary_rows* r) {
 // an output that the caller gave for x
 bool fits(const at::Tensor& out, const at::Tensor& x, const at::Tensor* other, const at::Tensor& pos,
           const at::Tensor& inv) {
-  return out.scalar_type() == x.scalar_type() && out.sizes() == x.sizes() && out.get_device() == x.get_device() &&
-         out.is_cuda() && distinct(out) && (same_view(out, x) || apart(out, x)) && (!other || apart(out, *other)) &&
+  return out.scalar_type() == x.scalar_type() && out.sizes() == x.sizes() && out.device() == x.device() &&
+         distinct(out) && (same_view(out, x) || apart(out, x)) && (!other || apart(out, *other)) &&
          apart(out, pos) && apart(out, inv);
 }
 
@@ -263,18 +285,14 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (k) ok = gk ? *gk : empty(k->sizes(), type, *k);
   ltx_rotary_rows rq, rk;
   if (!side(*q, oq, &rq) || (k && !side(*k, ok, &rk))) return general();
-  if (entry.rotary(&rq, k ? &rk : nullptr, dtype, batch, tokens, dh, d, pos->const_data_ptr(), pos_type, own ? tokens : 0,
-                   inv->const_data_ptr<double>(), factor, (int)flags, stream) != LTX_OK)
-    return general();
-  PyObject* po = THPVariable_Wrap(std::move(oq));
-  PyObject* pk = k ? THPVariable_Wrap(std::move(ok)) : (Py_INCREF(Py_None), Py_None);
-  PyObject* r = po && pk ? PyTuple_Pack(2, po, pk) : nullptr;
-  Py_XDECREF(po);
-  Py_XDECREF(pk);
-  return r;
+  PyObject* result = pair(oq, ok);
+  if (!result) return nullptr;
+  return outcome(entry.rotary(&rq, k ? &rk : nullptr, dtype, batch, tokens, dh, d, pos->const_data_ptr(), pos_type,
+                              own ? tokens : 0, inv->const_data_ptr<double>(), factor, (int)flags, stream),
+                 result);
 }
 
-// a C++ exception (no memory for an output) becomes a Python one
+// a C++ exception (no memory for an output; nothing throws after a launch)
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   try {

@@ -220,6 +220,14 @@ def fast_stream(t: torch.Tensor) -> tuple[int, int] | None:
     return device, _raw_stream(device)
 
 
+def launched(result, name: str, detail: str = ""):
+    """The result of a native host call that did not pass the call on; a status
+    that it came back with raises."""
+    if type(result) is int:
+        raise LtxKernelError(name, result, detail)
+    return result
+
+
 def same_device(*tensors: torch.Tensor | None) -> int:
     """The GPU index of the given tensors; raises unless all are on one GPU."""
     device = tensors[0].get_device()

@@ -462,7 +462,7 @@ def quantize_rows_mxfp4(x: torch.Tensor) -> Mx4Rows:
         where = _lib.fast_stream(x)
         rows = None if where is None else _lib.CALLS.quantize(x, *where)
         if rows is not None:
-            return Mx4Rows(*rows)
+            return Mx4Rows(*_lib.launched(rows, "ltx_quantize_mxfp4"))
     k = x.shape[-1]
     dtype = _QUANT_DTYPES.get(x.dtype)
     if dtype is None:
@@ -493,7 +493,7 @@ def dequantize_rows_mxfp4(rows: Mx4Rows) -> torch.Tensor:
         where = _lib.fast_stream(codes)
         out = None if where is None else _lib.CALLS.dequantize(codes, scales, *where)
         if out is not None:
-            return out
+            return _lib.launched(out, "ltx_dequantize_mxfp4_bf16")
     m, k, ldq, lds = _check_mxfp4("dequantize_rows_mxfp4", codes, scales)
     out = codes.new_empty((m, k), dtype=torch.bfloat16)
     if m:
@@ -525,7 +525,7 @@ def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int
                                   residual, gate, -1 if sigmoid_from is None else max(int(sigmoid_from), 0), out,
                                   *where)
             if y is not None:
-                return y
+                return _lib.launched(y, "ltx_gemm_mxfp4_bf16" if xs is None else "ltx_gemm_mx4_bf16")
     n, k, ldw, ldws = _check_mxfp4("weight", w, scale)
     quantised = isinstance(x, Mx4Rows)
     if quantised:

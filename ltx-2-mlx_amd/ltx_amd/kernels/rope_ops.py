@@ -174,7 +174,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
         where = _lib.fast_stream(q)
         rotated = None if where is None else _lib.CALLS.rotary(q, k, positions, inv_freq, flags, factor, oq, ok, *where)
         if rotated is not None:
-            return rotated
+            return _lib.launched(rotated, "ltx_rotary")
     shape = q.shape
     dtype = _ROTARY_DTYPES.get(q.dtype)
     if dtype is None or not 3 <= len(shape) <= 4:

@@ -1,0 +1,95 @@
+"""The native host calls against stand-ins for the entry points, on host
+tensors: what they pass on, what they raise, and that nothing is launched twice."""
+
+from __future__ import annotations
+
+import ctypes
+import importlib.util
+import shutil
+
+import pytest
+import torch
+
+OK, INVALID, UNSUPPORTED, HIP, ALIGN = 0, -1, -2, -3, -4
+HOST = (-1, 0)  # device and stream of host tensors
+
+
+@pytest.fixture
+def calls(tmp_path, monkeypatch):
+    """A copy of the module whose entry points return ``calls.status`` and count,
+    taking the place of the library's (ltx_amd._lib.CALLS)."""
+    from ltx_amd import _lib
+
+    if not _lib.LIB_PATH.with_name("_calls.so").exists():
+        pytest.skip("_calls.so not built")
+    _lib.lib()
+    copy = tmp_path / "_calls.so"
+    shutil.copy(_lib.LIB_PATH.with_name("_calls.so"), copy)
+    spec = importlib.util.spec_from_file_location("stand_in._calls", copy)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+
+    class Calls:
+        status = OK
+        count = 0
+        native = module
+
+    state, keep = Calls(), []
+    for name in _lib._CALLS_ENTRIES:
+        size = name in _lib.SIZES
+
+        def stub(*_, size=size):
+            if size:
+                return 0
+            state.count += 1
+            return state.status
+
+        keep.append(ctypes.CFUNCTYPE(ctypes.c_int64 if size else ctypes.c_int, *_lib.SIGNATURES[name])(stub))
+    module.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in keep))
+    state.keep = keep
+    monkeypatch.setattr(_lib, "CALLS", module)
+    monkeypatch.setattr(_lib, "fast_stream", lambda t: HOST)
+    monkeypatch.setattr(_lib, "launch", lambda *a: pytest.fail("the call was made again"))
+    return state
+
+
+def _every_call():
+    from ltx_amd.kernels import gemm, rope_ops
+
+    w = gemm.LinearWeight("mxfp4", torch.zeros(64, 64, dtype=torch.uint8), torch.zeros(1, 64, dtype=torch.int32))
+    rows = gemm.Mx4Rows(torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(1, 4, dtype=torch.int32))
+    x = torch.zeros(4, 128, dtype=torch.bfloat16)
+    res, gate = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(64)
+    q, k, pos = torch.zeros(4, 2, 64), torch.zeros(4, 1, 64), torch.arange(4)
+    inv, _ = rope_ops.rotary_frequencies(64, device="cpu")
+    add = dict(epilogue=gemm.EPI_RESIDUAL, residual=res, gate=gate, out=res)
+    return [lambda: gemm.linear(x, w), lambda: gemm.linear(x, w, **add), lambda: gemm.linear(rows, w, **add),
+            lambda: gemm.quantize_rows_mxfp4(x), lambda: gemm.dequantize_rows_mxfp4(rows),
+            lambda: rope_ops.rotary(q, k, pos, inv), lambda: rope_ops.rotary(q, k, pos, inv, out=(q, k)),
+            lambda: rope_ops.rotary(q, None, pos, inv)]
+
+
+def test_a_failed_launch_raises_and_is_not_made_again(calls):
+    from ltx_amd import _lib
+
+    for status in (HIP, -5, 7):
+        for i, call in enumerate(_every_call()):
+            calls.status, calls.count = status, 0
+            with pytest.raises(_lib.LtxKernelError):
+                call()
+            assert calls.count == 1, (i, status)
+
+
+def test_a_launch_is_made_once(calls):
+    for i, call in enumerate(_every_call()):
+        calls.count = 0
+        assert call() is not None
+        assert calls.count == 1, i
+
+
+def test_a_refusal_goes_to_the_python_path(calls):
+    for status in (INVALID, UNSUPPORTED, ALIGN):
+        for call in _every_call():
+            calls.status = status
+            with pytest.raises(ValueError, match="on one GPU"):  # its checks, met by host tensors
+                call()
