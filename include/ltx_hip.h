@@ -393,7 +393,8 @@ int ltx_gemm_mx_gelu_mxfp8(const uint8_t* A, int64_t lda, const uint8_t* a_scale
  * in bytes; scale words (ceil(K / 128), ld), word [k / 128][row] holding the
  * E8M0 bytes of the row's four blocks of those 128 k, the first in its low
  * byte; ld (in words) at least the rows, a multiple of 4.  Bytes of a last
- * word that lie past K are not used, nor are words past the rows.  No
+ * word that lie past K are not used, nor are words past the rows; a word row is
+ * read up to the next multiple of 4 rows, the last one too.  No
  * counterpart in the reference, whose caches hold MXFP8.
  *
  * ltx_gemm_mxfp4_bf16: bf16 rows A (M, K) x MXFP4 weights (N, K), decoded to

@@ -62,6 +62,24 @@ static void check_pair_loads() {
   }
 }
 
+// Every 16-byte load of scale words, for the rows that tiles of `tile` rows ask for,
+// ends inside the operand's own words (rows up to a multiple of 4, whatever the
+// stride), and brings the words of the rows asked for wherever those exist.
+static void check_word_loads() {
+  for (int rows = 1; rows <= 600; rows += rows < 20 ? 1 : 29)
+    for (int words : {1, 2, 5})
+      for (int64_t ld : {int64_t((rows + 3) / 4 * 4), int64_t(1024)}) {
+        const int64_t own = ((words - 1) * ld + (rows + 3) / 4 * 4) * 4;
+        EXPECT(ltx::word_bytes(words, ld, rows), own);
+        for (int tile : {64, 128, 256})
+          for (int row = 0; row < (rows + tile - 1) / tile * tile; row += 4) {
+            const int piece = ltx::word_piece(row, rows);
+            EXPECT(piece >= 0 && piece % 4 == 0 && ((words - 1) * ld + piece) * 4 + 16 <= own, 1);
+            if (row < rows) EXPECT(piece, row);
+          }
+      }
+}
+
 int main(int argc, char** argv) {
   if (argc > 1 && std::strcmp(argv[1], "--overflow-selftest") == 0) {
     // proves the sanitizer is live: one byte past a heap block
@@ -84,6 +102,7 @@ int main(int argc, char** argv) {
   EXPECT(ltx_device_clock_stamp(reinterpret_cast<uint64_t*>(static_cast<char*>(m) + 4), nullptr), LTX_ERR_ALIGNMENT);
 
   check_pair_loads();
+  check_word_loads();
   static const char no_args[1024] = {};  // never read: refused before
   const ltx::GemmArgs& none = *reinterpret_cast<const ltx::GemmArgs*>(no_args);
   EXPECT(ltx::kg_launch(0, none, 5, 64, 1, nullptr), 0);  // the MX kernel's epilogue

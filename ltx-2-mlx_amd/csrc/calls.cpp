@@ -118,14 +118,22 @@ bool same_view(const at::Tensor& a, const at::Tensor& b) {
 }
 
 // dense-column (rows, K / 2) codes with scale words that cover them
-bool mxfp4(const at::Tensor* codes, const at::Tensor* words, int64_t device, int64_t* rows, int64_t* k) {
+// (`ld`: their row stride; that of an axis of one entry says nothing)
+bool mxfp4(const at::Tensor* codes, const at::Tensor* words, int64_t device, int64_t* rows, int64_t* k, int64_t* ld) {
   if (!codes || !words || codes->scalar_type() != at::kByte || words->scalar_type() != at::kInt || codes->dim() != 2 ||
       words->dim() != 2 || !on(*codes, device) || !on(*words, device))
     return false;
   *rows = codes->size(0);
   *k = codes->size(1) * 2;
+  *ld = words->size(0) > 1 ? words->stride(0) : (words->size(1) + 3) / 4 * 4;
   return codes->stride(1) == 1 && words->stride(1) == 1 && codes->stride(0) >= codes->size(1) &&
-         words->stride(0) >= words->size(1) && words->size(0) * 128 >= *k && words->size(1) >= *rows;
+         *ld >= words->size(1) && words->size(0) * 128 >= *k && words->size(1) >= *rows;
+}
+
+// whether the words' memory goes on to a multiple of 4 rows, as products read them
+bool whole_words(const at::Tensor& words, int64_t rows, int64_t k, int64_t ld) {
+  return rows % 4 == 0 || (words.storage_offset() + (k - 1) / 128 * ld + (rows + 3) / 4 * 4) * 4 <=
+                              static_cast<int64_t>(words.storage().nbytes());
 }
 
 // linear(x, x_words or None, codes, words, bias or None, flags, epilogue, residual or None, gate or None,
@@ -138,10 +146,10 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 device = PyLong_AsLongLong(a[11]);
   void* stream = PyLong_AsVoidPtr(a[12]);
   if (PyErr_Occurred()) return nullptr;
-  int64_t N, K, M, kx;
-  if (!x || (!xs && a[1] != Py_None) || (!bias && a[4] != Py_None) || (!given && a[10] != Py_None) || !mxfp4(w, ws, device, &N, &K)) return general();
+  int64_t N, K, M, kx, ldws, ldxs = 0;
+  if (!x || (!xs && a[1] != Py_None) || (!bias && a[4] != Py_None) || (!given && a[10] != Py_None) || !mxfp4(w, ws, device, &N, &K, &ldws)) return general();
   if (xs) {
-    if (!mxfp4(x, xs, device, &M, &kx)) return general();
+    if (!mxfp4(x, xs, device, &M, &kx, &ldxs) || !whole_words(*xs, M, kx, ldxs)) return general();
   } else {
     if (x->dim() != 2 || x->scalar_type() != at::kBFloat16 || !on(*x, device) || x->stride(1) != 1) return general();
     M = x->size(0);
@@ -186,10 +194,9 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   PyObject* result = THPVariable_Wrap(out);  // (before the launch: it may fail)
   if (!result) return nullptr;
   const int st = xs ? entry.mx4(static_cast<const uint8_t*>(x->const_data_ptr()), lda,
-                                static_cast<const uint32_t*>(xs->const_data_ptr()), xs->stride(0), wc, ldw, wsp,
-                                ws->stride(0), bp, out.data_ptr(), ldc, M, N, K, (int)(epi | flags), rp, ldr, gp, from, wp,
+                                static_cast<const uint32_t*>(xs->const_data_ptr()), ldxs, wc, ldw, wsp, ldws, bp, out.data_ptr(), ldc, M, N, K, (int)(epi | flags), rp, ldr, gp, from, wp,
                                 bytes, stream)
-                    : entry.gemm(x->const_data_ptr(), lda, wc, ldw, wsp, ws->stride(0), bp, out.data_ptr(), ldc, M, N, K,
+                    : entry.gemm(x->const_data_ptr(), lda, wc, ldw, wsp, ldws, bp, out.data_ptr(), ldc, M, N, K,
                                  (int)(epi | flags), rp, ldr, gp, from, wp, bytes, stream);
   return outcome(st, result);
 }
@@ -222,14 +229,14 @@ PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t device = PyLong_AsLongLong(a[2]);
   void* stream = PyLong_AsVoidPtr(a[3]);
   if (PyErr_Occurred()) return nullptr;
-  int64_t rows, k;
-  if (!mxfp4(codes, words, device, &rows, &k) || rows < 1 || k < 1) return general();
+  int64_t rows, k, ld;
+  if (!mxfp4(codes, words, device, &rows, &k, &ld) || rows < 1 || k < 1) return general();
   at::Tensor out = empty({rows, k}, at::kBFloat16, *codes);
   PyObject* result = THPVariable_Wrap(out);
   if (!result) return nullptr;
   return outcome(entry.dequantize(static_cast<const uint8_t*>(codes->const_data_ptr()),
                                   rows > 1 ? codes->stride(0) : k / 2,
-                                  static_cast<const uint32_t*>(words->const_data_ptr()), words->stride(0), rows, k,
+                                  static_cast<const uint32_t*>(words->const_data_ptr()), ld, rows, k,
                                   out.data_ptr(), k, stream),
                  result);
 }

@@ -314,14 +314,13 @@ __global__ __launch_bounds__(kG8Threads, 1) void gemm8_kernel(GemmArgs p) {
   // MXFP4: an octet is four rows of 256 scale words, one per wave of group 1.
   constexpr bool SCALED = BKIND == B_MXFP8 || MX || FP4;
   const int sc_words = (p.K + 127) >> 7;
-  const int sc_records = FP4 ? (int)((int64_t)sc_words * p.ld_scale * 4) : (SCALED ? (int)((int64_t)p.N * p.ld_scale) : 0);
+  const int sc_records = FP4 ? (int)word_bytes(sc_words, p.ld_scale, p.N) : (SCALED ? (int)((int64_t)p.N * p.ld_scale) : 0);
   const int asc_records = MX ? (int)((int64_t)p.M * p.ld_ascale) : 0;
   const int sc_read = Cfg::SC_OFF + (wn * WN + (S16 ? r16 : fr)) * (FP4 ? 4 : 16);
   const int asc_read = Cfg::SC_OFF + 2 * Cfg::SC_OCT + (wm * WM + fr) * 16;
   uint32_t sc_src = 0;
-  if constexpr (FP4) {  // past the padded rows: the last ones again
-    const int row = n0 + 4 * lane;
-    sc_src = (uint32_t)(row + 4 <= (int)p.ld_scale ? row : (int)p.ld_scale - 4) * 4;
+  if constexpr (FP4) {
+    sc_src = (uint32_t)word_piece(n0 + 4 * lane, p.N) * 4;
   } else if (grp == 0 || !MX) {
     int gn = n0 + (wave & 3) * 64 + lane;
     gn = gn < p.N ? gn : p.N - 1;

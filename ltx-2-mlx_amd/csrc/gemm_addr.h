@@ -26,4 +26,12 @@ constexpr int stage_pairs(int stages) { return (stages + 1) >> 1; }
 constexpr bool half_pair(int u, int stages) { return (stages & 1) != 0 && u == stage_pairs(stages) - 1; }
 constexpr int half_pair_back(int lane) { return (pair_chunk(lane) & 4) * 16; }
 
+// MXFP4 scale words (K / 128, ld): a load takes four rows' words of one word row.
+// A tile's piece `row` (a multiple of 4) past the operand's last one re-reads
+// that one: what lies between the rows and the stride may be another tensor's, or
+// past the end of memory.  word_bytes: from the first word to the end of the last
+// piece.
+constexpr int word_piece(int row, int rows) { return row < rows ? row : (rows - 1) & ~3; }
+constexpr long long word_bytes(int words, long long ld, int rows) { return ((words - 1) * ld + ((rows + 3) & ~3)) * 4; }
+
 }  // namespace ltx

@@ -96,13 +96,13 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
     b_src[d] = (uint32_t)((int64_t)gn * p.ldb + k0 / 2) + chunk * 16;
   }
   // Scales: 16 bytes (4 rows' words) per lane.  Piece i of an operand's stage
-  // (BM or BN words for each of the two k-steps) is words 4 i .. 4 i + 3.  Rows
-  // past the padded count and k-steps past the last re-read the last.
+  // (BM or BN words for each of the two k-steps) is words 4 i .. 4 i + 3.  Pieces
+  // past the operand's rows (word_piece) and k-steps past the last re-read the last.
   constexpr int S_DMA = Cfg::S_DMA, SA_DMA = Cfg::SA_DMA, SB_DMA = Cfg::SB_DMA;
   const int words = p.K / 128;
   const void* s_base[S_DMA];
   int s_ld[S_DMA], s_dst[S_DMA];
-  int s_row[S_DMA], s_ks[S_DMA];
+  int s_row[S_DMA], s_ks[S_DMA], s_records[S_DMA];
 #pragma unroll
   for (int d = 0; d < S_DMA; ++d) {
     int i = (WAVES * d + wave) % (SA_DMA + SB_DMA);  // the activations' instructions, then the weights'
@@ -113,8 +113,8 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
     s_ld[d] = (int)(of_a ? p.ld_ascale : p.ld_scale);
     s_dst[d] = (of_a ? Cfg::SA_OFF : Cfg::SB_OFF) + i * 1024;
     s_ks[d] = k0 / 128 + piece * 4 / rows;
-    const int row = (of_a ? m0 : n0) + piece * 4 % rows;
-    s_row[d] = row + 4 <= s_ld[d] ? row : s_ld[d] - 4;
+    s_row[d] = word_piece((of_a ? m0 : n0) + piece * 4 % rows, of_a ? p.M : p.N);
+    s_records[d] = (int)word_bytes(words, s_ld[d], of_a ? p.M : p.N);
   }
   // load instruction l of stage t: code rows, then scales
   auto load = [&](int t, int slot, int l) __attribute__((always_inline)) {
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_mx4_kernel(GemmArgs p, i
       const int d = l >= A_DMA + B_DMA ? l - A_DMA - B_DMA : 0;
       int kw = s_ks[d] + 2 * t;
       kw = kw < words ? kw : words - 1;
-      buffer_dma16(s_base[d], words * s_ld[d] * 4, (uint32_t)(kw * s_ld[d] + s_row[d]) * 4, 0, S + s_dst[d]);
+      buffer_dma16(s_base[d], s_records[d], (uint32_t)(kw * s_ld[d] + s_row[d]) * 4, 0, S + s_dst[d]);
     }
   };
 

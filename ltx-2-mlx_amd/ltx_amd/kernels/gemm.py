@@ -434,6 +434,15 @@ def _check_mxfp4(what: str, codes: torch.Tensor, scales: torch.Tensor) -> tuple[
                      f"{None if scales is None else (scales.dtype, tuple(scales.shape))}")
 
 
+def _whole_words(scales: torch.Tensor, rows: int, k: int, ld: int) -> tuple[torch.Tensor, int]:
+    """(words, row stride) whose memory goes on to a multiple of 4 rows, as products
+    read them: the given ones, or a copy."""
+    end = scales.storage_offset() + (k - 1) // 128 * ld + (rows + 3) // 4 * 4
+    if rows % 4 == 0 or end * 4 <= scales.untyped_storage().nbytes():
+        return scales, ld
+    return torch.nn.functional.pad(scales[:, :rows], (0, -rows % 4)), (rows + 3) // 4 * 4
+
+
 def mxfp4_scale_words(scales: torch.Tensor) -> torch.Tensor:
     """E8M0 bytes (rows, K/32) uint8 as the scale words that MXFP4 operands
     hold: int32 (ceil(K/128), rows rounded up to 4)."""
@@ -531,6 +540,7 @@ def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int
     if quantised:
         src, xs = x.codes, x.scales
         m, kx, lda, ldas = _check_mxfp4("activations", src, xs)
+        xs, ldas = _whole_words(xs, m, kx, ldas)
         shape = (m, n)
     else:
         if x.dtype is not torch.bfloat16:

@@ -93,3 +93,33 @@ def test_a_refusal_goes_to_the_python_path(calls):
             calls.status = status
             with pytest.raises(ValueError, match="on one GPU"):  # its checks, met by host tensors
                 call()
+
+
+@pytest.mark.parametrize("rows,k", [(5, 128), (3, 256), (70, 640)])
+def test_scale_words_are_read_up_to_a_multiple_of_four_rows(calls, monkeypatch, rows, k):
+    """Words whose memory ends with the rows go to the kernel as a copy that goes on;
+    a column range of wider words goes as it is, natively."""
+    from ltx_amd import _lib
+    from ltx_amd.kernels import gemm
+
+    seen = []
+    monkeypatch.setattr(_lib, "same_device", lambda *t: -1)
+    monkeypatch.setattr(_lib, "launch", lambda *a: seen.append(a) or 0)
+    w = gemm.LinearWeight("mxfp4", torch.zeros(64, k // 2, dtype=torch.uint8),
+                          torch.zeros(k // 128, 64, dtype=torch.int32))
+    codes = torch.zeros(rows, k // 2, dtype=torch.uint8)
+    ld, words = -(-rows // 4) * 4, k // 128
+    wide = torch.arange(words * (ld + 8), dtype=torch.int32).view(words, ld + 8)
+    held = []
+    pad = torch.nn.functional.pad
+    monkeypatch.setattr(torch.nn.functional, "pad", lambda *a, **kw: held.append(pad(*a, **kw)) or held[-1])
+    for given, whole in ((wide[:, 8:], True), (wide[:, 4:4 + rows], True),
+                         (wide.flatten()[8:8 + (words - 1) * (ld + 8) + rows].clone().as_strided(
+                             (words, rows), (ld + 8, 1)), False)):
+        calls.count, seen[:], held[:] = 0, [], []
+        gemm.linear(gemm.Mx4Rows(codes, given), w)
+        assert calls.count == int(whole) and len(seen) == int(not whole)
+        if not whole:
+            _, name, _, _, ptr, stride = seen[0][:6]
+            assert name == "ltx_gemm_mx4_bf16" and ptr == held[0].data_ptr() and stride == ld
+            assert held[0].shape == (words, ld) and torch.equal(held[0][:, :rows], given)
