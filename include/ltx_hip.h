@@ -178,7 +178,7 @@ int ltx_qknorm_rope_axes_bf16(void* q, int64_t q_stride, int64_t rows_q, const f
  * positions: (batch, tokens) of pos_type 0 int32, 1 int64, 2 fp32, 3 fp64,
  * batch stride pos_batch (0: one row for all), token stride 1.  inv_freq: fp64
  * (rotary_dim / 2) device values.  rotary_dim even, at most head_dim; head_dim
- * at most 512; at most 2^26 - 4 tokens over the batch.
+ * at most 512; at most 2^30 heads and 2^26 - 4 tokens over the batch.
  */
 #define LTX_ROTARY_INTERLEAVED 1
 #define LTX_ROTARY_TRANSPOSE 2

@@ -24,6 +24,7 @@ namespace ltx {
 constexpr int kRotThreads = 256, kRotTokens = 16, kRotMaxDim = 512;
 constexpr int kRotTable = 2048;  // cosines (and sines) of a workgroup
 constexpr int64_t kRotBlocks = (1 << 24) - 1;  // a launch has fewer than 2^32 threads
+constexpr int64_t kRotHeads = 1 << 30;         // an item's head index runs up to kRotThreads + 1 past them
 
 struct RotArgs {
   ltx_rotary_rows side[2];
@@ -235,7 +236,8 @@ extern "C" int ltx_rotary(const ltx_rotary_rows* q, const ltx_rotary_rows* k, in
   int64_t bits = interleaved ? rotary_dim : rotary_dim / 2;
   bits |= head_dim - rotary_dim;
   for (const ltx_rotary_rows& r : p.side) {
-    if (r.heads < 0 || r.heads > INT32_MAX) return LTX_ERR_INVALID_ARG;
+    if (r.heads < 0) return LTX_ERR_INVALID_ARG;
+    if (r.heads > kRotHeads) return LTX_ERR_UNSUPPORTED;
     if (r.heads == 0) continue;
     if (!r.x || !r.out) return LTX_ERR_INVALID_ARG;
     if ((uintptr_t)r.x % size || (uintptr_t)r.out % size) return LTX_ERR_ALIGNMENT;
