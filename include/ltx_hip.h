@@ -406,7 +406,8 @@ int ltx_gemm_mx_gelu_mxfp8(const uint8_t* A, int64_t lda, const uint8_t* a_scale
  * sigmoid_from as above, except that GELU, the head gate and EPI_RESIDUAL act
  * on the fp32 value (no bf16 rounding before them).  Code and row strides 16-byte
  * multiples, pointers 16-byte aligned (bias and gate 4).
- * At most 2^27 rows or columns and 2^34 outputs.
+ * At most 2^27 rows or columns and 2^34 outputs.  C may be the residual with its
+ * stride; it must not overlap the operands in any other way.
  * Products of few tiles split K: they need `workspace` (device memory, 16-byte
  * aligned) of ltx_gemm_*_workspace_bytes(M, N, K) bytes, 0 where none is
  * needed (workspace may then be NULL); calls that may run at the same time

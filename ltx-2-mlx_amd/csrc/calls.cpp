@@ -173,9 +173,10 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int64_t ldc = N;
   if (given) {
     if (given->dim() != 2 || given->scalar_type() != at::kBFloat16 || given->size(0) != M || given->size(1) != N ||
-        given->stride(1) != 1 || !on(*given, device) || !apart(*given, *x) ||
-        (resid && !same_view(*given, *res) && !apart(*given, *res)))
+        given->stride(1) != 1 || !on(*given, device) || (resid && !same_view(*given, *res) && !apart(*given, *res)))
       return general();
+    for (const at::Tensor* t : {x, xs, w, ws, bias, resid ? gate : nullptr})
+      if (t && !apart(*given, *t)) return general();
     if (M > 1) ldc = given->stride(0);
     if (ldc < N) return general();
   }

@@ -595,9 +595,9 @@ def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int
         bptr = bias.data_ptr()
         if weight.qlinear:
             flags |= _lib.GEMM_ROUND_THEN_BIAS
-    if given and (_lib.overlaps(out, src) or (
+    if given and (any(t is not None and _lib.overlaps(out, t) for t in (src, xs, w, scale, bias, gate)) or (
             residual is not None and (out.data_ptr() != rptr or ldc != ldr) and _lib.overlaps(out, residual))):
-        raise ValueError("out overlaps the activations, or the residual without being it")
+        raise ValueError("out overlaps an operand, or the residual without being it")
     device = _lib.same_device(src, xs, w, scale, bias, out, residual, gate)
     if m == 0:
         return out
@@ -701,7 +701,8 @@ def linear(x: torch.Tensor | MxRows | Mx4Rows, weight: LinearWeight, *, epilogue
     """``epilogue(x @ W.T + b)`` for x (..., K) bf16; returns (..., N) bf16.
 
     For the residual epilogues, ``residual`` (..., N) bf16 and ``gate`` fp32
-    (N) are required; ``out`` may be ``residual`` itself (in-place update).
+    (N) are required; ``out`` may be ``residual`` itself (in-place update);
+    on MXFP4 weights anything else that it shares with an operand is refused.
     With ``EPI_BIAS``, columns ``n >= sigmoid_from`` get the 2*sigmoid head
     gate instead (fused gate-logit columns of a Q/QKV projection).
     ``splits``: split-K factor (None: ``auto_splits`` with the automatic tile

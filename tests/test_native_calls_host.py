@@ -123,3 +123,44 @@ def test_scale_words_are_read_up_to_a_multiple_of_four_rows(calls, monkeypatch, 
             _, name, _, _, ptr, stride = seen[0][:6]
             assert name == "ltx_gemm_mx4_bf16" and ptr == held[0].data_ptr() and stride == ld
             assert held[0].shape == (words, ld) and torch.equal(held[0][:, :rows], given)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_outputs_over_other_operands_are_refused(calls, monkeypatch, native):
+    """A given output that shares memory with anything that a product reads."""
+    from ltx_amd import _lib
+    from ltx_amd.kernels import gemm
+
+    if not native:
+        monkeypatch.setattr(_lib, "CALLS", None)
+    buf = torch.zeros(1 << 15, dtype=torch.uint8)
+
+    def at(offset, dtype, *shape):
+        return buf[offset:].view(dtype)[:torch.Size(shape).numel()].view(shape)
+
+    free = dict(x=torch.zeros(4, 128, dtype=torch.bfloat16), xc=torch.zeros(4, 64, dtype=torch.uint8),
+                xs=torch.zeros(1, 4, dtype=torch.int32), w=torch.zeros(64, 64, dtype=torch.uint8),
+                ws=torch.zeros(1, 64, dtype=torch.int32), bias=torch.zeros(64), gate=torch.zeros(64),
+                res=torch.zeros(4, 64, dtype=torch.bfloat16))
+    out = at(4096, torch.bfloat16, 4, 64)  # bytes 4096 to 4608
+    over = dict(x=at(4608 - 16, torch.bfloat16, 4, 128), xc=at(4096 - 240, torch.uint8, 4, 64),
+                xs=at(4096, torch.int32, 1, 4), w=at(4352, torch.uint8, 64, 64), ws=at(4096 - 64, torch.int32, 1, 64),
+                bias=at(4600, torch.float32, 64), gate=at(4096 - 252, torch.float32, 64),
+                res=at(4096 - 16, torch.bfloat16, 4, 64))
+
+    def product(t, quantised):
+        x = gemm.Mx4Rows(t["xc"], t["xs"]) if quantised else t["x"]
+        return gemm.linear(x, gemm.LinearWeight("mxfp4", t["w"], t["ws"], t["bias"]), epilogue=gemm.EPI_RESIDUAL,
+                           residual=t["res"], gate=t["gate"], out=out)
+
+    for quantised in (False, True):
+        for name in free:
+            if name in (("x",) if quantised else ("xc", "xs")):
+                continue
+            with pytest.raises(ValueError, match="overlaps"):
+                product({**free, name: over[name]}, quantised)
+        assert calls.count == 0
+        if native:
+            assert product(free, quantised) is out and calls.count == 1
+            assert product({**free, "res": out}, quantised) is out and calls.count == 2  # in place
+            calls.count = 0
