@@ -69,6 +69,7 @@ def build_calls() -> Path:
     tmp = out.with_suffix(".so.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DLTX_CALLS_BUILT_FOR="torch {torch.__version__}, Python {sys.version_info[0]}.{sys.version_info[1]}"',
            *(f for p in include_paths() for f in ("-isystem", p)), f"-I{sysconfig.get_paths()['include']}",
            str(CSRC / "calls.cpp"), "-o", str(tmp), f"-L{lib_dir}", "-ltorch_python", "-ltorch_cpu", "-lc10",
            f"-Wl,-rpath,{lib_dir}"]

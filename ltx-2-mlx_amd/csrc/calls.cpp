@@ -334,4 +334,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nul
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__calls() { return PyModule_Create(&module); }
+// (BUILT_FOR: the build's torch and Python, whose ABI this is)
+PyMODINIT_FUNC PyInit__calls() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "BUILT_FOR", LTX_CALLS_BUILT_FOR) < 0) Py_CLEAR(m);
+  return m;
+}

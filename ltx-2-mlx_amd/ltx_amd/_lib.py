@@ -8,7 +8,10 @@ entry points.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
+import sys
+import warnings
 from pathlib import Path
 
 import torch
@@ -140,8 +143,9 @@ ERR_SCRATCH_LIMIT = -5
 ATTN_NOALLOC_SCRATCH_BYTES = 32 << 20
 
 _LIB: ctypes.CDLL | None = None
-# Native host side of the small MXFP4 and rotary calls (csrc/calls.cpp), once the
-# library is loaded; None where it was not built: their Python path does the same
+# Native host side of the small MXFP4 and rotary calls (csrc/calls.cpp, the _calls.so
+# beside the library), once that is loaded; None where there is none for this Python and
+# torch: their Python path does the same
 CALLS = None
 _CALLS_ENTRIES = ("ltx_gemm_mxfp4_bf16", "ltx_gemm_mxfp4_workspace_bytes", "ltx_gemm_mx4_bf16",
                   "ltx_gemm_mx4_workspace_bytes", "ltx_quantize_mxfp4", "ltx_dequantize_mxfp4_bf16", "ltx_rotary")
@@ -177,13 +181,30 @@ def lib() -> ctypes.CDLL:
         handle.ltx_gemm_rows_counter_words.restype = _i64
         handle.ltx_status_string.argtypes = [ctypes.c_int]
         handle.ltx_status_string.restype = ctypes.c_char_p
-        if LIB_PATH.with_name("_calls.so").exists():
-            from . import _calls
-
-            _calls.bind(*(ctypes.cast(getattr(handle, name), _vp).value for name in _CALLS_ENTRIES))
-            CALLS = _calls
+        CALLS = _load_calls(LIB_PATH.with_name("_calls.so"), handle)
         _LIB = handle
     return _LIB
+
+
+def _load_calls(path: Path, handle: ctypes.CDLL):
+    """The native host calls of ``path``, bound to the library's entry points; None
+    (and, where there is a file, a warning) if they are not for this Python and torch."""
+    if not path.exists():
+        return None
+    want = f"torch {torch.__version__}, Python {sys.version_info[0]}.{sys.version_info[1]}"
+    spec = importlib.util.spec_from_file_location(f"{__package__}._calls", path)
+    try:
+        calls = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(calls)
+        built_for = calls.BUILT_FOR
+    except (ImportError, AttributeError) as e:
+        built_for = str(e)
+    if built_for != want:
+        warnings.warn(f"{path} is built for something other than {want} ({built_for}): small MXFP4 and rotary calls "
+                      f"go through Python; build again", RuntimeWarning, stacklevel=2)
+        return None
+    calls.bind(*(ctypes.cast(getattr(handle, name), _vp).value for name in _CALLS_ENTRIES))
+    return calls
 
 
 class LtxKernelError(RuntimeError):
