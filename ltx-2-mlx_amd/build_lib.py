@@ -58,24 +58,36 @@ def _compile(src: Path) -> Path:
     return obj
 
 
-def build_calls() -> Path:
+def build_calls() -> Path | None:
     """ltx_amd/_calls.so: the native host calls (a CPython module on torch's
-    headers; the kernels stay behind the C ABI)."""
+    headers; the kernels stay behind the C ABI).  Without a host compiler or the
+    headers of Python and torch there is none (an earlier one goes too): the same
+    calls then run through Python."""
     import torch
     from torch.utils.cpp_extension import include_paths
 
     lib_dir = Path(torch.__file__).parent / "lib"
     out = LIB_PATH.with_name("_calls.so")
     tmp = out.with_suffix(".so.tmp")
-    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+    python_include = Path(sysconfig.get_paths()["include"])
+    compiler = next((c for c in ("g++", "clang++", "/opt/rocm/llvm/bin/clang++") if shutil.which(c)), None)
+    torch_header = "torch/csrc/autograd/python_variable.h"
+    missing = ("a C++ compiler" if compiler is None else
+               f"{python_include}/Python.h" if not (python_include / "Python.h").exists() else
+               torch_header if not any((Path(p) / torch_header).exists() for p in include_paths()) else None)
+    if missing:
+        out.unlink(missing_ok=True)
+        print(f"no {missing}: {out.name} is not built, small MXFP4 and rotary calls go through Python")
+        return None
+    cmd = [compiler, "-O2", "-std=c++17", "-shared", "-fPIC",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            f'-DLTX_CALLS_BUILT_FOR="torch {torch.__version__}, Python {sys.version_info[0]}.{sys.version_info[1]}"',
-           *(f for p in include_paths() for f in ("-isystem", p)), f"-I{sysconfig.get_paths()['include']}",
+           *(f for p in include_paths() for f in ("-isystem", p)), f"-I{python_include}",
            str(CSRC / "calls.cpp"), "-o", str(tmp), f"-L{lib_dir}", "-ltorch_python", "-ltorch_cpu", "-lc10",
            f"-Wl,-rpath,{lib_dir}"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
-        raise RuntimeError(f"g++ failed for calls.cpp:\n{proc.stderr}")
+        raise RuntimeError(f"{compiler} failed for calls.cpp:\n{proc.stderr}")
     os.replace(tmp, out)
     return out
 
