@@ -174,7 +174,8 @@ __global__ __launch_bounds__(kG8Threads, 1) void gemm8_kernel(GemmArgs p) {
   // the stage's advance as the scalar offset and the LDS destination in M0
   // -- no vector instructions per load (vector instructions of one wave take
   // matrix-pipe slots from the other).  The descriptors' record counts bound the
-  // lane offsets to their operand (g8_ok checks the 32-bit extents), the clamps
+  // lane offsets to their operand (the launchers check the 31-bit extents: g8_ok, for
+  // MXFP4 fp4_rows_per_launch), the clamps
   // on the stage the scalar offset, which the counts do not cover.
   const int a_records = (int)((int64_t)p.M * p.lda * (MX ? 1 : 2)),
             b_records = FP4 ? (int)((int64_t)(p.N - 1) * p.ldb + p.K / 2)
@@ -832,13 +833,12 @@ static bool g8_ok(const GemmArgs& p) {
   // operand extents are 31-bit buffer record counts in the kernel
   if ((int64_t)p.M * p.lda * (BKIND == B_MX ? 1 : 2) >= ((int64_t)1 << 31) ||
       (int64_t)p.N * p.ldb * (BKIND == B_BF16 ? 2 : 1) >= ((int64_t)1 << 31) ||
-      (BKIND != B_MXFP4 && (int64_t)p.N * p.ld_scale >= ((int64_t)1 << 31)))
+      (int64_t)p.N * p.ld_scale >= ((int64_t)1 << 31))
     return false;
   if (BKIND == B_MX)
     return p.K % 512 == 0 && p.ld_scale % 16 == 0 && ((uintptr_t)p.bscale & 15u) == 0 &&
            p.ld_ascale % 16 == 0 && ((uintptr_t)p.ascale & 15u) == 0 &&
            (int64_t)p.M * p.ld_ascale < ((int64_t)1 << 31);
-  if (BKIND == B_MXFP4) return (int64_t)((p.K + 127) / 128) * p.ld_scale < ((int64_t)1 << 29);
   if (BKIND == B_MXFP8)
     return p.K % 512 == 0 && p.ld_scale % 16 == 0 && ((uintptr_t)p.bscale & 15u) == 0;
   return true;

@@ -380,6 +380,16 @@ static void fp4_launch(const GemmArgs& p, const Fp4Plan& pl, hipStream_t s) {
   }
 }
 
+// Rows of activations that one launch of the mid-size or the 8-wave kernel takes: their
+// operands' byte offsets have 31 bits.  All rows, or fewer in whole tiles (of 64, 128,
+// 192 or 256 rows); 0: those kernels do not take the product (weights, scale words or a
+// single tile's rows of 2 GiB), the few-row tiles do.
+static int64_t fp4_rows_per_launch(const GemmArgs& p, int64_t rows) {
+  const int64_t lim = ((int64_t)1 << 31) - 1, most = lim / (p.lda * 2);
+  if (p.N > lim / p.ldb || p.ld_scale > lim / 4 / ((p.K + 127) / 128)) return 0;
+  return rows <= most ? rows : most / 768 * 768;
+}
+
 }  // namespace ltx
 
 using namespace ltx;
@@ -410,9 +420,7 @@ extern "C" int ltx_gemm_mxfp4_bf16(const void* A, int64_t lda, const uint8_t* Wq
   hipStream_t s = (hipStream_t)stream;
   const int epi = epilogue & 0xff;
   if (pl.splits > 1) {
-    // (the mid-size kernel addresses its operands by 31-bit byte offsets)
-    const int64_t lim = ((int64_t)1 << 31) - 1;
-    if (pl.kernel == kFp4Mid && (M > lim / (lda * 2) || N > lim / ldw || ld_scale > lim / 4 / ((K + 127) / 128))) {
+    if (pl.kernel == kFp4Mid && fp4_rows_per_launch(p, M) < M) {
       pl.kernel = kFp4Rows;
       pl.bm = 64;
     }
@@ -421,24 +429,21 @@ extern "C" int ltx_gemm_mxfp4_bf16(const void* A, int64_t lda, const uint8_t* Wq
     const int e = ltx_launch_status();
     return e != LTX_OK ? e : fp4_combine(p, epi, pl.splits, s);
   }
-  // rows [r0, r1) on a kernel: the mid-size and 8-wave kernels in pieces of whole
-  // tiles below 2 GiB of activations; what does not fit them otherwise (a weight
-  // of 2 GiB) on the few-row tiles
+  // rows [r0, r1) on a kernel: the mid-size and 8-wave kernels in pieces of as many
+  // as a launch takes; what they do not take on the few-row tiles
   auto run = [&](int64_t r0, int64_t r1, bool head) {
     int64_t piece = r1 - r0;
     Fp4Plan q = pl;
     bool large = head;
     if (head || q.kernel == kFp4Mid || q.kernel == kFp4Large) {
-      const int64_t lim = ((int64_t)1 << 31) - 1, rows = lim / (lda * 2);
-      const bool w_fits = N <= lim / ldw && ld_scale <= lim / 4 / ((K + 127) / 128);
-      if (!w_fits || (piece > rows && rows < 768)) {
+      piece = fp4_rows_per_launch(p, r1 - r0);
+      if (piece == 0) {
+        piece = r1 - r0;
         q.kernel = kFp4Rows;
         q.bm = 64;
         q.splits = 1;
         q.k_split = (int)((K + 127) / 128 * 128);
         large = false;
-      } else if (piece > rows) {
-        piece = rows / 768 * 768;  // tiles of 64, 128, 192, 256 rows
       }
     }
     for (; r0 < r1; r0 += piece) {
