@@ -165,7 +165,8 @@ int ltx_qknorm_rope_axes_bf16(void* q, int64_t q_stride, int64_t rows_q, const f
  * positions and frequencies instead of tables:
  *   a' = factor * (a cos t - b sin t),  b' = factor * (b cos t + a sin t),
  *   t = position * inv_freq[i],  i < rotary_dim / 2,
- * on the first rotary_dim channels of every head, the others copied: pairs
+ * the same for all heads, on the first rotary_dim channels of each, the others
+ * copied: pairs
  * (i, i + rotary_dim / 2), or with LTX_ROTARY_INTERLEAVED (2 i, 2 i + 1) -- the
  * reference's split and interleaved layouts (rope.py:16-89).  With
  * LTX_ROTARY_TRANSPOSE the angle is negated: the map from output gradients to
@@ -395,7 +396,7 @@ int ltx_gemm_mx_gelu_mxfp8(const uint8_t* A, int64_t lda, const uint8_t* a_scale
  * byte; ld (in words) at least the rows, a multiple of 4.  Bytes of a last
  * word that lie past K are not used, nor are words past the rows; a word row is
  * read up to the next multiple of 4 rows, the last one too.  No
- * counterpart in the reference, whose caches hold MXFP8.
+ * counterpart in the reference's default caches, which hold MXFP8.
  *
  * ltx_gemm_mxfp4_bf16: bf16 rows A (M, K) x MXFP4 weights (N, K), decoded to
  * bf16 exactly.  K % 64 == 0, N % 8 == 0.

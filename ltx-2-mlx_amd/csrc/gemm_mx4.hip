@@ -13,11 +13,14 @@
 // block's byte.  The fragments of the next k-step are read while the MFMAs of the
 // current one run, also across the one barrier per stage.
 //
-// What bounds it: 256 x 256 tiles with all CUs busy run at 3.9-4.1 PFLOP/s (3456 x
-// 16384 -> 4096 115 us, 1.75 us per stage).  A loop of nothing but these MFMAs on
-// random codes reaches 5.9-6.4 at the chip's power limit (9.8 on zeros, and this
-// kernel 4.9); its loads and fragment reads alone take 1.15 us per stage, the
-// MFMAs without loads 1.65.  Measured beside it: the 16 x 16 x 128 form 117 us; four
+// What bounds it: a stage of 256 x 256 tiles takes 1.69-1.74 us with every CU busy,
+// 4.9-5.1 PFLOP/s (4096 x K -> 4096 and 6144 x K -> 16384, over K), 1.58 on 224 CUs
+// (3456 x 16384 -> 4096: 109-114 us in all, 4.1-4.25 PFLOP/s).  A loop of nothing but
+// these MFMAs on random codes reaches 5.9-6.4 at the chip's power limit (9.8 on
+// zeros; this kernel whole, 3456 x 16384 -> 4096, 5.6); its loads and fragment reads
+// alone take 1.15 us per stage, the MFMAs without loads 1.65.  First loads and
+// epilogue take 5.5 us a round with no MFMAs beside them, one workgroup per CU, and
+// GELU 4 more: 60 of the 222 us of 6144 x 4096 -> 16384.  Measured beside it: the 16 x 16 x 128 form 117 us; four
 // waves of 128 x 128 117 (a third less LDS traffic); all loads in one k-step 117
 // against 113 for two; touching the lines two stages ahead, to take the L2
 // misses off the loads, 116: no change.

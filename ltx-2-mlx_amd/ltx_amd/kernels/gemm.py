@@ -21,12 +21,12 @@ weights multiply MXFP8-quantised activations on the scaled fp8 MFMA
 arithmetic -- its MXFP8 path keeps the activations in bf16 -- and the
 activations' E4M3 rounding moves outputs by a few percent of their range.
 
-MXFP4 (E2M1 codes, an E8M0 scale per 32 along K) has no counterpart in the
-reference: weights at half MXFP8's bytes, times bf16 activations in
-:func:`linear`, or times MXFP4 activations (:class:`Mx4Rows`, from
-:func:`quantize_rows_mxfp4`) on the scaled FP4 MFMA.  Its GELU, head gate
-and ``EPI_RESIDUAL`` act on the fp32 value, without the bf16 rounding before
-them.
+MXFP4 (E2M1 codes, an E8M0 scale per 32 along K; the reference has it as a
+quantisation mode of its feed-forward cache, which is not read): weights at
+half MXFP8's bytes, times bf16 activations in :func:`linear`, or times MXFP4
+activations (:class:`Mx4Rows`, from :func:`quantize_rows_mxfp4`) on the scaled
+FP4 MFMA.  Its GELU, head gate and ``EPI_RESIDUAL`` act on the fp32 value,
+without the bf16 rounding before them.
 """
 
 from __future__ import annotations

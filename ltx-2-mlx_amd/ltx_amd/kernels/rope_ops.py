@@ -159,7 +159,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     2 * len(inv_freq) channels of a head rotate, the others are copied:
     channels (i, i + d/2) in the "half" layout, (2i, 2i+1) "interleaved" -- the
     reference's split and interleaved forms (model/transformer/rope.py:16-89)
-    -- by the angle positions * inv_freq[i], scaled by ``factor``
+    -- by the angle positions * inv_freq[i], the same for all heads, scaled by ``factor``
     (:func:`rotary_frequencies`).  positions: (T) for every sequence of the
     batch, or (B, T); int32, int64, fp32 or fp64.  ``transpose`` rotates back
     (times ``factor`` again): with the outputs' gradients for q and k it gives
