@@ -56,11 +56,19 @@ at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const at::Tensor& li
   return at::empty(size, like.options().dtype(type));
 }
 
-// The axes of more than one entry, by ascending stride (in bytes; up to 4)
+// The axes of more than one entry, by ascending stride (in bytes).  A dense tensor
+// is one axis, whatever its shape (a bias may have any); others have up to 4.
 struct Axes {
   int n = 0;
   int64_t stride[4], size[4], unit;
   explicit Axes(const at::Tensor& t) : unit(t.element_size()) {
+    if (t.is_contiguous()) {
+      n = 1;
+      stride[0] = unit;
+      size[0] = t.numel();
+      return;
+    }
+    TORCH_CHECK(t.dim() <= 4);
     for (int64_t d = 0; d < t.dim(); ++d) {
       if (t.size(d) == 1) continue;
       int i = n++;

@@ -164,3 +164,33 @@ def test_outputs_over_other_operands_are_refused(calls, monkeypatch, native):
             assert product(free, quantised) is out and calls.count == 1
             assert product({**free, "res": out}, quantised) is out and calls.count == 2  # in place
             calls.count = 0
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_bias_and_gate_of_many_axes(calls, monkeypatch, native):
+    """N values in any shape; the overlap check counts their bytes, not their axes."""
+    from ltx_amd import _lib
+    from ltx_amd.kernels import gemm
+
+    if not native:
+        monkeypatch.setattr(_lib, "CALLS", None)
+    shape = (1, 2, 2, 2, 2, 2, 2)
+    w = torch.zeros(64, 64, dtype=torch.uint8), torch.zeros(1, 64, dtype=torch.int32)
+    x = torch.zeros(4, 128, dtype=torch.bfloat16)
+    buf = torch.zeros(1024, dtype=torch.float32)  # out in bytes 0 to 512, the values after it or over its end
+    out = buf[:128].view(torch.bfloat16).view(4, 64)
+    apart, over = buf[128:192].view(shape), buf[127:191].view(shape)
+    for bias, gate, fine in ((apart, apart, True), (over, apart, False), (apart, over, False)):
+        def product():
+            return gemm.linear(x, gemm.LinearWeight("mxfp4", *w, bias), epilogue=gemm.EPI_RESIDUAL, residual=out,
+                               gate=gate, out=out)
+
+        calls.count = 0
+        if not fine:
+            with pytest.raises(ValueError, match="overlaps"):
+                product()
+        elif native:
+            assert product() is out and calls.count == 1
+        else:
+            with pytest.raises(ValueError, match="on one GPU"):
+                product()
