@@ -155,7 +155,9 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* stream = PyLong_AsVoidPtr(a[12]);
   if (PyErr_Occurred()) return nullptr;
   int64_t N, K, M, kx, ldws, ldxs = 0;
-  if (!x || (!xs && a[1] != Py_None) || (!bias && a[4] != Py_None) || (!given && a[10] != Py_None) || !mxfp4(w, ws, device, &N, &K, &ldws)) return general();
+  if (!x || (!xs && a[1] != Py_None) || (!bias && a[4] != Py_None) || (!given && a[10] != Py_None) ||
+      !mxfp4(w, ws, device, &N, &K, &ldws))
+    return general();
   if (xs) {
     if (!mxfp4(x, xs, device, &M, &kx, &ldxs) || !whole_words(*xs, M, kx, ldxs)) return general();
   } else {
@@ -203,8 +205,8 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   PyObject* result = THPVariable_Wrap(out);  // (before the launch: it may fail)
   if (!result) return nullptr;
   const int st = xs ? entry.mx4(static_cast<const uint8_t*>(x->const_data_ptr()), lda,
-                                static_cast<const uint32_t*>(xs->const_data_ptr()), ldxs, wc, ldw, wsp, ldws, bp, out.data_ptr(), ldc, M, N, K, (int)(epi | flags), rp, ldr, gp, from, wp,
-                                bytes, stream)
+                                static_cast<const uint32_t*>(xs->const_data_ptr()), ldxs, wc, ldw, wsp, ldws, bp,
+                                out.data_ptr(), ldc, M, N, K, (int)(epi | flags), rp, ldr, gp, from, wp, bytes, stream)
                     : entry.gemm(x->const_data_ptr(), lda, wc, ldw, wsp, ldws, bp, out.data_ptr(), ldc, M, N, K,
                                  (int)(epi | flags), rp, ldr, gp, from, wp, bytes, stream);
   return outcome(st, result);
