@@ -27,6 +27,8 @@
  *   ltx_qknorm_rope_bf16        <- model/transformer/attention.py:578-584
  *                                  (RMSNorm :320-329 + rope.py:16-89)
  *   ltx_rotary                  <- rope.py:16-89 (both layouts, no norm)
+ *   ltx_headnorm_rotary         <- (no counterpart: a norm per head; the
+ *                                  reference's spans the inner width)
  *   ltx_output_norm_modulate_bf16 <- model/transformer/model.py:1312-1342
  *   ltx_euler_x0_step_bf16      <- model.py:1519-1525 (X0Model.denoise) +
  *                                  components/diffusion_steps.py:19-69
@@ -193,6 +195,47 @@ typedef struct ltx_rotary_rows {
 int ltx_rotary(const ltx_rotary_rows* q, const ltx_rotary_rows* k, int dtype, int64_t batch, int64_t tokens,
                int64_t head_dim, int64_t rotary_dim, const void* positions, int pos_type, int64_t pos_batch,
                const double* inv_freq, double factor, int flags, void* stream);
+
+/*
+ * RMS norm of every query and key head, its weights and rotary positions, in one
+ * pass over both (k NULL: no keys):
+ *   r = (mean over the head of x^2 + eps)^-1/2,
+ *   y = R(position) (r x (weight_offset + weight)),
+ * R as ltx_rotary (factor included) on the first rotary_dim channels, 0 for no
+ * rotation (positions and inv_freq are then not used).  weight: fp32 (head_dim),
+ * the same for all heads of a side, or NULL for r x alone.  All arithmetic fp32,
+ * rounded once.  ltx_headnorm_rotary_grad: from the gradients g of y
+ *   dx = r (gn - r x mean(gn r x)),  gn = (weight_offset + weight) R^T g,
+ *   dweight = sum over tokens and heads of r x R^T g   (fp32 (head_dim), or NULL),
+ * with x the same inputs as the forward call's.
+ * Tensors, positions, frequencies and limits as ltx_rotary; `out` may be x (in
+ * the gradient: x or g) with the same strides and must not overlap anything else.
+ * g and dweight are not used by the forward call.  A side of no heads, or a call of
+ * no tokens, leaves dweight zero.  The sum over tokens and heads is taken in an order that the sizes fix:
+ * workgroups' shares go to `workspace` (device memory, 4-byte aligned, of
+ * ltx_headnorm_rotary_grad_workspace_bytes(head_dim) bytes; may be NULL without
+ * dweight), and calls that may run at the same time need their own.
+ */
+typedef struct ltx_headnorm_rows {
+  const void* x;
+  int64_t x_batch, x_token, x_head;
+  void* out;
+  int64_t out_batch, out_token, out_head;
+  const void* g;
+  int64_t g_batch, g_token, g_head;
+  const float* weight;
+  float* dweight;
+  int64_t heads;
+} ltx_headnorm_rows;
+int ltx_headnorm_rotary(const ltx_headnorm_rows* q, const ltx_headnorm_rows* k, int dtype, int64_t batch,
+                        int64_t tokens, int64_t head_dim, int64_t rotary_dim, const void* positions, int pos_type,
+                        int64_t pos_batch, const double* inv_freq, double factor, double eps, double weight_offset,
+                        int flags, void* stream);
+int64_t ltx_headnorm_rotary_grad_workspace_bytes(int64_t head_dim);
+int ltx_headnorm_rotary_grad(const ltx_headnorm_rows* q, const ltx_headnorm_rows* k, int dtype, int64_t batch,
+                             int64_t tokens, int64_t head_dim, int64_t rotary_dim, const void* positions, int pos_type,
+                             int64_t pos_batch, const double* inv_freq, double factor, double eps,
+                             double weight_offset, int flags, float* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Output head modulation (model.py:1312-1342):
@@ -426,6 +469,30 @@ int ltx_gemm_mx4_bf16(const uint8_t* A, int64_t lda, const uint32_t* a_scale, in
                       const float* gate, int64_t sigmoid_from, float* workspace, int64_t workspace_bytes,
                       void* stream);
 
+/* ---- int8 products ----------------------------------------------------------
+ * C[m, n] = epilogue( (sum_k A[m, k] Wq[n, k]) a_scale[m] w_scale[n] + bias[n] ):
+ * int8 rows (a scale per row: ltx_quantize_int8) times int8 weights (a scale per
+ * output channel: ltx_quantize_w8_bf16) on the int8 MFMA
+ * (v_mfma_i32_16x16x64_i8).  The sum is exact, in int32; scales, bias and epilogue
+ * are fp32, in the order (sum * a_scale[m]) * w_scale[n] + bias[n], so every way
+ * of splitting the work gives the same bits.  Opt-in arithmetic with no
+ * counterpart in the reference (ltx_gemm_w8a16_bf16 keeps the activations in
+ * bf16).  Epilogues LTX_GEMM_EPI_*, LTX_GEMM_ROUND_THEN_BIAS and sigmoid_from as
+ * for the MXFP4 products: on the fp32 value.
+ * K % 64 == 0, at most 131008 (a sum of 128 * 128 * K fits 31 bits), N % 8 == 0; strides of codes
+ * multiples of 16, code and output pointers 16-byte aligned (scales, bias and
+ * gate 4).  At most 2^27 rows or columns and 2^34 outputs.  C may be the
+ * residual with its stride; it must not overlap the operands in any other way.
+ * `workspace` (16-byte aligned) of ltx_gemm_i8_workspace_bytes(M, N, K) bytes, 0
+ * where none is needed (workspace may then be NULL); calls that may run at the
+ * same time need their own.
+ */
+int64_t ltx_gemm_i8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int ltx_gemm_i8_bf16(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* Wq, int64_t ldw,
+                     const float* w_scale, const float* bias, void* C, int64_t ldc, int64_t M, int64_t N, int64_t K,
+                     int epilogue, const void* residual, int64_t ldr, const float* gate, int64_t sigmoid_from,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Split-K forms of the three GEMMs for products of few output tiles (the
  * 68-token audio stream, short clips): `splits` blocks per output tile each
  * accumulate K / splits of the product into an fp32 partial tile in
@@ -534,6 +601,16 @@ int ltx_quantize_mxfp4(const void* x, int dtype, int64_t ldx, int64_t rows, int6
                        uint32_t* scales, int64_t ld_scale, void* stream);
 int ltx_dequantize_mxfp4_bf16(const uint8_t* q, int64_t ldq, const uint32_t* scales, int64_t ld_scale,
                               int64_t rows, int64_t K, void* out, int64_t ldo, void* stream);
+
+/* Activation rows in int8, a scale per row (the int8 weights' rule):
+ *   scale[m] = max|x[m,:]| / 127,  q = clamp(rint(x / scale), -127, 127),
+ * both quotients rounded to fp32, rint to even; a row of zeros has scale 0 and
+ * codes 0, a row with a NaN or an infinity scale NaN and codes 0 (it decodes to
+ * NaN).  x: (rows, K) of dtype 0 bf16, 1 fp16, 2 fp32, row stride ldx, 16-byte
+ * aligned rows of x and q; K % 16 == 0; at most 2^24 - 1 rows.
+ * ltx_dequantize_w8_bf16 decodes. */
+int ltx_quantize_int8(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t K, int8_t* q, int64_t ldq,
+                      float* scale, void* stream);
 
 /* FP8 checkpoint tensor dequantisation -- the numeric step of
  * loader/transformer_cache.py:658-708 (_iter_fp8_checkpoint_weights):

@@ -14,6 +14,8 @@
 // int8 W8A16 (per output channel, symmetric):
 //     s[n] = max_k |w[n,k]| / 127 (fp32), q = clamp(rint(w / s), -127, 127);
 //     a zero row has s = 0 and q = 0.  Decode: w' = bf16(fp32(q) * s).
+//   Activation rows (int8 x int8 products) by the same rule; a row with a NaN or an
+//   infinity has s = NaN and q = 0.
 // MXFP4 (OCP Microscaling v1.0, element E2M1, block 32 along K, scale E8M0):
 //     X = floor(log2(max|v|)) - 2 (2 = E2M1 emax), clamped to [-127, 127],
 //     scale byte = X + 127, code = E2M1(v / 2^X) rounded to nearest-even and
@@ -110,6 +112,7 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
 // 68 x 2048 4.1 and 2.6, a launch.
 constexpr int kQ4Rows = 16;
 constexpr int64_t kQ4Blocks = (1 << 24) - 1;  // of 256 threads: a launch has fewer than 2^32
+constexpr int64_t kI8Rows = (1 << 24) - 1;    // (up to a workgroup of 256 threads each)
 template <typename T>
 __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows,
                                                              int64_t K, uint8_t* __restrict__ q, int64_t ldq,
@@ -230,6 +233,48 @@ __global__ void w8_dequantize_kernel(const int8_t* __restrict__ q, int64_t ldq,
   *reinterpret_cast<bf16x8*>(out + n * ldo + c * 8) = o;
 }
 
+// Activation rows, one wave each: the row's largest magnitude, then the codes from
+// a second read of it.
+template <typename T>
+__global__ __launch_bounds__(256) void int8_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t K,
+                                                        int8_t* __restrict__ q, int64_t ldq,
+                                                        float* __restrict__ scale) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  // the largest magnitude as bits: those of a NaN or an infinity are above every finite one's
+  uint32_t top = 0;
+  for (int64_t k = lane * 8; k < K; k += 512) {
+    float v[8];
+    load8(x + r * ldx + k, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t b = __float_as_uint(v[e]) & 0x7fffffffu;
+      top = b > top ? b : top;
+    }
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    const uint32_t t = __shfl_xor(top, off, 64);
+    top = t > top ? t : top;
+  }
+  const bool bad = top >= 0x7f800000u;
+  const float s = __fdiv_rn(__uint_as_float(top), 127.0f);
+  if (lane == 0) scale[r] = bad ? __uint_as_float(0x7fc00000u) : s;
+  for (int64_t k = lane * 8; k < K; k += 512) {
+    float v[8];
+    load8(x + r * ldx + k, v);
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float c = s > 0.0f && !bad ? rintf(__fdiv_rn(v[e], s)) : 0.0f;
+      c = fminf(fmaxf(c, -127.0f), 127.0f);  // (a subnormal scale may be off by more than a step)
+      w[e / 4] |= ((uint32_t)(int32_t)c & 0xffu) << (8 * (e % 4));
+    }
+    *reinterpret_cast<u32x2*>(q + r * ldq + k) = u32x2{w[0], w[1]};
+  }
+}
+
 // E4M3 code -> float, exact: (-1)^s 2^(e-7) (1 + m/8), subnormals (e = 0)
 // m 2^-9, 0x7F / 0xFF NaN, no infinities.  The subnormals are formed from
 // the integer m rather than an fp32 denormal, so the decode does not depend on
@@ -331,10 +376,27 @@ extern "C" int ltx_dequantize_w8_bf16(const int8_t* q, int64_t ldq, const float*
   if (K % 8) return LTX_ERR_UNSUPPORTED;
   if (ldq < K || ldo < K) return LTX_ERR_INVALID_ARG;
   if (!a16(out) || (uintptr_t)q % 8 || ldq % 8 || ldo % 8) return LTX_ERR_ALIGNMENT;
+  if (N == 0 || K == 0) return LTX_OK;
+  if (K / 8 > kQ4Blocks * 256 / N) return LTX_ERR_UNSUPPORTED;
   const int64_t total = N * (K / 8);
-  if (total == 0) return LTX_OK;
   w8_dequantize_kernel<<<(int)((total + 255) / 256), 256, 0, (hipStream_t)stream>>>(
       q, ldq, scale, N, K, (bf16*)out, ldo);
+  return ltx_launch_status();
+}
+
+extern "C" int ltx_quantize_int8(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t K, int8_t* q,
+                                 int64_t ldq, float* scale, void* stream) {
+  if (!x || !q || !scale || rows < 0 || K < 0) return LTX_ERR_INVALID_ARG;
+  if (dtype < 0 || dtype > 2 || K % 16) return LTX_ERR_UNSUPPORTED;
+  if (ldx < K || ldq < K) return LTX_ERR_INVALID_ARG;
+  if (!a16(x) || !a16(q) || (uintptr_t)scale % 4 || ldx % (dtype == 2 ? 4 : 8) || ldq % 16) return LTX_ERR_ALIGNMENT;
+  if (rows > kI8Rows) return LTX_ERR_UNSUPPORTED;
+  if (rows == 0) return LTX_OK;
+  const int blocks = (int)((rows + 3) / 4);
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == 0) int8_rows_kernel<<<blocks, 256, 0, s>>>((const bf16*)x, ldx, rows, K, q, ldq, scale);
+  else if (dtype == 1) int8_rows_kernel<<<blocks, 256, 0, s>>>((const _Float16*)x, ldx, rows, K, q, ldq, scale);
+  else int8_rows_kernel<<<blocks, 256, 0, s>>>((const float*)x, ldx, rows, K, q, ldq, scale);
   return ltx_launch_status();
 }
 

@@ -80,6 +80,14 @@ SIGNATURES: dict[str, list] = {
     "ltx_quantize_mxfp4": [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp],
     "ltx_dequantize_mxfp4_bf16": [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp],
     "ltx_rotary": [_vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _int, _i64, _vp, _f64, _int, _vp],
+    "ltx_headnorm_rotary": [_vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _int, _i64, _vp, _f64, _f64, _f64, _int, _vp],
+    "ltx_headnorm_rotary_grad_workspace_bytes": [_i64],
+    "ltx_headnorm_rotary_grad": [_vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _int, _i64, _vp, _f64, _f64, _f64, _int,
+                                 _vp, _i64, _vp],
+    "ltx_quantize_int8": [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp],
+    "ltx_gemm_i8_workspace_bytes": [_i64, _i64, _i64],
+    "ltx_gemm_i8_bf16": [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _vp, _i64, _vp, _i64,
+                         _vp, _i64, _vp],
     "ltx_dequantize_fp8_e4m3": [_vp, _i64, _vp, _vp, _int, _vp],
     "ltx_attn_transpose_v_bf16": [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp],
     "ltx_flash_attn_bf16": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _vp],
@@ -108,7 +116,8 @@ SIGNATURES: dict[str, list] = {
 }
 
 # Functions of SIGNATURES whose result is a size (int64)
-SIZES = ("ltx_gemm_mxfp4_workspace_bytes", "ltx_gemm_mx4_workspace_bytes")
+SIZES = ("ltx_gemm_mxfp4_workspace_bytes", "ltx_gemm_mx4_workspace_bytes", "ltx_gemm_i8_workspace_bytes",
+         "ltx_headnorm_rotary_grad_workspace_bytes")
 
 
 class RotaryRows(ctypes.Structure):
@@ -116,6 +125,16 @@ class RotaryRows(ctypes.Structure):
 
     _fields_ = [("x", _vp), ("x_batch", _i64), ("x_token", _i64), ("x_head", _i64),
                 ("out", _vp), ("out_batch", _i64), ("out_token", _i64), ("out_head", _i64), ("heads", _i64)]
+
+
+class HeadnormRows(ctypes.Structure):
+    """``ltx_headnorm_rows``: a tensor, where its result goes, the gradient of the
+    forward result, the norm weights and where their gradient goes."""
+
+    _fields_ = [("x", _vp), ("x_batch", _i64), ("x_token", _i64), ("x_head", _i64),
+                ("out", _vp), ("out_batch", _i64), ("out_token", _i64), ("out_head", _i64),
+                ("g", _vp), ("g_batch", _i64), ("g_token", _i64), ("g_head", _i64),
+                ("weight", _vp), ("dweight", _vp), ("heads", _i64)]
 
 
 # Flag values (include/ltx_hip.h)

@@ -27,6 +27,10 @@ half MXFP8's bytes, times bf16 activations in :func:`linear`, or times MXFP4
 activations (:class:`Mx4Rows`, from :func:`quantize_rows_mxfp4`) on the scaled
 FP4 MFMA.  Its GELU, head gate and ``EPI_RESIDUAL`` act on the fp32 value,
 without the bf16 rounding before them.
+
+int8 weights take int8 activations as well (:class:`Int8Rows`, a scale per
+row, from :func:`quantize_rows_int8`): the int8 MFMA at twice the bf16 rate,
+exact int32 sums, epilogues on the fp32 value as MXFP4's.
 """
 
 from __future__ import annotations
@@ -621,6 +625,144 @@ def _linear_mxfp4(x: torch.Tensor | Mx4Rows, weight: LinearWeight, epilogue: int
     return out
 
 
+@dataclass
+class Int8Rows:
+    """Activation rows in int8: codes (M, K) int8 and fp32 scales (M); a row's
+    values are its codes times its scale."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+
+def _check_int8(what: str, codes: torch.Tensor, scales: torch.Tensor | None) -> tuple[int, int, int]:
+    """(rows, K, code row stride) of int8 codes with a scale for each row."""
+    if codes.dtype is torch.int8 and codes.dim() == 2 and scales is not None and scales.dtype is torch.float32 \
+            and scales.dim() == 1 and scales.is_contiguous():
+        rows, k = codes.shape
+        ld, unit = codes.stride()
+        if k > 0 and scales.shape[0] == rows and unit == 1 and (rows <= 1 or ld >= k):
+            return rows, k, ld if rows > 1 else (k + 15) // 16 * 16  # (the stride of an axis of one entry says nothing)
+    raise ValueError(f"{what}: int8 operands are codes (rows, K) int8 of unit column stride and contiguous fp32 scales "
+                     f"(rows), got {codes.dtype} {tuple(codes.shape)} and "
+                     f"{None if scales is None else (scales.dtype, tuple(scales.shape))}")
+
+
+def quantize_rows_int8(x: torch.Tensor) -> Int8Rows:
+    """int8 of the rows of x (..., K) bf16, fp16 or fp32 by the int8 weights' rule:
+    scale = max|v| / 127, codes v / scale to the nearest, ties to even (both
+    quotients in fp32).  A row of zeros has scale 0; one with a NaN or an infinity
+    scale NaN, which its products and its decoded values take."""
+    k = x.shape[-1]
+    dtype = _QUANT_DTYPES.get(x.dtype)
+    if dtype is None:
+        raise TypeError(f"quantize_rows_int8 takes bf16, fp16 or fp32 rows, got {x.dtype}")
+    if k % 16 or k == 0:
+        raise ValueError(f"K={k} is not a positive multiple of 16")
+    xv, ldx = _lib.row_view(x, k)
+    m = x.numel() // k
+    if m == 1:
+        ldx = k  # (the stride of an axis of one entry says nothing)
+    elif ldx < k:  # one row for all
+        xv, ldx = xv.contiguous(), k
+    codes = x.new_empty((m, k), dtype=torch.int8)
+    scales = x.new_empty(m, dtype=torch.float32)
+    if m:
+        st = _lib.launch(_lib.same_device(xv), "ltx_quantize_int8", xv.data_ptr(), dtype, ldx, m, k, codes.data_ptr(), k,
+                         scales.data_ptr())
+        if st:
+            raise _lib.LtxKernelError("ltx_quantize_int8", st, f"{x.dtype} rows M={m} K={k} ld={ldx}")
+    return Int8Rows(codes, scales)
+
+
+def dequantize_rows_int8(rows: Int8Rows) -> torch.Tensor:
+    """bf16 (M, K) values of int8 rows: codes times scales, rounded once."""
+    codes, scales = rows.codes, rows.scales
+    m, k, ldq = _check_int8("dequantize_rows_int8", codes, scales)
+    out = codes.new_empty((m, k), dtype=torch.bfloat16)
+    if m:
+        st = _lib.launch(_lib.same_device(codes, scales), "ltx_dequantize_w8_bf16", codes.data_ptr(), ldq,
+                         scales.data_ptr(), m, k, out.data_ptr(), k)
+        if st:
+            raise _lib.LtxKernelError("ltx_dequantize_w8_bf16", st, f"M={m} K={k}")
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _int8_workspace_bytes(m: int, n: int, k: int) -> int:
+    return _lib.lib().ltx_gemm_i8_workspace_bytes(m, n, k)
+
+
+def _linear_int8(x: Int8Rows, weight: LinearWeight, epilogue: int, out: torch.Tensor | None,
+                 residual: torch.Tensor | None, gate: torch.Tensor | None, sigmoid_from: int | None) -> torch.Tensor:
+    """:func:`linear` for int8 rows and int8 weights."""
+    w, scale, bias = weight.w, weight.scale, weight.bias
+    codes, xs = x.codes, x.scales
+    n, k, ldw = _check_int8("weight", w, scale)
+    m, kx, lda = _check_int8("activations", codes, xs)
+    if kx != k:
+        raise ValueError(f"activations have K={kx}, the weight {k}")
+    given = out is not None
+    if not given:
+        out = codes.new_empty((m, n), dtype=torch.bfloat16)
+        ldc = n
+    else:
+        if out.dtype is not torch.bfloat16 or out.shape != (m, n):
+            raise ValueError(f"out must be bf16 {(m, n)}, got {out.dtype} {tuple(out.shape)}")
+        ov, ldc = _lib.row_view(out, n)
+        if ov.data_ptr() != out.data_ptr() or (ldc < n and m > 1):
+            raise ValueError("out must be a row-strided view")
+        ldc = ldc if m > 1 else n
+    rptr, ldr, gptr = None, 0, None
+    if epilogue == EPI_RESIDUAL or epilogue == EPI_RESIDUAL_ROUND:
+        if residual is None or gate is None:
+            raise ValueError("residual epilogues need residual and gate")
+        if residual.dtype is not torch.bfloat16 or residual.shape[-1] != n or residual.numel() != m * n:
+            raise ValueError(f"residual must be bf16 ({m}, {n}), got {residual.dtype} {tuple(residual.shape)}")
+        rv, ldr = _lib.row_view(residual, n)
+        rptr = rv.data_ptr()
+        if rptr != residual.data_ptr() or (ldr < n and m > 1):
+            raise ValueError("residual must be a row-strided view")
+        ldr = ldr if m > 1 else n
+        if gate.dtype is not torch.float32 or gate.numel() != n:
+            raise ValueError("gate must be fp32 with N elements")
+        gate = _lib.flat(gate)
+        gptr = gate.data_ptr()
+    else:
+        residual = gate = None
+    flags, bptr = epilogue, None
+    if bias is not None:
+        if bias.dtype is not torch.float32 or bias.numel() != n or not bias.is_contiguous():
+            raise ValueError(f"bias must be {n} contiguous fp32 values")
+        bptr = bias.data_ptr()
+        if weight.qlinear:
+            flags |= _lib.GEMM_ROUND_THEN_BIAS
+    if given and (any(t is not None and _lib.overlaps(out, t) for t in (codes, xs, w, scale, bias, gate)) or (
+            residual is not None and (out.data_ptr() != rptr or ldc != ldr) and _lib.overlaps(out, residual))):
+        raise ValueError("out overlaps an operand, or the residual without being it")
+    device = _lib.same_device(codes, xs, w, scale, bias, out, residual, gate)
+    if m == 0:
+        return out
+    ws_bytes = _int8_workspace_bytes(m, n, k)
+    ws = codes.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    hook = LAUNCH_HOOK
+    info = (weight.kind, m, n, k, epilogue)
+    if hook is not None:
+        hook("pre", info)
+    st = _lib.launch(device, "ltx_gemm_i8_bf16", codes.data_ptr(), lda, xs.data_ptr(), w.data_ptr(), ldw,
+                     scale.data_ptr(), bptr, out.data_ptr(), ldc, m, n, k, flags, rptr, ldr, gptr,
+                     n if sigmoid_from is None else int(sigmoid_from), None if ws is None else ws.data_ptr(), ws_bytes)
+    if st:
+        raise _lib.LtxKernelError("ltx_gemm_i8_bf16", st, f"M={m} N={n} K={k} epi={epilogue} lda={lda} ldw={ldw} "
+                                                         f"ldc={ldc}")
+    if hook is not None:
+        hook("post", info)
+    return out
+
+
 def _mx_eligible(m: int, n: int, k: int, weight: LinearWeight, tile: int) -> bool:
     return (MX_ACTIVATIONS and weight.kind == "mxfp8" and tile in (TILE_AUTO, TILE_G8) and k % 512 == 0
             and ((m + 255) // 256) * ((n + 255) // 256) >= MX_MIN_TILES)
@@ -694,7 +836,7 @@ def linear_rowss(x: torch.Tensor, weight: LinearWeight, ss_cols: int, *, sigmoid
     return out, ss
 
 
-def linear(x: torch.Tensor | MxRows | Mx4Rows, weight: LinearWeight, *, epilogue: int = EPI_BIAS,
+def linear(x: torch.Tensor | MxRows | Mx4Rows | Int8Rows, weight: LinearWeight, *, epilogue: int = EPI_BIAS,
            out: torch.Tensor | None = None, residual: torch.Tensor | None = None,
            gate: torch.Tensor | None = None, tile: int = TILE_AUTO,
            sigmoid_from: int | None = None, splits: int | None = None) -> torch.Tensor:
@@ -711,8 +853,15 @@ def linear(x: torch.Tensor | MxRows | Mx4Rows, weight: LinearWeight, *, epilogue
     With ``ROWS_KERNEL`` set, few-row products with ``splits=None`` and the
     automatic tile choice run on :func:`linear_rows`.
     MXFP4 weights take bf16 rows or :class:`Mx4Rows` and choose tiles and
-    splits themselves (``tile`` and ``splits`` stay at their defaults).
+    splits themselves (``tile`` and ``splits`` stay at their defaults); so do
+    int8 weights with :class:`Int8Rows`, which refuse the same outputs.
     """
+    if isinstance(x, Int8Rows):
+        if weight.kind != "int8":
+            raise ValueError(f"Int8Rows activations do not go with {weight.kind} weights")
+        if tile != TILE_AUTO or splits is not None:
+            raise ValueError("products of int8 rows take no explicit tile or split count")
+        return _linear_int8(x, weight, epilogue, out, residual, gate, sigmoid_from)
     if weight.kind == "mxfp4" or isinstance(x, Mx4Rows):
         if weight.kind != "mxfp4" or isinstance(x, MxRows):
             raise ValueError(f"{type(x).__name__} activations do not go with {weight.kind} weights")

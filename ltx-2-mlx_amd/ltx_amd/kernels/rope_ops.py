@@ -1,5 +1,6 @@
-"""QK-RMSNorm + split RoPE (in place), the RoPE table layout, and rotary
-positions without a norm (:func:`rotary`).
+"""QK-RMSNorm + split RoPE (in place), the RoPE table layout, rotary
+positions without a norm (:func:`rotary`) and after a norm of every head
+(:func:`headnorm_rotary`, :func:`headnorm_rotary_grad`).
 
 Replaces the ``q_norm``/``k_norm`` + ``apply_rotary_emb`` sequence of
 ``Attention.__call__`` (model/transformer/attention.py:578-584) with one HIP
@@ -217,3 +218,142 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     if st:
         raise _lib.LtxKernelError("ltx_rotary", st, f"{q.dtype} B={batch} T={tokens} dh={dh} rotary={d}")
     return oq, ok
+
+
+_HEADNORM_ROWS = struct.Struct("15q").pack  # ltx_headnorm_rows: x, out, g with their strides, weight, dweight, heads
+
+
+def _head_strides(name: str, t: torch.Tensor) -> tuple[int, int, int]:
+    """Strides of batch, token and head."""
+    st = t.stride()
+    if st[-1] != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name} must have unit channel stride")
+    return (0, st[0], st[1]) if len(st) == 3 else (st[0], st[1], st[2])
+
+
+def _headnorm(name: str, q, k, gq, gk, wq, wk, positions, inv_freq, eps, weight_offset, layout, factor, out):
+    """Both calls of the per-head norm (gradients: gq is given): checks, outputs, launch."""
+    if layout not in ROTARY_LAYOUTS:
+        raise ValueError(f"layout must be one of {ROTARY_LAYOUTS}, got {layout!r}")
+    grad = gq is not None
+    shape = q.shape
+    dtype = _ROTARY_DTYPES.get(q.dtype)
+    if dtype is None or not 3 <= len(shape) <= 4:
+        raise ValueError(f"q must be (T, H, dh) or (B, T, H, dh) in bf16, fp16 or fp32, got {q.dtype} {tuple(shape)}")
+    *lead, _, dh = shape
+    if k is None:
+        if wk is not None or gk is not None:
+            raise ValueError("weights or a gradient for k, but there is no k")
+    else:
+        *lead_k, _, dk = k.shape
+        if k.dtype is not q.dtype or lead_k != lead or dk != dh:
+            raise ValueError(f"k {k.dtype} {tuple(k.shape)} does not go with q {q.dtype} {tuple(shape)}")
+    batch, tokens = lead if len(lead) == 2 else (1, lead[0])
+    if (positions is None) != (inv_freq is None):
+        raise ValueError("positions and inv_freq go together")
+    d, pos_type, pos_batch = 0, 0, 0
+    if positions is not None:
+        if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+            raise ValueError("inv_freq must be a contiguous fp64 vector (rotary_frequencies)")
+        d = 2 * inv_freq.numel()
+        if not 2 <= d <= dh:
+            raise ValueError(f"{d} rotary channels do not fit heads of {dh}")
+        pos_type, pos_shape = _POSITION_DTYPES.get(positions.dtype), positions.shape
+        if pos_type is None or (pos_shape != (tokens,) and pos_shape != (batch, tokens)):
+            raise ValueError(f"positions must be int32, int64, fp32 or fp64 ({tokens},) or ({batch}, {tokens}), got "
+                             f"{positions.dtype} {tuple(pos_shape)}")
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
+        pos_batch = tokens if len(pos_shape) == 2 else 0
+    elif factor != 1.0:
+        raise ValueError("a factor belongs to the rotation, which has no positions")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    given = out if out is not None else (None, None)
+    if k is None and given[1] is not None:
+        raise ValueError("out has a tensor for k, but there is no k")
+    sides = []
+    for n, x, g, w, o in (("q", q, gq, wq, given[0]), ("k", k, gk, wk, given[1])):
+        if x is None:
+            sides.append((None, None, None, None, None))
+            continue
+        if w is not None and (w.dtype is not torch.float32 or w.shape != (dh,) or not w.is_contiguous()):
+            raise ValueError(f"the norm weights of {n} must be {dh} contiguous fp32 values")
+        if grad and (g is None or g.dtype is not x.dtype or g.shape != x.shape):
+            raise ValueError(f"the gradient of {n}' must be {x.dtype} {tuple(x.shape)}, got "
+                             f"{None if g is None else (g.dtype, tuple(g.shape))}")
+        if o is None:
+            o = x.new_empty(x.shape)  # dense, whatever the strides of x
+        elif o.shape != x.shape or o.dtype is not x.dtype:
+            raise ValueError(f"{n}'s out must be {x.dtype} {tuple(x.shape)}, got {o.dtype} {tuple(o.shape)}")
+        elif _lib.self_overlaps(o):
+            raise ValueError(f"{n}'s out has one element in several places")
+        dw = x.new_empty(dh, dtype=torch.float32) if grad and w is not None else None
+        rows = _HEADNORM_ROWS(x.data_ptr(), *_head_strides(n, x), o.data_ptr(), *_head_strides(f"{n}'s out", o),
+                              g.data_ptr() if grad else 0, *(_head_strides(f"the gradient of {n}'", g) if grad else (0, 0, 0)),
+                              0 if w is None else w.data_ptr(), 0 if dw is None else dw.data_ptr(), x.shape[-2])
+        sides.append((rows, o, dw, x, g))
+    (rq, oq, dwq, _, _), (rk, ok, dwk, _, _) = sides
+    if out is not None:
+        # workgroups read and write in any order: an output may be its own input (or its
+        # gradient), and must keep off everything else that is read or written
+        for i, (mine, own) in enumerate(((given[0], (q, gq)), (given[1], (k, gk)))):
+            if mine is None:
+                continue
+            others = [t for t in (*(sides[1 - i][3:]), sides[1 - i][1], wq, wk, positions, inv_freq) if t is not None]
+            if any(t is not None and not _lib.same_view(mine, t) and _lib.overlaps(mine, t) for t in own) or any(
+                    _lib.overlaps(mine, t) for t in others):
+                raise ValueError("an output of the per-head norm overlaps another tensor of the call")
+    device = _lib.same_device(q, k, gq, gk, wq, wk, positions, inv_freq, oq, ok)
+    args = [rq, rk, dtype, batch, tokens, dh, d, None if positions is None else positions.data_ptr(), pos_type, pos_batch,
+            None if inv_freq is None else inv_freq.data_ptr(), factor, eps, weight_offset,
+            _lib.ROTARY_INTERLEAVED if layout == "interleaved" else 0]
+    if grad:
+        sums = dwq is not None or dwk is not None
+        if batch * tokens == 0 and not sums:
+            return oq, ok, dwq, dwk
+        size = _lib.lib().ltx_headnorm_rotary_grad_workspace_bytes(dh) if sums else 0
+        work = q.new_empty(size, dtype=torch.uint8) if sums else None
+        args += [None if work is None else work.data_ptr(), size]
+    elif batch * tokens == 0:
+        return oq, ok
+    st = _lib.launch(device, name, *args)
+    if st:
+        raise _lib.LtxKernelError(name, st, f"{q.dtype} B={batch} T={tokens} dh={dh} rotary={d}")
+    return (oq, ok, dwq, dwk) if grad else (oq, ok)
+
+
+def headnorm_rotary(q: torch.Tensor, k: torch.Tensor | None, wq: torch.Tensor | None, wk: torch.Tensor | None,
+                    positions: torch.Tensor | None, inv_freq: torch.Tensor | None, *, eps: float = 1e-6,
+                    weight_offset: float = 0.0, layout: str = "half", factor: float = 1.0,
+                    out: tuple[torch.Tensor, torch.Tensor | None] | None = None
+                    ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """RMS norm of every query and key head and its rotary position, one launch:
+    returns (q', k') = rotary(r x (weight_offset + w)), r = (mean over the head of
+    x^2 + eps)^-1/2, all in fp32 and rounded once.
+
+    q, k, positions, inv_freq, layout and factor as in :func:`rotary`;
+    positions and inv_freq None: the norm alone.  wq / wk: fp32 (dh), the same for
+    all heads (``weight_offset`` 1 for weights held as their difference from one),
+    or None for r x alone.  ``out`` may be (q, k) itself (in place); its tensors
+    must not overlap the others in any other way.
+    """
+    return _headnorm("ltx_headnorm_rotary", q, k, None, None, wq, wk, positions, inv_freq, eps, weight_offset, layout,
+                     factor, out)
+
+
+def headnorm_rotary_grad(gq: torch.Tensor, gk: torch.Tensor | None, q: torch.Tensor, k: torch.Tensor | None,
+                         wq: torch.Tensor | None, wk: torch.Tensor | None, positions: torch.Tensor | None,
+                         inv_freq: torch.Tensor | None, *, eps: float = 1e-6, weight_offset: float = 0.0,
+                         layout: str = "half", factor: float = 1.0,
+                         out: tuple[torch.Tensor, torch.Tensor | None] | None = None
+                         ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
+    """The gradients of :func:`headnorm_rotary`: from those of its results, gq and
+    gk, and its inputs returns (dq, dk, dwq, dwk), the norm weights' in fp32
+    (None where there are none), summed over batch, tokens and heads in a fixed
+    order.  ``out``: where dq and dk go; each may be its own gradient or input (q and k
+    are read, so an output over them ends their use)."""
+    if gq is None:
+        raise ValueError("headnorm_rotary_grad needs the gradient of q'")
+    return _headnorm("ltx_headnorm_rotary_grad", q, k, gq, gk, wq, wk, positions, inv_freq, eps, weight_offset, layout,
+                     factor, out)
