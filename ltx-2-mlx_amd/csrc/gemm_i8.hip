@@ -114,6 +114,354 @@ static void i8_launch_rows(GemmArgs p, int epi, hipStream_t s) {
   i8_rows_kernel<MB, NB><<<p.tiles_m * p.tiles_n, kI8Waves * 64, 0, s>>>(p, epi);
 }
 
+// ---- tiles -----------------------------------------------------------------------
+// A workgroup computes a BM x BN tile.  A stage is 128 k: rows of 128 bytes, one line
+// each, which reach LDS by direct loads into a ring of NST stages.  A stage has two
+// k-steps of 64, each in two halves of the wave's rows: while the MFMAs of one half
+// run, the fragments of the next are read, also across the one barrier per stage, so
+// that only a quarter of a wave's activations and two k-steps of its weights are in
+// registers beside the sums.
+template <int BM_, int BN_, int WAVES_M_, int WAVES_N_, int NST_>
+struct I8Tile {
+  static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, NST = NST_;
+  static constexpr int WAVES = WAVES_M * WAVES_N, THREADS = WAVES * 64;
+  static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N;
+  static constexpr int TM = WM / 16, TN = WN / 16, HM = TM / 2;
+  static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, B_OFF = A_BYTES, STAGE = A_BYTES + B_BYTES;
+  // direct loads of a wave per stage
+  static constexpr int A_DMA = BM / 8 / WAVES, B_DMA = BN / 8 / WAVES, DMA = A_DMA + B_DMA;
+  // staged output rows of a wave: its tile as bf16, or half of it as fp32 (a residual's branch)
+  static constexpr int EPI_ROWB = WN * 2, R_ROWB = WN * 4, EPI_WAVE = WM * EPI_ROWB;
+  static constexpr int RING = NST * STAGE, EPI = WAVES * EPI_WAVE;
+  static constexpr int LDS_BYTES = RING > EPI ? RING : EPI;
+  static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole direct-load instructions per wave");
+  static_assert(TM % 2 == 0 && TN >= 2, "halves of whole fragments");
+  static_assert(LDS_BYTES <= 160 * 1024 && (NST - 1) * DMA < 60, "LDS, vmcnt range");
+};
+
+template <class Cfg, int EPI>
+__global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, int k_split) {
+  constexpr int BM = Cfg::BM, BN = Cfg::BN, WM = Cfg::WM, WN = Cfg::WN, TM = Cfg::TM, TN = Cfg::TN, HM = Cfg::HM;
+  constexpr int NST = Cfg::NST, A_DMA = Cfg::A_DMA, B_DMA = Cfg::B_DMA, WAVES = Cfg::WAVES;
+  constexpr bool RESID = EPI == LTX_GEMM_EPI_RESIDUAL || EPI == LTX_GEMM_EPI_RESIDUAL_ROUND;
+  __shared__ __attribute__((aligned(1024))) char lds[Cfg::LDS_BYTES];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % Cfg::WAVES_M, wn = wave / Cfg::WAVES_M;
+  const int r16 = lane & 15, q = lane >> 4;
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int kz = EPI == kEpiPartial ? (int)blockIdx.x / tiles : 0;
+  int tmi, tni;
+  tile_coords(EPI == kEpiPartial ? (int)blockIdx.x % tiles : (int)blockIdx.x, tiles, p.tiles_m, p.tiles_n, tmi, tni);
+  const int m0 = tmi * BM, n0 = tni * BN;
+  const int k0 = kz * k_split;
+  const int depth = p.K - k0 < k_split ? p.K - k0 : k_split;  // a multiple of 64
+  const int T = (depth + 127) / 128;
+  const bool half = (depth & 64) != 0;  // the last stage has one k-step
+
+  // ---- direct-load sources (bytes from the operand's start).  Instruction d of a
+  // wave fills 8 LDS rows of 128 bytes, lane j the 16-byte slot j & 7 of row j >> 3
+  // (the chunk that the row's swizzle puts there).  Rows past M / N re-read the last
+  // one.  A last half stage: the lanes of the missing k-step load the other's bytes.
+  const int a_records = (int)((int64_t)(p.M - 1) * p.lda + p.K);
+  const int b_records = (int)((int64_t)(p.N - 1) * p.ldb + p.K);
+  const int chunk = (lane & 7) ^ g8_swz128(lane >> 3, true);  // (8 rows on, the swizzle repeats)
+  const int back = (chunk & 4) * 16;
+  uint32_t a_src[A_DMA], b_src[B_DMA];
+#pragma unroll
+  for (int d = 0; d < A_DMA; ++d) {
+    int gm = m0 + 8 * (WAVES * d + wave) + (lane >> 3);
+    gm = gm < p.M ? gm : p.M - 1;
+    a_src[d] = (uint32_t)((int64_t)gm * p.lda + k0) + chunk * 16;
+  }
+#pragma unroll
+  for (int d = 0; d < B_DMA; ++d) {
+    int gn = n0 + 8 * (WAVES * d + wave) + (lane >> 3);
+    gn = gn < p.N ? gn : p.N - 1;
+    b_src[d] = (uint32_t)((int64_t)gn * p.ldb + k0) + chunk * 16;
+  }
+  // load instruction l of stage t (past the last stage: the last again)
+  auto load = [&](int t, int slot, int l) __attribute__((always_inline)) {
+    t = t < T ? t : T - 1;
+    char* S = lds + slot * Cfg::STAGE;
+    const uint32_t bk = half && t == T - 1 ? back : 0;
+    if (l < A_DMA) {
+      buffer_dma16(p.A, a_records, a_src[l < A_DMA ? l : 0] - bk, t * 128, S + (WAVES * l + wave) * 1024);
+    } else {
+      const int d = l >= A_DMA ? l - A_DMA : 0;
+      buffer_dma16(p.B, b_records, b_src[d] - bk, t * 128, S + Cfg::B_OFF + (WAVES * d + wave) * 1024);
+    }
+  };
+
+  // ---- fragments of a k-step: lane (row r16, quarter q) holds the 16 bytes of chunk 4 ks + q
+  i32x4 a[2][HM], w[2][TN];
+  int c_off[2];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) c_off[ks] = ((4 * ks + q) ^ g8_swz128(r16, true)) * 16;
+  const int a_rd = (wm * WM + r16) * 128, w_rd = Cfg::B_OFF + (wn * WN + r16) * 128;
+  auto read_a = [&](i32x4& f, int slot, int ks, int i) __attribute__((always_inline)) {
+    f = *reinterpret_cast<const i32x4*>(lds + slot * Cfg::STAGE + a_rd + c_off[ks] + i * 2048);
+  };
+  auto read_w = [&](i32x4& f, int slot, int ks, int j) __attribute__((always_inline)) {
+    f = *reinterpret_cast<const i32x4*>(lds + slot * Cfg::STAGE + w_rd + c_off[ks] + j * 2048);
+  };
+  // share j of TN of the reads of half h of k-step ks (of its weights too, where `weights`)
+  auto read_share = [&](int slot, int ks, int h, bool weights, int j) __attribute__((always_inline)) {
+    if (weights) read_w(w[ks][j], slot, ks, j);
+#pragma unroll
+    for (int i = 0; i < HM; ++i)
+      if (i * TN / HM == j) read_a(a[h][i], slot, ks, h * HM + i);
+  };
+  i32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+  // the MFMAs of half h of k-step ks in groups of one weight fragment (weights as the
+  // MFMA's first operand: a lane then holds four consecutive output columns); f(j) issues
+  // what goes beside group j
+  auto step = [&](auto kc, auto hc, auto f) __attribute__((always_inline)) {
+    constexpr int KS = decltype(kc)::value, H = decltype(hc)::value;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      f(j);
+#pragma unroll
+      for (int i = 0; i < HM; ++i)
+        acc[H * HM + i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[KS][j], a[H][i], acc[H * HM + i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  constexpr std::integral_constant<int, 0> c0;
+  constexpr std::integral_constant<int, 1> c1;
+
+  // ---- prologue: the ring filled (of the last slot's stage the first HL loads), stage 0 landed
+  constexpr int HL = (Cfg::DMA + 1) / 2;
+#pragma unroll
+  for (int t = 0; t < NST; ++t)
+#pragma unroll
+    for (int l = 0; l < (t < NST - 1 ? Cfg::DMA : HL); ++l) load(t, t, l);
+  wait_vmcnt<(NST - 2) * Cfg::DMA + HL>();
+  barrier_nofence();
+#pragma unroll
+  for (int j = 0; j < TN; ++j) read_share(0, 0, 0, true, j);
+
+  // Stage t: before its last half step, with every read of the stage done and stage
+  // t + 1 landed, the barrier, after which the loads of stage t + NST go into this slot.
+  int slot = 0;
+  constexpr int LPJ = (HL + TN - 1) / TN;  // load instructions per group
+  int prev = NST - 1;                      // the slot of stage t - 1
+  for (int t = 0; t < depth / 128; ++t) {
+    step(c0, c0, [&](int j) __attribute__((always_inline)) {
+      read_share(slot, 0, 1, false, j);
+#pragma unroll
+      for (int l = HL; l < Cfg::DMA; ++l)
+        if ((l - HL) / LPJ == j) load(t + NST - 1, prev, l);
+    });
+    step(c0, c1, [&](int j) __attribute__((always_inline)) { read_share(slot, 1, 0, true, j); });
+    step(c1, c0, [&](int j) __attribute__((always_inline)) { read_share(slot, 1, 1, false, j); });
+    wait_lgkmcnt0();
+    wait_vmcnt<(NST - 2) * Cfg::DMA>();
+    barrier_nofence();
+    prev = slot;
+    slot = slot + 1 < NST ? slot + 1 : 0;
+    step(c1, c1, [&](int j) __attribute__((always_inline)) {
+      read_share(slot, 0, 0, true, j);
+#pragma unroll
+      for (int l = 0; l < HL; ++l)
+        if (l / LPJ == j) load(t + NST, prev, l);
+    });
+  }
+  if (half) {
+    step(c0, c0, [&](int j) __attribute__((always_inline)) { read_share(slot, 0, 1, false, j); });
+    step(c0, c1, [](int) {});
+  }
+  wait_vmcnt<0>();
+  if constexpr (EPI == kEpiPartial) {
+    int32_t* P = (int32_t*)p.partial + (int64_t)kz * p.M * p.N;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int gm = m0 + wm * WM + i * 16 + r16;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int gn = n0 + wn * WN + j * 16 + 4 * q;  // N % 8 == 0: four columns inside or outside
+        if (gm < p.M && gn < p.N) *reinterpret_cast<i32x4*>(P + (int64_t)gm * p.N + gn) = acc[i][j];
+      }
+    }
+    return;
+  } else {
+    // ---- epilogue: the tile through LDS, 16-byte chunks XORed by the row so that
+    // both the writes and the 16-byte reads spread over the banks
+    __syncthreads();
+    constexpr int CH = WN / 8, RPI = 64 / CH;
+    char* E = lds + wave * Cfg::EPI_WAVE;  // a wave reads back only what it wrote itself
+    const int ch = lane % CH, rsub = lane / CH;
+    const int gn = n0 + wn * WN + ch * 8;
+    float sa[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int gm = m0 + wm * WM + i * 16 + r16;
+      sa[i] = i8_row_scale(p)[gm < p.M ? gm : p.M - 1];
+    }
+    // the values of fragment column j's columns 4 q on, rows of blocks i0 to i1, to put(i, j, value)
+    auto branch = [&](int i0, int i1, auto sig_tag, auto rtb_tag, auto put) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int c = n0 + wn * WN + j * 16 + 4 * q;
+        const bool in = c < p.N;
+        const f32x4 sw = i8_four(i8_col_scale(p) + (in ? c : 0));
+        f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (p.bias) bias = i8_four(p.bias + (in ? c : 0));
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          if (i < i0 || i >= i1) continue;
+          put(i, j, fp4_branch4<EPI, decltype(sig_tag)::value, decltype(rtb_tag)::value>(p, i8_value(acc[i][j], sa[i], sw),
+                                                                                         bias, c));
+        }
+      }
+    };
+    if constexpr (RESID) {
+      constexpr int ROWB = Cfg::R_ROWB, C4 = WN / 4, ITS = HM * 16 / RPI;
+      float g8[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g8[e] = gn < p.N ? p.gate[gn + e] : 0.0f;
+#pragma unroll
+      for (int i0 = 0; i0 < TM; i0 += HM) {
+        auto put = [&](int i, int j, f32x4 y) __attribute__((always_inline)) {
+          const int row = (i - i0) * 16 + r16;
+          *reinterpret_cast<f32x4*>(E + row * ROWB + (((4 * j + q) ^ row) & (C4 - 1)) * 16) = y;
+        };
+        if (p.round_then_bias) branch(i0, i0 + HM, std::false_type{}, std::true_type{}, put);
+        else branch(i0, i0 + HM, std::false_type{}, std::false_type{}, put);
+        bf16x8 res[ITS];
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) {
+          int gm = m0 + wm * WM + i0 * 16 + it * RPI + rsub;
+          gm = gm < p.M ? gm : p.M - 1;
+          res[it] = *reinterpret_cast<const bf16x8*>(p.R + (int64_t)gm * p.ldr + (gn < p.N ? gn : 0));
+        }
+        wait_lgkmcnt0();
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) {
+          const int row = it * RPI + rsub, gm = m0 + wm * WM + i0 * 16 + row;
+          const f32x4 lo = *reinterpret_cast<const f32x4*>(E + row * ROWB + (((2 * ch) ^ row) & (C4 - 1)) * 16);
+          const f32x4 hi = *reinterpret_cast<const f32x4*>(E + row * ROWB + (((2 * ch + 1) ^ row) & (C4 - 1)) * 16);
+          bf16x8 v;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = fp4_residual<EPI>(e < 4 ? lo[e & 3] : hi[e & 3], res[it][e], g8[e]);
+          if (gm < p.M && gn < p.N) *reinterpret_cast<bf16x8*>(p.C + (int64_t)gm * p.ldc + gn) = v;
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    } else {
+      constexpr int ITS = WM / RPI;
+      auto swz = [](int row) { return CH == 8 ? (row >> 1) & 7 : (row >> 2) & 3; };
+      auto put = [&](int i, int j, f32x4 y) __attribute__((always_inline)) {
+        const int row = i * 16 + r16;
+        *reinterpret_cast<bf16x4*>(E + row * Cfg::EPI_ROWB + ((2 * j + (q >> 1)) ^ swz(row)) * 16 + (q & 1) * 8) = fp4_bf16(y);
+      };
+      const bool sig = EPI == LTX_GEMM_EPI_BIAS && n0 + wn * WN + WN > p.sig_from;
+      if (p.round_then_bias) {
+        if (sig) branch(0, TM, std::true_type{}, std::true_type{}, put);
+        else branch(0, TM, std::false_type{}, std::true_type{}, put);
+      } else {
+        if (sig) branch(0, TM, std::true_type{}, std::false_type{}, put);
+        else branch(0, TM, std::false_type{}, std::false_type{}, put);
+      }
+      wait_lgkmcnt0();
+      __builtin_amdgcn_wave_barrier();
+      if (gn >= p.N) return;
+#pragma unroll
+      for (int it = 0; it < ITS; ++it) {
+        const int row = it * RPI + rsub, gm = m0 + wm * WM + row;
+        if (gm >= p.M) break;
+        *reinterpret_cast<bf16x8*>(p.C + (int64_t)gm * p.ldc + gn) =
+            *reinterpret_cast<const bf16x8*>(E + row * Cfg::EPI_ROWB + (ch ^ swz(row)) * 16);
+      }
+    }
+  }
+}
+
+using I8Large = I8Tile<256, 256, 2, 4, 2>;
+using I8Tall = I8Tile<256, 128, 4, 2, 3>;
+using I8Mid = I8Tile<128, 128, 2, 4, 4>;
+using I8Small = I8Tile<64, 128, 2, 4, 4>;
+
+// sum of the K ranges' partial products, then the epilogue
+__global__ __launch_bounds__(256) void i8_combine_kernel(GemmArgs p, int epi, int splits) {
+  const int per_row = p.N / 4;
+  const int64_t total = (int64_t)p.M * per_row, plane = (int64_t)p.M * p.N;
+  for (int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x; idx < total; idx += (int64_t)gridDim.x * 256) {
+    const int m = (int)(idx / per_row), n = (int)(idx % per_row) * 4;
+    const int32_t* P = (const int32_t*)p.partial + (int64_t)m * p.N + n;
+    i32x4 a = *reinterpret_cast<const i32x4*>(P);
+    for (int z = 1; z < splits; ++z) a += *reinterpret_cast<const i32x4*>(P + z * plane);
+    i8_store4(p, epi, a, m, n);
+  }
+}
+
+// ---- which kernel ------------------------------------------------------------------
+struct I8Plan {
+  int bm, bn;   // bn 0: the few-row kernel, bm its rows
+  int splits;   // K ranges (tiles)
+  int k_split;  // k of one, a multiple of 128
+};
+
+// Modelled time (us): a round of one workgroup per CU costs `fixed` (first loads and
+// epilogue) and per 128 k `idle` to `full`, as it fills the CUs; a split's second launch and
+// its partials.
+static double i8_time(int64_t M, int64_t N, int bm, int bn, int splits, double per) {
+  const double wgs = (double)(((M + bm - 1) / bm) * ((N + bn - 1) / bn) * splits);
+  double fixed = 2.2, idle = 0.30, full = 0.36;
+  if (bm == 256 && bn == 256) fixed = 5.5, idle = 1.0, full = 1.4;
+  else if (bm == 256) fixed = 4.3, idle = 0.6, full = 0.8;
+  else if (bm == 128) fixed = 2.6, idle = 0.42, full = 0.5;
+  const double rounds = (double)(int64_t)(wgs / 256), rest = wgs / 256 - rounds;
+  double t = 2.2 + rounds * (fixed + per * full);
+  if (rest > 0) t += fixed + per * (idle + (full - idle) * rest);
+  if (splits > 1) t += 2.5 + (double)(M * N) * splits * 8 / 4e6;
+  return t;
+}
+
+static I8Plan i8_plan(int64_t M, int64_t N, int64_t K) {
+  static const int tile[4][2] = {{256, 256}, {256, 128}, {128, 128}, {64, 128}};
+  if (M <= 32) return {M <= 16 ? 16 : 64, 0, 1, (int)K};
+  const int64_t units = (K + 127) / 128;
+  I8Plan pl = {64, 128, 1, (int)(units * 128)};
+  double best = 1e30;
+  for (const auto& t : tile) {
+    const int64_t tiles = ((M + t[0] - 1) / t[0]) * ((N + t[1] - 1) / t[1]);
+    for (int want = 1; want <= 16; ++want) {
+      // splits: at least two stages each, within one round of the CUs, 10 % faster
+      if (want > 1 && (units / want < 2 || tiles * want > 256)) break;
+      const int64_t per = (units + want - 1) / want;
+      const int s = (int)((units + per - 1) / per);
+      const double us = i8_time(M, N, t[0], t[1], s, (double)per);
+      if (us < best * (s > 1 ? 0.9 : 1.0)) {
+        best = us;
+        pl = {t[0], t[1], s, (int)(per * 128)};
+      }
+    }
+  }
+  return pl;
+}
+
+template <int EPI>
+static void i8_launch_tiles(GemmArgs p, const I8Plan& pl, hipStream_t s) {
+  p.tiles_m = (p.M + pl.bm - 1) / pl.bm;
+  p.tiles_n = (p.N + pl.bn - 1) / pl.bn;
+  const int blocks = p.tiles_m * p.tiles_n * pl.splits;
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    gemm_i8_kernel<T, EPI><<<blocks, T::THREADS, 0, s>>>(p, pl.k_split);
+  };
+  if (pl.bm == 256 && pl.bn == 256) go(I8Large{});
+  else if (pl.bm == 256) go(I8Tall{});
+  else if (pl.bm == 128) go(I8Mid{});
+  else go(I8Small{});
+}
+
 static inline int i8_check(const void* A, int64_t lda, const float* a_scale, const void* W, int64_t ldw,
                            const float* w_scale, const float* bias, const void* C, int64_t ldc, int64_t M, int64_t N,
                            int64_t K, int epilogue, const void* R, int64_t ldr, const float* gate) {
@@ -140,19 +488,23 @@ using namespace ltx;
 
 extern "C" int64_t ltx_gemm_i8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   if (M < 0 || N < 0 || K < 0) return -1;
-  return 0;
+  if (M == 0 || N == 0 || K == 0 || M > INT32_MAX / 2 || N > INT32_MAX / 2 || K > INT32_MAX / 2) return 0;
+  const I8Plan pl = i8_plan(M, N, K);
+  return pl.splits > 1 ? (int64_t)pl.splits * M * N * 4 : 0;
 }
 
 extern "C" int ltx_gemm_i8_bf16(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* Wq, int64_t ldw,
                                 const float* w_scale, const float* bias, void* C, int64_t ldc, int64_t M, int64_t N,
                                 int64_t K, int epilogue, const void* residual, int64_t ldr, const float* gate,
                                 int64_t sigmoid_from, void* workspace, int64_t workspace_bytes, void* stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   const int st = i8_check(A, lda, a_scale, Wq, ldw, w_scale, bias, C, ldc, M, N, K, epilogue, residual, ldr, gate);
   if (st != LTX_OK) return st;
   if (M == 0 || N == 0) return LTX_OK;
   if (K == 0) return LTX_ERR_UNSUPPORTED;
+  const I8Plan pl = i8_plan(M, N, K);
+  const int64_t need = pl.splits > 1 ? (int64_t)pl.splits * M * N * 4 : 0;
+  if (need > 0 && (!workspace || workspace_bytes < need)) return LTX_ERR_INVALID_ARG;
+  if (need > 0 && ((uintptr_t)workspace & 15u)) return LTX_ERR_ALIGNMENT;
   GemmArgs p = {};
   p.A = (const bf16*)A;
   p.lda = lda;
@@ -173,7 +525,48 @@ extern "C" int ltx_gemm_i8_bf16(const int8_t* A, int64_t lda, const float* a_sca
   p.K = (int)K;
   hipStream_t s = (hipStream_t)stream;
   const int epi = epilogue & 0xff;
-  if (M <= 16) i8_launch_rows<1, 1>(p, epi, s);
-  else i8_launch_rows<4, 2>(p, epi, s);
-  return ltx_launch_status();
+  auto rows = [&](int bm) {
+    if (bm == 16 && N >= 32 * 256) i8_launch_rows<1, 2>(p, epi, s);
+    else if (bm == 16) i8_launch_rows<1, 1>(p, epi, s);
+    else i8_launch_rows<4, 2>(p, epi, s);
+  };
+  if (pl.bn == 0) {
+    rows(pl.bm);
+    return ltx_launch_status();
+  }
+  // Rows that one launch of the tile kernel takes: its operands' byte offsets have 31
+  // bits.  Rows past them in further launches; none where a tile's rows, or the weights,
+  // are past them: then the few-row kernel, whose addresses have 64 bits
+  const int64_t lim = ((int64_t)1 << 31) - 1;
+  int64_t piece = lim / lda;
+  if (N > lim / ldw) piece = 0;
+  if (piece < M) piece = piece / 256 * 256;
+  if (piece == 0) {
+    rows(64);
+    return ltx_launch_status();
+  }
+  if (pl.splits > 1 && piece >= M) {
+    p.partial = (float*)workspace;
+    i8_launch_tiles<kEpiPartial>(p, pl, s);
+    const int e = ltx_launch_status();
+    if (e != LTX_OK) return e;
+    const int64_t total = M * (N / 4);
+    i8_combine_kernel<<<(int)(total + 255 < 4096 * 256 ? (total + 255) / 256 : 4096), 256, 0, s>>>(p, epi, pl.splits);
+    return ltx_launch_status();
+  }
+  I8Plan whole = pl;
+  whole.splits = 1;
+  whole.k_split = (int)((K + 127) / 128 * 128);
+  for (int64_t r = 0; r < M; r += piece) {
+    GemmArgs part = p;
+    part.A = (const bf16*)(A + r * lda);
+    part.ascale = (const uint8_t*)(a_scale + r);
+    part.C = p.C + r * ldc;
+    if (p.R) part.R = p.R + r * ldr;
+    part.M = (int)(M - r < piece ? M - r : piece);
+    fp4_epilogue(epi, [&](auto e) { i8_launch_tiles<decltype(e)::value>(part, whole, s); });
+    const int e = ltx_launch_status();
+    if (e != LTX_OK) return e;
+  }
+  return LTX_OK;
 }
