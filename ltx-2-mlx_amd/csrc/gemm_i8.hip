@@ -130,12 +130,9 @@ struct I8Tile {
   static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, B_OFF = A_BYTES, STAGE = A_BYTES + B_BYTES;
   // direct loads of a wave per stage
   static constexpr int A_DMA = BM / 8 / WAVES, B_DMA = BN / 8 / WAVES, DMA = A_DMA + B_DMA;
-  // staged output rows of a wave: its tile as bf16, or half of it as fp32 (a residual's branch)
-  static constexpr int EPI_ROWB = WN * 2, R_ROWB = WN * 4, EPI_WAVE = WM * EPI_ROWB;
-  static constexpr int RING = NST * STAGE, EPI = WAVES * EPI_WAVE;
-  static constexpr int LDS_BYTES = RING > EPI ? RING : EPI;
+  static constexpr int LDS_BYTES = NST * STAGE;
   static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole direct-load instructions per wave");
-  static_assert(TM % 2 == 0 && TN >= 2, "halves of whole fragments");
+  static_assert(TM % 2 == 0 && TN % 2 == 0, "halves of whole fragments, pairs of weight fragments");
   static_assert(LDS_BYTES <= 160 * 1024 && (NST - 1) * DMA < 60, "LDS, vmcnt range");
 };
 
@@ -163,11 +160,16 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
   // ---- direct-load sources (bytes from the operand's start).  Instruction d of a
   // wave fills 8 LDS rows of 128 bytes, lane j the 16-byte slot j & 7 of row j >> 3
   // (the chunk that the row's swizzle puts there).  Rows past M / N re-read the last
-  // one.  A last half stage: the lanes of the missing k-step load the other's bytes.
+  // one.  A k-step takes every other chunk (the reads' pattern for which g8_swz128 leaves
+  // no bank conflicts), so a last half stage's four chunks go to the even places.
   const int a_records = (int)((int64_t)(p.M - 1) * p.lda + p.K);
   const int b_records = (int)((int64_t)(p.N - 1) * p.ldb + p.K);
+  // Weight fragments j and j + 1 (j even) of a wave hold its columns 16 j + 8 (r16 / 4) +
+  // r16 % 4 and the ones 4 further on, so that a lane's sums of the two are eight
+  // neighbouring columns; their rows' swizzle takes bit 3 where the activations' takes bit 2.
   const int chunk = (lane & 7) ^ g8_swz128(lane >> 3, true);  // (8 rows on, the swizzle repeats)
-  const int back = (chunk & 4) * 16;
+  const int b_chunk = (lane & 7) ^ g8_swz128(((lane >> 3) & 3) | (wave & 1) << 2, true);
+  const int back = (chunk - (chunk >> 1)) * 16, b_back = (b_chunk - (b_chunk >> 1)) * 16;
   uint32_t a_src[A_DMA], b_src[B_DMA];
 #pragma unroll
   for (int d = 0; d < A_DMA; ++d) {
@@ -179,32 +181,32 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
   for (int d = 0; d < B_DMA; ++d) {
     int gn = n0 + 8 * (WAVES * d + wave) + (lane >> 3);
     gn = gn < p.N ? gn : p.N - 1;
-    b_src[d] = (uint32_t)((int64_t)gn * p.ldb + k0) + chunk * 16;
+    b_src[d] = (uint32_t)((int64_t)gn * p.ldb + k0) + b_chunk * 16;
   }
   // load instruction l of stage t (past the last stage: the last again)
   auto load = [&](int t, int slot, int l) __attribute__((always_inline)) {
     t = t < T ? t : T - 1;
     char* S = lds + slot * Cfg::STAGE;
-    const uint32_t bk = half && t == T - 1 ? back : 0;
+    const bool last = half && t == T - 1;
     if (l < A_DMA) {
-      buffer_dma16(p.A, a_records, a_src[l < A_DMA ? l : 0] - bk, t * 128, S + (WAVES * l + wave) * 1024);
+      buffer_dma16(p.A, a_records, a_src[l < A_DMA ? l : 0] - (last ? back : 0), t * 128, S + (WAVES * l + wave) * 1024);
     } else {
       const int d = l >= A_DMA ? l - A_DMA : 0;
-      buffer_dma16(p.B, b_records, b_src[d] - bk, t * 128, S + Cfg::B_OFF + (WAVES * d + wave) * 1024);
+      buffer_dma16(p.B, b_records, b_src[d] - (last ? b_back : 0), t * 128, S + Cfg::B_OFF + (WAVES * d + wave) * 1024);
     }
   };
 
-  // ---- fragments of a k-step: lane (row r16, quarter q) holds the 16 bytes of chunk 4 ks + q
+  // ---- fragments of a k-step: lane (row r16, quarter q) holds the 16 bytes of chunk 2 q + ks
   i32x4 a[2][HM], w[2][TN];
   int c_off[2];
 #pragma unroll
-  for (int ks = 0; ks < 2; ++ks) c_off[ks] = ((4 * ks + q) ^ g8_swz128(r16, true)) * 16;
-  const int a_rd = (wm * WM + r16) * 128, w_rd = Cfg::B_OFF + (wn * WN + r16) * 128;
+  for (int ks = 0; ks < 2; ++ks) c_off[ks] = ((2 * q + ks) ^ g8_swz128(r16, true)) * 16;
+  const int a_rd = (wm * WM + r16) * 128, w_rd = Cfg::B_OFF + (wn * WN + 8 * (r16 >> 2) + (r16 & 3)) * 128;
   auto read_a = [&](i32x4& f, int slot, int ks, int i) __attribute__((always_inline)) {
     f = *reinterpret_cast<const i32x4*>(lds + slot * Cfg::STAGE + a_rd + c_off[ks] + i * 2048);
   };
   auto read_w = [&](i32x4& f, int slot, int ks, int j) __attribute__((always_inline)) {
-    f = *reinterpret_cast<const i32x4*>(lds + slot * Cfg::STAGE + w_rd + c_off[ks] + j * 2048);
+    f = *reinterpret_cast<const i32x4*>(lds + slot * Cfg::STAGE + w_rd + c_off[ks] + (j >> 1) * 4096 + (j & 1) * 512);
   };
   // share j of TN of the reads of half h of k-step ks (of its weights too, where `weights`)
   auto read_share = [&](int slot, int ks, int h, bool weights, int j) __attribute__((always_inline)) {
@@ -277,107 +279,63 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
     step(c0, c1, [](int) {});
   }
   wait_vmcnt<0>();
-  if constexpr (EPI == kEpiPartial) {
-    int32_t* P = (int32_t*)p.partial + (int64_t)kz * p.M * p.N;
+  // ---- epilogue: from registers, 16 bytes per lane and row, 64 side by side
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int gm = m0 + wm * WM + i * 16 + r16;
+  for (int h = 0; h < TN / 2; ++h) {
+    const int n = n0 + wn * WN + 32 * h + 8 * q;
+    if (n >= p.N) continue;  // N % 8 == 0: eight columns inside or outside
+    if constexpr (EPI == kEpiPartial) {
+      int32_t* P = (int32_t*)p.partial + (int64_t)kz * p.M * p.N;
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int gn = n0 + wn * WN + j * 16 + 4 * q;  // N % 8 == 0: four columns inside or outside
-        if (gm < p.M && gn < p.N) *reinterpret_cast<i32x4*>(P + (int64_t)gm * p.N + gn) = acc[i][j];
-      }
-    }
-    return;
-  } else {
-    // ---- epilogue: the tile through LDS, 16-byte chunks XORed by the row so that
-    // both the writes and the 16-byte reads spread over the banks
-    __syncthreads();
-    constexpr int CH = WN / 8, RPI = 64 / CH;
-    char* E = lds + wave * Cfg::EPI_WAVE;  // a wave reads back only what it wrote itself
-    const int ch = lane % CH, rsub = lane / CH;
-    const int gn = n0 + wn * WN + ch * 8;
-    float sa[TM];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int gm = m0 + wm * WM + i * 16 + r16;
-      sa[i] = i8_row_scale(p)[gm < p.M ? gm : p.M - 1];
-    }
-    // the values of fragment column j's columns 4 q on, rows of blocks i0 to i1, to put(i, j, value)
-    auto branch = [&](int i0, int i1, auto sig_tag, auto rtb_tag, auto put) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int c = n0 + wn * WN + j * 16 + 4 * q;
-        const bool in = c < p.N;
-        const f32x4 sw = i8_four(i8_col_scale(p) + (in ? c : 0));
-        f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (p.bias) bias = i8_four(p.bias + (in ? c : 0));
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          if (i < i0 || i >= i1) continue;
-          put(i, j, fp4_branch4<EPI, decltype(sig_tag)::value, decltype(rtb_tag)::value>(p, i8_value(acc[i][j], sa[i], sw),
-                                                                                         bias, c));
-        }
-      }
-    };
-    if constexpr (RESID) {
-      constexpr int ROWB = Cfg::R_ROWB, C4 = WN / 4, ITS = HM * 16 / RPI;
-      float g8[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) g8[e] = gn < p.N ? p.gate[gn + e] : 0.0f;
-#pragma unroll
-      for (int i0 = 0; i0 < TM; i0 += HM) {
-        auto put = [&](int i, int j, f32x4 y) __attribute__((always_inline)) {
-          const int row = (i - i0) * 16 + r16;
-          *reinterpret_cast<f32x4*>(E + row * ROWB + (((4 * j + q) ^ row) & (C4 - 1)) * 16) = y;
-        };
-        if (p.round_then_bias) branch(i0, i0 + HM, std::false_type{}, std::true_type{}, put);
-        else branch(i0, i0 + HM, std::false_type{}, std::false_type{}, put);
-        bf16x8 res[ITS];
-#pragma unroll
-        for (int it = 0; it < ITS; ++it) {
-          int gm = m0 + wm * WM + i0 * 16 + it * RPI + rsub;
-          gm = gm < p.M ? gm : p.M - 1;
-          res[it] = *reinterpret_cast<const bf16x8*>(p.R + (int64_t)gm * p.ldr + (gn < p.N ? gn : 0));
-        }
-        wait_lgkmcnt0();
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int it = 0; it < ITS; ++it) {
-          const int row = it * RPI + rsub, gm = m0 + wm * WM + i0 * 16 + row;
-          const f32x4 lo = *reinterpret_cast<const f32x4*>(E + row * ROWB + (((2 * ch) ^ row) & (C4 - 1)) * 16);
-          const f32x4 hi = *reinterpret_cast<const f32x4*>(E + row * ROWB + (((2 * ch + 1) ^ row) & (C4 - 1)) * 16);
-          bf16x8 v;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = fp4_residual<EPI>(e < 4 ? lo[e & 3] : hi[e & 3], res[it][e], g8[e]);
-          if (gm < p.M && gn < p.N) *reinterpret_cast<bf16x8*>(p.C + (int64_t)gm * p.ldc + gn) = v;
-        }
-        __builtin_amdgcn_wave_barrier();
+      for (int i = 0; i < TM; ++i) {
+        const int m = m0 + wm * WM + i * 16 + r16;
+        if (m >= p.M) continue;
+        *reinterpret_cast<i32x4*>(P + (int64_t)m * p.N + n) = acc[i][2 * h];
+        *reinterpret_cast<i32x4*>(P + (int64_t)m * p.N + n + 4) = acc[i][2 * h + 1];
       }
     } else {
-      constexpr int ITS = WM / RPI;
-      auto swz = [](int row) { return CH == 8 ? (row >> 1) & 7 : (row >> 2) & 3; };
-      auto put = [&](int i, int j, f32x4 y) __attribute__((always_inline)) {
-        const int row = i * 16 + r16;
-        *reinterpret_cast<bf16x4*>(E + row * Cfg::EPI_ROWB + ((2 * j + (q >> 1)) ^ swz(row)) * 16 + (q & 1) * 8) = fp4_bf16(y);
+      f32x4 sw[2], bias[2], gate[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        sw[c] = i8_four(i8_col_scale(p) + n + 4 * c);
+        bias[c] = p.bias ? i8_four(p.bias + n + 4 * c) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (RESID) gate[c] = i8_four(p.gate + n + 4 * c);
+      }
+      bf16x8 res[TM];
+      if constexpr (RESID) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          int m = m0 + wm * WM + i * 16 + r16;
+          m = m < p.M ? m : p.M - 1;
+          res[i] = *reinterpret_cast<const bf16x8*>(p.R + (int64_t)m * p.ldr + n);
+        }
+      }
+      auto rows = [&](auto sig_tag, auto rtb_tag) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const int m = m0 + wm * WM + i * 16 + r16;
+          const float sa = i8_row_scale(p)[m < p.M ? m : p.M - 1];
+          bf16x8 v;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const f32x4 y = fp4_branch4<EPI, decltype(sig_tag)::value, decltype(rtb_tag)::value>(
+                p, i8_value(acc[i][2 * h + c], sa, sw[c]), bias[c], n + 4 * c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (RESID) v[4 * c + e] = fp4_residual<EPI>(y[e], res[i][4 * c + e], gate[c][e]);
+              else v[4 * c + e] = (bf16)y[e];
+            }
+          }
+          if (m < p.M) *reinterpret_cast<bf16x8*>(p.C + (int64_t)m * p.ldc + n) = v;
+        }
       };
       const bool sig = EPI == LTX_GEMM_EPI_BIAS && n0 + wn * WN + WN > p.sig_from;
       if (p.round_then_bias) {
-        if (sig) branch(0, TM, std::true_type{}, std::true_type{}, put);
-        else branch(0, TM, std::false_type{}, std::true_type{}, put);
+        if (sig) rows(std::true_type{}, std::true_type{});
+        else rows(std::false_type{}, std::true_type{});
       } else {
-        if (sig) branch(0, TM, std::true_type{}, std::false_type{}, put);
-        else branch(0, TM, std::false_type{}, std::false_type{}, put);
-      }
-      wait_lgkmcnt0();
-      __builtin_amdgcn_wave_barrier();
-      if (gn >= p.N) return;
-#pragma unroll
-      for (int it = 0; it < ITS; ++it) {
-        const int row = it * RPI + rsub, gm = m0 + wm * WM + row;
-        if (gm >= p.M) break;
-        *reinterpret_cast<bf16x8*>(p.C + (int64_t)gm * p.ldc + gn) =
-            *reinterpret_cast<const bf16x8*>(E + row * Cfg::EPI_ROWB + (ch ^ swz(row)) * 16);
+        if (sig) rows(std::true_type{}, std::false_type{});
+        else rows(std::false_type{}, std::false_type{});
       }
     }
   }
