@@ -115,12 +115,23 @@ static void i8_launch_rows(GemmArgs p, int epi, hipStream_t s) {
 }
 
 // ---- tiles -----------------------------------------------------------------------
-// A workgroup computes a BM x BN tile.  A stage is 128 k: rows of 128 bytes, one line
-// each, which reach LDS by direct loads into a ring of NST stages.  A stage has two
-// k-steps of 64, each in two halves of the wave's rows: while the MFMAs of one half
-// run, the fragments of the next are read, also across the one barrier per stage, so
-// that only a quarter of a wave's activations and two k-steps of its weights are in
-// registers beside the sums.
+// A workgroup computes BM x BN tiles, one after another.  A stage is 128 k: rows of 128
+// bytes, one line each, which reach LDS by direct loads into a ring of NST stages, one
+// stream over all its tiles (the next tile's first stages travel during the last
+// stages and the epilogue of this one).  A stage has two k-steps of 64, each in two halves of the
+// wave's rows: while the MFMAs of one half run, the fragments of the next are read, also
+// across the one barrier per stage, so that only a quarter of a wave's activations and two
+// k-steps of its weights are in registers beside the sums.
+//
+// What bounds it: the chip's power.  A stage of 256 x 256 tiles takes 1.4 us with every CU
+// busy, 3.0 PO/s (6144 x 4096 -> 16384 without its epilogues 275 us), 1.08 us on zeros; a loop
+// of nothing but these MFMAs on such codes reaches 4.1 (32 x 32 x 32: 3.5); the stage without its
+// loads takes 1.19 us, without its fragment reads 1.21, without MFMAs 0.99.  Epilogues take 25
+// us of that product's 300 with bias, GELU 17 more.  Measured beside it: four waves of 128 x 128, sums
+// in AGPRs (a third less LDS traffic), 152 against 148 us (4096 x 12288 -> 4096); 320-row tiles 334
+// against 340 (6144 x 4096 -> 16384, rounds of 256 rows' tiles elsewhere); loads in one half step, all
+// fragment reads in the first group, fewer vector instructions in the loop: no change; two
+// workgroups per CU of 128 x 128: 459.
 template <int BM_, int BN_, int WAVES_M_, int WAVES_N_, int NST_>
 struct I8Tile {
   static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, NST = NST_;
@@ -147,15 +158,17 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % Cfg::WAVES_M, wn = wave / Cfg::WAVES_M;
   const int r16 = lane & 15, q = lane >> 4;
-  const int tiles = p.tiles_m * p.tiles_n;
-  const int kz = EPI == kEpiPartial ? (int)blockIdx.x / tiles : 0;
-  int tmi, tni;
-  tile_coords(EPI == kEpiPartial ? (int)blockIdx.x % tiles : (int)blockIdx.x, tiles, p.tiles_m, p.tiles_n, tmi, tni);
-  const int m0 = tmi * BM, n0 = tni * BN;
-  const int k0 = kz * k_split;
-  const int depth = p.K - k0 < k_split ? p.K - k0 : k_split;  // a multiple of 64
-  const int T = (depth + 127) / 128;
-  const bool half = (depth & 64) != 0;  // the last stage has one k-step
+  const int tiles = p.tiles_m * p.tiles_n, total = tiles * (EPI == kEpiPartial ? (p.K + k_split - 1) / k_split : 1);
+  // tile `id`: its first row and column, and its K range
+  auto locate = [&](int id, int& m0, int& n0, int& k0, int& depth) __attribute__((always_inline)) {
+    const int kz = EPI == kEpiPartial ? id / tiles : 0;
+    int tm, tn;
+    tile_coords(id - kz * tiles, tiles, p.tiles_m, p.tiles_n, tm, tn);
+    m0 = tm * BM;
+    n0 = tn * BN;
+    k0 = kz * k_split;
+    depth = p.K - k0 < k_split ? p.K - k0 : k_split;  // a multiple of 64
+  };
 
   // ---- direct-load sources (bytes from the operand's start).  Instruction d of a
   // wave fills 8 LDS rows of 128 bytes, lane j the 16-byte slot j & 7 of row j >> 3
@@ -171,28 +184,49 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
   const int b_chunk = (lane & 7) ^ g8_swz128(((lane >> 3) & 3) | (wave & 1) << 2, true);
   const int back = (chunk - (chunk >> 1)) * 16, b_back = (b_chunk - (b_chunk >> 1)) * 16;
   uint32_t a_src[A_DMA], b_src[B_DMA];
+  int next = (int)blockIdx.x;  // the tile being loaded
+  int lt, lT;                  // its stage, and its stages
+  bool lhalf;                  // whether its last one is a half
+  auto aim = [&]() __attribute__((always_inline)) {
+    int m0, n0, k0, depth;
+    locate(next, m0, n0, k0, depth);
+    lt = 0;
+    lT = (depth + 127) / 128;
+    lhalf = (depth & 64) != 0;
 #pragma unroll
-  for (int d = 0; d < A_DMA; ++d) {
-    int gm = m0 + 8 * (WAVES * d + wave) + (lane >> 3);
-    gm = gm < p.M ? gm : p.M - 1;
-    a_src[d] = (uint32_t)((int64_t)gm * p.lda + k0) + chunk * 16;
-  }
+    for (int d = 0; d < A_DMA; ++d) {
+      int gm = m0 + 8 * (WAVES * d + wave) + (lane >> 3);
+      gm = gm < p.M ? gm : p.M - 1;
+      a_src[d] = (uint32_t)((int64_t)gm * p.lda + k0) + chunk * 16;
+    }
 #pragma unroll
-  for (int d = 0; d < B_DMA; ++d) {
-    int gn = n0 + 8 * (WAVES * d + wave) + (lane >> 3);
-    gn = gn < p.N ? gn : p.N - 1;
-    b_src[d] = (uint32_t)((int64_t)gn * p.ldb + k0) + b_chunk * 16;
-  }
-  // load instruction l of stage t (past the last stage: the last again)
-  auto load = [&](int t, int slot, int l) __attribute__((always_inline)) {
-    t = t < T ? t : T - 1;
+    for (int d = 0; d < B_DMA; ++d) {
+      int gn = n0 + 8 * (WAVES * d + wave) + (lane >> 3);
+      gn = gn < p.N ? gn : p.N - 1;
+      b_src[d] = (uint32_t)((int64_t)gn * p.ldb + k0) + b_chunk * 16;
+    }
+  };
+  // load instruction l of the stage, and the step to the stage behind it (past the last
+  // tile's: that one again)
+  auto load = [&](int slot, int l) __attribute__((always_inline)) {
     char* S = lds + slot * Cfg::STAGE;
-    const bool last = half && t == T - 1;
+    const bool last = lhalf && lt == lT - 1;
     if (l < A_DMA) {
-      buffer_dma16(p.A, a_records, a_src[l < A_DMA ? l : 0] - (last ? back : 0), t * 128, S + (WAVES * l + wave) * 1024);
+      buffer_dma16(p.A, a_records, a_src[l < A_DMA ? l : 0] - (last ? back : 0), lt * 128,
+                   S + (WAVES * l + wave) * 1024);
     } else {
       const int d = l >= A_DMA ? l - A_DMA : 0;
-      buffer_dma16(p.B, b_records, b_src[d] - (last ? b_back : 0), t * 128, S + Cfg::B_OFF + (WAVES * d + wave) * 1024);
+      buffer_dma16(p.B, b_records, b_src[d] - (last ? b_back : 0), lt * 128,
+                   S + Cfg::B_OFF + (WAVES * d + wave) * 1024);
+    }
+  };
+  auto advance = [&]() __attribute__((always_inline)) {
+    if (++lt < lT) return;
+    if (next + (int)gridDim.x < total) {
+      next += (int)gridDim.x;
+      aim();
+    } else {
+      lt = lT - 1;
     }
   };
 
@@ -216,10 +250,6 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
       if (i * TN / HM == j) read_a(a[h][i], slot, ks, h * HM + i);
   };
   i32x4 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
   // the MFMAs of half h of k-step ks in groups of one weight fragment (weights as the
   // MFMA's first operand: a lane then holds four consecutive output columns); f(j) issues
   // what goes beside group j
@@ -239,94 +269,158 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
 
   // ---- prologue: the ring filled (of the last slot's stage the first HL loads), stage 0 landed
   constexpr int HL = (Cfg::DMA + 1) / 2;
+  aim();
+#pragma unroll 1
+  for (int t = 0; t < NST - 1; ++t) {
 #pragma unroll
-  for (int t = 0; t < NST; ++t)
+    for (int l = 0; l < Cfg::DMA; ++l) load(t, l);
+    advance();
+  }
 #pragma unroll
-    for (int l = 0; l < (t < NST - 1 ? Cfg::DMA : HL); ++l) load(t, t, l);
+  for (int l = 0; l < HL; ++l) load(NST - 1, l);
   wait_vmcnt<(NST - 2) * Cfg::DMA + HL>();
   barrier_nofence();
 #pragma unroll
   for (int j = 0; j < TN; ++j) read_share(0, 0, 0, true, j);
 
-  // Stage t: before its last half step, with every read of the stage done and stage
-  // t + 1 landed, the barrier, after which the loads of stage t + NST go into this slot.
+  // The stages of all the workgroup's tiles are one stream.  A stage: before its last half
+  // step, with every read of it done and the next stage landed, the barrier, after which
+  // the loads of NST stages further on go into its slot.
   int slot = 0;
   constexpr int LPJ = (HL + TN - 1) / TN;  // load instructions per group
-  int prev = NST - 1;                      // the slot of stage t - 1
-  for (int t = 0; t < depth / 128; ++t) {
-    step(c0, c0, [&](int j) __attribute__((always_inline)) {
-      read_share(slot, 0, 1, false, j);
+  int prev = NST - 1;                      // the slot of the stage before
+  auto late = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-      for (int l = HL; l < Cfg::DMA; ++l)
-        if ((l - HL) / LPJ == j) load(t + NST - 1, prev, l);
-    });
-    step(c0, c1, [&](int j) __attribute__((always_inline)) { read_share(slot, 1, 0, true, j); });
-    step(c1, c0, [&](int j) __attribute__((always_inline)) { read_share(slot, 1, 1, false, j); });
+    for (int l = HL; l < Cfg::DMA; ++l)
+      if ((l - HL) / LPJ == j) load(prev, l);
+  };
+  auto early = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+    for (int l = 0; l < HL; ++l)
+      if (l / LPJ == j) load(prev, l);
+  };
+  auto turn = [&]() __attribute__((always_inline)) {
     wait_lgkmcnt0();
     wait_vmcnt<(NST - 2) * Cfg::DMA>();
     barrier_nofence();
     prev = slot;
     slot = slot + 1 < NST ? slot + 1 : 0;
-    step(c1, c1, [&](int j) __attribute__((always_inline)) {
-      read_share(slot, 0, 0, true, j);
+  };
+  for (int id = (int)blockIdx.x; id < total; id += (int)gridDim.x) {
+    int m0, n0, k0, depth;
+    locate(id, m0, n0, k0, depth);
 #pragma unroll
-      for (int l = 0; l < HL; ++l)
-        if (l / LPJ == j) load(t + NST, prev, l);
-    });
-  }
-  if (half) {
-    step(c0, c0, [&](int j) __attribute__((always_inline)) { read_share(slot, 0, 1, false, j); });
-    step(c0, c1, [](int) {});
-  }
-  wait_vmcnt<0>();
-  // ---- epilogue: from registers, 16 bytes per lane and row, 64 side by side
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-  for (int h = 0; h < TN / 2; ++h) {
-    const int n = n0 + wn * WN + 32 * h + 8 * q;
-    if (n >= p.N) continue;  // N % 8 == 0: eight columns inside or outside
+      for (int j = 0; j < TN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    for (int t = 0; t < depth / 128; ++t) {
+      step(c0, c0, [&](int j) __attribute__((always_inline)) {
+        read_share(slot, 0, 1, false, j);
+        late(j);
+      });
+      advance();
+      step(c0, c1, [&](int j) __attribute__((always_inline)) { read_share(slot, 1, 0, true, j); });
+      step(c1, c0, [&](int j) __attribute__((always_inline)) { read_share(slot, 1, 1, false, j); });
+      turn();
+      step(c1, c1, [&](int j) __attribute__((always_inline)) {
+        read_share(slot, 0, 0, true, j);
+        early(j);
+      });
+    }
+    if ((depth & 64) != 0) {  // the last stage has one k-step
+      step(c0, c0, [&](int j) __attribute__((always_inline)) {
+        read_share(slot, 0, 1, false, j);
+        late(j);
+      });
+      advance();
+      turn();
+      step(c0, c1, early);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) read_share(slot, 0, 0, true, j);
+    }
+    // ---- epilogue: from registers, 16 bytes per lane and row, 64 side by side.  Everything
+    // that is loaded is loaded before the first store: loads wait for the stores before them.
+    int er = r16, eq = q;
+    asm volatile("" : "+v"(er), "+v"(eq));  // (keeps what depends on them out of the registers of the stages)
     if constexpr (EPI == kEpiPartial) {
-      int32_t* P = (int32_t*)p.partial + (int64_t)kz * p.M * p.N;
+      int32_t* P = (int32_t*)p.partial + (int64_t)(id / tiles) * p.M * p.N;
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const int m = m0 + wm * WM + i * 16 + r16;
-        if (m >= p.M) continue;
-        *reinterpret_cast<i32x4*>(P + (int64_t)m * p.N + n) = acc[i][2 * h];
-        *reinterpret_cast<i32x4*>(P + (int64_t)m * p.N + n + 4) = acc[i][2 * h + 1];
-      }
-    } else {
-      f32x4 sw[2], bias[2], gate[2];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        sw[c] = i8_four(i8_col_scale(p) + n + 4 * c);
-        bias[c] = p.bias ? i8_four(p.bias + n + 4 * c) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if constexpr (RESID) gate[c] = i8_four(p.gate + n + 4 * c);
-      }
-      bf16x8 res[TM];
-      if constexpr (RESID) {
+      for (int h = 0; h < TN / 2; ++h) {
+        const int n = n0 + wn * WN + 32 * h + 8 * eq;
+        if (n >= p.N) continue;  // N % 8 == 0: eight columns inside or outside
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-          int m = m0 + wm * WM + i * 16 + r16;
-          m = m < p.M ? m : p.M - 1;
-          res[i] = *reinterpret_cast<const bf16x8*>(p.R + (int64_t)m * p.ldr + n);
+          const int m = m0 + wm * WM + i * 16 + er;
+          if (m >= p.M) continue;
+          *reinterpret_cast<i32x4*>(P + (int64_t)m * p.N + n) = acc[i][2 * h];
+          *reinterpret_cast<i32x4*>(P + (int64_t)m * p.N + n + 4) = acc[i][2 * h + 1];
         }
       }
-      auto rows = [&](auto sig_tag, auto rtb_tag) __attribute__((always_inline)) {
+    } else {
+      float sa[TM];
+      f32x4 sw[TN], bias[TN], gate[TN];
+      auto columns = [&](int j) __attribute__((always_inline)) {
+        int n = n0 + wn * WN + 32 * (j >> 1) + 8 * eq;
+        n = (n < p.N ? n : 0) + 4 * (j & 1);
+        sw[j] = i8_four(i8_col_scale(p) + n);
+        bias[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (p.bias) bias[j] = i8_four(p.bias + n);
+        if constexpr (RESID) gate[j] = i8_four(p.gate + n);
+      };
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          const int m = m0 + wm * WM + i * 16 + r16;
-          const float sa = i8_row_scale(p)[m < p.M ? m : p.M - 1];
+      for (int i = 0; i < TM; ++i) {
+        const int m = m0 + wm * WM + i * 16 + er;
+        sa[i] = i8_row_scale(p)[m < p.M ? m : p.M - 1];
+      }
+      auto store = [&](int i, int h, bf16x8 v) __attribute__((always_inline)) {
+        const int m = m0 + wm * WM + i * 16 + er, n = n0 + wn * WN + 32 * h + 8 * eq;
+        if (m < p.M && n < p.N) *reinterpret_cast<bf16x8*>(p.C + (int64_t)m * p.ldc + n) = v;  // N % 8 == 0
+      };
+      auto rows = [&](auto sig_tag, auto rtb_tag) __attribute__((always_inline)) {
+        auto eight = [&](int i, int h, auto finish) __attribute__((always_inline)) {
+          const int n = n0 + wn * WN + 32 * h + 8 * eq;
           bf16x8 v;
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const f32x4 y = fp4_branch4<EPI, decltype(sig_tag)::value, decltype(rtb_tag)::value>(
-                p, i8_value(acc[i][2 * h + c], sa, sw[c]), bias[c], n + 4 * c);
+                p, i8_value(acc[i][2 * h + c], sa[i], sw[2 * h + c]), bias[2 * h + c], n + 4 * c);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if constexpr (RESID) v[4 * c + e] = fp4_residual<EPI>(y[e], res[i][4 * c + e], gate[c][e]);
-              else v[4 * c + e] = (bf16)y[e];
+            for (int e = 0; e < 4; ++e) v[4 * c + e] = finish(y[e], c, e);
+          }
+          store(i, h, v);
+        };
+        if constexpr (RESID) {
+          // 32 columns at a time (all at once do not fit the registers)
+#pragma unroll
+          for (int h = 0; h < TN / 2; ++h) {
+            columns(2 * h);
+            columns(2 * h + 1);
+            bf16x8 res[TM];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+              int m = m0 + wm * WM + i * 16 + er;
+              m = m < p.M ? m : p.M - 1;
+              const int n = n0 + wn * WN + 32 * h + 8 * eq;
+              res[i] = *reinterpret_cast<const bf16x8*>(p.R + (int64_t)m * p.ldr + (n < p.N ? n : 0));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            wait_vmcnt<0>();  // (for the compiler too: no register waits for a load past here)
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+              eight(i, h, [&](float y, int c, int e) {
+                return fp4_residual<EPI>(y, res[i][4 * c + e], gate[2 * h + c][e]);
+              });
+              __builtin_amdgcn_sched_barrier(0);
             }
           }
-          if (m < p.M) *reinterpret_cast<bf16x8*>(p.C + (int64_t)m * p.ldc + n) = v;
+        } else {
+#pragma unroll
+          for (int j = 0; j < TN; ++j) columns(j);
+          wait_vmcnt<0>();  // (likewise)
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int h = 0; h < TN / 2; ++h) eight(i, h, [](float y, int, int) { return (bf16)y; });
         }
       };
       const bool sig = EPI == LTX_GEMM_EPI_BIAS && n0 + wn * WN + WN > p.sig_from;
@@ -338,7 +432,11 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
         else rows(std::false_type{}, std::false_type{});
       }
     }
+    // the next tile's first fragments again: the epilogue had their registers
+#pragma unroll
+    for (int j = 0; j < TN; ++j) read_share(slot, 0, 0, true, j);
   }
+  wait_vmcnt<0>();  // (the loads past the last stage: LDS is theirs until then)
 }
 
 using I8Large = I8Tile<256, 256, 2, 4, 2>;
@@ -361,33 +459,44 @@ __global__ __launch_bounds__(256) void i8_combine_kernel(GemmArgs p, int epi, in
 
 // ---- which kernel ------------------------------------------------------------------
 struct I8Plan {
-  int bm, bn;   // bn 0: the few-row kernel, bm its rows
+  int bm, bn;   // rows and columns of a tile; bn < 0: the few-row kernel, bm rows and -16 bn columns
   int splits;   // K ranges (tiles)
   int k_split;  // k of one, a multiple of 128
 };
 
-// Modelled time (us): a round of one workgroup per CU costs `fixed` (first loads and
-// epilogue) and per 128 k `idle` to `full`, as it fills the CUs; a split's second launch and
-// its partials.
+// Modelled times (us).  Tiles: a round of one workgroup per CU costs `fixed` (epilogue) and per
+// 128 k `idle` to `full`, as it fills the CUs (they share the L2s and the chip's power); a
+// split's second launch and its partials.  Model against measured (weights from HBM): 1296 x
+// 4096 -> 4096 in tiles of 256 x 256, 256 x 128, 128 x 128, 64 x 128 40 / 28 / 33 / 40
+// against 53 / 31 / 37 / 44, 3456 x 4096 -> 16384 202 / 220 / 260 / 335 against 208 / 218 / 261 / 337, 512 x 4096 -> 4096 64 x 128 16 / 17, 68 x 8192 -> 2048 in
+// 8 ranges 11 / 14.
 static double i8_time(int64_t M, int64_t N, int bm, int bn, int splits, double per) {
   const double wgs = (double)(((M + bm - 1) / bm) * ((N + bn - 1) / bn) * splits);
-  double fixed = 2.2, idle = 0.30, full = 0.36;
-  if (bm == 256 && bn == 256) fixed = 5.5, idle = 1.0, full = 1.4;
-  else if (bm == 256) fixed = 4.3, idle = 0.6, full = 0.8;
-  else if (bm == 128) fixed = 2.6, idle = 0.42, full = 0.5;
+  double fixed = 1.6, idle = 0.30, full = 0.34;
+  if (bm == 256 && bn == 256) fixed = 6.0, idle = 0.85, full = 1.40;
+  else if (bm == 256) fixed = 4.6, idle = 0.62, full = 0.78;
+  else if (bm == 128) fixed = 2.5, idle = 0.42, full = 0.48;
   const double rounds = (double)(int64_t)(wgs / 256), rest = wgs / 256 - rounds;
-  double t = 2.2 + rounds * (fixed + per * full);
+  double t = 4.0 + rounds * (fixed + per * full);
   if (rest > 0) t += fixed + per * (idle + (full - idle) * rest);
   if (splits > 1) t += 2.5 + (double)(M * N) * splits * 8 / 4e6;
   return t;
 }
+// The few-row kernel: a CU gets 33 bytes of operands per ns.
+static double i8_rows_time(int64_t M, int64_t N, int64_t K, int mb, int nb) {
+  const double wgs = (double)(((M + 16 * mb - 1) / (16 * mb)) * ((N + 16 * nb - 1) / (16 * nb)));
+  const double rounds = wgs < 256 ? 1.0 : wgs / 256;
+  return 3.2 + rounds * (double)(16 * (mb + nb) * K) / 33e3;
+}
 
 static I8Plan i8_plan(int64_t M, int64_t N, int64_t K) {
   static const int tile[4][2] = {{256, 256}, {256, 128}, {128, 128}, {64, 128}};
-  if (M <= 32) return {M <= 16 ? 16 : 64, 0, 1, (int)K};
+  // rows of the few-row kernel; 32 columns where that leaves a workgroup for every CU
+  const int mb = M <= 16 ? 1 : (M <= 32 ? 2 : 4), nb = N >= 32 * 256 ? 2 : 1;
   const int64_t units = (K + 127) / 128;
-  I8Plan pl = {64, 128, 1, (int)(units * 128)};
-  double best = 1e30;
+  I8Plan pl = {16 * mb, -nb, 1, (int)K};
+  double best = i8_rows_time(M, N, K, mb, nb);
+  if (M <= 32) return pl;
   for (const auto& t : tile) {
     const int64_t tiles = ((M + t[0] - 1) / t[0]) * ((N + t[1] - 1) / t[1]);
     for (int want = 1; want <= 16; ++want) {
@@ -409,7 +518,7 @@ template <int EPI>
 static void i8_launch_tiles(GemmArgs p, const I8Plan& pl, hipStream_t s) {
   p.tiles_m = (p.M + pl.bm - 1) / pl.bm;
   p.tiles_n = (p.N + pl.bn - 1) / pl.bn;
-  const int blocks = p.tiles_m * p.tiles_n * pl.splits;
+  const int all = p.tiles_m * p.tiles_n * pl.splits, blocks = all < 256 ? all : 256;
   auto go = [&](auto t) {
     using T = decltype(t);
     gemm_i8_kernel<T, EPI><<<blocks, T::THREADS, 0, s>>>(p, pl.k_split);
@@ -483,15 +592,16 @@ extern "C" int ltx_gemm_i8_bf16(const int8_t* A, int64_t lda, const float* a_sca
   p.K = (int)K;
   hipStream_t s = (hipStream_t)stream;
   const int epi = epilogue & 0xff;
-  auto rows = [&](int bm) {
-    if (bm == 16 && N >= 32 * 256) i8_launch_rows<1, 2>(p, epi, s);
-    else if (bm == 16) i8_launch_rows<1, 1>(p, epi, s);
+  auto rows = [&](int bm, int nb) {
+    if (bm == 16 && nb == 1) i8_launch_rows<1, 1>(p, epi, s);
+    else if (bm == 16) i8_launch_rows<1, 2>(p, epi, s);
+    else if (bm == 32 && nb == 1) i8_launch_rows<2, 1>(p, epi, s);
+    else if (bm == 32) i8_launch_rows<2, 2>(p, epi, s);
+    else if (nb == 1) i8_launch_rows<4, 1>(p, epi, s);
     else i8_launch_rows<4, 2>(p, epi, s);
-  };
-  if (pl.bn == 0) {
-    rows(pl.bm);
     return ltx_launch_status();
-  }
+  };
+  if (pl.bn < 0) return rows(pl.bm, -pl.bn);
   // Rows that one launch of the tile kernel takes: its operands' byte offsets have 31
   // bits.  Rows past them in further launches; none where a tile's rows, or the weights,
   // are past them: then the few-row kernel, whose addresses have 64 bits
@@ -499,10 +609,7 @@ extern "C" int ltx_gemm_i8_bf16(const int8_t* A, int64_t lda, const float* a_sca
   int64_t piece = lim / lda;
   if (N > lim / ldw) piece = 0;
   if (piece < M) piece = piece / 256 * 256;
-  if (piece == 0) {
-    rows(64);
-    return ltx_launch_status();
-  }
+  if (piece == 0) return rows(64, 2);
   if (pl.splits > 1 && piece >= M) {
     p.partial = (float*)workspace;
     i8_launch_tiles<kEpiPartial>(p, pl, s);
