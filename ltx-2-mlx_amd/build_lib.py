@@ -77,7 +77,7 @@ def build_calls() -> Path | None:
                torch_header if not any((Path(p) / torch_header).exists() for p in include_paths()) else None)
     if missing:
         out.unlink(missing_ok=True)
-        print(f"no {missing}: {out.name} is not built, small MXFP4 and rotary calls go through Python")
+        print(f"no {missing}: {out.name} is not built, small MXFP4, int8, rotary and per-head norm calls go through Python")
         return None
     cmd = [compiler, "-O2", "-std=c++17", "-shared", "-fPIC",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",

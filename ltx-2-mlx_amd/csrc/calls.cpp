@@ -1,7 +1,7 @@
-// Host side of the small MXFP4 and rotary calls: argument checks, output
-// allocation and the launch in one native call.  A product of one row or the
-// rotation of one token takes the GPU 3-6 us; checking the tensors and making
-// the call from Python takes 7-10, from here 4-6.
+// Host side of the small MXFP4, int8, rotary and per-head norm calls: argument
+// checks, output allocation and the launch in one native call.  A product of one
+// row or the rotation of one token takes the GPU 3-6 us; checking the tensors and
+// making the call from Python takes 7-13, from here 4-6.
 //
 // Every function does the usual case only and returns None for anything else
 // (an unusual stride, a type or size that does not fit, a refusal of the entry
@@ -26,6 +26,13 @@ struct Entry {
   decltype(&ltx_quantize_mxfp4) quantize;
   decltype(&ltx_dequantize_mxfp4_bf16) dequantize;
   decltype(&ltx_rotary) rotary;
+  decltype(&ltx_quantize_int8) quantize8;
+  decltype(&ltx_dequantize_w8_bf16) dequantize8;
+  decltype(&ltx_gemm_i8_bf16) gemm8;
+  decltype(&ltx_gemm_i8_workspace_bytes) gemm8_ws;
+  decltype(&ltx_headnorm_rotary) headnorm;
+  decltype(&ltx_headnorm_rotary_grad) headnorm_grad;
+  decltype(&ltx_headnorm_rotary_grad_workspace_bytes) headnorm_ws;
 } entry = {};
 
 PyObject* general() { Py_RETURN_NONE; }
@@ -44,7 +51,7 @@ PyObject* outcome(int status, PyObject* result) {
   return PyLong_FromLong(status);
 }
 PyObject* pair(at::Tensor a, at::Tensor b) {
-  PyObject* pa = THPVariable_Wrap(std::move(a));
+  PyObject* pa = a.defined() ? THPVariable_Wrap(std::move(a)) : (Py_INCREF(Py_None), Py_None);
   PyObject* pb = b.defined() ? THPVariable_Wrap(std::move(b)) : (Py_INCREF(Py_None), Py_None);
   PyObject* r = pa && pb ? PyTuple_Pack(2, pa, pb) : nullptr;
   Py_XDECREF(pa);
@@ -144,6 +151,33 @@ bool whole_words(const at::Tensor& words, int64_t rows, int64_t k, int64_t ld) {
                               static_cast<int64_t>(words.storage().nbytes());
 }
 
+// Row strides of a product's residual (0 without one) and of its output, new (M, N) or
+// `given`; false for what needs the general path.
+bool outputs(const at::Tensor* res, const at::Tensor* gate, const at::Tensor* given, bool resid, int64_t M, int64_t N,
+             int64_t device, std::initializer_list<const at::Tensor*> operands, int64_t* ldr, int64_t* ldc) {
+  *ldr = 0;
+  *ldc = N;
+  if (resid) {
+    if (!res || !gate || res->dim() != 2 || res->scalar_type() != at::kBFloat16 || res->size(0) != M ||
+        res->size(1) != N || res->stride(1) != 1 || !on(*res, device) || gate->scalar_type() != at::kFloat ||
+        gate->numel() != N || !gate->is_contiguous() || !on(*gate, device))
+      return false;
+    *ldr = M > 1 ? res->stride(0) : N;
+    if (*ldr < N) return false;
+  }
+  if (given) {
+    if (given->dim() != 2 || given->scalar_type() != at::kBFloat16 || given->size(0) != M || given->size(1) != N ||
+        given->stride(1) != 1 || !on(*given, device) || (resid && !same_view(*given, *res) && !apart(*given, *res)))
+      return false;
+    for (const at::Tensor* t : operands)
+      if (t && !apart(*given, *t)) return false;
+    if (resid && !apart(*given, *gate)) return false;
+    if (M > 1) *ldc = given->stride(0);
+    if (*ldc < N) return false;
+  }
+  return true;
+}
+
 // linear(x, x_words or None, codes, words, bias or None, flags, epilogue, residual or None, gate or None,
 //        sigmoid_from or -1, out or None, device, stream)
 PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -171,25 +205,8 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (bias && (bias->scalar_type() != at::kFloat || bias->numel() != N || !bias->is_contiguous() || !on(*bias, device)))
     return general();
   const bool resid = epi == LTX_GEMM_EPI_RESIDUAL || epi == LTX_GEMM_EPI_RESIDUAL_ROUND;
-  int64_t ldr = 0;
-  if (resid) {
-    if (!res || !gate || res->dim() != 2 || res->scalar_type() != at::kBFloat16 || res->size(0) != M ||
-        res->size(1) != N || res->stride(1) != 1 || !on(*res, device) || gate->scalar_type() != at::kFloat ||
-        gate->numel() != N || !gate->is_contiguous() || !on(*gate, device))
-      return general();
-    ldr = M > 1 ? res->stride(0) : N;
-    if (ldr < N) return general();
-  }
-  int64_t ldc = N;
-  if (given) {
-    if (given->dim() != 2 || given->scalar_type() != at::kBFloat16 || given->size(0) != M || given->size(1) != N ||
-        given->stride(1) != 1 || !on(*given, device) || (resid && !same_view(*given, *res) && !apart(*given, *res)))
-      return general();
-    for (const at::Tensor* t : {x, xs, w, ws, bias, resid ? gate : nullptr})
-      if (t && !apart(*given, *t)) return general();
-    if (M > 1) ldc = given->stride(0);
-    if (ldc < N) return general();
-  }
+  int64_t ldr, ldc;
+  if (!outputs(res, gate, given, resid, M, N, device, {x, xs, w, ws, bias}, &ldr, &ldc)) return general();
   at::Tensor out = given ? *given : empty({M, N}, at::kBFloat16, *x);
   const int64_t bytes = xs ? entry.mx4_ws(M, N, K) : entry.gemm_ws(M, N, K);
   at::Tensor work;
@@ -252,6 +269,92 @@ PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
                  result);
 }
 
+int float_type(const at::Tensor& t) {
+  const auto type = t.scalar_type();
+  return type == at::kBFloat16 ? 0 : (type == at::kHalf ? 1 : (type == at::kFloat ? 2 : -1));
+}
+
+// dense-column (rows, k) int8 codes with a scale for each row
+bool int8(const at::Tensor* codes, const at::Tensor* scales, int64_t device, int64_t* rows, int64_t* k, int64_t* ld) {
+  if (!codes || !scales || codes->scalar_type() != at::kChar || scales->scalar_type() != at::kFloat ||
+      codes->dim() != 2 || scales->dim() != 1 || !on(*codes, device) || !on(*scales, device))
+    return false;
+  *rows = codes->size(0);
+  *k = codes->size(1);
+  *ld = *rows > 1 ? codes->stride(0) : *k;
+  return *rows > 0 && *k > 0 && codes->stride(1) == 1 && *ld >= *k && scales->size(0) == *rows && scales->is_contiguous();
+}
+
+// quantize8(x, device, stream) -> (codes, scales)
+PyObject* quantize8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 3 || !entry.quantize8) return general();
+  const at::Tensor* x = tensor(a[0]);
+  const int64_t device = PyLong_AsLongLong(a[1]);
+  void* stream = PyLong_AsVoidPtr(a[2]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!x || x->dim() != 2 || !on(*x, device) || x->stride(1) != 1) return general();
+  const int dtype = float_type(*x);
+  const int64_t rows = x->size(0), k = x->size(1), ldx = rows > 1 ? x->stride(0) : k;
+  if (dtype < 0 || rows < 1 || k < 16 || k % 16 || ldx < k) return general();
+  at::Tensor codes = empty({rows, k}, at::kChar, *x), scales = empty({rows}, at::kFloat, *x);
+  PyObject* result = pair(codes, scales);
+  if (!result) return nullptr;
+  return outcome(entry.quantize8(x->const_data_ptr(), dtype, ldx, rows, k, static_cast<int8_t*>(codes.data_ptr()), k,
+                                 static_cast<float*>(scales.data_ptr()), stream),
+                 result);
+}
+
+// dequantize8(codes, scales, device, stream)
+PyObject* dequantize8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 4 || !entry.dequantize8) return general();
+  const at::Tensor *codes = tensor(a[0]), *scales = tensor(a[1]);
+  const int64_t device = PyLong_AsLongLong(a[2]);
+  void* stream = PyLong_AsVoidPtr(a[3]);
+  if (PyErr_Occurred()) return nullptr;
+  int64_t rows, k, ld;
+  if (!int8(codes, scales, device, &rows, &k, &ld)) return general();
+  at::Tensor out = empty({rows, k}, at::kBFloat16, *codes);
+  PyObject* result = THPVariable_Wrap(out);
+  if (!result) return nullptr;
+  return outcome(entry.dequantize8(static_cast<const int8_t*>(codes->const_data_ptr()), ld,
+                                   scales->const_data_ptr<float>(), rows, k, out.data_ptr(), k, stream),
+                 result);
+}
+
+// linear8(codes, scales, weight codes, weight scales, bias or None, flags, epilogue, residual or None, gate or None,
+//         sigmoid_from or -1, out or None, device, stream)
+PyObject* linear8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 13 || !entry.gemm8) return general();
+  const at::Tensor *x = tensor(a[0]), *xs = tensor(a[1]), *w = tensor(a[2]), *ws = tensor(a[3]), *bias = tensor(a[4]),
+                   *res = tensor(a[7]), *gate = tensor(a[8]), *given = tensor(a[10]);
+  const int64_t flags = PyLong_AsLongLong(a[5]), epi = PyLong_AsLongLong(a[6]), sig = PyLong_AsLongLong(a[9]),
+                device = PyLong_AsLongLong(a[11]);
+  void* stream = PyLong_AsVoidPtr(a[12]);
+  if (PyErr_Occurred()) return nullptr;
+  int64_t M, N, K, kx, lda, ldw;
+  if ((!bias && a[4] != Py_None) || (!given && a[10] != Py_None) || !int8(w, ws, device, &N, &K, &ldw) ||
+      !int8(x, xs, device, &M, &kx, &lda) || kx != K)
+    return general();
+  if (bias && (bias->scalar_type() != at::kFloat || bias->numel() != N || !bias->is_contiguous() || !on(*bias, device)))
+    return general();
+  const bool resid = epi == LTX_GEMM_EPI_RESIDUAL || epi == LTX_GEMM_EPI_RESIDUAL_ROUND;
+  int64_t ldr, ldc;
+  if (!outputs(res, gate, given, resid, M, N, device, {x, xs, w, ws, bias}, &ldr, &ldc)) return general();
+  at::Tensor out = given ? *given : empty({M, N}, at::kBFloat16, *x);
+  const int64_t bytes = entry.gemm8_ws(M, N, K);
+  at::Tensor work;
+  if (bytes > 0) work = empty({bytes}, at::kByte, *x);
+  PyObject* result = THPVariable_Wrap(out);  // (before the launch: it may fail)
+  if (!result) return nullptr;
+  return outcome(entry.gemm8(static_cast<const int8_t*>(x->const_data_ptr()), lda, xs->const_data_ptr<float>(),
+                             static_cast<const int8_t*>(w->const_data_ptr()), ldw, ws->const_data_ptr<float>(),
+                             bias ? bias->const_data_ptr<float>() : nullptr, out.data_ptr(), ldc, M, N, K,
+                             (int)(epi | flags), resid ? res->const_data_ptr() : nullptr, ldr,
+                             resid ? gate->const_data_ptr<float>() : nullptr, sig < 0 ? N : sig,
+                             bytes > 0 ? work.data_ptr() : nullptr, bytes, stream),
+                 result);
+}
+
 // one side of a rotation
 bool side(const at::Tensor& x, const at::Tensor& out, ltx_rotary_rows* r) {
   const int b = x.dim() == 4 ? 1 : 0;
@@ -310,6 +413,108 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
                  result);
 }
 
+// One side of the per-head norm (g, dw: of its gradient) and its output, new or `given`; false
+// for what needs the general path.
+bool head_side(const at::Tensor& x, const at::Tensor* g, const at::Tensor* w, const at::Tensor* given, int64_t device,
+               at::Tensor* out, at::Tensor* dw, ltx_headnorm_rows* r) {
+  const int b = x.dim() == 4 ? 1 : 0;
+  const int64_t dh = x.size(b + 2);
+  if (!on(x, device) || x.stride(b + 2) != 1 || x.size(b + 1) < 1) return false;
+  if (w && (w->scalar_type() != at::kFloat || w->dim() != 1 || w->size(0) != dh || !w->is_contiguous() || !on(*w, device)))
+    return false;
+  if (g && (g->scalar_type() != x.scalar_type() || g->sizes() != x.sizes() || g->stride(b + 2) != 1 || !on(*g, device)))
+    return false;
+  if (given && (given->scalar_type() != x.scalar_type() || given->sizes() != x.sizes() || given->stride(b + 2) != 1 ||
+                !on(*given, device) || !distinct(*given)))
+    return false;
+  *out = given ? *given : empty(x.sizes(), x.scalar_type(), x);
+  if (g && w) *dw = empty({dh}, at::kFloat, x);
+  auto batch = [&](const at::Tensor& t) { return b ? t.stride(0) : 0; };
+  *r = {x.const_data_ptr(), batch(x), x.stride(b), x.stride(b + 1),
+        out->data_ptr(), batch(*out), out->stride(b), out->stride(b + 1),
+        g ? g->const_data_ptr() : nullptr, g ? batch(*g) : 0, g ? g->stride(b) : 0, g ? g->stride(b + 1) : 0,
+        w ? w->const_data_ptr<float>() : nullptr, dw->defined() ? static_cast<float*>(dw->data_ptr()) : nullptr,
+        x.size(b + 1)};
+  return true;
+}
+
+// [gq, gk or None,] q, k or None, wq or None, wk or None, positions, inv_freq, flags, factor, eps, weight_offset,
+// q' or None, k' or None, device, stream -> (q', k' or None) or (dq, dk or None, dwq or None, dwk or None)
+template <bool GRAD>
+PyObject* head_call(PyObject* const* a, Py_ssize_t n) {
+  constexpr int G = GRAD ? 2 : 0;
+  if (n != 14 + G || !(GRAD ? (void*)entry.headnorm_grad : (void*)entry.headnorm)) return general();
+  const at::Tensor *gq = GRAD ? tensor(a[0]) : nullptr, *gk = GRAD ? tensor(a[1]) : nullptr;
+  a += G;
+  const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *wq = tensor(a[2]), *wk = tensor(a[3]), *pos = tensor(a[4]),
+                   *inv = tensor(a[5]), *oq = tensor(a[10]), *ok = tensor(a[11]);
+  const int64_t flags = PyLong_AsLongLong(a[6]), device = PyLong_AsLongLong(a[12]);
+  const double factor = PyFloat_AsDouble(a[7]), eps = PyFloat_AsDouble(a[8]), offset = PyFloat_AsDouble(a[9]);
+  void* stream = PyLong_AsVoidPtr(a[13]);
+  if (PyErr_Occurred()) return nullptr;
+  auto odd = [&](int i, const at::Tensor* t) { return !t && a[i] != Py_None; };
+  if (!q || odd(1, k) || odd(2, wq) || odd(3, wk) || odd(10, oq) || odd(11, ok) || !pos || !inv ||
+      (q->dim() != 3 && q->dim() != 4) || (!k && (wk || gk || ok)) || (GRAD && (!gq || (k && !gk))))
+    return general();
+  const int64_t dims = q->dim(), batch = dims == 4 ? q->size(0) : 1, tokens = q->size(dims - 3), dh = q->size(dims - 1);
+  const int dtype = float_type(*q);
+  const auto ptype = pos->scalar_type();
+  const int pos_type = ptype == at::kInt ? 0 : (ptype == at::kLong ? 1 : (ptype == at::kFloat ? 2 : (ptype == at::kDouble ? 3 : -1)));
+  if (dtype < 0 || pos_type < 0 || batch < 1 || tokens < 1 || !on(*pos, device) || !on(*inv, device) ||
+      inv->scalar_type() != at::kDouble || inv->dim() != 1 || !inv->is_contiguous() || !pos->is_contiguous())
+    return general();
+  const bool own = pos->dim() == 2;
+  if ((own && (pos->size(0) != batch || pos->size(1) != tokens)) || (!own && (pos->dim() != 1 || pos->size(0) != tokens)))
+    return general();
+  const int64_t d = 2 * inv->numel();
+  if (d < 2 || d > dh) return general();
+  if (k && (k->dim() != dims || k->scalar_type() != q->scalar_type() || k->size(dims - 1) != dh ||
+            k->size(dims - 3) != tokens || (dims == 4 && k->size(0) != batch)))
+    return general();
+  at::Tensor out[2], dw[2], work;
+  ltx_headnorm_rows rows[2];
+  if (!head_side(*q, gq, wq, oq, device, &out[0], &dw[0], &rows[0]) ||
+      (k && !head_side(*k, gk, wk, ok, device, &out[1], &dw[1], &rows[1])))
+    return general();
+  // an output may be its own input (or gradient), and keeps off everything else
+  auto fits8 = [&](const at::Tensor* mine, std::initializer_list<const at::Tensor*> own_ones,
+                   std::initializer_list<const at::Tensor*> others) {
+    if (!mine) return true;
+    for (const at::Tensor* t : own_ones)
+      if (t && !same_view(*mine, *t) && !apart(*mine, *t)) return false;
+    for (const at::Tensor* t : others)
+      if (t && !apart(*mine, *t)) return false;
+    return true;
+  };
+  if (!fits8(oq, {q, gq}, {k, gk, ok, wq, wk, pos, inv}) || !fits8(ok, {k, gk}, {q, gq, oq, wq, wk, pos, inv}))
+    return general();
+  const bool sums = dw[0].defined() || dw[1].defined();
+  const int64_t bytes = sums ? entry.headnorm_ws(dh) : 0;
+  if (sums) work = empty({bytes}, at::kByte, *q);
+  PyObject* result = pair(out[0], out[1]);
+  if (result && GRAD) {
+    PyObject* both = pair(dw[0], dw[1]);
+    PyObject* four = both ? PySequence_Concat(result, both) : nullptr;
+    Py_XDECREF(both);
+    Py_DECREF(result);
+    result = four;
+  }
+  if (!result) return nullptr;
+  const int64_t pos_batch = own ? tokens : 0;
+  const double* freq = inv->const_data_ptr<double>();
+  if constexpr (GRAD)
+    return outcome(entry.headnorm_grad(&rows[0], k ? &rows[1] : nullptr, dtype, batch, tokens, dh, d,
+                                       pos->const_data_ptr(), pos_type, pos_batch, freq, factor, eps, offset, (int)flags,
+                                       sums ? static_cast<float*>(work.data_ptr()) : nullptr, bytes, stream),
+                   result);
+  else
+    return outcome(entry.headnorm(&rows[0], k ? &rows[1] : nullptr, dtype, batch, tokens, dh, d, pos->const_data_ptr(),
+                                  pos_type, pos_batch, freq, factor, eps, offset, (int)flags, stream),
+                   result);
+}
+PyObject* headnorm(PyObject*, PyObject* const* a, Py_ssize_t n) { return head_call<false>(a, n); }
+PyObject* headnorm_grad(PyObject*, PyObject* const* a, Py_ssize_t n) { return head_call<true>(a, n); }
+
 // a C++ exception (no memory for an output; nothing throws after a launch)
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
@@ -322,13 +527,17 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 
 // bind(addresses of the entry points, in the order of Entry)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  void** slots[] = {(void**)&entry.gemm,     (void**)&entry.gemm_ws,    (void**)&entry.mx4,   (void**)&entry.mx4_ws,
-                    (void**)&entry.quantize, (void**)&entry.dequantize, (void**)&entry.rotary};
-  if (n != 7) {
-    PyErr_SetString(PyExc_TypeError, "bind takes seven addresses");
+  void** slots[] = {(void**)&entry.gemm,       (void**)&entry.gemm_ws,       (void**)&entry.mx4,
+                    (void**)&entry.mx4_ws,     (void**)&entry.quantize,      (void**)&entry.dequantize,
+                    (void**)&entry.rotary,     (void**)&entry.quantize8,     (void**)&entry.dequantize8,
+                    (void**)&entry.gemm8,      (void**)&entry.gemm8_ws,      (void**)&entry.headnorm,
+                    (void**)&entry.headnorm_grad, (void**)&entry.headnorm_ws};
+  constexpr int kSlots = sizeof(slots) / sizeof(slots[0]);
+  if (n != kSlots) {
+    PyErr_Format(PyExc_TypeError, "bind takes %d addresses", kSlots);
     return nullptr;
   }
-  for (int i = 0; i < 7; ++i) *slots[i] = PyLong_AsVoidPtr(a[i]);
+  for (int i = 0; i < kSlots; ++i) *slots[i] = PyLong_AsVoidPtr(a[i]);
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
@@ -339,6 +548,11 @@ PyMethodDef methods[] = {
     {"quantize", (PyCFunction)(void (*)())guarded<quantize>, METH_FASTCALL, "rows to MXFP4, or None"},
     {"dequantize", (PyCFunction)(void (*)())guarded<dequantize>, METH_FASTCALL, "MXFP4 rows to bf16, or None"},
     {"rotary", (PyCFunction)(void (*)())guarded<rotary>, METH_FASTCALL, "rotary positions, or None"},
+    {"quantize8", (PyCFunction)(void (*)())guarded<quantize8>, METH_FASTCALL, "rows to int8, or None"},
+    {"dequantize8", (PyCFunction)(void (*)())guarded<dequantize8>, METH_FASTCALL, "int8 rows to bf16, or None"},
+    {"linear8", (PyCFunction)(void (*)())guarded<linear8>, METH_FASTCALL, "an int8 product, or None"},
+    {"headnorm", (PyCFunction)(void (*)())guarded<headnorm>, METH_FASTCALL, "per-head norm and rotation, or None"},
+    {"headnorm_grad", (PyCFunction)(void (*)())guarded<headnorm_grad>, METH_FASTCALL, "its gradients, or None"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

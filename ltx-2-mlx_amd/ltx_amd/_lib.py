@@ -162,12 +162,14 @@ ERR_SCRATCH_LIMIT = -5
 ATTN_NOALLOC_SCRATCH_BYTES = 32 << 20
 
 _LIB: ctypes.CDLL | None = None
-# Native host side of the small MXFP4 and rotary calls (csrc/calls.cpp, the _calls.so
-# beside the library), once that is loaded; None where there is none for this Python and
+# Native host side of the small MXFP4, int8, rotary and per-head norm calls (csrc/calls.cpp,
+# the _calls.so beside the library), once that is loaded; None where there is none for this Python and
 # torch: their Python path does the same
 CALLS = None
 _CALLS_ENTRIES = ("ltx_gemm_mxfp4_bf16", "ltx_gemm_mxfp4_workspace_bytes", "ltx_gemm_mx4_bf16",
-                  "ltx_gemm_mx4_workspace_bytes", "ltx_quantize_mxfp4", "ltx_dequantize_mxfp4_bf16", "ltx_rotary")
+                  "ltx_gemm_mx4_workspace_bytes", "ltx_quantize_mxfp4", "ltx_dequantize_mxfp4_bf16", "ltx_rotary",
+                  "ltx_quantize_int8", "ltx_dequantize_w8_bf16", "ltx_gemm_i8_bf16", "ltx_gemm_i8_workspace_bytes",
+                  "ltx_headnorm_rotary", "ltx_headnorm_rotary_grad", "ltx_headnorm_rotary_grad_workspace_bytes")
 _current_device = getattr(torch._C, "_cuda_getDevice", None)  # (None: a torch without a GPU backend)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -219,8 +221,8 @@ def _load_calls(path: Path, handle: ctypes.CDLL):
     except (ImportError, AttributeError) as e:
         built_for = str(e)
     if built_for != want:
-        warnings.warn(f"{path} is built for something other than {want} ({built_for}): small MXFP4 and rotary calls "
-                      f"go through Python; build again", RuntimeWarning, stacklevel=2)
+        warnings.warn(f"{path} is built for something other than {want} ({built_for}): small MXFP4, int8, rotary "
+                      f"and per-head norm calls go through Python; build again", RuntimeWarning, stacklevel=2)
         return None
     calls.bind(*(ctypes.cast(getattr(handle, name), _vp).value for name in _CALLS_ENTRIES))
     return calls

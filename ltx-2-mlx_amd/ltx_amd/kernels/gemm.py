@@ -656,6 +656,11 @@ def quantize_rows_int8(x: torch.Tensor) -> Int8Rows:
     scale = max|v| / 127, codes v / scale to the nearest, ties to even (both
     quotients in fp32).  A row of zeros has scale 0; one with a NaN or an infinity
     scale NaN, which its products and its decoded values take."""
+    if _lib.CALLS is not None:
+        where = _lib.fast_stream(x)
+        rows = None if where is None else _lib.CALLS.quantize8(x, *where)
+        if rows is not None:
+            return Int8Rows(*_lib.launched(rows, "ltx_quantize_int8"))
     k = x.shape[-1]
     dtype = _QUANT_DTYPES.get(x.dtype)
     if dtype is None:
@@ -681,6 +686,11 @@ def quantize_rows_int8(x: torch.Tensor) -> Int8Rows:
 def dequantize_rows_int8(rows: Int8Rows) -> torch.Tensor:
     """bf16 (M, K) values of int8 rows: codes times scales, rounded once."""
     codes, scales = rows.codes, rows.scales
+    if _lib.CALLS is not None:
+        where = _lib.fast_stream(codes)
+        out = None if where is None else _lib.CALLS.dequantize8(codes, scales, *where)
+        if out is not None:
+            return _lib.launched(out, "ltx_dequantize_w8_bf16")
     m, k, ldq = _check_int8("dequantize_rows_int8", codes, scales)
     out = codes.new_empty((m, k), dtype=torch.bfloat16)
     if m:
@@ -701,6 +711,15 @@ def _linear_int8(x: Int8Rows, weight: LinearWeight, epilogue: int, out: torch.Te
     """:func:`linear` for int8 rows and int8 weights."""
     w, scale, bias = weight.w, weight.scale, weight.bias
     codes, xs = x.codes, x.scales
+    if _lib.CALLS is not None and LAUNCH_HOOK is None:
+        where = _lib.fast_stream(w)
+        if where is not None:
+            y = _lib.CALLS.linear8(codes, xs, w, scale, bias,
+                                   _lib.GEMM_ROUND_THEN_BIAS if weight.qlinear and bias is not None else 0, epilogue,
+                                   residual, gate, -1 if sigmoid_from is None else max(int(sigmoid_from), 0), out,
+                                   *where)
+            if y is not None:
+                return _lib.launched(y, "ltx_gemm_i8_bf16")
     n, k, ldw = _check_int8("weight", w, scale)
     m, kx, lda = _check_int8("activations", codes, xs)
     if kx != k:

@@ -236,6 +236,15 @@ def _headnorm(name: str, q, k, gq, gk, wq, wk, positions, inv_freq, eps, weight_
     if layout not in ROTARY_LAYOUTS:
         raise ValueError(f"layout must be one of {ROTARY_LAYOUTS}, got {layout!r}")
     grad = gq is not None
+    flags = _lib.ROTARY_INTERLEAVED if layout == "interleaved" else 0
+    given = out if out is not None else (None, None)
+    if _lib.CALLS is not None and positions is not None:
+        where = _lib.fast_stream(q)
+        if where is not None:
+            args = (q, k, wq, wk, positions, inv_freq, flags, factor, eps, weight_offset, *given, *where)
+            done = _lib.CALLS.headnorm_grad(gq, gk, *args) if grad else _lib.CALLS.headnorm(*args)
+            if done is not None:
+                return _lib.launched(done, name)
     shape = q.shape
     dtype = _ROTARY_DTYPES.get(q.dtype)
     if dtype is None or not 3 <= len(shape) <= 4:
@@ -269,7 +278,6 @@ def _headnorm(name: str, q, k, gq, gk, wq, wk, positions, inv_freq, eps, weight_
         raise ValueError("a factor belongs to the rotation, which has no positions")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    given = out if out is not None else (None, None)
     if k is None and given[1] is not None:
         raise ValueError("out has a tensor for k, but there is no k")
     sides = []
@@ -306,8 +314,7 @@ def _headnorm(name: str, q, k, gq, gk, wq, wk, positions, inv_freq, eps, weight_
                 raise ValueError("an output of the per-head norm overlaps another tensor of the call")
     device = _lib.same_device(q, k, gq, gk, wq, wk, positions, inv_freq, oq, ok)
     args = [rq, rk, dtype, batch, tokens, dh, d, None if positions is None else positions.data_ptr(), pos_type, pos_batch,
-            None if inv_freq is None else inv_freq.data_ptr(), factor, eps, weight_offset,
-            _lib.ROTARY_INTERLEAVED if layout == "interleaved" else 0]
+            None if inv_freq is None else inv_freq.data_ptr(), factor, eps, weight_offset, flags]
     if grad:
         sums = dwq is not None or dwk is not None
         if batch * tokens == 0 and not sums:
