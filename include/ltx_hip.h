@@ -208,7 +208,8 @@ int ltx_rotary(const ltx_rotary_rows* q, const ltx_rotary_rows* k, int dtype, in
  *   dx = r (gn - r x mean(gn r x)),  gn = (weight_offset + weight) R^T g,
  *   dweight = sum over tokens and heads of r x R^T g   (fp32 (head_dim), or NULL),
  * with x the same inputs as the forward call's.
- * Tensors, positions, frequencies and limits as ltx_rotary; `out` may be x (in
+ * Tensors, positions, frequencies and limits as ltx_rotary, but at most 2^25 - 4
+ * tokens over the batch and token and head strides below 2^32; `out` may be x (in
  * the gradient: x or g) with the same strides and must not overlap anything else.
  * g and dweight are not used by the forward call.  A side of no heads, or a call of
  * no tokens, leaves dweight zero.  The sum over tokens and heads is taken in an order that the sizes fix:

@@ -8,13 +8,23 @@
 // with R the rotation of rotary.hip (pairs (i, i + rotary / 2) or (2 i, 2 i + 1) of
 // the first `rotary` channels, the others as they are; rotary 0: no rotation).
 //
-// Bound by memory: every element is read and written once.  A head lives in the
+// Bound by memory: every element is read and written once.  A workgroup takes the
+// query heads or the key heads of a few tokens.  A head lives in the
 // registers of a group of lanes (a power of two of them, each with one item: the two
 // halves of VEC pairs, or two vectors of neighbouring pairs or of plain channels), so
 // the sums over its channels are a few lane exchanges.  A lane keeps its channels
 // for all heads, and with them the norm weights and, in the gradient, its share of dw.
+// The first heads are on their way while the workgroup computes its tokens' cosines and
+// sines, the next ones while it works on these.
 // Sums, r and dw are fp32, cosines and sines as in rotary.hip from fp64 angles; one
 // rounding at the end.
+// Measured: 3456 tokens x 64 heads of 128 bf16 29 us (3.9 TB/s; the rotation alone 22), 14640 x 40
+// heads of 128 bf16 65 (4.6 TB/s), 14639 x 40 heads of 64 fp32 60 (5.0 TB/s), one token 4.7, its gradient at
+// 14640 x 40 heads of 128 bf16 94 (4.8 TB/s, 4 of them the second launch), 3456 x 64 heads 46.  About
+// 300 vector instructions per eight heads of 128 lie beside the loads.  Beside it: both sides in one
+// workgroup 43, 88 and 127 us (3456 and 14640 tokens, gradient); two heads on their way and one at work
+// (29, 70, 102); as many workgroups as the CUs hold, each with tiles of the same size (28, 70, 101); positions in
+// batches of four, a pair per thread (29, 65, 109).
 #include <type_traits>
 
 #include "ltx_common.h"
@@ -23,24 +33,30 @@ namespace ltx {
 
 constexpr int kHnThreads = 256, kHnTokens = 16, kHnMaxDim = 512;
 constexpr int kHnTable = 2048;  // cosines (and sines) of a workgroup
-constexpr int64_t kHnBlocks = (1 << 24) - 1;  // a launch has fewer than 2^32 threads
+constexpr int64_t kHnBlocks = (1 << 23) - 1;  // of a side: a launch has fewer than 2^32 threads
 constexpr int64_t kHnHeads = 1 << 30;
-constexpr int kHnGradBlocks = 1024;  // workgroups of the gradient, each with a share of dw
+// Workgroups of a side of the gradient, each with a share of dw and one tile after another.  384 /
+// 512 / 1024: 14640 x 32 and 8 heads of 128 bf16 96 / 94 / 98 us, 3456 x 32 heads of each side
+// 43 / 46 / 52, 9000 x 12 and 4 heads of 80 fp16 27 / 24 / 23.
+constexpr int kHnGradBlocks = 512;
 
+struct HnSide {
+  ltx_headnorm_rows r;
+  int per_block;      // tokens of a tile
+  int tiles, blocks;  // (forward: a workgroup each)
+};
 struct HnArgs {
-  ltx_headnorm_rows side[2];
-  int64_t batch, tokens;
+  HnSide side[2];
+  int batch, tokens, all;
   int head_dim, rotary;
   const void* positions;
   int64_t pos_batch;
   int pos_type;
   const double* inv_freq;
   float factor, eps, offset;
-  int lanes;      // of a head's group
-  int per_block;  // tokens of a tile
-  int table;      // table entries of a token: its pairs, up to a multiple of 4
-  int64_t tiles;
-  float* partial;  // gradient: dw of each workgroup, (blocks, 2, head_dim)
+  int lanes;       // of a head's group
+  int table;       // table entries of a token: its pairs, up to a multiple of 4
+  float* partial;  // gradient: dw of each workgroup, (blocks, head_dim)
 };
 
 __device__ __forceinline__ double hn_position(const HnArgs& p, int64_t i) {
@@ -50,6 +66,31 @@ __device__ __forceinline__ double hn_position(const HnArgs& p, int64_t i) {
     case 2: return (double)((const float*)p.positions)[i];
     default: return ((const double*)p.positions)[i];
   }
+}
+
+// sum over the lanes of a group (of G consecutive ones, a power of two)
+template <int CTRL>
+__device__ __forceinline__ float hn_dpp(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int N>
+__device__ __forceinline__ void hn_group_sum(float (&v)[N], int G) {
+  auto all = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = f(v[e]);
+  };
+  if (G < 2) return;
+  all([](float x) { return hn_dpp<0xB1>(x); });  // the neighbour
+  if (G < 4) return;
+  all([](float x) { return hn_dpp<0x4E>(x); });  // the other pair of four
+  if (G < 8) return;
+  all([](float x) { return hn_dpp<0x141>(x); });  // eight lanes mirrored
+  if (G < 16) return;
+  all([](float x) { return hn_dpp<0x140>(x); });  // sixteen mirrored
+  if (G < 32) return;
+  all([](float x) { return x + __shfl_xor(x, 16, kWave); });
+  if (G < 64) return;
+  all([](float x) { return x + __shfl_xor(x, 32, kWave); });
 }
 
 template <typename T, int VEC>
@@ -103,249 +144,283 @@ static int hn_items(int vec, bool interleaved, int head_dim, int rotary) {
   return (rot_vecs + 1) / 2 + ((head_dim - rotary) / vec + 1) / 2;
 }
 
-// the rotation of an item's values (fp32), cosines and sines of its token at cv, sv
+// the rotation of an item's values (fp32), cosines and sines of its token at cv, sv (16-byte aligned)
 template <int VEC, bool INTERLEAVED>
 __device__ __forceinline__ void hn_rotate(const HnItem& it, const float* cv, const float* sv, float (&a)[VEC],
                                           float (&b)[VEC]) {
   if (!it.rot) return;
   if constexpr (INTERLEAVED && VEC > 1) {
+    using P = HnVec<float, VEC / 2>;
+    const P c0 = *reinterpret_cast<const P*>(cv + it.at), s0 = *reinterpret_cast<const P*>(sv + it.at);
+    const P c1 = *reinterpret_cast<const P*>(cv + it.at1), s1 = *reinterpret_cast<const P*>(sv + it.at1);
 #pragma unroll
-    for (int k = 0; k < VEC; k += 2) {
-      const float ca = cv[it.at + k / 2], sa = sv[it.at + k / 2], cb = cv[it.at1 + k / 2], sb = sv[it.at1 + k / 2];
-      const float u = a[k], w = a[k + 1], y = b[k], z = b[k + 1];
-      a[k] = u * ca - w * sa;
-      a[k + 1] = w * ca + u * sa;
-      b[k] = y * cb - z * sb;
-      b[k + 1] = z * cb + y * sb;
+    for (int k = 0; k < VEC / 2; ++k) {
+      const float u = a[2 * k], w = a[2 * k + 1], y = b[2 * k], z = b[2 * k + 1];
+      a[2 * k] = u * c0.v[k] - w * s0.v[k];
+      a[2 * k + 1] = w * c0.v[k] + u * s0.v[k];
+      b[2 * k] = y * c1.v[k] - z * s1.v[k];
+      b[2 * k + 1] = z * c1.v[k] + y * s1.v[k];
     }
   } else {
+    constexpr int Q = VEC < 4 ? VEC : 4;
+    using P = HnVec<float, Q>;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      const float c = cv[it.at + k], s = sv[it.at + k], u = a[k], w = b[k];
-      a[k] = u * c - w * s;
-      b[k] = w * c + u * s;
+    for (int k = 0; k < VEC; k += Q) {
+      const P c = *reinterpret_cast<const P*>(cv + it.at + k), s = *reinterpret_cast<const P*>(sv + it.at + k);
+#pragma unroll
+      for (int e = 0; e < Q; ++e) {
+        const float u = a[k + e], w = b[k + e];
+        a[k + e] = u * c.v[e] - w * s.v[e];
+        b[k + e] = w * c.v[e] + u * s.v[e];
+      }
     }
   }
 }
 
-// IPL items per lane (more than one only where a head has more than 64); BATCH
-// heads of a group in flight.
+// IPL items per lane (more than one only where a head has more than 64); BATCH heads of
+// a group at work, as many on their way.
 template <typename T, int VEC, bool INTERLEAVED, int IPL, bool GRAD>
 __global__ __launch_bounds__(kHnThreads) void headnorm_kernel(HnArgs p) {
   using V = HnVec<T, VEC>;
-  constexpr int BATCH = IPL > 1 ? 1 : (GRAD ? 2 : 4);
+  constexpr int BATCH = IPL > 1 || GRAD ? 1 : 2;
   __shared__ __attribute__((aligned(16))) float cs[kHnTable], sn[kHnTable];
-  __shared__ int64_t row_x[2][kHnTokens], row_out[2][kHnTokens], row_g[2][GRAD ? kHnTokens : 1];
-  const int pairs = p.rotary / 2;
-  const int64_t all = p.batch * p.tokens;
+  const bool keys = (int)blockIdx.x >= p.side[0].blocks;
+  const HnSide& side = p.side[keys];
+  const ltx_headnorm_rows& r = side.r;
+  const int block = (int)blockIdx.x - (keys ? p.side[0].blocks : 0);
+  const int pairs = p.rotary / 2, heads = (int)r.heads;
   const int G = p.lanes, groups = kHnThreads / G;
   const int group = threadIdx.x / G, lane = threadIdx.x % G;
   HnItem it[IPL];
 #pragma unroll
   for (int s = 0; s < IPL; ++s) it[s] = hn_item<VEC, INTERLEAVED>(lane + s * G, p.head_dim, p.rotary);
-  float u0[2][IPL][VEC], u1[2][IPL][VEC], d0[2][IPL][VEC], d1[2][IPL][VEC];
-#pragma unroll
-  for (int side = 0; side < 2; ++side)
-#pragma unroll
-    for (int s = 0; s < IPL; ++s)
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const float* w = p.side[side].weight;
-        u0[side][s][k] = w && it[s].have ? p.offset + w[it[s].c0 + k] : 1.0f;
-        u1[side][s][k] = w && it[s].have ? p.offset + w[it[s].c1 + k] : 1.0f;
-        d0[side][s][k] = d1[side][s][k] = 0.0f;
-      }
-  const float mean = 1.0f / (float)p.head_dim;
 
-  for (int64_t tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
-    const int64_t first = tile * p.per_block;
-    const int count = (int)(all - first < p.per_block ? all - first : p.per_block);
-    if (GRAD && tile != blockIdx.x) __syncthreads();
-    for (int i = threadIdx.x; i < count * pairs; i += kHnThreads) {
-      const int t = i / pairs, j = i % pairs;
-      const int64_t row = first + t;
-      const double pos = hn_position(p, row / p.tokens * p.pos_batch + row % p.tokens);
-      double turns = pos * p.inv_freq[j] * 0.15915494309189533576888;  // 1 / (2 pi)
-      turns -= rint(turns);
-      float s, c;
-      sincospif((float)(2.0 * turns), &s, &c);
-      cs[t * p.table + j] = c * p.factor;
-      sn[t * p.table + j] = (GRAD ? -s : s) * p.factor;
+  // Heads of a group in flight.  Loads past the tile's tokens repeat its last one's, those of
+  // a lane without an item the head's first vector: no branch waits for them.
+  struct Heads {
+    V xa[BATCH][IPL], xb[BATCH][IPL], ga[GRAD ? BATCH : 1][IPL], gb[GRAD ? BATCH : 1][IPL];
+    int t[BATCH], h[BATCH];
+  };
+  const int dh = groups % heads, dt = groups / heads;
+  int first = 0, count = 0, t = 0, h = 0;  // the tile; (token, head) of the group's next load
+  // element (token t of the tile, head h) of a tensor
+  auto offset = [&](int tt, int hh, int64_t batch, int64_t token, int64_t head) __attribute__((always_inline)) {
+    uint32_t row = (uint32_t)(first + tt);
+    int64_t at = 0;
+    if (p.batch > 1) {
+      const uint32_t b = row / (uint32_t)p.tokens;
+      row -= b * (uint32_t)p.tokens;
+      at = (int64_t)b * batch;
     }
-    if (threadIdx.x < 2 * kHnTokens) {
-      const int side = threadIdx.x / kHnTokens, t = threadIdx.x % kHnTokens;
-      const ltx_headnorm_rows& r = p.side[side];
-      const int64_t row = first + t, b = row / p.tokens, tok = row % p.tokens;
-      row_x[side][t] = b * r.x_batch + tok * r.x_token;
-      row_out[side][t] = b * r.out_batch + tok * r.out_token;
-      if constexpr (GRAD) row_g[side][t] = b * r.g_batch + tok * r.g_token;
-    }
-    __syncthreads();
+    // (token and head strides below 2^32)
+    return at + (int64_t)((uint64_t)row * (uint32_t)token) + (int64_t)((uint64_t)(uint32_t)hh * (uint32_t)head);
+  };
+  auto load = [&](Heads& n) __attribute__((always_inline)) {
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const ltx_headnorm_rows& r = p.side[side];
-      const int heads = (int)r.heads;
-      if (heads == 0) continue;
-      const T* x = (const T*)r.x;
-      const T* g = (const T*)r.g;
-      T* out = (T*)r.out;
-      // (token, head) of this group, and what `groups` heads add to it
-      int h = group % heads, t = group / heads;
-      const int dh = groups % heads, dt = groups / heads;
-      while (t < count) {
-        V xa[BATCH][IPL], xb[BATCH][IPL], ga[BATCH][IPL], gb[BATCH][IPL];
-        int at[BATCH], ah[BATCH];
+    for (int e = 0; e < BATCH; ++e) {
+      n.t[e] = t;
+      n.h[e] = h;
+      const int tt = t < count ? t : count - 1;
+      const T* src = (const T*)r.x + offset(tt, h, r.x_batch, r.x_token, r.x_head);
 #pragma unroll
-        for (int e = 0; e < BATCH; ++e) {
-          at[e] = t;
-          ah[e] = h;
+      for (int s = 0; s < IPL; ++s) {
+        n.xa[e][s] = *reinterpret_cast<const V*>(src + it[s].c0);
+        n.xb[e][s] = *reinterpret_cast<const V*>(src + it[s].c1);
+      }
+      if constexpr (GRAD) {
+        const T* up = (const T*)r.g + offset(tt, h, r.g_batch, r.g_token, r.g_head);
 #pragma unroll
-          for (int s = 0; s < IPL; ++s) {
-            xa[e][s] = xb[e][s] = V{};
-            if constexpr (GRAD) ga[e][s] = gb[e][s] = V{};
-            if (t < count && it[s].have) {
-              const T* src = x + row_x[side][t] + h * r.x_head;
-              xa[e][s] = *reinterpret_cast<const V*>(src + it[s].c0);
-              xb[e][s] = *reinterpret_cast<const V*>(src + it[s].c1);
-              if constexpr (GRAD) {
-                const T* up = g + row_g[side][t] + h * r.g_head;
-                ga[e][s] = *reinterpret_cast<const V*>(up + it[s].c0);
-                gb[e][s] = *reinterpret_cast<const V*>(up + it[s].c1);
-              }
-            }
-          }
-          h += dh;
-          t += dt;
-          if (h >= heads) {
-            h -= heads;
-            ++t;
-          }
-        }
-        float ss[BATCH], sg[BATCH];
-        float za[BATCH][IPL][VEC], zb[BATCH][IPL][VEC];  // gz
-#pragma unroll
-        for (int e = 0; e < BATCH; ++e) {
-          ss[e] = sg[e] = 0.0f;
-#pragma unroll
-          for (int s = 0; s < IPL; ++s) {
-            if constexpr (GRAD) {
-#pragma unroll
-              for (int k = 0; k < VEC; ++k) {
-                za[e][s][k] = (float)ga[e][s].v[k];
-                zb[e][s][k] = (float)gb[e][s].v[k];
-              }
-              const int tt = at[e] < count ? at[e] : 0;
-              hn_rotate<VEC, INTERLEAVED>(it[s], (const float*)__builtin_assume_aligned(cs + tt * p.table, 16),
-                                          (const float*)__builtin_assume_aligned(sn + tt * p.table, 16), za[e][s],
-                                          zb[e][s]);
-            }
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-              const float va = (float)xa[e][s].v[k], vb = it[s].two ? (float)xb[e][s].v[k] : 0.0f;
-              ss[e] += va * va + vb * vb;
-              if constexpr (GRAD) sg[e] += va * za[e][s][k] * u0[side][s][k] + vb * zb[e][s][k] * u1[side][s][k];
-            }
-          }
-        }
-        for (int off = 1; off < G; off <<= 1)
-#pragma unroll
-          for (int e = 0; e < BATCH; ++e) {
-            ss[e] += __shfl_xor(ss[e], off, kWave);
-            if constexpr (GRAD) sg[e] += __shfl_xor(sg[e], off, kWave);
-          }
-#pragma unroll
-        for (int e = 0; e < BATCH; ++e) {
-          if (at[e] >= count) break;
-          const float rn = rsqrt_rn(ss[e] * mean + p.eps);
-          const float kk = sg[e] * mean * rn;
-          T* dst = out + row_out[side][at[e]] + ah[e] * r.out_head;
-          const float* cv = (const float*)__builtin_assume_aligned(cs + at[e] * p.table, 16);
-          const float* sv = (const float*)__builtin_assume_aligned(sn + at[e] * p.table, 16);
-#pragma unroll
-          for (int s = 0; s < IPL; ++s) {
-            if (!it[s].have) continue;
-            float a[VEC], b[VEC];
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-              const float na = (float)xa[e][s].v[k] * rn, nb = (float)xb[e][s].v[k] * rn;
-              if constexpr (GRAD) {
-                d0[side][s][k] += za[e][s][k] * na;
-                d1[side][s][k] += zb[e][s][k] * nb;
-                a[k] = rn * (za[e][s][k] * u0[side][s][k] - na * kk);
-                b[k] = rn * (zb[e][s][k] * u1[side][s][k] - nb * kk);
-              } else {
-                a[k] = na * u0[side][s][k];
-                b[k] = nb * u1[side][s][k];
-              }
-            }
-            if constexpr (!GRAD) hn_rotate<VEC, INTERLEAVED>(it[s], cv, sv, a, b);
-            V oa, ob;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-              oa.v[k] = (T)a[k];
-              ob.v[k] = (T)b[k];
-            }
-            *reinterpret_cast<V*>(dst + it[s].c0) = oa;
-            *reinterpret_cast<V*>(dst + it[s].c1) = ob;
-          }
+        for (int s = 0; s < IPL; ++s) {
+          n.ga[e][s] = *reinterpret_cast<const V*>(up + it[s].c0);
+          n.gb[e][s] = *reinterpret_cast<const V*>(up + it[s].c1);
         }
       }
+      h += dh;
+      t += dt;
+      if (h >= heads) {
+        h -= heads;
+        ++t;
+      }
     }
-  }
-  if constexpr (GRAD) {
-    // the workgroup's share of dw: the groups of a wave by lane exchanges, the waves through LDS
-    // (the tables' place), in wave order
-    static_assert(2 * kHnTable >= 4 * kHnMaxDim, "room for the waves' shares");
-    const int wave = threadIdx.x / kWave;
+  };
+
+  float u0[IPL][VEC], u1[IPL][VEC], d0[GRAD ? IPL : 1][VEC], d1[GRAD ? IPL : 1][VEC];
+  const float mean = 1.0f / (float)p.head_dim;
+  auto work = [&](const Heads& c) __attribute__((always_inline)) {
+    float sums[GRAD ? 2 * BATCH : BATCH];            // of x^2, of gz u x
+    float za[BATCH][IPL][VEC], zb[BATCH][IPL][VEC];  // gz
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      if (p.side[side].dweight == nullptr) continue;
-      __syncthreads();
+    for (int e = 0; e < BATCH; ++e) {
+      float ss = 0.0f, sg = 0.0f;
+#pragma unroll
+      for (int s = 0; s < IPL; ++s) {
+        if constexpr (GRAD) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            za[e][s][k] = (float)c.ga[e][s].v[k];
+            zb[e][s][k] = (float)c.gb[e][s].v[k];
+          }
+          const int at = (c.t[e] < count ? c.t[e] : 0) * p.table;
+          hn_rotate<VEC, INTERLEAVED>(it[s], cs + at, sn + at, za[e][s], zb[e][s]);
+        }
+        float sa = 0.0f, sb = 0.0f, ta = 0.0f, tb = 0.0f;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const float va = (float)c.xa[e][s].v[k], vb = (float)c.xb[e][s].v[k];
+          sa += va * va;
+          sb += vb * vb;
+          if constexpr (GRAD) {
+            ta += va * (za[e][s][k] * u0[s][k]);
+            tb += vb * (zb[e][s][k] * u1[s][k]);
+          }
+        }
+        ss += it[s].have ? sa + (it[s].two ? sb : 0.0f) : 0.0f;
+        if constexpr (GRAD) sg += it[s].have ? ta + (it[s].two ? tb : 0.0f) : 0.0f;
+      }
+      sums[e] = ss;
+      if constexpr (GRAD) sums[BATCH + e] = sg;
+    }
+    hn_group_sum(sums, G);
+#pragma unroll
+    for (int e = 0; e < BATCH; ++e) {
+      if (c.t[e] >= count) break;
+      const float rn = rsqrt_rn(sums[e] * mean + p.eps);
+      T* dst = (T*)r.out + offset(c.t[e], c.h[e], r.out_batch, r.out_token, r.out_head);
+      const int at = c.t[e] * p.table;
+#pragma unroll
+      for (int s = 0; s < IPL; ++s) {
+        if (!it[s].have) continue;
+        float va[VEC], vb[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const float na = (float)c.xa[e][s].v[k] * rn, nb = (float)c.xb[e][s].v[k] * rn;
+          if constexpr (GRAD) {
+            const float kk = sums[BATCH + e] * mean * rn;
+            d0[s][k] += za[e][s][k] * na;
+            d1[s][k] += zb[e][s][k] * nb;
+            va[k] = rn * (za[e][s][k] * u0[s][k] - na * kk);
+            vb[k] = rn * (zb[e][s][k] * u1[s][k] - nb * kk);
+          } else {
+            va[k] = na * u0[s][k];
+            vb[k] = nb * u1[s][k];
+          }
+        }
+        if constexpr (!GRAD) hn_rotate<VEC, INTERLEAVED>(it[s], cs + at, sn + at, va, vb);
+        V oa, ob;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          oa.v[k] = (T)va[k];
+          ob.v[k] = (T)vb[k];
+        }
+        *reinterpret_cast<V*>(dst + it[s].c0) = oa;
+        *reinterpret_cast<V*>(dst + it[s].c1) = ob;
+      }
+    }
+  };
+  for (int tile = block; tile < side.tiles; tile += side.blocks) {
+    first = tile * side.per_block;
+    count = p.all - first < side.per_block ? p.all - first : side.per_block;
+    t = group / heads;
+    h = group % heads;
+    Heads now;
+    load(now);
+    if (!GRAD || tile == block) {
 #pragma unroll
       for (int s = 0; s < IPL; ++s)
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-          float a = d0[side][s][k], b = d1[side][s][k];
-          for (int off = G; off < kWave; off <<= 1) {
-            a += __shfl_xor(a, off, kWave);
-            b += __shfl_xor(b, off, kWave);
-          }
-          if (threadIdx.x % kWave < G && it[s].have) {
-            float* dst = (wave < 2 ? cs : sn) + (wave & 1) * kHnMaxDim;
-            dst[it[s].c0 + k] = a;
-            if (it[s].two) dst[it[s].c1 + k] = b;
-          }
+          u0[s][k] = r.weight ? p.offset + r.weight[it[s].c0 + k] : 1.0f;
+          u1[s][k] = r.weight ? p.offset + r.weight[it[s].c1 + k] : 1.0f;
+          if constexpr (GRAD) d0[s][k] = d1[s][k] = 0.0f;
         }
-      __syncthreads();
-      for (int c = threadIdx.x; c < p.head_dim; c += kHnThreads)
-        p.partial[((int64_t)blockIdx.x * 2 + side) * p.head_dim + c] =
-            (cs[c] + cs[kHnMaxDim + c]) + (sn[c] + sn[kHnMaxDim + c]);
+    } else {
+      __syncthreads();  // the last tile's table
     }
+    for (int i = threadIdx.x; i < count * pairs; i += kHnThreads) {
+      const int tt = i / pairs, j = i - tt * pairs;
+      uint32_t row = (uint32_t)(first + tt);
+      int64_t at = 0;
+      if (p.batch > 1) {
+        at = (int64_t)(row / (uint32_t)p.tokens) * p.pos_batch;
+        row %= (uint32_t)p.tokens;
+      }
+      double turns = hn_position(p, at + row) * p.inv_freq[j] * 0.15915494309189533576888;  // 1 / (2 pi)
+      turns -= rint(turns);
+      float sine, cosine;
+      sincospif((float)(2.0 * turns), &sine, &cosine);
+      cs[tt * p.table + j] = cosine * p.factor;
+      sn[tt * p.table + j] = (GRAD ? -sine : sine) * p.factor;
+    }
+    __syncthreads();
+    const int turns = (int)(((int64_t)count * heads + groups * BATCH - 1) / (groups * BATCH));
+    for (int i = 1; i < turns; ++i) {
+      Heads next;
+      load(next);
+      work(now);
+      now = next;
+    }
+    work(now);
+  }
+  if constexpr (GRAD) {
+    if (r.dweight == nullptr) return;
+    // the workgroup's share of dw: the groups of a wave by lane exchanges, the waves through LDS
+    // (the tables' place), in wave order
+    static_assert(2 * kHnTable >= 4 * kHnMaxDim, "room for the waves' shares");
+    const int wave = threadIdx.x / kWave;
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < IPL; ++s)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        float va = d0[s][k], vb = d1[s][k];
+        for (int off = G; off < kWave; off <<= 1) {
+          va += __shfl_xor(va, off, kWave);
+          vb += __shfl_xor(vb, off, kWave);
+        }
+        if (threadIdx.x % kWave < G && it[s].have) {
+          float* dst = (wave < 2 ? cs : sn) + (wave & 1) * kHnMaxDim;
+          dst[it[s].c0 + k] = va;
+          if (it[s].two) dst[it[s].c1 + k] = vb;
+        }
+      }
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.head_dim; c += kHnThreads)
+      p.partial[(int64_t)blockIdx.x * p.head_dim + c] = (cs[c] + cs[kHnMaxDim + c]) + (sn[c] + sn[kHnMaxDim + c]);
   }
 }
 
-// dw from the workgroups' shares: eight channels per workgroup, 32 threads each
-__global__ __launch_bounds__(256) void headnorm_dw_kernel(const float* __restrict__ partial, int blocks, int head_dim,
-                                                          float* dwq, float* dwk) {
-  const int side = blockIdx.y, c = blockIdx.x * 8 + threadIdx.x % 8, part = threadIdx.x / 8;
-  float* dw = side == 0 ? dwq : dwk;
+// dw from the workgroups' shares: eight channels per workgroup, 64 threads each
+__global__ __launch_bounds__(512) void headnorm_dw_kernel(const float* __restrict__ partial, int blocks_q, int blocks_k,
+                                                          int head_dim, float* dwq, float* dwk) {
+  const bool keys = blockIdx.y != 0;
+  const int c = blockIdx.x * 8 + threadIdx.x % 8, part = threadIdx.x / 8;
+  const int from = keys ? blocks_q : 0, to = keys ? blocks_q + blocks_k : blocks_q;
+  float* dw = keys ? dwk : dwq;
   if (dw == nullptr) return;
-  __shared__ double sum[256];
+  __shared__ double sum[512];
   double a = 0.0;
-  if (c < head_dim)
-    for (int b = part; b < blocks; b += 32) a += (double)partial[((int64_t)b * 2 + side) * head_dim + c];
+  if (c < head_dim) {
+#pragma unroll 8
+    for (int b = from + part; b < to; b += 64) a += (double)partial[(int64_t)b * head_dim + c];
+  }
   sum[threadIdx.x] = a;
   __syncthreads();
-  if (part == 0 && c < head_dim) {
-    for (int i = 1; i < 32; ++i) a += sum[i * 8 + threadIdx.x];
-    dw[c] = (float)a;
+  for (int n = 256; n >= 8; n /= 2) {
+    if ((int)threadIdx.x < n) sum[threadIdx.x] += sum[threadIdx.x + n];
+    __syncthreads();
   }
+  if (part == 0 && c < head_dim) dw[c] = (float)sum[threadIdx.x];
 }
 
-static int hn_tokens(int64_t all, int64_t token_bytes, int table) {
+// Tokens of a tile: a power of two, of up to 96 KiB of heads (48 KiB in fp32, with half the
+// arithmetic per byte, and in the gradient) where 300 tiles remain.  24 / 48 / 96 / 192 KiB: 3456 x 32 heads of 128
+// bf16 of each side 40 / 31 / 29 / 29 us, 14640 x 32 and 8 heads 90 / 68 / 65 / 67, 14639 x 32
+// and 8 heads of 64 fp32 71 / 59 / 62 / 66.
+static int hn_tokens(int64_t all, int64_t token_bytes, bool small, int table) {
+  const int64_t most = small ? 49152 : 98304;
   int n = 1;
   while (2 * n <= kHnTokens && 2 * n * table <= kHnTable &&
-         ((2 * n * token_bytes <= 49152 && 2 * n <= all / (n < 4 ? 448 : 640)) || all / n > kHnBlocks))
+         ((2 * n * token_bytes <= most && 2 * n <= all / 300) || all / n > kHnBlocks))
     n *= 2;
   return n;
 }
@@ -373,14 +448,15 @@ static void hn_launch_vec(const HnArgs& p, int vec, bool interleaved, int items,
   }
 }
 template <bool GRAD>
-static void hn_launch_type(const HnArgs& p, int dtype, int vec, bool interleaved, int items, int blocks, hipStream_t s) {
+static void hn_launch_type(const HnArgs& p, int dtype, int vec, bool interleaved, int items, int blocks,
+                           hipStream_t s) {
   if (dtype == 0) hn_launch_vec<bf16, GRAD>(p, vec, interleaved, items, blocks, s);
   else if (dtype == 1) hn_launch_vec<_Float16, GRAD>(p, vec, interleaved, items, blocks, s);
   else hn_launch_vec<float, GRAD>(p, vec, interleaved, items, blocks, s);
 }
 
 // Checks and arguments of both entry points; *vec and *items: the kernel's form.
-// LTX_OK with p->tiles == 0: nothing to do.
+// LTX_OK with no tiles on either side: nothing to do.
 static int hn_args(const ltx_headnorm_rows* q, const ltx_headnorm_rows* k, bool grad, int dtype, int64_t batch,
                    int64_t tokens, int64_t head_dim, int64_t rotary_dim, const void* positions, int pos_type,
                    int64_t pos_batch, const double* inv_freq, double factor, double eps, double offset, int flags,
@@ -397,14 +473,15 @@ static int hn_args(const ltx_headnorm_rows* q, const ltx_headnorm_rows* k, bool 
     if ((uintptr_t)positions % pos_size || (uintptr_t)inv_freq % 8) return LTX_ERR_ALIGNMENT;
   }
   *p = {};
-  p->side[0] = *q;
-  if (k) p->side[1] = *k;
+  p->side[0].r = *q;
+  if (k) p->side[1].r = *k;
   const bool interleaved = (flags & LTX_ROTARY_INTERLEAVED) != 0;
   // the widest vector that divides every extent, stride and address
   int64_t bits = interleaved ? rotary_dim : rotary_dim / 2;
   bits |= head_dim - rotary_dim;
   int64_t heads = 0;
-  for (ltx_headnorm_rows& r : p->side) {
+  for (HnSide& side : p->side) {
+    ltx_headnorm_rows& r = side.r;
     if (!grad) r.dweight = nullptr;
     if (r.heads < 0 || (r.dweight && !r.weight)) return LTX_ERR_INVALID_ARG;
     if (r.heads > kHnHeads) return LTX_ERR_UNSUPPORTED;
@@ -414,20 +491,27 @@ static int hn_args(const ltx_headnorm_rows* q, const ltx_headnorm_rows* k, bool 
     if (!r.x || !r.out || (grad && !r.g)) return LTX_ERR_INVALID_ARG;
     if ((uintptr_t)r.x % size || (uintptr_t)r.out % size || (grad && (uintptr_t)r.g % size)) return LTX_ERR_ALIGNMENT;
     bits |= (int64_t)((uintptr_t)r.x / size | (uintptr_t)r.out / size | (grad ? (uintptr_t)r.g / size : 0));
-    // the stride of an axis of one entry is never used
+    // the stride of an axis of one entry is never used; offsets of tokens and heads are products of 32 bits
+    auto narrow = [grad](int64_t x, int64_t out, int64_t g) {
+      return (uint64_t)x >> 32 == 0 && (uint64_t)out >> 32 == 0 && (!grad || (uint64_t)g >> 32 == 0);
+    };
+    if ((tokens > 1 && !narrow(r.x_token, r.out_token, r.g_token)) ||
+        (r.heads > 1 && !narrow(r.x_head, r.out_head, r.g_head)))
+      return LTX_ERR_UNSUPPORTED;
     if (batch > 1) bits |= r.x_batch | r.out_batch | (grad ? r.g_batch : 0);
     if (tokens > 1) bits |= r.x_token | r.out_token | (grad ? r.g_token : 0);
     if (r.heads > 1) bits |= r.x_head | r.out_head | (grad ? r.g_head : 0);
   }
   if (heads == 0) return LTX_OK;
-  if (tokens > 4 * kHnBlocks / batch) return LTX_ERR_UNSUPPORTED;  // (4 tokens of any width fit a workgroup)
+  if (tokens > 4 * kHnBlocks / batch) return LTX_ERR_UNSUPPORTED;  // (4 tokens of any width fit a tile)
   *vec = (int)(16 / size);
   while (*vec > 1 && (bits & (*vec - 1))) *vec >>= 1;
   *items = hn_items(*vec, interleaved, (int)head_dim, (int)rotary_dim);
   p->lanes = 1;
   while (p->lanes < *items && p->lanes < kWave) p->lanes *= 2;
-  p->batch = batch;
-  p->tokens = tokens;
+  p->batch = (int)batch;
+  p->tokens = (int)tokens;
+  p->all = (int)(batch * tokens);
   p->head_dim = (int)head_dim;
   p->rotary = (int)rotary_dim;
   p->positions = positions;
@@ -438,9 +522,12 @@ static int hn_args(const ltx_headnorm_rows* q, const ltx_headnorm_rows* k, bool 
   p->eps = (float)eps;
   p->offset = (float)offset;
   p->table = (int)(rotary_dim / 2 + 3) / 4 * 4;
-  const int64_t all = batch * tokens;
-  p->per_block = hn_tokens(all, heads * head_dim * (int64_t)size, p->table);
-  p->tiles = (all + p->per_block - 1) / p->per_block;
+  for (HnSide& side : p->side) {
+    if (side.r.heads == 0) continue;
+    side.per_block = hn_tokens(p->all, side.r.heads * head_dim * (int64_t)size, size == 4 || grad, p->table);
+    side.tiles = (p->all + side.per_block - 1) / side.per_block;
+    side.blocks = !grad || side.tiles < kHnGradBlocks ? side.tiles : kHnGradBlocks;
+  }
   return LTX_OK;
 }
 
@@ -456,8 +543,9 @@ extern "C" int ltx_headnorm_rotary(const ltx_headnorm_rows* q, const ltx_headnor
   int vec, items;
   const int st = hn_args(q, k, false, dtype, batch, tokens, head_dim, rotary_dim, positions, pos_type, pos_batch,
                          inv_freq, factor, eps, weight_offset, flags, &p, &vec, &items);
-  if (st != LTX_OK || p.tiles == 0) return st;
-  hn_launch_type<false>(p, dtype, vec, (flags & LTX_ROTARY_INTERLEAVED) != 0, items, (int)p.tiles, (hipStream_t)stream);
+  const int blocks = p.side[0].blocks + p.side[1].blocks;
+  if (st != LTX_OK || blocks == 0) return st;
+  hn_launch_type<false>(p, dtype, vec, (flags & LTX_ROTARY_INTERLEAVED) != 0, items, blocks, (hipStream_t)stream);
   return ltx_launch_status();
 }
 
@@ -475,22 +563,21 @@ extern "C" int ltx_headnorm_rotary_grad(const ltx_headnorm_rows* q, const ltx_he
   const int st = hn_args(q, k, true, dtype, batch, tokens, head_dim, rotary_dim, positions, pos_type, pos_batch,
                          inv_freq, factor, eps, weight_offset, flags, &p, &vec, &items);
   if (st != LTX_OK) return st;
-  const bool sums = p.side[0].dweight || p.side[1].dweight;
-  if (p.tiles > 0 && sums) {
+  float *dwq = p.side[0].r.dweight, *dwk = p.side[1].r.dweight;
+  const int blocks = p.side[0].blocks + p.side[1].blocks;
+  if (blocks > 0 && (dwq || dwk)) {
     if (!workspace || workspace_bytes < ltx_headnorm_rotary_grad_workspace_bytes(head_dim)) return LTX_ERR_INVALID_ARG;
     if ((uintptr_t)workspace % 4) return LTX_ERR_ALIGNMENT;
   }
   hipStream_t s = (hipStream_t)stream;
-  int blocks = 0;
-  if (p.tiles > 0) {
+  if (blocks > 0) {
     p.partial = workspace;
-    blocks = (int)(p.tiles < kHnGradBlocks ? p.tiles : kHnGradBlocks);
     hn_launch_type<true>(p, dtype, vec, (flags & LTX_ROTARY_INTERLEAVED) != 0, items, blocks, s);
     const int e = ltx_launch_status();
     if (e != LTX_OK) return e;
   }
-  if (!sums) return LTX_OK;
-  headnorm_dw_kernel<<<dim3((unsigned)(head_dim + 7) / 8, 2), 256, 0, s>>>(workspace, blocks, (int)head_dim,
-                                                                          p.side[0].dweight, p.side[1].dweight);
+  if (!dwq && !dwk) return LTX_OK;
+  headnorm_dw_kernel<<<dim3((unsigned)(head_dim + 7) / 8, 2), 512, 0, s>>>(
+      workspace, p.side[0].blocks, p.side[1].blocks, (int)head_dim, dwq, dwk);
   return ltx_launch_status();
 }
