@@ -215,64 +215,194 @@ __global__ __launch_bounds__(256) void w8_quantize_kernel(const bf16* __restrict
   }
 }
 
-__global__ void w8_dequantize_kernel(const int8_t* __restrict__ q, int64_t ldq,
+// C codes (8 or 16) per thread.
+template <int C>
+__global__ __launch_bounds__(256) void w8_dequantize_kernel(const int8_t* __restrict__ q, int64_t ldq,
                                      const float* __restrict__ scale, int64_t N, int64_t K,
                                      bf16* __restrict__ out, int64_t ldo) {
-  const int64_t per_row = K / 8;
+  const int64_t per_row = K / C;
   const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (idx >= N * per_row) return;
   const int64_t n = idx / per_row, c = idx % per_row;
-  const u32x2 raw = *reinterpret_cast<const u32x2*>(q + n * ldq + c * 8);
+  typedef uint32_t words __attribute__((ext_vector_type(C / 4)));
+  const words raw = *reinterpret_cast<const words*>(q + n * ldq + c * C);
   const float s = scale[n];
-  bf16x8 o;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int32_t v = (int32_t)(int8_t)((raw[e / 4] >> (8 * (e % 4))) & 0xffu);
-    o[e] = (bf16)mul_rn((float)v, s);
+  for (int h = 0; h < C; h += 8) {
+    bf16x8 o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int32_t v = (int32_t)(int8_t)((raw[(h + e) / 4] >> (8 * (e % 4))) & 0xffu);
+      o[e] = (bf16)mul_rn((float)v, s);
+    }
+    *reinterpret_cast<bf16x8*>(out + n * ldo + c * C + h) = o;
   }
-  *reinterpret_cast<bf16x8*>(out + n * ldo + c * 8) = o;
 }
 
-// Activation rows, one wave each: the row's largest magnitude, then the codes from
-// a second read of it.
+// ---- int8 rows -----------------------------------------------------------------
+// The code of the rule, rint(fp32(v / s)), of eight values.  v (1 / s) is within 2^-16.4 of the
+// fp32 quotient (|v / s| < 128: 2^-17 by the reciprocal's rounding, 2^-18 by the quotient's), so its
+// nearest integer is the code's unless it lies that close to a half; then the divisions are made.
+// The sum with 1.5 * 2^23 has the integer in its low byte.
+__device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
+  const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(d), __float_as_uint(c), 0x04000c0cu);
+  return lo | hi;
+}
+__device__ __forceinline__ u32x2 int8_codes8(const float (&v)[8], float s, float inv) {
+  constexpr float kMagic = 12582912.0f;
+  float t[8];
+  bool near = !(s >= 0x1p-126f);  // a subnormal scale's reciprocal may not be finite
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    t[e] = fmaf(v[e], inv, kMagic);
+    near |= fabsf(fmaf(v[e], inv, -(t[e] - kMagic))) > 0.5f - 0x1p-15f;
+  }
+  if (near) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float c = s > 0.0f ? rintf(__fdiv_rn(v[e], s)) : 0.0f;
+      t[e] = fminf(fmaxf(c, -127.0f), 127.0f) + kMagic;  // (a subnormal scale may be off by more than a step)
+    }
+  }
+  return u32x2{low_bytes(t[0], t[1], t[2], t[3]), low_bytes(t[4], t[5], t[6], t[7])};
+}
+
+// The magnitude bits of eight elements: those of a NaN or an infinity are above every
+// finite one's, in each type's own bits.
 template <typename T>
+struct Bits8 {
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  static constexpr uint32_t kInf =
+      std::is_same_v<T, float> ? 0x7f800000u : (std::is_same_v<T, bf16> ? 0x7f80u : 0x7c00u);
+  t8 x;
+  // largest so far of the even and the odd elements (fp32: one value)
+  __device__ __forceinline__ uint32_t top(uint32_t t) const {
+    if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t b = __float_as_uint(x[e]) & 0x7fffffffu;
+        t = b > t ? b : t;
+      }
+      return t;
+    } else {
+      const u32x4 w = __builtin_bit_cast(u32x4, x);
+      u16x2 m = __builtin_bit_cast(u16x2, t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu));
+      return __builtin_bit_cast(uint32_t, m);
+    }
+  }
+  static __device__ __forceinline__ uint32_t one(uint32_t t) {
+    if constexpr (std::is_same_v<T, float>) return t;
+    else return (t >> 16) > (t & 0xffffu) ? t >> 16 : t & 0xffffu;
+  }
+  static __device__ __forceinline__ float value(uint32_t bits) {
+    if constexpr (std::is_same_v<T, float>) return __uint_as_float(bits);
+    else return (float)__builtin_bit_cast(T, (uint16_t)bits);
+  }
+};
+
+// A row stays in the registers of WPR waves between its maximum and its codes: NC pieces of
+// 512 * WPR elements, eight per lane.  Bound by HBM: 14640 x 4096 bf16 35 us (5.2 TB/s; read twice, with
+// a division per element, 52), fp32 54 (5.5), 3456 x 16384 bf16 39 (4.3), 68 x 2048 4.2, a launch; the decoder
+// 14640 x 4096 32 (5.7).
+template <typename T, int WPR, int NC>
 __global__ __launch_bounds__(256) void int8_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t K,
                                                         int8_t* __restrict__ q, int64_t ldq,
                                                         float* __restrict__ scale) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= rows) return;
-  // the largest magnitude as bits: those of a NaN or an infinity are above every finite one's
-  uint32_t top = 0;
-  for (int64_t k = lane * 8; k < K; k += 512) {
-    float v[8];
-    load8(x + r * ldx + k, v);
+  __shared__ uint32_t tops[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t r = WPR == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
+  if (r >= rows) return;  // (WPR 4: no workgroup is past them)
+  const int64_t first = (WPR == 1 ? lane : (int)threadIdx.x) * 8;
+  Bits8<T> v[NC];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t b = __float_as_uint(v[e]) & 0x7fffffffu;
-      top = b > top ? b : top;
-    }
+  for (int c = 0; c < NC; ++c) {
+    const int64_t k = first + c * (512 * WPR);
+    // (past K: the last ones)
+    v[c].x = *reinterpret_cast<const typename Bits8<T>::t8*>(x + r * ldx + (k < K ? k : K - 8));
   }
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) top = v[c].top(top);
+  top = Bits8<T>::one(top);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
     const uint32_t t = __shfl_xor(top, off, 64);
     top = t > top ? t : top;
   }
-  const bool bad = top >= 0x7f800000u;
-  const float s = __fdiv_rn(__uint_as_float(top), 127.0f);
-  if (lane == 0) scale[r] = bad ? __uint_as_float(0x7fc00000u) : s;
-  for (int64_t k = lane * 8; k < K; k += 512) {
-    float v[8];
-    load8(x + r * ldx + k, v);
-    uint32_t w[2] = {0, 0};
+  if constexpr (WPR == 4) {
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float c = s > 0.0f && !bad ? rintf(__fdiv_rn(v[e], s)) : 0.0f;
-      c = fminf(fmaxf(c, -127.0f), 127.0f);  // (a subnormal scale may be off by more than a step)
-      w[e / 4] |= ((uint32_t)(int32_t)c & 0xffu) << (8 * (e % 4));
-    }
-    *reinterpret_cast<u32x2*>(q + r * ldq + k) = u32x2{w[0], w[1]};
+    for (int w = 0; w < 4; ++w) top = tops[w] > top ? tops[w] : top;
   }
+  const bool bad = top >= Bits8<T>::kInf;
+  const float s = bad ? 0.0f : __fdiv_rn(Bits8<T>::value(top), 127.0f), inv = __fdiv_rn(1.0f, s);
+  if (lane == 0 && (WPR == 1 || wave == 0)) scale[r] = bad ? __uint_as_float(0x7fc00000u) : s;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int64_t k = first + c * (512 * WPR);
+    if (k >= K) break;
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (float)v[c].x[e];
+    *reinterpret_cast<u32x2*>(q + r * ldq + k) = int8_codes8(f, s, inv);
+  }
+}
+
+// Rows of more than 16384: a workgroup each, read twice.
+template <typename T>
+__global__ __launch_bounds__(256) void int8_long_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t K,
+                                                             int8_t* __restrict__ q, int64_t ldq,
+                                                             float* __restrict__ scale) {
+  __shared__ uint32_t tops[4];
+  const int64_t r = blockIdx.x;
+  uint32_t top = 0;
+  for (int64_t k = threadIdx.x * 8; k < K; k += 2048)
+    top = Bits8<T>{*reinterpret_cast<const typename Bits8<T>::t8*>(x + r * ldx + k)}.top(top);
+  top = Bits8<T>::one(top);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    const uint32_t t = __shfl_xor(top, off, 64);
+    top = t > top ? t : top;
+  }
+  if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) top = tops[w] > top ? tops[w] : top;
+  const bool bad = top >= Bits8<T>::kInf;
+  const float s = bad ? 0.0f : __fdiv_rn(Bits8<T>::value(top), 127.0f), inv = __fdiv_rn(1.0f, s);
+  if (threadIdx.x == 0) scale[r] = bad ? __uint_as_float(0x7fc00000u) : s;
+  for (int64_t k = threadIdx.x * 8; k < K; k += 2048) {
+    float f[8];
+    load8(x + r * ldx + k, f);
+    *reinterpret_cast<u32x2*>(q + r * ldq + k) = int8_codes8(f, s, inv);
+  }
+}
+
+// One wave per row for many short ones, four otherwise: one / four 30000 x 512 fp16 11 / 21 us,
+// 14640 x 1024 bf16 12 / 16, x 2048 22 / 23, x 4096 42 / 35, 3456 x 4096 16 / 12.
+template <typename T>
+static void int8_rows_launch(const T* x, int64_t ldx, int64_t rows, int64_t K, int8_t* q, int64_t ldq, float* scale,
+                             hipStream_t s) {
+  const bool one = K <= 2048 && rows >= 2048;
+  const int64_t pieces = (K + (one ? 511 : 2047)) / (one ? 512 : 2048);
+  auto go = [&](auto wpr, auto nc) {
+    constexpr int W = decltype(wpr)::value, N = decltype(nc)::value;
+    int8_rows_kernel<T, W, N><<<(int)(W == 1 ? (rows + 3) / 4 : rows), 256, 0, s>>>(x, ldx, rows, K, q, ldq, scale);
+  };
+  auto pick = [&](auto wpr) {
+    if (pieces <= 1) go(wpr, std::integral_constant<int, 1>{});
+    else if (pieces <= 2) go(wpr, std::integral_constant<int, 2>{});
+    else if (pieces <= 4) go(wpr, std::integral_constant<int, 4>{});
+    else go(wpr, std::integral_constant<int, 8>{});
+  };
+  if (pieces > 8) int8_long_rows_kernel<<<(int)rows, 256, 0, s>>>(x, ldx, K, q, ldq, scale);
+  else if (one) pick(std::integral_constant<int, 1>{});
+  else pick(std::integral_constant<int, 4>{});
 }
 
 // E4M3 code -> float, exact: (-1)^s 2^(e-7) (1 + m/8), subnormals (e = 0)
@@ -378,9 +508,11 @@ extern "C" int ltx_dequantize_w8_bf16(const int8_t* q, int64_t ldq, const float*
   if (!a16(out) || (uintptr_t)q % 8 || ldq % 8 || ldo % 8) return LTX_ERR_ALIGNMENT;
   if (N == 0 || K == 0) return LTX_OK;
   if (K / 8 > kQ4Blocks * 256 / N) return LTX_ERR_UNSUPPORTED;
-  const int64_t total = N * (K / 8);
-  w8_dequantize_kernel<<<(int)((total + 255) / 256), 256, 0, (hipStream_t)stream>>>(
-      q, ldq, scale, N, K, (bf16*)out, ldo);
+  hipStream_t st = (hipStream_t)stream;
+  if (K % 16 == 0 && ldq % 16 == 0 && (uintptr_t)q % 16 == 0)
+    w8_dequantize_kernel<16><<<(int)((N * (K / 16) + 255) / 256), 256, 0, st>>>(q, ldq, scale, N, K, (bf16*)out, ldo);
+  else
+    w8_dequantize_kernel<8><<<(int)((N * (K / 8) + 255) / 256), 256, 0, st>>>(q, ldq, scale, N, K, (bf16*)out, ldo);
   return ltx_launch_status();
 }
 
@@ -392,11 +524,11 @@ extern "C" int ltx_quantize_int8(const void* x, int dtype, int64_t ldx, int64_t 
   if (!a16(x) || !a16(q) || (uintptr_t)scale % 4 || ldx % (dtype == 2 ? 4 : 8) || ldq % 16) return LTX_ERR_ALIGNMENT;
   if (rows > kI8Rows) return LTX_ERR_UNSUPPORTED;
   if (rows == 0) return LTX_OK;
-  const int blocks = (int)((rows + 3) / 4);
+  if (K == 0) return LTX_ERR_UNSUPPORTED;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == 0) int8_rows_kernel<<<blocks, 256, 0, s>>>((const bf16*)x, ldx, rows, K, q, ldq, scale);
-  else if (dtype == 1) int8_rows_kernel<<<blocks, 256, 0, s>>>((const _Float16*)x, ldx, rows, K, q, ldq, scale);
-  else int8_rows_kernel<<<blocks, 256, 0, s>>>((const float*)x, ldx, rows, K, q, ldq, scale);
+  if (dtype == 0) int8_rows_launch((const bf16*)x, ldx, rows, K, q, ldq, scale, s);
+  else if (dtype == 1) int8_rows_launch((const _Float16*)x, ldx, rows, K, q, ldq, scale, s);
+  else int8_rows_launch((const float*)x, ldx, rows, K, q, ldq, scale, s);
   return ltx_launch_status();
 }
 
