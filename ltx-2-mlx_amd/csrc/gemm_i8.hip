@@ -459,6 +459,8 @@ __global__ __launch_bounds__(256) void i8_combine_kernel(GemmArgs p, int epi, in
 
 // ---- which kernel ------------------------------------------------------------------
 struct I8Plan {
+  int64_t head;  // rows on 256 x head_bn tiles in a launch before the others' (0: none)
+  int head_bn;
   int bm, bn;   // rows and columns of a tile; bn < 0: the few-row kernel, bm rows and -16 bn columns
   int splits;   // K ranges (tiles)
   int k_split;  // k of one, a multiple of 128
@@ -468,8 +470,8 @@ struct I8Plan {
 // 128 k `idle` to `full`, as it fills the CUs (they share the L2s and the chip's power); a
 // split's second launch and its partials.  Model against measured (weights from HBM): 1296 x
 // 4096 -> 4096 in tiles of 256 x 256, 256 x 128, 128 x 128, 64 x 128 40 / 28 / 33 / 40
-// against 53 / 31 / 37 / 44, 3456 x 4096 -> 16384 202 / 220 / 260 / 335 against 208 / 218 / 261 / 337, 512 x 4096 -> 4096 64 x 128 16 / 17, 68 x 8192 -> 2048 in
-// 8 ranges 11 / 14.
+// against 53 / 31 / 37 / 44, 3456 x 4096 -> 16384 202 / 220 / 260 / 335 against 208 /
+// 218 / 261 / 337, 512 x 4096 -> 4096 64 x 128 16 / 17, 68 x 8192 -> 2048 in 8 ranges 11 / 14.
 static double i8_time(int64_t M, int64_t N, int bm, int bn, int splits, double per) {
   const double wgs = (double)(((M + bm - 1) / bm) * ((N + bn - 1) / bn) * splits);
   double fixed = 1.6, idle = 0.30, full = 0.34;
@@ -489,17 +491,18 @@ static double i8_rows_time(int64_t M, int64_t N, int64_t K, int mb, int nb) {
   return 3.2 + rounds * (double)(16 * (mb + nb) * K) / 33e3;
 }
 
-static I8Plan i8_plan(int64_t M, int64_t N, int64_t K) {
+// The fastest single launch (or, where `split`, K ranges and a combining one) and its time
+static double i8_one(int64_t M, int64_t N, int64_t K, bool split, I8Plan* pl) {
   static const int tile[4][2] = {{256, 256}, {256, 128}, {128, 128}, {64, 128}};
   // rows of the few-row kernel; 32 columns where that leaves a workgroup for every CU
   const int mb = M <= 16 ? 1 : (M <= 32 ? 2 : 4), nb = N >= 32 * 256 ? 2 : 1;
   const int64_t units = (K + 127) / 128;
-  I8Plan pl = {16 * mb, -nb, 1, (int)K};
+  *pl = {0, 0, 16 * mb, -nb, 1, (int)K};
   double best = i8_rows_time(M, N, K, mb, nb);
-  if (M <= 32) return pl;
+  if (M <= 32) return best;
   for (const auto& t : tile) {
     const int64_t tiles = ((M + t[0] - 1) / t[0]) * ((N + t[1] - 1) / t[1]);
-    for (int want = 1; want <= 16; ++want) {
+    for (int want = 1; want <= (split ? 16 : 1); ++want) {
       // splits: at least two stages each, within one round of the CUs, 10 % faster
       if (want > 1 && (units / want < 2 || tiles * want > 256)) break;
       const int64_t per = (units + want - 1) / want;
@@ -507,7 +510,30 @@ static I8Plan i8_plan(int64_t M, int64_t N, int64_t K) {
       const double us = i8_time(M, N, t[0], t[1], s, (double)per);
       if (us < best * (s > 1 ? 0.9 : 1.0)) {
         best = us;
-        pl = {t[0], t[1], s, (int)(per * 128)};
+        *pl = {0, 0, t[0], t[1], s, (int)(per * 128)};
+      }
+    }
+  }
+  return best;
+}
+
+// Rows [0, head) on 256-row tiles, where those make (nearly) whole rounds of the CUs and another
+// kernel takes the rows left over for less than one more round: 1296 x 4096 -> 12320 as 1280
+// rows of 256 x 256 and 16 of the few-row kernel 74 us, in one launch 83.
+static I8Plan i8_plan(int64_t M, int64_t N, int64_t K) {
+  I8Plan pl;
+  double best = i8_one(M, N, K, true, &pl);
+  const double units = (double)((K + 127) / 128);
+  for (int64_t b = (M - 1) / 256, tries = 0; b >= 1 && tries < 8; --b, ++tries) {
+    I8Plan rest;
+    const double left = i8_one(M - 256 * b, N, K, false, &rest);
+    for (int bn = 128; bn <= 256; bn += 128) {
+      const double t = i8_time(256 * b, N, 256, bn, 1, units) + left;
+      if (t < 0.95 * best) {
+        best = t;
+        pl = rest;
+        pl.head = 256 * b;
+        pl.head_bn = bn;
       }
     }
   }
@@ -587,30 +613,49 @@ extern "C" int ltx_gemm_i8_bf16(const int8_t* A, int64_t lda, const float* a_sca
   p.gate = gate;
   p.sig_from = (int)(sigmoid_from < N ? (sigmoid_from < 0 ? 0 : sigmoid_from) : N);
   p.round_then_bias = (epilogue & LTX_GEMM_ROUND_THEN_BIAS) != 0;
-  p.M = (int)M;
   p.N = (int)N;
   p.K = (int)K;
   hipStream_t s = (hipStream_t)stream;
   const int epi = epilogue & 0xff;
-  auto rows = [&](int bm, int nb) {
-    if (bm == 16 && nb == 1) i8_launch_rows<1, 1>(p, epi, s);
-    else if (bm == 16) i8_launch_rows<1, 2>(p, epi, s);
-    else if (bm == 32 && nb == 1) i8_launch_rows<2, 1>(p, epi, s);
-    else if (bm == 32) i8_launch_rows<2, 2>(p, epi, s);
-    else if (nb == 1) i8_launch_rows<4, 1>(p, epi, s);
-    else i8_launch_rows<4, 2>(p, epi, s);
-    return ltx_launch_status();
+  // rows [r0, r1) by a plan's kernel in one pass over K
+  auto run = [&](int64_t r0, int64_t r1, int bm, int bn) {
+    const I8Plan whole = {0, 0, bm, bn, 1, (int)((K + 127) / 128 * 128)};
+    // Rows that one launch of the tile kernel takes: its operands' byte offsets have 31 bits.
+    // None where a tile's rows, or the weights, are past them: then the few-row kernel, whose
+    // addresses have 64 bits
+    const int64_t lim = ((int64_t)1 << 31) - 1;
+    int64_t piece = r1 - r0;
+    if (bn > 0) {
+      if (N > lim / ldw) piece = 0;
+      else if (lim / lda < piece) piece = lim / lda / 256 * 256;
+      if (piece == 0) {
+        piece = r1 - r0;
+        bm = 64;
+        bn = -2;
+      }
+    }
+    for (; r0 < r1; r0 += piece) {
+      GemmArgs part = p;
+      part.A = (const bf16*)(A + r0 * lda);
+      part.ascale = (const uint8_t*)(a_scale + r0);
+      part.C = p.C + r0 * ldc;
+      if (p.R) part.R = p.R + r0 * ldr;
+      part.M = (int)(r1 - r0 < piece ? r1 - r0 : piece);
+      if (bn > 0) fp4_epilogue(epi, [&](auto e) { i8_launch_tiles<decltype(e)::value>(part, whole, s); });
+      else if (bm == 16 && bn == -1) i8_launch_rows<1, 1>(part, epi, s);
+      else if (bm == 16) i8_launch_rows<1, 2>(part, epi, s);
+      else if (bm == 32 && bn == -1) i8_launch_rows<2, 1>(part, epi, s);
+      else if (bm == 32) i8_launch_rows<2, 2>(part, epi, s);
+      else if (bn == -1) i8_launch_rows<4, 1>(part, epi, s);
+      else i8_launch_rows<4, 2>(part, epi, s);
+      const int e = ltx_launch_status();
+      if (e != LTX_OK) return e;
+    }
+    return LTX_OK;
   };
-  if (pl.bn < 0) return rows(pl.bm, -pl.bn);
-  // Rows that one launch of the tile kernel takes: its operands' byte offsets have 31
-  // bits.  Rows past them in further launches; none where a tile's rows, or the weights,
-  // are past them: then the few-row kernel, whose addresses have 64 bits
   const int64_t lim = ((int64_t)1 << 31) - 1;
-  int64_t piece = lim / lda;
-  if (N > lim / ldw) piece = 0;
-  if (piece < M) piece = piece / 256 * 256;
-  if (piece == 0) return rows(64, 2);
-  if (pl.splits > 1 && piece >= M) {
+  if (pl.splits > 1 && N <= lim / ldw && M <= lim / lda) {
+    p.M = (int)M;
     p.partial = (float*)workspace;
     i8_launch_tiles<kEpiPartial>(p, pl, s);
     const int e = ltx_launch_status();
@@ -619,19 +664,9 @@ extern "C" int ltx_gemm_i8_bf16(const int8_t* A, int64_t lda, const float* a_sca
     i8_combine_kernel<<<(int)(total + 255 < 4096 * 256 ? (total + 255) / 256 : 4096), 256, 0, s>>>(p, epi, pl.splits);
     return ltx_launch_status();
   }
-  I8Plan whole = pl;
-  whole.splits = 1;
-  whole.k_split = (int)((K + 127) / 128 * 128);
-  for (int64_t r = 0; r < M; r += piece) {
-    GemmArgs part = p;
-    part.A = (const bf16*)(A + r * lda);
-    part.ascale = (const uint8_t*)(a_scale + r);
-    part.C = p.C + r * ldc;
-    if (p.R) part.R = p.R + r * ldr;
-    part.M = (int)(M - r < piece ? M - r : piece);
-    fp4_epilogue(epi, [&](auto e) { i8_launch_tiles<decltype(e)::value>(part, whole, s); });
-    const int e = ltx_launch_status();
+  if (pl.head > 0) {
+    const int e = run(0, pl.head, 256, pl.head_bn);
     if (e != LTX_OK) return e;
   }
-  return LTX_OK;
+  return run(pl.head, M, pl.bm, pl.bn);
 }
