@@ -116,12 +116,18 @@ static void i8_launch_rows(GemmArgs p, int epi, hipStream_t s) {
 
 // ---- tiles -----------------------------------------------------------------------
 // A workgroup computes BM x BN tiles, one after another.  A stage is 128 k: rows of 128
-// bytes, one line each, which reach LDS by direct loads into a ring of NST stages, one
+// bytes, one line each, which reach LDS by direct loads into a ring of stages per operand, one
 // stream over all its tiles (the next tile's first stages travel during the last
 // stages and the epilogue of this one).  A stage has two k-steps of 64, each in two halves of the
 // wave's rows: while the MFMAs of one half run, the fragments of the next are read, also
 // across the one barrier per stage, so that only a quarter of a wave's activations and two
 // k-steps of its weights are in registers beside the sums.
+//
+// The rings: LDS holds two stages of 256 x 256 tiles and one operand's third.  The weights have it:
+// their loads leave two stages ahead, and they are what comes from HBM (every row tile of a
+// round reads the same activations from the L2s).  With eight sets of operands in turn 3456 x 16384 ->
+// 4096 takes 192 us, 208 with two stages each, 180 with one set; 6144 x 4096 -> 16384 333 / 344 / 322.
+// More stages of the smaller tiles: 0 to 4 % slower (their first loads are as many more).
 //
 // What bounds it: the chip's power.  A stage of 256 x 256 tiles takes 1.4 us with every CU
 // busy, 3.0 PO/s (6144 x 4096 -> 16384 without its epilogues 275 us), 1.08 us on zeros; a loop
@@ -132,25 +138,31 @@ static void i8_launch_rows(GemmArgs p, int epi, hipStream_t s) {
 // against 340 (6144 x 4096 -> 16384, rounds of 256 rows' tiles elsewhere); loads in one half step, all
 // fragment reads in the first group, fewer vector instructions in the loop: no change; two
 // workgroups per CU of 128 x 128: 459.
-template <int BM_, int BN_, int WAVES_M_, int WAVES_N_, int NST_>
+template <int BM_, int BN_, int WAVES_M_, int WAVES_N_, int NA_, int NB_>
 struct I8Tile {
-  static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, NST = NST_;
+  static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_;
   static constexpr int WAVES = WAVES_M * WAVES_N, THREADS = WAVES * 64;
   static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N;
   static constexpr int TM = WM / 16, TN = WN / 16, HM = TM / 2;
-  static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, B_OFF = A_BYTES, STAGE = A_BYTES + B_BYTES;
+  // rings of NA stages of activations and NB of weights
+  static constexpr int NA = NA_, NB = NB_, A_BYTES = BM * 128, B_BYTES = BN * 128, B_OFF = NA * A_BYTES;
   // direct loads of a wave per stage
-  static constexpr int A_DMA = BM / 8 / WAVES, B_DMA = BN / 8 / WAVES, DMA = A_DMA + B_DMA;
-  static constexpr int LDS_BYTES = NST * STAGE;
+  static constexpr int A_DMA = BM / 8 / WAVES, B_DMA = BN / 8 / WAVES;
+  // loads that may be outstanding when the next stage has to be in LDS: those issued after its
+  // activations, and after its weights (see the kernel)
+  static constexpr int A_LEFT = (NA - 1) * B_DMA + (NA - 2) * A_DMA, B_LEFT = (NB - 2) * (A_DMA + B_DMA);
+  static constexpr int LEFT = A_LEFT < B_LEFT ? A_LEFT : B_LEFT;
+  static constexpr int LDS_BYTES = B_OFF + NB * B_BYTES;
   static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole direct-load instructions per wave");
   static_assert(TM % 2 == 0 && TN % 2 == 0, "halves of whole fragments, pairs of weight fragments");
-  static_assert(LDS_BYTES <= 160 * 1024 && (NST - 1) * DMA < 60, "LDS, vmcnt range");
+  static_assert(NB >= NA && LDS_BYTES <= 160 * 1024, "LDS");
+  static_assert(NA * A_DMA + (NB - 1) * B_DMA < 60, "vmcnt range");
 };
 
 template <class Cfg, int EPI>
 __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, int k_split) {
   constexpr int BM = Cfg::BM, BN = Cfg::BN, WM = Cfg::WM, WN = Cfg::WN, TM = Cfg::TM, TN = Cfg::TN, HM = Cfg::HM;
-  constexpr int NST = Cfg::NST, A_DMA = Cfg::A_DMA, B_DMA = Cfg::B_DMA, WAVES = Cfg::WAVES;
+  constexpr int NA = Cfg::NA, NB = Cfg::NB, A_DMA = Cfg::A_DMA, B_DMA = Cfg::B_DMA, WAVES = Cfg::WAVES;
   constexpr bool RESID = EPI == LTX_GEMM_EPI_RESIDUAL || EPI == LTX_GEMM_EPI_RESIDUAL_ROUND;
   __shared__ __attribute__((aligned(1024))) char lds[Cfg::LDS_BYTES];
 
@@ -184,49 +196,53 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
   const int b_chunk = (lane & 7) ^ g8_swz128(((lane >> 3) & 3) | (wave & 1) << 2, true);
   const int back = (chunk - (chunk >> 1)) * 16, b_back = (b_chunk - (b_chunk >> 1)) * 16;
   uint32_t a_src[A_DMA], b_src[B_DMA];
-  int next = (int)blockIdx.x;  // the tile being loaded
-  int lt, lT;                  // its stage, and its stages
-  bool lhalf;                  // whether its last one is a half
-  auto aim = [&]() __attribute__((always_inline)) {
+  // the stage that an operand's loads are at: its tile, its number there, and the tile's stages
+  struct Place {
+    int tile, t, stages;
+    bool half;  // whether the last stage is a half
+  } pa, pb;
+  pa.tile = pb.tile = (int)blockIdx.x;
+  auto aim = [&](Place& l, bool of_a) __attribute__((always_inline)) {
     int m0, n0, k0, depth;
-    locate(next, m0, n0, k0, depth);
-    lt = 0;
-    lT = (depth + 127) / 128;
-    lhalf = (depth & 64) != 0;
+    locate(l.tile, m0, n0, k0, depth);
+    l.t = 0;
+    l.stages = (depth + 127) / 128;
+    l.half = (depth & 64) != 0;
+    if (of_a) {
 #pragma unroll
-    for (int d = 0; d < A_DMA; ++d) {
-      int gm = m0 + 8 * (WAVES * d + wave) + (lane >> 3);
-      gm = gm < p.M ? gm : p.M - 1;
-      a_src[d] = (uint32_t)((int64_t)gm * p.lda + k0) + chunk * 16;
-    }
+      for (int d = 0; d < A_DMA; ++d) {
+        int gm = m0 + 8 * (WAVES * d + wave) + (lane >> 3);
+        gm = gm < p.M ? gm : p.M - 1;
+        a_src[d] = (uint32_t)((int64_t)gm * p.lda + k0) + chunk * 16;
+      }
+    } else {
 #pragma unroll
-    for (int d = 0; d < B_DMA; ++d) {
-      int gn = n0 + 8 * (WAVES * d + wave) + (lane >> 3);
-      gn = gn < p.N ? gn : p.N - 1;
-      b_src[d] = (uint32_t)((int64_t)gn * p.ldb + k0) + b_chunk * 16;
+      for (int d = 0; d < B_DMA; ++d) {
+        int gn = n0 + 8 * (WAVES * d + wave) + (lane >> 3);
+        gn = gn < p.N ? gn : p.N - 1;
+        b_src[d] = (uint32_t)((int64_t)gn * p.ldb + k0) + b_chunk * 16;
+      }
     }
   };
-  // load instruction l of the stage, and the step to the stage behind it (past the last
-  // tile's: that one again)
-  auto load = [&](int slot, int l) __attribute__((always_inline)) {
-    char* S = lds + slot * Cfg::STAGE;
-    const bool last = lhalf && lt == lT - 1;
-    if (l < A_DMA) {
-      buffer_dma16(p.A, a_records, a_src[l < A_DMA ? l : 0] - (last ? back : 0), lt * 128,
-                   S + (WAVES * l + wave) * 1024);
-    } else {
-      const int d = l >= A_DMA ? l - A_DMA : 0;
-      buffer_dma16(p.B, b_records, b_src[d] - (last ? b_back : 0), lt * 128,
-                   S + Cfg::B_OFF + (WAVES * d + wave) * 1024);
-    }
+  // load instruction l of the operand's stage, and the step to the stage behind it (past the
+  // last tile's: that one again)
+  auto load_a = [&](int slot, int l) __attribute__((always_inline)) {
+    const bool last = pa.half && pa.t == pa.stages - 1;
+    buffer_dma16(p.A, a_records, a_src[l] - (last ? back : 0), pa.t * 128,
+                 lds + slot * Cfg::A_BYTES + (WAVES * l + wave) * 1024);
   };
-  auto advance = [&]() __attribute__((always_inline)) {
-    if (++lt < lT) return;
-    if (next + (int)gridDim.x < total) {
-      next += (int)gridDim.x;
-      aim();
+  auto load_b = [&](int slot, int l) __attribute__((always_inline)) {
+    const bool last = pb.half && pb.t == pb.stages - 1;
+    buffer_dma16(p.B, b_records, b_src[l] - (last ? b_back : 0), pb.t * 128,
+                 lds + Cfg::B_OFF + slot * Cfg::B_BYTES + (WAVES * l + wave) * 1024);
+  };
+  auto advance = [&](Place& l, bool of_a) __attribute__((always_inline)) {
+    if (++l.t < l.stages) return;
+    if (l.tile + (int)gridDim.x < total) {
+      l.tile += (int)gridDim.x;
+      aim(l, of_a);
     } else {
-      lt = lT - 1;
+      l.t = l.stages - 1;
     }
   };
 
@@ -236,18 +252,19 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) c_off[ks] = ((2 * q + ks) ^ g8_swz128(r16, true)) * 16;
   const int a_rd = (wm * WM + r16) * 128, w_rd = Cfg::B_OFF + (wn * WN + 8 * (r16 >> 2) + (r16 & 3)) * 128;
-  auto read_a = [&](i32x4& f, int slot, int ks, int i) __attribute__((always_inline)) {
-    f = *reinterpret_cast<const i32x4*>(lds + slot * Cfg::STAGE + a_rd + c_off[ks] + i * 2048);
+  int slot_a = 0, slot_b = 0;  // of the stage at work
+  auto read_a = [&](i32x4& f, int ks, int i) __attribute__((always_inline)) {
+    f = *reinterpret_cast<const i32x4*>(lds + slot_a * Cfg::A_BYTES + a_rd + c_off[ks] + i * 2048);
   };
-  auto read_w = [&](i32x4& f, int slot, int ks, int j) __attribute__((always_inline)) {
-    f = *reinterpret_cast<const i32x4*>(lds + slot * Cfg::STAGE + w_rd + c_off[ks] + (j >> 1) * 4096 + (j & 1) * 512);
+  auto read_w = [&](i32x4& f, int ks, int j) __attribute__((always_inline)) {
+    f = *reinterpret_cast<const i32x4*>(lds + slot_b * Cfg::B_BYTES + w_rd + c_off[ks] + (j >> 1) * 4096 + (j & 1) * 512);
   };
   // share j of TN of the reads of half h of k-step ks (of its weights too, where `weights`)
-  auto read_share = [&](int slot, int ks, int h, bool weights, int j) __attribute__((always_inline)) {
-    if (weights) read_w(w[ks][j], slot, ks, j);
+  auto read_share = [&](int ks, int h, bool weights, int j) __attribute__((always_inline)) {
+    if (weights) read_w(w[ks][j], ks, j);
 #pragma unroll
     for (int i = 0; i < HM; ++i)
-      if (i * TN / HM == j) read_a(a[h][i], slot, ks, h * HM + i);
+      if (i * TN / HM == j) read_a(a[h][i], ks, h * HM + i);
   };
   i32x4 acc[TM][TN];
   // the MFMAs of half h of k-step ks in groups of one weight fragment (weights as the
@@ -267,44 +284,54 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
   constexpr std::integral_constant<int, 0> c0;
   constexpr std::integral_constant<int, 1> c1;
 
-  // ---- prologue: the ring filled (of the last slot's stage the first HL loads), stage 0 landed
-  constexpr int HL = (Cfg::DMA + 1) / 2;
-  aim();
+  // ---- prologue: stages 0 to NA - 1 of the activations and to NB - 2 of the weights, the first landed
+  aim(pa, true);
+  aim(pb, false);
 #pragma unroll 1
-  for (int t = 0; t < NST - 1; ++t) {
+  for (int t = 0; t < NB - 1; ++t) {
+    if (t < NA) {
 #pragma unroll
-    for (int l = 0; l < Cfg::DMA; ++l) load(t, l);
-    advance();
+      for (int l = 0; l < A_DMA; ++l) load_a(t, l);
+      advance(pa, true);
+    }
+#pragma unroll
+    for (int l = 0; l < B_DMA; ++l) load_b(t, l);
+    advance(pb, false);
   }
+  if constexpr (NA == NB) {
 #pragma unroll
-  for (int l = 0; l < HL; ++l) load(NST - 1, l);
-  wait_vmcnt<(NST - 2) * Cfg::DMA + HL>();
+    for (int l = 0; l < A_DMA; ++l) load_a(NA - 1, l);
+    advance(pa, true);
+  }
+  wait_vmcnt<(NA - 1) * A_DMA + (NB - 2) * B_DMA>();
   barrier_nofence();
 #pragma unroll
-  for (int j = 0; j < TN; ++j) read_share(0, 0, 0, true, j);
+  for (int j = 0; j < TN; ++j) read_share(0, 0, true, j);
 
-  // The stages of all the workgroup's tiles are one stream.  A stage: before its last half
-  // step, with every read of it done and the next stage landed, the barrier, after which
-  // the loads of NST stages further on go into its slot.
-  int slot = 0;
-  constexpr int LPJ = (HL + TN - 1) / TN;  // load instructions per group
-  int prev = NST - 1;                      // the slot of the stage before
+  // The stages of all the workgroup's tiles are one stream.  A stage t: the weights of stage t + NB -
+  // 1 are loaded into the slot that stage t - 1 left.  Before its last half step, with every
+  // read of it done and the next stage landed, the barrier, after which the activations of
+  // stage t + NA are loaded into its slot.  (So after the activations of stage t + 1 those of NA - 2
+  // stages and the weights of NA - 1 have been issued, after its weights NB - 2 of both.)
+  int free_a = 0, free_b = NB - 1;
   auto late = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-    for (int l = HL; l < Cfg::DMA; ++l)
-      if ((l - HL) / LPJ == j) load(prev, l);
+    for (int l = 0; l < B_DMA; ++l)
+      if (l * TN / B_DMA == j) load_b(free_b, l);
   };
   auto early = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-    for (int l = 0; l < HL; ++l)
-      if (l / LPJ == j) load(prev, l);
+    for (int l = 0; l < A_DMA; ++l)
+      if (l * TN / A_DMA == j) load_a(free_a, l);
   };
   auto turn = [&]() __attribute__((always_inline)) {
     wait_lgkmcnt0();
-    wait_vmcnt<(NST - 2) * Cfg::DMA>();
+    wait_vmcnt<Cfg::LEFT>();
     barrier_nofence();
-    prev = slot;
-    slot = slot + 1 < NST ? slot + 1 : 0;
+    free_a = slot_a;
+    free_b = slot_b;
+    slot_a = slot_a + 1 < NA ? slot_a + 1 : 0;
+    slot_b = slot_b + 1 < NB ? slot_b + 1 : 0;
   };
   for (int id = (int)blockIdx.x; id < total; id += (int)gridDim.x) {
     int m0, n0, k0, depth;
@@ -315,28 +342,30 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
       for (int j = 0; j < TN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
     for (int t = 0; t < depth / 128; ++t) {
       step(c0, c0, [&](int j) __attribute__((always_inline)) {
-        read_share(slot, 0, 1, false, j);
+        read_share(0, 1, false, j);
         late(j);
       });
-      advance();
-      step(c0, c1, [&](int j) __attribute__((always_inline)) { read_share(slot, 1, 0, true, j); });
-      step(c1, c0, [&](int j) __attribute__((always_inline)) { read_share(slot, 1, 1, false, j); });
+      advance(pb, false);
+      step(c0, c1, [&](int j) __attribute__((always_inline)) { read_share(1, 0, true, j); });
+      step(c1, c0, [&](int j) __attribute__((always_inline)) { read_share(1, 1, false, j); });
       turn();
       step(c1, c1, [&](int j) __attribute__((always_inline)) {
-        read_share(slot, 0, 0, true, j);
+        read_share(0, 0, true, j);
         early(j);
       });
+      advance(pa, true);
     }
     if ((depth & 64) != 0) {  // the last stage has one k-step
       step(c0, c0, [&](int j) __attribute__((always_inline)) {
-        read_share(slot, 0, 1, false, j);
+        read_share(0, 1, false, j);
         late(j);
       });
-      advance();
+      advance(pb, false);
       turn();
       step(c0, c1, early);
+      advance(pa, true);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) read_share(slot, 0, 0, true, j);
+      for (int j = 0; j < TN; ++j) read_share(0, 0, true, j);
     }
     // ---- epilogue: from registers, 16 bytes per lane and row, 64 side by side.  Everything
     // that is loaded is loaded before the first store: loads wait for the stores before them.
@@ -434,15 +463,15 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
     }
     // the next tile's first fragments again: the epilogue had their registers
 #pragma unroll
-    for (int j = 0; j < TN; ++j) read_share(slot, 0, 0, true, j);
+    for (int j = 0; j < TN; ++j) read_share(0, 0, true, j);
   }
   wait_vmcnt<0>();  // (the loads past the last stage: LDS is theirs until then)
 }
 
-using I8Large = I8Tile<256, 256, 2, 4, 2>;
-using I8Tall = I8Tile<256, 128, 4, 2, 3>;
-using I8Mid = I8Tile<128, 128, 2, 4, 4>;
-using I8Small = I8Tile<64, 128, 2, 4, 4>;
+using I8Large = I8Tile<256, 256, 2, 4, 2, 3>;
+using I8Tall = I8Tile<256, 128, 4, 2, 3, 3>;
+using I8Mid = I8Tile<128, 128, 2, 4, 4, 4>;
+using I8Small = I8Tile<64, 128, 2, 4, 4, 4>;
 
 // sum of the K ranges' partial products, then the epilogue
 __global__ __launch_bounds__(256) void i8_combine_kernel(GemmArgs p, int epi, int splits) {
