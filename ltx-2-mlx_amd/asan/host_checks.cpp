@@ -285,6 +285,89 @@ int main(int argc, char** argv) {
   mlps[1].h1 = nullptr;
   EXPECT(ltx_adaln_mlps_f32(mlps, 2, nullptr), LTX_ERR_INVALID_ARG);
 
+  // int8 rows and products
+  int8_t* cd = static_cast<int8_t*>(d);
+  EXPECT(ltx_quantize_int8(nullptr, 0, 64, 4, 64, cd, 64, fo, nullptr), LTX_ERR_INVALID_ARG);
+  EXPECT(ltx_quantize_int8(d, 3, 64, 4, 64, cd, 64, fo, nullptr), LTX_ERR_UNSUPPORTED);
+  EXPECT(ltx_quantize_int8(d, 0, 64, 4, 56, cd, 64, fo, nullptr), LTX_ERR_UNSUPPORTED);
+  EXPECT(ltx_quantize_int8(d, 0, 48, 4, 64, cd, 64, fo, nullptr), LTX_ERR_INVALID_ARG);
+  EXPECT(ltx_quantize_int8(m, 0, 64, 4, 64, cd, 64, fo, nullptr), LTX_ERR_ALIGNMENT);
+  EXPECT(ltx_quantize_int8(d, 0, 64, 1 << 24, 64, cd, 64, fo, nullptr), LTX_ERR_UNSUPPORTED);
+  EXPECT(ltx_quantize_int8(d, 0, 64, 0, 64, cd, 64, fo, nullptr), LTX_OK);
+  const auto product8 = [&](const void* a, int64_t lda, int64_t ldw, void* c, int64_t ldc, int64_t rows, int64_t cols,
+                      int64_t depth, int epi, const void* r, int64_t ldr, void* ws, int64_t bytes) {
+    return ltx_gemm_i8_bf16(static_cast<const int8_t*>(a), lda, fd, cd, ldw, fd, fd, c, ldc, rows, cols, depth, epi, r,
+                            ldr, fd, cols, ws, bytes, nullptr);
+  };
+  EXPECT(product8(nullptr, 64, 64, d, 64, 4, 64, 64, 0, nullptr, 0, nullptr, 0), LTX_ERR_INVALID_ARG);
+  EXPECT(product8(d, 64, 64, d, 64, 4, 64, 64, 9, nullptr, 0, nullptr, 0), LTX_ERR_INVALID_ARG);
+  EXPECT(product8(d, 64, 64, d, 64, 4, 64, 64, LTX_GEMM_EPI_RESIDUAL, nullptr, 64, nullptr, 0), LTX_ERR_INVALID_ARG);
+  EXPECT(product8(d, 64, 64, d, 64, 4, 64, 64, LTX_GEMM_EPI_RESIDUAL, d, 56, nullptr, 0), LTX_ERR_INVALID_ARG);
+  EXPECT(product8(d, 96, 96, d, 64, 4, 64, 96, 0, nullptr, 0, nullptr, 0), LTX_ERR_UNSUPPORTED);
+  EXPECT(product8(d, 1 << 17, 1 << 17, d, 64, 4, 64, 1 << 17, 0, nullptr, 0, nullptr, 0), LTX_ERR_UNSUPPORTED);
+  EXPECT(product8(d, 64, 64, d, 64, 4, 60, 64, 0, nullptr, 0, nullptr, 0), LTX_ERR_UNSUPPORTED);
+  EXPECT(product8(d, 64, 64, d, 64, int64_t(1) << 40, 64, 64, 0, nullptr, 0, nullptr, 0), LTX_ERR_UNSUPPORTED);
+  EXPECT(product8(d, 64, 64, d, INT64_MAX, 4, 64, 64, 0, nullptr, 0, nullptr, 0), LTX_ERR_UNSUPPORTED);
+  EXPECT(product8(d, 56, 64, d, 64, 4, 64, 64, 0, nullptr, 0, nullptr, 0), LTX_ERR_INVALID_ARG);
+  EXPECT(product8(d, 72, 64, d, 64, 4, 64, 64, 0, nullptr, 0, nullptr, 0), LTX_ERR_ALIGNMENT);
+  EXPECT(product8(m, 64, 64, d, 64, 4, 64, 64, 0, nullptr, 0, nullptr, 0), LTX_ERR_ALIGNMENT);
+  EXPECT(product8(d, 64, 64, d, 64, 0, 64, 64, 0, nullptr, 0, nullptr, 0), LTX_OK);
+  const int64_t i8_need = ltx_gemm_i8_workspace_bytes(128, 2048, 16384);
+  EXPECT(i8_need > 0, 1);
+  EXPECT(product8(d, 16384, 16384, d, 2048, 128, 2048, 16384, 0, nullptr, 0, nullptr, 0), LTX_ERR_INVALID_ARG);
+  EXPECT(product8(d, 16384, 16384, d, 2048, 128, 2048, 16384, 0, nullptr, 0, d, i8_need - 1), LTX_ERR_INVALID_ARG);
+  EXPECT(product8(d, 16384, 16384, d, 2048, 128, 2048, 16384, 0, nullptr, 0, m, i8_need), LTX_ERR_ALIGNMENT);
+  EXPECT(ltx_gemm_i8_workspace_bytes(-1, 64, 64), -1);
+  for (int64_t v : {int64_t(0), int64_t(1), int64_t(1) << 27, int64_t(1) << 40, INT64_MAX})
+    for (int64_t w : {int64_t(0), int64_t(1), int64_t(1) << 27, INT64_MAX}) {
+      EXPECT(ltx_gemm_i8_workspace_bytes(v, w, 4096) >= 0, 1);
+      EXPECT(ltx_gemm_i8_workspace_bytes(v, w, v) >= 0, 1);
+    }
+
+  // norm of the query and key heads with rotary positions, and its gradient
+  const ltx_headnorm_rows head_rows = {d, 0, 4096, 128, d, 0, 4096, 128, d, 0, 4096, 128, fd, fo, 32};
+  const auto headnorm = [&](const ltx_headnorm_rows* q, int dtype, int64_t batch, int64_t tokens, int64_t head_dim,
+                            int64_t rotary_dim, const void* positions, int pos_type, double eps, int flags) {
+    return ltx_headnorm_rotary(q, nullptr, dtype, batch, tokens, head_dim, rotary_dim, positions, pos_type, 0,
+                               static_cast<const double*>(d), 1.0, eps, 0.0, flags, nullptr);
+  };
+  EXPECT(headnorm(nullptr, 0, 1, 4, 128, 64, d, 0, 1e-6, 0), LTX_ERR_INVALID_ARG);
+  EXPECT(headnorm(&head_rows, 0, 1, 4, 128, 130, d, 0, 1e-6, 0), LTX_ERR_INVALID_ARG);
+  EXPECT(headnorm(&head_rows, 0, 1, 4, 128, 63, d, 0, 1e-6, 0), LTX_ERR_INVALID_ARG);
+  EXPECT(headnorm(&head_rows, 3, 1, 4, 128, 64, d, 0, 1e-6, 0), LTX_ERR_UNSUPPORTED);
+  EXPECT(headnorm(&head_rows, 0, 1, 4, 128, 64, d, 4, 1e-6, 0), LTX_ERR_UNSUPPORTED);
+  EXPECT(headnorm(&head_rows, 0, 1, 4, 128, 64, nullptr, 0, 1e-6, 0), LTX_ERR_INVALID_ARG);
+  EXPECT(headnorm(&head_rows, 0, 1, 4, 128, 64, static_cast<char*>(d) + 4, 1, 1e-6, 0), LTX_ERR_ALIGNMENT);
+  EXPECT(headnorm(&head_rows, 0, 1, 4, 128, 64, d, 0, -1.0, 0), LTX_ERR_INVALID_ARG);
+  EXPECT(headnorm(&head_rows, 0, 1, 4, 128, 64, d, 0, 1e-6, LTX_ROTARY_TRANSPOSE), LTX_ERR_INVALID_ARG);
+  EXPECT(headnorm(&head_rows, 0, 1, 4, 514, 64, d, 0, 1e-6, 0), LTX_ERR_UNSUPPORTED);
+  EXPECT(headnorm(&head_rows, 0, 1 << 20, 1 << 20, 128, 64, d, 0, 1e-6, 0), LTX_ERR_UNSUPPORTED);
+  EXPECT(headnorm(&head_rows, 0, 1, 0, 128, 64, nullptr, 0, 1e-6, 0), LTX_OK);
+  ltx_headnorm_rows bad_rows = head_rows;
+  bad_rows.x = nullptr;
+  EXPECT(headnorm(&bad_rows, 0, 1, 4, 128, 64, d, 0, 1e-6, 0), LTX_ERR_INVALID_ARG);
+  bad_rows = head_rows;
+  bad_rows.x_token = int64_t(1) << 32;
+  EXPECT(headnorm(&bad_rows, 0, 1, 4, 128, 64, d, 0, 1e-6, 0), LTX_ERR_UNSUPPORTED);
+  bad_rows = head_rows;
+  bad_rows.heads = -1;
+  EXPECT(headnorm(&bad_rows, 0, 1, 4, 128, 64, d, 0, 1e-6, 0), LTX_ERR_INVALID_ARG);
+  const auto headnorm_grad = [&](const ltx_headnorm_rows* q, float* ws, int64_t bytes) {
+    return ltx_headnorm_rotary_grad(q, &head_rows, 0, 1, 4, 128, 64, d, 0, 0, static_cast<const double*>(d), 1.0, 1e-6,
+                                    0.0, 0, ws, bytes, nullptr);
+  };
+  const int64_t head_need = ltx_headnorm_rotary_grad_workspace_bytes(128);
+  EXPECT(head_need > 0, 1);
+  EXPECT(ltx_headnorm_rotary_grad_workspace_bytes(-1), -1);
+  EXPECT(headnorm_grad(&head_rows, nullptr, 0), LTX_ERR_INVALID_ARG);
+  EXPECT(headnorm_grad(&head_rows, fo, head_need - 1), LTX_ERR_INVALID_ARG);
+  bad_rows = head_rows;
+  bad_rows.g = nullptr;
+  EXPECT(headnorm_grad(&bad_rows, fo, head_need), LTX_ERR_INVALID_ARG);
+  bad_rows = head_rows;
+  bad_rows.weight = nullptr;  // a gradient of no weight
+  EXPECT(headnorm_grad(&bad_rows, fo, head_need), LTX_ERR_INVALID_ARG);
+
   // automatic GEMM choices, also of sizes that no launch could take
   for (int wf = -1; wf <= 3; ++wf) {
     for (int64_t v : {int64_t(-1), int64_t(0), int64_t(1), int64_t(68), int64_t(188160), INT64_MAX / 4}) {
@@ -457,6 +540,29 @@ int main(int argc, char** argv) {
           const int64_t need4 = ltx_gemm_mx4_workspace_bytes(m, n, k);
           EXPECT(ltx_gemm_mx4_bf16(bd, k / 2, ud, (m + 3) / 4 * 4, bd, k / 2, ud, ld, fd, d, n, m, n, k, 1, nullptr, 0,
                                    nullptr, n, fo, need4, nullptr), k % 128 ? LTX_ERR_UNSUPPORTED : LTX_ERR_HIP);
+        }
+    // int8 rows and products (every kernel of the choice), the heads' norm
+    for (int64_t k : {int64_t(16), int64_t(4096), int64_t(4112), int64_t(65536)})
+      for (int type : {0, 1, 2})
+        EXPECT(ltx_quantize_int8(d, type, k, 3456, k, static_cast<int8_t*>(d), k, fo, nullptr), LTX_ERR_HIP);
+    for (int64_t m : {int64_t(1), int64_t(16), int64_t(33), int64_t(68), int64_t(300), int64_t(1296), int64_t(3456),
+                      int64_t(1) << 20})
+      for (int64_t k : {int64_t(64), int64_t(1088), int64_t(4096), int64_t(131008)})
+        for (int64_t n : {int64_t(8), int64_t(2048), int64_t(12320)})
+          for (int epi = 0; epi <= LTX_GEMM_EPI_SIGMOID2; ++epi) {
+            const int64_t need = ltx_gemm_i8_workspace_bytes(m, n, k);
+            EXPECT(need >= 0, 1);
+            EXPECT(ltx_gemm_i8_bf16(static_cast<const int8_t*>(d), k, fd, static_cast<const int8_t*>(d), k, fd, fd, d, n,
+                                    m, n, k, epi, d, n, fd, n, fo, need, nullptr), LTX_ERR_HIP);
+          }
+    for (int type : {0, 1, 2})
+      for (int64_t tokens : {int64_t(1), int64_t(257), int64_t(14640)})
+        for (int64_t rotary_dim : {int64_t(0), int64_t(62), int64_t(128)}) {
+          EXPECT(ltx_headnorm_rotary(&head_rows, &head_rows, type, 2, tokens, 128, rotary_dim, d, 1, 0,
+                                     static_cast<const double*>(d), 1.0, 1e-6, 1.0, 0, nullptr), LTX_ERR_HIP);
+          EXPECT(ltx_headnorm_rotary_grad(&head_rows, &head_rows, type, 2, tokens, 128, rotary_dim, d, 1, 0,
+                                          static_cast<const double*>(d), 1.0, 1e-6, 1.0, LTX_ROTARY_INTERLEAVED, fo,
+                                          head_need, nullptr), LTX_ERR_HIP);
         }
     const ltx_rotary_rows rows = {d, 0, 4096, 128, d, 0, 4096, 128, 32};
     for (int type : {0, 1, 2})
