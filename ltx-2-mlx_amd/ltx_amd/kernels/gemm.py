@@ -30,7 +30,10 @@ without the bf16 rounding before them.
 
 int8 weights take int8 activations as well (:class:`Int8Rows`, a scale per
 row, from :func:`quantize_rows_int8`): the int8 MFMA at twice the bf16 rate,
-exact int32 sums, epilogues on the fp32 value as MXFP4's.
+exact int32 sums, epilogues on the fp32 value as MXFP4's.  Opt-in
+(``INT8_ACTIVATIONS``, environment ``LTX_INT8_ACTIVATIONS=1``): :func:`linear`
+quantises bf16 rows for every int8 weight, as the model's projections use it;
+not the reference's arithmetic either.
 """
 
 from __future__ import annotations
@@ -58,6 +61,12 @@ FORMATS = ("bf16", "int8", "mxfp8", "mxfp4")
 # and run ltx_gemm_mx_bf16.
 MX_ACTIVATIONS = os.environ.get("LTX_MX_ACTIVATIONS", "0") == "1"
 MX_MIN_TILES = 100
+
+# The same for int8 weights, at all sizes: quantising the rows and the int8
+# product take less than the bf16 rows' product at every projection of the
+# model (us, weights from HBM): 16 x 2048 -> 2048 7.9 / 10.9, 68 x 8192 -> 2048
+# 18.9 / 19.1, 3456 x 4096 -> 16384 217 / 391, 3456 x 16384 -> 4096 216 / 374.
+INT8_ACTIVATIONS = os.environ.get("LTX_INT8_ACTIVATIONS", "0") == "1"
 
 # Optional launch observer: called as hook(phase, info) with phase "pre" /
 # "post" around every GEMM launch on the launching stream (used by bench.py
@@ -787,13 +796,39 @@ def _mx_eligible(m: int, n: int, k: int, weight: LinearWeight, tile: int) -> boo
             and ((m + 255) // 256) * ((n + 255) // 256) >= MX_MIN_TILES)
 
 
+def _int8_eligible(x, weight: LinearWeight, tile: int, splits: int | None) -> bool:
+    return (INT8_ACTIVATIONS and weight.kind == "int8" and tile in (TILE_AUTO, TILE_G8) and splits is None
+            and isinstance(x, torch.Tensor) and x.dtype is torch.bfloat16 and weight.in_features % 64 == 0
+            and weight.in_features < 1 << 17)
+
+
+def _linear_int8_rows(x: torch.Tensor, weight: LinearWeight, epilogue: int, out: torch.Tensor | None,
+                      residual: torch.Tensor | None, gate: torch.Tensor | None,
+                      sigmoid_from: int | None) -> torch.Tensor:
+    """:func:`linear` of bf16 rows (..., K) through int8 rows."""
+    lead, n = x.shape[:-1], weight.out_features
+    rows = quantize_rows_int8(x)
+    if len(lead) == 1:
+        return _linear_int8(rows, weight, epilogue, out, residual, gate, sigmoid_from)
+    if out is None:
+        return _linear_int8(rows, weight, epilogue, None, residual, gate, sigmoid_from).view(*lead, n)
+    if out.shape != (*lead, n):
+        raise ValueError(f"out must have the shape {(*lead, n)}, got {tuple(out.shape)}")
+    ov, ldc = _lib.row_view(out, n)
+    if ov.data_ptr() != out.data_ptr():
+        raise ValueError("out must be a row-strided view")
+    _linear_int8(rows, weight, epilogue, out.as_strided((rows.codes.shape[0], n), (ldc, 1)), residual, gate,
+                 sigmoid_from)
+    return out
+
+
 def rowss_eligible(x: torch.Tensor, weight: LinearWeight) -> bool:
     """Whether :func:`linear_rowss` takes this product: bf16 activations,
     weights of one of the three formats, at least 100 tiles of 256x256 (where
     the automatic choice is the 8-wave or the mid-size kernel, whose epilogues
     give the statistics, and the same one for :func:`linear`) and the 8-wave
     kernel's conditions (MXFP8 weights: K a multiple of 512), outside the
-    opt-in MX path.  Not bf16 products of 160 tiles on with fewer columns than
+    opt-in MX and int8 paths.  Not bf16 products of 160 tiles on with fewer columns than
     K (the A2V query projection of long clips): the attention with its norm
     inside measured slower than with the separate pass (6144 x 68 tokens 144
     against 138 us, 14640 x 68 324 against 316)."""
@@ -805,6 +840,8 @@ def rowss_eligible(x: torch.Tensor, weight: LinearWeight) -> bool:
     if tiles < 100 or (weight.kind == "bf16" and tiles >= 160 and n < k):
         return False
     if weight.kind == "mxfp8" and (k % 512 or _mx_eligible(m, n, k, weight, TILE_AUTO)):
+        return False
+    if _int8_eligible(x, weight, TILE_AUTO, None):
         return False
     return True
 
@@ -887,6 +924,8 @@ def linear(x: torch.Tensor | MxRows | Mx4Rows | Int8Rows, weight: LinearWeight, 
         if tile != TILE_AUTO or splits is not None:
             raise ValueError("MXFP4 products take no explicit tile or split count")
         return _linear_mxfp4(x, weight, epilogue, out, residual, gate, sigmoid_from)
+    if _int8_eligible(x, weight, tile, splits):
+        return _linear_int8_rows(x, weight, epilogue, out, residual, gate, sigmoid_from)
     k = weight.in_features
     n = weight.out_features
     if (splits is None and tile == TILE_AUTO and not isinstance(x, MxRows)
