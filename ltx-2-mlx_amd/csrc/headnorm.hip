@@ -18,7 +18,8 @@
 // sines, the next ones while it works on these.
 // Sums, r and dw are fp32, cosines and sines as in rotary.hip from fp64 angles; one
 // rounding at the end.
-// Measured: 3456 tokens x 64 heads of 128 bf16 29 us (3.9 TB/s; the rotation alone 22), 14640 x 40
+// Measured, inputs from HBM: 3456 tokens x 64 heads of 128 bf16 29 us (3.9 TB/s; 23 with part of them in a cache,
+// the rotation alone 22), 14640 x 40
 // heads of 128 bf16 65 (4.6 TB/s), 14639 x 40 heads of 64 fp32 60 (5.0 TB/s), one token 4.7, its gradient at
 // 14640 x 40 heads of 128 bf16 94 (4.8 TB/s, 4 of them the second launch), 3456 x 64 heads 46.  About
 // 300 vector instructions per eight heads of 128 lie beside the loads.  Beside it: both sides in one
