@@ -134,8 +134,8 @@ static void i8_launch_rows(GemmArgs p, int epi, hipStream_t s) {
 // of nothing but these MFMAs on such codes reaches 4.1 (32 x 32 x 32: 3.5); the stage without its
 // loads takes 1.19 us, without its fragment reads 1.21, without MFMAs 0.99.  Epilogues take 25
 // us of that product's 300 with bias, GELU 17 more.  Measured beside it: four waves of 128 x 128, sums
-// in AGPRs (a third less LDS traffic), 152 against 148 us (4096 x 12288 -> 4096); 320-row tiles 334
-// against 340 (6144 x 4096 -> 16384, rounds of 256 rows' tiles elsewhere); loads in one half step, all
+// in AGPRs (a third less LDS traffic), 152 against 148 us (4096 x 12288 -> 4096); 224-row tiles, which
+// give each CU one at 3456 x 16384 -> 4096, 178 against 181; loads in one half step, all
 // fragment reads in the first group, fewer vector instructions in the loop: no change; two
 // workgroups per CU of 128 x 128: 459.
 template <int BM_, int BN_, int WAVES_M_, int WAVES_N_, int NA_, int NB_>
@@ -143,18 +143,22 @@ struct I8Tile {
   static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_;
   static constexpr int WAVES = WAVES_M * WAVES_N, THREADS = WAVES * 64;
   static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N;
-  static constexpr int TM = WM / 16, TN = WN / 16, HM = TM / 2;
+  static constexpr int TM = WM / 16, TN = WN / 16;
+  // fragments of rows of the halves of a k-step: the first's, and the second's
+  static constexpr int HM = (TM + 1) / 2;
+  static constexpr int half(int h) { return h == 0 ? HM : TM - HM; }
+  // direct loads of a wave per stage, 8 rows each (of the activations' last some may repeat a row)
+  static constexpr int A_DMA = (BM + 8 * WAVES - 1) / (8 * WAVES), B_DMA = BN / 8 / WAVES;
   // rings of NA stages of activations and NB of weights
-  static constexpr int NA = NA_, NB = NB_, A_BYTES = BM * 128, B_BYTES = BN * 128, B_OFF = NA * A_BYTES;
-  // direct loads of a wave per stage
-  static constexpr int A_DMA = BM / 8 / WAVES, B_DMA = BN / 8 / WAVES;
+  static constexpr int NA = NA_, NB = NB_, A_BYTES = A_DMA * 8 * WAVES * 128, B_BYTES = BN * 128;
+  static constexpr int B_OFF = NA * A_BYTES;
   // loads that may be outstanding when the next stage has to be in LDS: those issued after its
   // activations, and after its weights (see the kernel)
   static constexpr int A_LEFT = (NA - 1) * B_DMA + (NA - 2) * A_DMA, B_LEFT = (NB - 2) * (A_DMA + B_DMA);
   static constexpr int LEFT = A_LEFT < B_LEFT ? A_LEFT : B_LEFT;
   static constexpr int LDS_BYTES = B_OFF + NB * B_BYTES;
-  static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole direct-load instructions per wave");
-  static_assert(TM % 2 == 0 && TN % 2 == 0, "halves of whole fragments, pairs of weight fragments");
+  static_assert(WM % 16 == 0 && BN % (8 * WAVES) == 0, "whole fragments, whole direct-load instructions per wave");
+  static_assert(TM >= 2 && TN % 2 == 0, "two halves, pairs of weight fragments");
   static_assert(NB >= NA && LDS_BYTES <= 160 * 1024, "LDS");
   static_assert(NA * A_DMA + (NB - 1) * B_DMA < 60, "vmcnt range");
 };
@@ -211,8 +215,9 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
     if (of_a) {
 #pragma unroll
       for (int d = 0; d < A_DMA; ++d) {
-        int gm = m0 + 8 * (WAVES * d + wave) + (lane >> 3);
-        gm = gm < p.M ? gm : p.M - 1;
+        int row = 8 * (WAVES * d + wave) + (lane >> 3);
+        if (BM % (8 * WAVES) != 0) row = row < BM ? row : BM - 1;
+        const int gm = m0 + row < p.M ? m0 + row : p.M - 1;
         a_src[d] = (uint32_t)((int64_t)gm * p.lda + k0) + chunk * 16;
       }
     } else {
@@ -263,7 +268,7 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
   auto read_share = [&](int ks, int h, bool weights, int j) __attribute__((always_inline)) {
     if (weights) read_w(w[ks][j], ks, j);
 #pragma unroll
-    for (int i = 0; i < HM; ++i)
+    for (int i = 0; i < Cfg::half(h); ++i)
       if (i * TN / HM == j) read_a(a[h][i], ks, h * HM + i);
   };
   i32x4 acc[TM][TN];
@@ -276,7 +281,7 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
     for (int j = 0; j < TN; ++j) {
       f(j);
 #pragma unroll
-      for (int i = 0; i < HM; ++i)
+      for (int i = 0; i < Cfg::half(H); ++i)
         acc[H * HM + i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[KS][j], a[H][i], acc[H * HM + i][j], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -468,6 +473,9 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
   wait_vmcnt<0>();  // (the loads past the last stage: LDS is theirs until then)
 }
 
+// 288 rows: where they make one round of the CUs less than 256 (below); the third stage of weights has no room
+// beside them, and the residual epilogue spills.
+using I8Huge = I8Tile<288, 256, 2, 4, 2, 2>;
 using I8Large = I8Tile<256, 256, 2, 4, 2, 3>;
 using I8Tall = I8Tile<256, 128, 4, 2, 3, 3>;
 using I8Mid = I8Tile<128, 128, 2, 4, 4, 4>;
@@ -499,12 +507,15 @@ struct I8Plan {
 // 128 k `idle` to `full`, as it fills the CUs (they share the L2s and the chip's power); a
 // split's second launch and its partials.  Model against measured (weights from HBM): 1296 x
 // 4096 -> 4096 in tiles of 256 x 256, 256 x 128, 128 x 128, 64 x 128 40 / 28 / 33 / 40
-// against 53 / 31 / 37 / 44, 3456 x 4096 -> 16384 202 / 220 / 260 / 335 against 208 /
-// 218 / 261 / 337, 512 x 4096 -> 4096 64 x 128 16 / 17, 68 x 8192 -> 2048 in 8 ranges 11 / 14.
+// against 45 / 31 / 37 / 41, 3456 x 4096 -> 16384 in tiles of 288 x 256 and these 174 / 202 / 220 / 260 / 335
+// against 176 / 195 / 209 / 254 / 330, 512 x 4096 -> 4096 64 x 128 16 / 17, 68 x 8192 -> 2048 in 8 ranges 11 / 13.
+// 288 rows take 12 % more than 256 where both fill as many rounds: 6144 x 4096 -> 16384 337 against 313;
+// one round instead of two: 4100 x 4096 -> 4096 61 against 82 (256 x 128).
 static double i8_time(int64_t M, int64_t N, int bm, int bn, int splits, double per) {
   const double wgs = (double)(((M + bm - 1) / bm) * ((N + bn - 1) / bn) * splits);
   double fixed = 1.6, idle = 0.30, full = 0.34;
-  if (bm == 256 && bn == 256) fixed = 6.0, idle = 0.85, full = 1.40;
+  if (bm == 288) fixed = 6.6, idle = 1.00, full = 1.56;
+  else if (bm == 256 && bn == 256) fixed = 6.0, idle = 0.85, full = 1.40;
   else if (bm == 256) fixed = 4.6, idle = 0.62, full = 0.78;
   else if (bm == 128) fixed = 2.5, idle = 0.42, full = 0.48;
   const double rounds = (double)(int64_t)(wgs / 256), rest = wgs / 256 - rounds;
@@ -522,7 +533,7 @@ static double i8_rows_time(int64_t M, int64_t N, int64_t K, int mb, int nb) {
 
 // The fastest single launch (or, where `split`, K ranges and a combining one) and its time
 static double i8_one(int64_t M, int64_t N, int64_t K, bool split, I8Plan* pl) {
-  static const int tile[4][2] = {{256, 256}, {256, 128}, {128, 128}, {64, 128}};
+  static const int tile[5][2] = {{288, 256}, {256, 256}, {256, 128}, {128, 128}, {64, 128}};
   // rows of the few-row kernel; 32 columns where that leaves a workgroup for every CU
   const int mb = M <= 16 ? 1 : (M <= 32 ? 2 : 4), nb = N >= 32 * 256 ? 2 : 1;
   const int64_t units = (K + 127) / 128;
@@ -547,8 +558,8 @@ static double i8_one(int64_t M, int64_t N, int64_t K, bool split, I8Plan* pl) {
 }
 
 // Rows [0, head) on 256-row tiles, where those make (nearly) whole rounds of the CUs and another
-// kernel takes the rows left over for less than one more round: 1296 x 4096 -> 12320 as 1280
-// rows of 256 x 256 and 16 of the few-row kernel 74 us, in one launch 83.
+// kernel takes the rows left over for less than one more round: 5120 x 4096 -> 4096 as 4096
+// rows of 256 x 256 tiles and 1024 of 128 x 128 77 us, in one launch 90; 1497 x 4032 -> 12744 77 and 93.
 static I8Plan i8_plan(int64_t M, int64_t N, int64_t K) {
   I8Plan pl;
   double best = i8_one(M, N, K, true, &pl);
@@ -579,6 +590,7 @@ static void i8_launch_tiles(GemmArgs p, const I8Plan& pl, hipStream_t s) {
     gemm_i8_kernel<T, EPI><<<blocks, T::THREADS, 0, s>>>(p, pl.k_split);
   };
   if (pl.bm == 256 && pl.bn == 256) go(I8Large{});
+  else if (pl.bm == 288) go(I8Huge{});
   else if (pl.bm == 256) go(I8Tall{});
   else if (pl.bm == 128) go(I8Mid{});
   else go(I8Small{});

@@ -151,6 +151,13 @@ def test_products(m, n, k):
         assert y.shape == (m, n) and y.dtype is torch.bfloat16 and over <= 0, (epilogue, sig, over)
 
 
+@pytest.mark.parametrize("m,n,k", [(520, 24576, 192), (1299, 12328, 576), (4100, 4104, 448), (1025, 4096, 16384),
+                                   (1500, 12744, 320)])
+def test_products_of_a_round_of_tall_tiles(m, n, k):
+    """Sizes that one round of the tallest tiles takes, a part of them in K ranges; and whole rounds with rows left over."""
+    test_products(m, n, k)
+
+
 @pytest.mark.parametrize("m", [1, 40, 300, 2100])
 def test_largest_sums_are_exact(m):
     """Codes of +-127 and -128 at the largest depth: sums near 2^31, whose fp32 value rounds once."""
