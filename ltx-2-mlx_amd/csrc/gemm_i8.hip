@@ -675,6 +675,10 @@ extern "C" int ltx_gemm_i8_bf16(const int8_t* A, int64_t lda, const float* a_sca
         bn = -2;
       }
     }
+    if (bn < 0) {  // (a launch has fewer than 2^32 threads)
+      const int64_t most = (((int64_t)1 << 23) - 1) / ((N - 16 * bn - 1) / (-16 * bn)) * bm;
+      piece = most < piece ? most : piece;
+    }
     for (; r0 < r1; r0 += piece) {
       GemmArgs part = p;
       part.A = (const bf16*)(A + r0 * lda);
