@@ -1051,6 +1051,9 @@ def main(argv=None):
         "roofline": roofline,
         "gemm_classes": gemm_classes,
     }
+    if args.weights == "int8" and _gemm.INT8_ACTIVATIONS:
+        out["dtype"] = "int8"
+        out["config"]["activations"] = "int8 rows (LTX_INT8_ACTIVATIONS=1); the reference keeps bf16 activations"
     if gemm_classes and "video_stream" in gemm_classes:
         out["video_stream_gemm_mfma_pct"] = round(100 * gemm_classes["video_stream"]["frac_bf16_peak"], 1)
     del graphs
