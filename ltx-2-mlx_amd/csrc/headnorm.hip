@@ -40,6 +40,10 @@ constexpr int64_t kHnHeads = 1 << 30;
 // 512 / 1024: 14640 x 32 and 8 heads of 128 bf16 96 / 94 / 98 us, 3456 x 32 heads of each side
 // 43 / 46 / 52, 9000 x 12 and 4 heads of 80 fp16 27 / 24 / 23.
 constexpr int kHnGradBlocks = 512;
+// Heads of a group up to which one workgroup takes a side of the gradient, and its dw needs no
+// second launch.  One launch / two, 32 and 8 heads of 128 bf16: 1 token 6.7 / 8.9 us, 2 tokens 7.4 / 8.8, 4 (four
+// heads a group) 9.1 / 8.8, 6 11.1 / 8.9; a launch costs the host 3.
+constexpr int kHnAlone = 4;
 
 struct HnSide {
   ltx_headnorm_rows r;
@@ -58,6 +62,7 @@ struct HnArgs {
   int lanes;       // of a head's group
   int table;       // table entries of a token: its pairs, up to a multiple of 4
   float* partial;  // gradient: dw of each workgroup, (blocks, head_dim)
+  bool alone;      // gradient: a workgroup per side, whose dw is the result
 };
 
 __device__ __forceinline__ double hn_position(const HnArgs& p, int64_t i) {
@@ -385,8 +390,9 @@ __global__ __launch_bounds__(kHnThreads) void headnorm_kernel(HnArgs p) {
         }
       }
     __syncthreads();
+    float* dw = p.alone ? r.dweight : p.partial + (int64_t)blockIdx.x * p.head_dim;
     for (int c = threadIdx.x; c < p.head_dim; c += kHnThreads)
-      p.partial[(int64_t)blockIdx.x * p.head_dim + c] = (cs[c] + cs[kHnMaxDim + c]) + (sn[c] + sn[kHnMaxDim + c]);
+      dw[c] = (cs[c] + cs[kHnMaxDim + c]) + (sn[c] + sn[kHnMaxDim + c]);
   }
 }
 
@@ -523,11 +529,20 @@ static int hn_args(const ltx_headnorm_rows* q, const ltx_headnorm_rows* k, bool 
   p->eps = (float)eps;
   p->offset = (float)offset;
   p->table = (int)(rotary_dim / 2 + 3) / 4 * 4;
+  const int64_t groups = kHnThreads / p->lanes;
+  p->alone = grad;
+  for (const HnSide& side : p->side)
+    if (p->all * side.r.heads > kHnAlone * groups || (side.r.heads == 0 && side.r.dweight)) p->alone = false;
   for (HnSide& side : p->side) {
     if (side.r.heads == 0) continue;
-    side.per_block = hn_tokens(p->all, side.r.heads * head_dim * (int64_t)size, size == 4 || grad, p->table);
+    if (p->alone) {
+      side.per_block = 1;
+      while (side.per_block < p->all && 2 * side.per_block * p->table <= kHnTable) side.per_block *= 2;
+    } else {
+      side.per_block = hn_tokens(p->all, side.r.heads * head_dim * (int64_t)size, size == 4 || grad, p->table);
+    }
     side.tiles = (p->all + side.per_block - 1) / side.per_block;
-    side.blocks = !grad || side.tiles < kHnGradBlocks ? side.tiles : kHnGradBlocks;
+    side.blocks = p->alone ? 1 : (!grad || side.tiles < kHnGradBlocks ? side.tiles : kHnGradBlocks);
   }
   return LTX_OK;
 }
@@ -577,7 +592,7 @@ extern "C" int ltx_headnorm_rotary_grad(const ltx_headnorm_rows* q, const ltx_he
     const int e = ltx_launch_status();
     if (e != LTX_OK) return e;
   }
-  if (!dwq && !dwk) return LTX_OK;
+  if ((!dwq && !dwk) || p.alone) return LTX_OK;
   headnorm_dw_kernel<<<dim3((unsigned)(head_dim + 7) / 8, 2), 512, 0, s>>>(
       workspace, p.side[0].blocks, p.side[1].blocks, (int)head_dim, dwq, dwk);
   return ltx_launch_status();

@@ -354,3 +354,34 @@ def test_int8_attention_layer():
     stretch = torch.linalg.matrix_norm(gate.double()[:, None] * values(wo), 2)
     assert stretch * moved.norm() <= 0.5 * (gate.double() * branch).norm()  # (what a wrong operator would exceed)
     assert (y.double() - want).norm() <= stretch * moved.norm() + 2.0 ** -8 * want.norm()
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 30])
+def test_gradient_of_few_tokens_without_a_side_or_weights(tokens):
+    """Sizes around those that one workgroup per side takes: no key heads (their weights' gradient is zero, whatever the
+    memory held), weights on one side only, and graphs replayed."""
+    from ltx_amd.kernels import rope_ops
+
+    q, k, gq, gk, wq, wk, pos, inv = _inputs(tokens, 8, 4, 128, 64, torch.bfloat16)
+    want, sums = _gradient(gq, q, wq, pos, inv)
+    for _ in range(3):
+        junk = [torch.full((128,), float("nan"), device=DEV) for _ in range(8)]
+        del junk
+        dq, dk, dwq, dwk = rope_ops.headnorm_rotary_grad(gq, gk[:, :0], q, k[:, :0], wq, wk, pos, inv, eps=EPS)
+        _within(dq, want)
+        _within(dwq, sums)
+        assert dk.shape == (tokens, 0, 128) and (dwk == 0).all()
+    dq, dk, none, dwk = rope_ops.headnorm_rotary_grad(gq, gk, q, k, None, wk, pos, inv, eps=EPS)
+    assert none is None
+    _within(dq, _gradient(gq, q, None, pos, inv)[0])
+    _within(dk, _gradient(gk, k, wk, pos, inv)[0])
+    _within(dwk, _gradient(gk, k, wk, pos, inv)[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = rope_ops.headnorm_rotary_grad(gq, gk, q, k, wq, wk, pos, inv, eps=EPS)
+    for _ in range(3):
+        gq.copy_(torch.randn(gq.shape, device=DEV))
+        fresh = rope_ops.headnorm_rotary_grad(gq, gk, q, k, wq, wk, pos, inv, eps=EPS)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, fresh))
