@@ -3,6 +3,8 @@ the calls both take, the Python path's results for all others."""
 
 from __future__ import annotations
 
+import gc
+
 import pytest
 import torch
 
@@ -72,3 +74,30 @@ def test_headnorm(both):  # noqa: F811
                 both(lambda: f(q, k, w, v, None, None, eps=1e-5))
                 both(lambda: f(q, k, w, v, pos, inv, out=(torch.empty_like(q), None), **kw))
                 both(lambda: b(gq, gk, q, k, w, v, pos, inv, out=(None, gk.clone()), **kw))
+
+
+def test_outputs_are_ordinary_tensors():
+    """What the native calls return: of the caller's device and allocator, inference tensors in inference mode only, and
+    no part of a graph for inputs that record one."""
+    from ltx_amd.kernels import gemm, rope_ops
+
+    x = torch.randn(5, 64, device="cuda")
+    q, pos = torch.randn(5, 2, 64, device="cuda", requires_grad=True), torch.arange(5, device="cuda")
+    inv, _ = rope_ops.rotary_frequencies(64)
+    rows = gemm.quantize_rows_int8(x)
+    with torch.inference_mode():
+        again = gemm.quantize_rows_int8(x)
+    assert not rows.codes.is_inference() and again.codes.is_inference() and torch.equal(rows.codes, again.codes)
+    y, _ = rope_ops.headnorm_rotary(q, None, None, None, pos, inv)
+    assert not y.requires_grad and y.device == x.device
+    gc.collect()  # (what earlier tests left)
+    before = torch.cuda.memory_allocated()
+    big = gemm.dequantize_rows_int8(gemm.quantize_rows_int8(torch.zeros(1024, 1024, device="cuda", dtype=torch.bfloat16)))
+    assert torch.cuda.memory_allocated() - before >= big.numel() * 2
+    assert big.untyped_storage().device == x.untyped_storage().device
+    del big
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
+    for t in (rows.codes, rows.scales, y):  # as torch's own: resized, copied, added to
+        t.resize_(4 * t.numel())
+        t.clone().add_(1)
