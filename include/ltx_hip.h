@@ -212,8 +212,8 @@ int ltx_rotary(const ltx_rotary_rows* q, const ltx_rotary_rows* k, int dtype, in
  * tokens over the batch and token and head strides below 2^32; `out` may be x (in
  * the gradient: x or g) with the same strides and must not overlap anything else.
  * g and dweight are not used by the forward call.  A side of no heads, or a call of
- * no tokens, leaves dweight zero.  The sum over tokens and heads is taken in an order that the sizes fix:
- * workgroups' shares go to `workspace` (device memory, 4-byte aligned, of
+ * no tokens, leaves dweight zero.  The sum over tokens and heads is taken in an order that the sizes fix, in
+ * fp32 over at most 256 heads of a lane and some exchanges, in fp64 beyond: workgroups' shares go to `workspace` (device memory, 4-byte aligned, of
  * ltx_headnorm_rotary_grad_workspace_bytes(head_dim) bytes; may be NULL without
  * dweight), and calls that may run at the same time need their own.
  */

@@ -16,8 +16,9 @@
 // for all heads, and with them the norm weights and, in the gradient, its share of dw.
 // The first heads are on their way while the workgroup computes its tokens' cosines and
 // sines, the next ones while it works on these.
-// Sums, r and dw are fp32, cosines and sines as in rotary.hip from fp64 angles; one
-// rounding at the end.
+// Sums and r are fp32, cosines and sines as in rotary.hip from fp64 angles; one
+// rounding at the end.  A lane's share of dw is fp32 over kHnRun heads, then the workgroup's is added to
+// in fp64: however long a call is, its chains of fp32 sums are not longer.
 // Measured, inputs from HBM: 3456 tokens x 64 heads of 128 bf16 29 us (3.9 TB/s; 23 with part of them in a cache,
 // the rotation alone 22), 14640 x 40
 // heads of 128 bf16 65 (4.6 TB/s), 14639 x 40 heads of 64 fp32 60 (5.0 TB/s), one token 4.7, its gradient at
@@ -44,6 +45,8 @@ constexpr int kHnGradBlocks = 512;
 // second launch.  One launch / two, 32 and 8 heads of 128 bf16: 1 token 6.7 / 8.9 us, 2 tokens 7.4 / 8.8, 4 (four
 // heads a group) 9.1 / 8.8, 6 11.1 / 8.9; a launch costs the host 3.
 constexpr int kHnAlone = 4;
+// Heads that a lane adds to its fp32 share of dw before the workgroup's fp64 sums take it
+constexpr int kHnRun = 256;
 
 struct HnSide {
   ltx_headnorm_rows r;
@@ -190,6 +193,7 @@ __global__ __launch_bounds__(kHnThreads) void headnorm_kernel(HnArgs p) {
   using V = HnVec<T, VEC>;
   constexpr int BATCH = IPL > 1 || GRAD ? 1 : 2;
   __shared__ __attribute__((aligned(16))) float cs[kHnTable], sn[kHnTable];
+  __shared__ double dws[GRAD ? kHnMaxDim : 1];  // gradient: the workgroup's dw
   const bool keys = (int)blockIdx.x >= p.side[0].blocks;
   const HnSide& side = p.side[keys];
   const ltx_headnorm_rows& r = side.r;
@@ -323,6 +327,45 @@ __global__ __launch_bounds__(kHnThreads) void headnorm_kernel(HnArgs p) {
       }
     }
   };
+  // The lanes' shares of dw to the workgroup's sums: the groups of a wave by lane exchanges, the
+  // waves through LDS in wave order.  All threads, at the same turn.
+  int run = 0;
+  if (GRAD)
+    for (int c = threadIdx.x; c < p.head_dim; c += kHnThreads) dws[c] = 0.0;  // (a thread adds to its own ones only)
+  auto share = [&]() __attribute__((always_inline)) {
+    if constexpr (GRAD) {
+      __shared__ float waves[kHnThreads / kWave][kHnMaxDim];
+      int tid = threadIdx.x;
+      asm volatile("" : "+v"(tid));  // (keeps what depends on it out of the registers of the turns)
+      const int wave = tid / kWave, own = tid % kWave;
+      run = 0;
+      if (r.dweight == nullptr) return;
+      auto from = [](float v, int from_lane) __attribute__((always_inline)) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(from_lane * 4, __builtin_bit_cast(int, v)));
+      };
+      __syncthreads();
+#pragma unroll
+      for (int s = 0; s < IPL; ++s)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          float va = d0[s][k], vb = d1[s][k];
+          d0[s][k] = d1[s][k] = 0.0f;
+          for (int off = G; off < kWave; off <<= 1) {
+            va += from(va, own ^ off);
+            vb += from(vb, own ^ off);
+          }
+          if (own < G && it[s].have) {
+            waves[wave][it[s].c0 + k] = va;
+            if (it[s].two) waves[wave][it[s].c1 + k] = vb;
+          }
+        }
+      __syncthreads();
+      for (int c = tid; c < p.head_dim; c += kHnThreads) {
+        const float part = (waves[0][c] + waves[1][c]) + (waves[2][c] + waves[3][c]);
+        dws[c] += (double)part;
+      }
+    }
+  };
   for (int tile = block; tile < side.tiles; tile += side.blocks) {
     first = tile * side.per_block;
     count = p.all - first < side.per_block ? p.all - first : side.per_block;
@@ -364,35 +407,16 @@ __global__ __launch_bounds__(kHnThreads) void headnorm_kernel(HnArgs p) {
       load(next);
       work(now);
       now = next;
+      if (GRAD && ++run == kHnRun) share();
     }
     work(now);
+    if (GRAD && ++run == kHnRun) share();
   }
   if constexpr (GRAD) {
     if (r.dweight == nullptr) return;
-    // the workgroup's share of dw: the groups of a wave by lane exchanges, the waves through LDS
-    // (the tables' place), in wave order
-    static_assert(2 * kHnTable >= 4 * kHnMaxDim, "room for the waves' shares");
-    const int wave = threadIdx.x / kWave;
-    __syncthreads();
-#pragma unroll
-    for (int s = 0; s < IPL; ++s)
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        float va = d0[s][k], vb = d1[s][k];
-        for (int off = G; off < kWave; off <<= 1) {
-          va += __shfl_xor(va, off, kWave);
-          vb += __shfl_xor(vb, off, kWave);
-        }
-        if (threadIdx.x % kWave < G && it[s].have) {
-          float* dst = (wave < 2 ? cs : sn) + (wave & 1) * kHnMaxDim;
-          dst[it[s].c0 + k] = va;
-          if (it[s].two) dst[it[s].c1 + k] = vb;
-        }
-      }
-    __syncthreads();
+    share();
     float* dw = p.alone ? r.dweight : p.partial + (int64_t)blockIdx.x * p.head_dim;
-    for (int c = threadIdx.x; c < p.head_dim; c += kHnThreads)
-      dw[c] = (cs[c] + cs[kHnMaxDim + c]) + (sn[c] + sn[kHnMaxDim + c]);
+    for (int c = threadIdx.x; c < p.head_dim; c += kHnThreads) dw[c] = (float)dws[c];
   }
 }
 
