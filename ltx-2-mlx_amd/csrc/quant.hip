@@ -272,7 +272,8 @@ __device__ __forceinline__ u32x2 int8_codes8(const float (&v)[8], float s, float
 // finite one's, in each type's own bits.
 template <typename T>
 struct Bits8 {
-  typedef T t8 __attribute__((ext_vector_type(8)));
+  typedef T t8 __attribute__((ext_vector_type(8), aligned(16)));  // (eight fp32 are two loads of 16 bytes)
+  static_assert(alignof(t8) == 16, "rows are at multiples of 16 bytes");
   typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
   static constexpr uint32_t kInf =
       std::is_same_v<T, float> ? 0x7f800000u : (std::is_same_v<T, bf16> ? 0x7f80u : 0x7c00u);
