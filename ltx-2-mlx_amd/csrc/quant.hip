@@ -398,8 +398,8 @@ static void int8_rows_launch(const T* x, int64_t ldx, int64_t rows, int64_t K, i
   auto pick = [&](auto wpr) {
     if (pieces <= 1) go(wpr, std::integral_constant<int, 1>{});
     else if (pieces <= 2) go(wpr, std::integral_constant<int, 2>{});
-    else if (pieces <= 4) go(wpr, std::integral_constant<int, 4>{});
-    else go(wpr, std::integral_constant<int, 8>{});
+    else if (decltype(wpr)::value == 1 || pieces <= 4) go(wpr, std::integral_constant<int, 4>{});
+    else if constexpr (decltype(wpr)::value == 4) go(wpr, std::integral_constant<int, 8>{});  // (one wave: at most 2048)
   };
   if (pieces > 8) int8_long_rows_kernel<<<(int)rows, 256, 0, s>>>(x, ldx, K, q, ldq, scale);
   else if (one) pick(std::integral_constant<int, 1>{});
