@@ -28,7 +28,10 @@ Prints ONE JSON line.  Besides ms/step and tokens/s it carries:
                 clock stamps as the roofline kernel: launches, average us,
                 algorithmic flops / launch time and its fraction of the bf16
                 MFMA peak (the audio stream's and the contexts' launches run
-                beside the video stream's, sharing the chip);
+                beside the video stream's, sharing the chip); with int8
+                activations (LTX_INT8_ACTIVATIONS=1) of the int8 MFMA peak,
+                here and in roofline and gemm_shapes, the rows' quantisation
+                included in the launches' times;
   attention     the flash-attention calls of the block alone (video self at
                 3456 and 6144 tokens, the 3456 x 256 text cross-attention,
                 A2V 3456 x 68 and split-KV V2A 68 x 3456), each replayed from
@@ -81,7 +84,22 @@ sys.path.insert(0, str(ROOT / "ltx-2-mlx_amd"))
 
 METRIC = "ms per DiT denoise step (1 GPU, 768x512x65); fused-op HBM GB/s; GEMM MFMA %"
 PEAK_BF16_TFLOPS = 2500.0
+PEAK_INT8_TOPS = 5000.0
 PEAK_HBM_GBPS = 8000.0
+
+
+def mfma_peak(kind: str) -> tuple[str, float]:
+    """(name of the fraction, dense peak) that products of one kind (the first
+    of their launch info) are measured against: the int8 MFMA's for int8 rows
+    times int8 weights, the bf16 one's for the others."""
+    return ("frac_int8_peak", PEAK_INT8_TOPS) if kind == "w8a8" else ("frac_bf16_peak", PEAK_BF16_TFLOPS)
+
+
+def peak_fraction(kinds, flops: float, ms: float) -> dict:
+    """The fraction of the MFMA peak of launches of these kinds together;
+    nothing where they have different ones."""
+    peaks = {mfma_peak(kind) for kind in kinds}
+    return {name: round(flops / (ms * 1e-3) / 1e12 / peak, 4) for name, peak in peaks if len(peaks) == 1}
 
 
 def parse_args(argv=None):
@@ -414,17 +432,16 @@ def gemm_step_profile(run_step, steps, tv, torch, prefill=None):
         g[0] += 1
         g[1] += 2.0 * m * n * k
         g[2] += ms
+    kinds = {rec[0][0] for rec in recs}
     summary = {}
     tot = [0, 0.0, 0.0]
     for name, (cnt, fl, ms) in groups.items():
         tot = [tot[0] + cnt, tot[1] + fl, tot[2] + ms]
         summary[name] = {"launches_per_step": cnt // steps, "gflop_per_step": round(fl / steps / 1e9, 1),
                          "ms_per_step": round(ms / steps, 3),
-                         "tflops": round(fl / (ms * 1e-3) / 1e12, 1),
-                         "frac_bf16_peak": round(fl / (ms * 1e-3) / 1e12 / PEAK_BF16_TFLOPS, 4)}
+                         "tflops": round(fl / (ms * 1e-3) / 1e12, 1), **peak_fraction(kinds, fl, ms)}
     summary["all"] = {"gflop_per_step": round(tot[1] / steps / 1e9, 1), "ms_per_step": round(tot[2] / steps, 3),
-                      "tflops": round(tot[1] / (tot[2] * 1e-3) / 1e12, 1),
-                      "frac_bf16_peak": round(tot[1] / (tot[2] * 1e-3) / 1e12 / PEAK_BF16_TFLOPS, 4)}
+                      "tflops": round(tot[1] / (tot[2] * 1e-3) / 1e12, 1), **peak_fraction(kinds, tot[1], tot[2])}
     return ff_up, summary, host_ms
 
 
@@ -553,28 +570,28 @@ class LaunchStamps:
 
 def gemm_class_summary(records) -> dict:
     """Per GEMM class: launches, average us, algorithmic TFLOP/s and fraction
-    of the bf16 peak over the stamped launches; ``video_stream`` combines
+    of the MFMA peak over the stamped launches; ``video_stream`` combines
     the video-stream classes (flops over summed durations of one launch of
     each kind per block, i.e. weighted by how often the step runs them)."""
     acc = {}
-    for label, (_, m, n, k, _), ms in records:
-        a = acc.setdefault(label, [0, 0.0, 0.0])
+    for label, (kind, m, n, k, _), ms in records:
+        a = acc.setdefault(label, [0, 0.0, 0.0, set()])
         a[0] += 1
         a[1] += 2.0 * m * n * k
         a[2] += ms
+        a[3].add(kind)
     res = {}
-    for label, (cnt, fl, ms) in sorted(acc.items()):
+    for label, (cnt, fl, ms, kinds) in sorted(acc.items()):
         res[label] = {"launches": cnt, "avg_us": round(ms / cnt * 1e3, 1),
                       "gflop_per_launch": round(fl / cnt / 1e9, 2),
-                      "tflops": round(fl / (ms * 1e-3) / 1e12, 1),
-                      "frac_bf16_peak": round(fl / (ms * 1e-3) / 1e12 / PEAK_BF16_TFLOPS, 4)}
+                      "tflops": round(fl / (ms * 1e-3) / 1e12, 1), **peak_fraction(kinds, fl, ms)}
     per_block = {"ff_up": 1, "ff_down": 1, "qkv": 1, "out": 2, "text_q": 1, "a2v_q": 1, "a2v_out": 1}
     if all(c in res for c in per_block):
         fl = sum(res[c]["gflop_per_launch"] * per_block[c] for c in per_block)
         us = sum(res[c]["avg_us"] * per_block[c] for c in per_block)
+        kinds = set().union(*(acc[c][3] for c in per_block))
         res["video_stream"] = {"us_per_block": round(us, 1), "gflop_per_block": round(fl, 1),
-                               "tflops": round(fl / us * 1e3, 1),
-                               "frac_bf16_peak": round(fl / us * 1e3 / PEAK_BF16_TFLOPS, 4)}
+                               "tflops": round(fl / us * 1e3, 1), **peak_fraction(kinds, fl * 1e9, us * 1e-3)}
     return res
 
 
@@ -595,6 +612,7 @@ def gemm_shapes(torch, fmt: str, m: int = 3456, tile=None) -> dict:
         w = (torch.randn((n, k), generator=g, device="cuda") * 0.02).bfloat16()
         wt = gemm.make_weight(w, torch.zeros(n, device="cuda"), kind=fmt)
         out = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+        frac, peak = mfma_peak("w8a8" if gemm._int8_eligible(x, wt, tile, None) else fmt)
         gemm.linear(x, wt, out=out, tile=tile)
         torch.cuda.synchronize()
         iters = 10
@@ -614,13 +632,13 @@ def gemm_shapes(torch, fmt: str, m: int = 3456, tile=None) -> dict:
             best = min(best, a.elapsed_time(b) / iters)
         fl = 2.0 * m * n * k
         res[name] = {"ms": round(best, 4), "tflops": round(fl / (best * 1e-3) / 1e12, 1),
-                     "frac_bf16_peak": round(fl / (best * 1e-3) / 1e12 / PEAK_BF16_TFLOPS, 4), "per_block": count}
+                     frac: round(fl / (best * 1e-3) / 1e12 / peak, 4), "per_block": count}
         tot_ms += best * count
         tot_fl += fl * count
         del graph, x, w, wt, out
     res["block_total"] = {"ms": round(tot_ms, 4), "gflop": round(tot_fl / 1e9, 1),
                           "tflops": round(tot_fl / (tot_ms * 1e-3) / 1e12, 1),
-                          "frac_bf16_peak": round(tot_fl / (tot_ms * 1e-3) / 1e12 / PEAK_BF16_TFLOPS, 4)}
+                          frac: round(tot_fl / (tot_ms * 1e-3) / 1e12 / peak, 4)}
     return res
 
 
@@ -937,6 +955,31 @@ def guided_step_ms(model, args, ta: int, s: int) -> dict:
             "loop": "CfgAvLoop: CFG-star video 3.0 / audio 7.0 + STG 1.0 (all blocks), LTX2Scheduler sigmas"}
 
 
+def ff_up_roofline(kind: str, tv: int, k_ms: float, launches: int, timing: str) -> dict:
+    """The roofline record of the dominant kernel: the video FF up-projection
+    of ``kind`` (a weight format; "w8a8": int8 rows times int8 weights), k_ms
+    per launch."""
+    k_flop = 2.0 * tv * 4096 * 16384
+    achieved = k_flop / (k_ms * 1e-3) / 1e12
+    _, peak = mfma_peak(kind)
+    if kind == "w8a8":
+        kname, how, unit = "gemm_i8_kernel<GELU>", "int8 MFMA; a launch is int8_rows_kernel and the product", "TOP/s"
+    else:
+        # the kernel the automatic tile choice runs for this shape: the 8-wave
+        # kernel for every weight format, its 256-row tiles for the first rows and
+        # (when that shortens the partial last round, e.g. rows 3072-3455 of the
+        # 3456-token step) 128-row tiles for the rest in a second launch; a launch
+        # here is the product, i.e. both launches
+        kname, unit = f"gemm8_kernel<{kind},GELU>", "TFLOP/s"
+        how = "bf16 MFMA; the automatic row split into 256- and 128-row tiles"
+    return {"bound": "mfma", "kernel": f"{kname} (video FF up, M={tv} K=4096 N=16384; {how})",
+            "achieved": round(achieved, 1), "peak": peak, "unit": unit,
+            "frac": round(achieved / peak, 4), "traffic": measured_traffic(kname, kind),
+            "launch_us": round(k_ms * 1e3, 1), "launches_timed": launches,
+            "launch_timing": timing,
+            "algorithmic_flop_per_launch": k_flop}
+
+
 def main(argv=None):
     args = parse_args(argv)
     if args.gpus != 1:
@@ -1020,21 +1063,8 @@ def main(argv=None):
         durs, _, _ = gemm_step_profile(run_step, args.kernel_steps, tv, torch)
         timing = "stream events around each launch in eager steps"
     k_ms = sum(durs) / len(durs)
-    k_flop = 2.0 * tv * 4096 * 16384
-    achieved = k_flop / (k_ms * 1e-3) / 1e12
-    # the kernel the automatic tile choice runs for this shape: the 8-wave
-    # kernel for every weight format, its 256-row tiles for the first rows and
-    # (when that shortens the partial last round, e.g. rows 3072-3455 of the
-    # 3456-token step) 128-row tiles for the rest in a second launch; a launch
-    # here is the product, i.e. both launches
-    kname = f"gemm8_kernel<{args.weights},GELU>"
-    roofline = {"bound": "mfma", "kernel": f"{kname} (video FF up, M={tv} K=4096 N=16384; bf16 MFMA; "
-                                           "the automatic row split into 256- and 128-row tiles)",
-                "achieved": round(achieved, 1), "peak": PEAK_BF16_TFLOPS, "unit": "TFLOP/s",
-                "frac": round(achieved / PEAK_BF16_TFLOPS, 4), "traffic": measured_traffic(kname, args.weights),
-                "launch_us": round(k_ms * 1e3, 1), "launches_timed": len(durs),
-                "launch_timing": timing,
-                "algorithmic_flop_per_launch": k_flop}
+    rows8 = args.weights == "int8" and _gemm.INT8_ACTIVATIONS
+    roofline = ff_up_roofline("w8a8" if rows8 else args.weights, tv, k_ms, len(durs), timing)
     flops = step_flops(tv, ta, s, args.layers)
     out = {
         "metric": METRIC, "value": round(ms, 3), "unit": "ms/step", "n_gpus": 1, "steps": args.steps,
@@ -1047,15 +1077,16 @@ def main(argv=None):
                    "weights": args.weights, "timing": "hip-graph replay, FF-up launches bracketed by device clock stamps" if graphs else "eager"},
         "tokens_per_s": round((tv + ta) / (ms * 1e-3), 1),
         "step_tflop": round(flops / 1e12, 2), "step_tflops_achieved": round(flops / (ms * 1e-3) / 1e12, 1),
-        "ff_up_mfma_pct": round(100 * achieved / PEAK_BF16_TFLOPS, 1),
+        "ff_up_mfma_pct": round(100 * roofline["frac"], 1),
         "roofline": roofline,
         "gemm_classes": gemm_classes,
     }
-    if args.weights == "int8" and _gemm.INT8_ACTIVATIONS:
+    if rows8:
         out["dtype"] = "int8"
         out["config"]["activations"] = "int8 rows (LTX_INT8_ACTIVATIONS=1); the reference keeps bf16 activations"
     if gemm_classes and "video_stream" in gemm_classes:
-        out["video_stream_gemm_mfma_pct"] = round(100 * gemm_classes["video_stream"]["frac_bf16_peak"], 1)
+        vs = gemm_classes["video_stream"]
+        out["video_stream_gemm_mfma_pct"] = round(100 * vs[mfma_peak("w8a8" if rows8 else args.weights)[0]], 1)
     del graphs
     if args.weights == "mxfp8" and not args.no_mx:
         print("# opt-in MX path: step graphs with MXFP8 activations", file=sys.stderr, flush=True)

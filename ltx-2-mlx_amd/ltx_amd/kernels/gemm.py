@@ -70,7 +70,9 @@ INT8_ACTIVATIONS = os.environ.get("LTX_INT8_ACTIVATIONS", "0") == "1"
 
 # Optional launch observer: called as hook(phase, info) with phase "pre" /
 # "post" around every GEMM launch on the launching stream (used by bench.py
-# to time chosen launches with stream events).  None in normal operation.
+# to time chosen launches with stream events), what quantises its rows
+# included.  info: (weight format, "w8a8" where int8 rows meet int8 weights;
+# M, N, K, epilogue).  None in normal operation.
 LAUNCH_HOOK = None
 
 
@@ -716,11 +718,13 @@ def _int8_workspace_bytes(m: int, n: int, k: int) -> int:
 
 
 def _linear_int8(x: Int8Rows, weight: LinearWeight, epilogue: int, out: torch.Tensor | None,
-                 residual: torch.Tensor | None, gate: torch.Tensor | None, sigmoid_from: int | None) -> torch.Tensor:
-    """:func:`linear` for int8 rows and int8 weights."""
+                 residual: torch.Tensor | None, gate: torch.Tensor | None, sigmoid_from: int | None,
+                 watched: bool = False) -> torch.Tensor:
+    """:func:`linear` for int8 rows and int8 weights (``watched``: inside its caller's calls of the launch observer)."""
     w, scale, bias = weight.w, weight.scale, weight.bias
     codes, xs = x.codes, x.scales
-    if _lib.CALLS is not None and LAUNCH_HOOK is None:
+    hook = None if watched else LAUNCH_HOOK
+    if _lib.CALLS is not None and hook is None:
         where = _lib.fast_stream(w)
         if where is not None:
             y = _lib.CALLS.linear8(codes, xs, w, scale, bias,
@@ -776,8 +780,7 @@ def _linear_int8(x: Int8Rows, weight: LinearWeight, epilogue: int, out: torch.Te
         return out
     ws_bytes = _int8_workspace_bytes(m, n, k)
     ws = codes.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
-    hook = LAUNCH_HOOK
-    info = (weight.kind, m, n, k, epilogue)
+    info = ("w8a8", m, n, k, epilogue)
     if hook is not None:
         hook("pre", info)
     st = _lib.launch(device, "ltx_gemm_i8_bf16", codes.data_ptr(), lda, xs.data_ptr(), w.data_ptr(), ldw,
@@ -807,19 +810,26 @@ def _linear_int8_rows(x: torch.Tensor, weight: LinearWeight, epilogue: int, out:
                       sigmoid_from: int | None) -> torch.Tensor:
     """:func:`linear` of bf16 rows (..., K) through int8 rows."""
     lead, n = x.shape[:-1], weight.out_features
+    hook = LAUNCH_HOOK if x.numel() else None
+    info = ("w8a8", x.numel() // max(x.shape[-1], 1), n, weight.in_features, epilogue)
+    if hook is not None:
+        hook("pre", info)
     rows = quantize_rows_int8(x)
-    if len(lead) == 1:
-        return _linear_int8(rows, weight, epilogue, out, residual, gate, sigmoid_from)
-    if out is None:
-        return _linear_int8(rows, weight, epilogue, None, residual, gate, sigmoid_from).view(*lead, n)
-    if out.shape != (*lead, n):
-        raise ValueError(f"out must have the shape {(*lead, n)}, got {tuple(out.shape)}")
-    ov, ldc = _lib.row_view(out, n)
-    if ov.data_ptr() != out.data_ptr():
-        raise ValueError("out must be a row-strided view")
-    _linear_int8(rows, weight, epilogue, out.as_strided((rows.codes.shape[0], n), (ldc, 1)), residual, gate,
-                 sigmoid_from)
-    return out
+    rest = residual, gate, sigmoid_from, hook is not None
+    if len(lead) == 1 or out is None:
+        y = _linear_int8(rows, weight, epilogue, out, *rest)
+        y = y if len(lead) == 1 else y.view(*lead, n)
+    else:
+        if out.shape != (*lead, n):
+            raise ValueError(f"out must have the shape {(*lead, n)}, got {tuple(out.shape)}")
+        ov, ldc = _lib.row_view(out, n)
+        if ov.data_ptr() != out.data_ptr():
+            raise ValueError("out must be a row-strided view")
+        _linear_int8(rows, weight, epilogue, out.as_strided((rows.codes.shape[0], n), (ldc, 1)), *rest)
+        y = out
+    if hook is not None:
+        hook("post", info)
+    return y
 
 
 def rowss_eligible(x: torch.Tensor, weight: LinearWeight) -> bool:
