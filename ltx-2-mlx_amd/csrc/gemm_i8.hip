@@ -127,14 +127,15 @@ static void i8_launch_rows(GemmArgs p, int epi, hipStream_t s) {
 // The rings: LDS holds two stages of 256 x 256 tiles and one operand's third.  The weights have it:
 // their loads leave two stages ahead, and they are what comes from HBM (every row tile of a
 // round reads the same activations from the L2s).  With eight sets of operands in turn 3456 x 16384 ->
-// 4096 takes 192 us, 208 with two stages each, 180 with one set; 6144 x 4096 -> 16384 333 / 344 / 322.
+// 4096 takes 192 us, 208 with two stages each, 180 with one set; 6144 x 4096 -> 16384 333 / 344 / 322 (one
+// card; others take up to 8 % more: 208 / 191 and 350 / 337 in turn / with one set).
 // More stages of the smaller tiles: 0 to 4 % slower (their first loads are as many more).
 //
 // What bounds it: the chip's power.  A stage of 256 x 256 tiles takes 1.4 us with every CU
 // busy, 3.0 PO/s (6144 x 4096 -> 16384 without its epilogues 275 us), 1.08 us on zeros; a loop
 // of nothing but these MFMAs on such codes reaches 4.1 (32 x 32 x 32: 3.5); the stage without its
-// loads takes 1.19 us, without its fragment reads 1.21, without MFMAs 0.99.  Epilogues take 25
-// us of that product's 300 with bias, GELU 17 more.  Measured beside it: four waves of 128 x 128, sums
+// loads takes 1.19 us, without its fragment reads 1.21, without MFMAs 0.99.  With its epilogues that
+// product takes 312 us with bias and 330 with GELU (one set of operands).  Measured beside it, one set each: four waves of 128 x 128, sums
 // in AGPRs (a third less LDS traffic), 152 against 148 us (4096 x 12288 -> 4096); 224-row tiles, which
 // give each CU one at 3456 x 16384 -> 4096, 178 against 181; loads in one half step, all
 // fragment reads in the first group, fewer vector instructions in the loop: no change; two
@@ -475,7 +476,10 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(GemmArgs p, in
 }
 
 // 288 rows: where they make one round of the CUs less than 256 (below); the third stage of weights has no room
-// beside them, and the residual epilogue spills.
+// beside them.  The residual epilogues spill: at 256 x 256 19 to 21 registers, which stay in the epilogue, at 288
+// rows 67 to 69, whose reloads make the stages wait for part of their loads.  The choice does not know the epilogue; 288 rows
+// against the best other tiles, x 16384 -> 4096, sets of operands in turn (us): 4608 rows 229 / 249 with bias, 270 / 269
+// with residual, 9216 rows 453 / 476 and 517 / 494, 13824 rows 674 / 695 and 774 / 725.
 using I8Huge = I8Tile<288, 256, 2, 4, 2, 2>;
 using I8Large = I8Tile<256, 256, 2, 4, 2, 3>;
 using I8Tall = I8Tile<256, 128, 4, 2, 3, 3>;

@@ -20,7 +20,8 @@ struct I8Plan {
 // 4096 -> 4096 in tiles of 256 x 256, 256 x 128, 128 x 128, 64 x 128 40 / 28 / 33 / 40
 // against 45 / 31 / 37 / 41, 3456 x 4096 -> 16384 in tiles of 288 x 256 and these 174 / 202 / 220 / 260 / 335
 // against 176 / 195 / 209 / 254 / 330, 512 x 4096 -> 4096 64 x 128 16 / 17, 68 x 8192 -> 2048 in 8 ranges 11 / 13.
-// 288 rows take 12 % more than 256 where both fill as many rounds: 6144 x 4096 -> 16384 337 against 313;
+// 288 rows take 12 % more than 256 where both fill as many rounds: 6144 x 4096 -> 16384 337 against 313
+// (bias; with a residual their epilogue spills and they are up to 7 % slower also with a round less);
 // one round instead of two: 4100 x 4096 -> 4096 61 against 82 (256 x 128).
 inline double i8_time(int64_t M, int64_t N, int bm, int bn, int splits, double per) {
   const double wgs = (double)(((M + bm - 1) / bm) * ((N + bn - 1) / bn) * splits);

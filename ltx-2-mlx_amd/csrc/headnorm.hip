@@ -19,10 +19,12 @@
 // Sums and r are fp32, cosines and sines as in rotary.hip from fp64 angles; one
 // rounding at the end.  A lane's share of dw is fp32 over kHnRun heads, then the workgroup's is added to
 // in fp64: however long a call is, its chains of fp32 sums are not longer.
-// Measured, inputs from HBM: 3456 tokens x 64 heads of 128 bf16 29 us (3.9 TB/s; 23 with part of them in a cache,
+// Measured, inputs from HBM: 3456 tokens x 64 heads of 128 bf16 30 us (3.8 TB/s; 23 with part of them in a cache,
 // the rotation alone 22), 14640 x 40
-// heads of 128 bf16 65 (4.6 TB/s), 14639 x 40 heads of 64 fp32 60 (5.0 TB/s), one token 4.7, its gradient at
-// 14640 x 40 heads of 128 bf16 94 (4.8 TB/s, 4 of them the second launch), 3456 x 64 heads 46.  About
+// heads of 128 bf16 66 (4.5 TB/s), 14639 x 40 heads of 64 fp32 62 (4.8 TB/s), one token 4.3, its gradient at
+// 14640 x 40 heads of 128 bf16 94 (4.8 TB/s, 4 of them the second launch), 3456 x 64 heads 47 (39 with part of them
+// in a cache).  Heads of 80 and 96 have five and six items in groups of eight lanes: 9000 x 16 of them in fp16 20 and 22
+// us, the gradient 30 and 32, where a copy of as many bytes takes 9.0, 10.8, 13.5 and 16.2.  About
 // 300 vector instructions per eight heads of 128 lie beside the loads.  Beside it: both sides in one
 // workgroup 43, 88 and 127 us (3456 and 14640 tokens, gradient); two heads on their way and one at work
 // (29, 70, 102); as many workgroups as the CUs hold, each with tiles of the same size (28, 70, 101); positions in
@@ -38,8 +40,9 @@ constexpr int kHnTable = 2048;  // cosines (and sines) of a workgroup
 constexpr int64_t kHnBlocks = (1 << 23) - 1;  // of a side: a launch has fewer than 2^32 threads
 constexpr int64_t kHnHeads = 1 << 30;
 // Workgroups of a side of the gradient, each with a share of dw and one tile after another.  384 /
-// 512 / 1024: 14640 x 32 and 8 heads of 128 bf16 96 / 94 / 98 us, 3456 x 32 heads of each side
-// 43 / 46 / 52, 9000 x 12 and 4 heads of 80 fp16 27 / 24 / 23.
+// 512 / 1024, inputs from HBM: 14640 x 32 and 8 heads of 128 bf16 99 / 94 / 98 us, 3456 x 32 heads of each side
+// 44 / 47 / 53, 9000 x 12 and 4 heads of 80 fp16 31 / 30 / 30.  (147 registers: the chip holds 768 at a time, so of
+// two long sides' 1024 a quarter waits for a second round.)
 constexpr int kHnGradBlocks = 512;
 // Heads of a group up to which one workgroup takes a side of the gradient, and its dw needs no
 // second launch.  One launch / two, 32 and 8 heads of 128 bf16: 1 token 6.7 / 8.9 us, 2 tokens 7.4 / 8.8, 4 (four

@@ -306,9 +306,9 @@ struct Bits8 {
 };
 
 // A row stays in the registers of WPR waves between its maximum and its codes: NC pieces of
-// 512 * WPR elements, eight per lane.  Bound by HBM: 14640 x 4096 bf16 35 us (5.2 TB/s; read twice, with
-// a division per element, 52), fp32 54 (5.5), 3456 x 16384 bf16 39 (4.3), 68 x 2048 4.2, a launch; the decoder
-// 14640 x 4096 32 (5.7).
+// 512 * WPR elements, eight per lane.  Bound by HBM: from memory that no cache holds 14640 x 4096 bf16 37 us (4.8
+// TB/s; read twice, with a division per element, 52), fp32 53 (5.7), 3456 x 16384 bf16 37 (4.6), 68 x 2048 3.1, a
+// launch; the decoder 14640 x 4096 32 (5.6).  The same rows again, partly in the last-level cache: 29 and 29.
 template <typename T, int WPR, int NC>
 __global__ __launch_bounds__(256) void int8_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t K,
                                                         int8_t* __restrict__ q, int64_t ldq,
