@@ -967,8 +967,8 @@ def ff_up_roofline(kind: str, tv: int, k_ms: float, launches: int, timing: str) 
     else:
         # the kernel the automatic tile choice runs for this shape: the 8-wave
         # kernel for every weight format, its 256-row tiles for the first rows and
-        # (when that shortens the partial last round, e.g. rows 3072-3455 of the
-        # 3456-token step) 128-row tiles for the rest in a second launch; a launch
+        # (when that shortens the partial last round, e.g. the last 384 rows of
+        # the 3456-token step) 128-row tiles for the rest in a second launch; a launch
         # here is the product, i.e. both launches
         kname, unit = f"gemm8_kernel<{kind},GELU>", "TFLOP/s"
         how = "bf16 MFMA; the automatic row split into 256- and 128-row tiles"
